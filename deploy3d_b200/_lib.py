@@ -85,6 +85,7 @@ _sz = ctypes.c_size_t
 _descp = ctypes.POINTER(TensorDesc)
 _vpp = ctypes.POINTER(ctypes.c_void_p)
 _szp = ctypes.POINTER(ctypes.c_size_t)
+_int, _i64, _f32 = ctypes.c_int, ctypes.c_int64, ctypes.c_float
 
 
 def _enqueue_sig(params_t):
@@ -179,6 +180,20 @@ SIGNATURES = {
     "d3d_yolox3d_decode_enqueue": (ctypes.c_int, _enqueue_sig(ctypes.POINTER(YoloX3dDecodeParams))),
     "d3d_nms3d_enqueue_static": (ctypes.c_int, [ctypes.POINTER(Nms3dParams), _descp, ctypes.c_int, _descp,
                                                  ctypes.c_int, _vpp, _vpp, _vp]),
+    "d3d_layer_norm": (ctypes.c_int, [_int, _vp, _i64, _vp, _i64, _vp, _vp, _f32, _i64, _int] + [_vp] * 6),
+    "d3d_layer_norm_backward_workspace": (_sz, [_i64, _int]),
+    "d3d_layer_norm_backward": (ctypes.c_int, [_int, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _vp, _vp, _i64, _int, _vp, _vp,
+                                               _vp, _vp, _vp, _sz, _vp]),
+    "d3d_quantize_rows": (ctypes.c_int, [_int, _vp, _i64, _i64, _int, _vp, _vp, _i64, _vp, _vp]),
+    "d3d_layer_norm_int8": (ctypes.c_int, [_int, _vp, _i64, _vp, _i64, _vp, _vp, _f32, _i64, _int, _vp, _vp, _vp, _i64, _vp,
+                                           _vp]),
+    "d3d_gated_recurrence_state_rows": (_i64, [_i64]),
+    "d3d_gated_recurrence_workspace": (_sz, [_i64, _int]),
+    "d3d_gated_recurrence": (ctypes.c_int, [_int, _vp, _i64, _vp, _i64, _vp, _int, _i64, _int, _int, _vp, _vp, _vp, _vp, _vp,
+                                            _sz, _vp]),
+    "d3d_gated_recurrence_backward": (ctypes.c_int, [_int, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _int, _i64, _int, _int] +
+                                      [_vp] * 7 + [_sz, _vp]),
+    "d3d_gated_recurrence_step": (ctypes.c_int, [_int, _vp, _i64, _vp, _i64, _vp, _vp, _vp, _i64, _int, _vp]),
 }
 
 _LIB = None

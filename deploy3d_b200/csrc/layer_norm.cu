@@ -1,0 +1,586 @@
+// Layer norm over the channels of voxel rows, its backward pass, and rows in 8-bit integers.
+//   t = x + r,  y = (t - mean) rstd w + b,  rstd = 1 / sqrt(var + eps)
+//   dx = rstd (g - <g> - xhat <g xhat>),  g = dy w,  xhat = (t - mean) rstd,  dw = sum dy xhat,  db = sum dy
+//   s = max |y| / 127,  q = rint(y / s)
+// All of them move bytes: every tensor is read and written once, in 16-byte pieces, a row stays in the registers of
+// the threads that share it, and mean, variance and the two means of the backward pass are exact sums over those
+// registers (the variance of differences to the mean, not a difference of two large sums).
+#include <type_traits>
+
+#include "common.cuh"
+
+namespace d3d {
+namespace {
+
+template <class T, int V> struct alignas(sizeof(T) * V) Pack { T v[V]; };
+
+struct NormArgs {
+  const void *x, *residual;
+  int64_t x_ld, residual_ld;
+  const float *weight, *bias;
+  float eps;
+  int64_t rows;
+  int channels;
+  const int32_t* num_rows;  // live rows on the device, or null
+  void *total, *out;        // [rows][channels]
+  float *mean, *rstd;
+  int8_t* q;
+  int64_t q_ld;
+  float* scales;
+};
+
+__device__ __forceinline__ int64_t live_rows(int64_t rows, const int32_t* num_rows) {
+  if (!num_rows) return rows;
+  const int64_t n = __ldg(num_rows);
+  return n < 0 ? 0 : n < rows ? n : rows;
+}
+
+struct Add {
+  __device__ __forceinline__ float operator()(float a, float b) const { return a + b; }
+};
+struct MaxBits {
+  __device__ __forceinline__ uint32_t operator()(uint32_t a, uint32_t b) const { return a > b ? a : b; }
+};
+
+// Combines N values over the kLanes threads that share a row; every thread gets the results.  Within a warp by shuffles, beyond
+// it through `scratch` (two buffers of N words a warp, used in turn: one barrier per call).
+template <int kLanes, int N, class T, class Op>
+__device__ __forceinline__ void row_reduce(T (&v)[N], Op op, uint32_t* scratch, int& turn) {
+#pragma unroll
+  for (int d = (kLanes < 32 ? kLanes : 32) / 2; d >= 1; d >>= 1)
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = op(v[i], __shfl_xor_sync(0xffffffffu, v[i], d));
+  if (kLanes > 32) {
+    constexpr int kWarps = kLanes > 32 ? kLanes / 32 : 1;
+    T* s = reinterpret_cast<T*>(scratch) + turn * (kWarps * N);
+    turn ^= 1;
+    if (lane_id() == 0)
+#pragma unroll
+      for (int i = 0; i < N; ++i) s[(threadIdx.x >> 5) * N + i] = v[i];
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      v[i] = s[i];
+#pragma unroll
+      for (int w = 1; w < kWarps; ++w) v[i] = op(v[i], s[w * N + i]);
+    }
+  }
+}
+
+// The integer nearest to v / s, ties to even, as if the quotient were exact: the product with 1 / s is at most one step
+// off, and what is left over, v - r s, has no rounding error near the border (s / 2) that decides.
+__device__ __forceinline__ int nearest_step(float v, float s, float inv) {
+  float r = rintf(v * inv);
+  const float left = fmaf(-r, s, v), half = 0.5f * s;
+  const bool odd = ((int)r & 1) != 0;
+  if (left > half || (odd && left == half)) r += 1.f;
+  else if (left < -half || (odd && left == -half)) r -= 1.f;
+  return (int)fminf(fmaxf(r, -127.f), 127.f);
+}
+// Scale of a row whose largest magnitude has these bits.  A row that is not finite has no scale (NaN, which every product
+// with it becomes), one below 127 times the smallest normal number counts as zeros.
+__device__ __forceinline__ float step_of(uint32_t amax_bits, float* inv) {
+  if (amax_bits >= 0x7f800000u) {
+    *inv = 0.f;
+    return __uint_as_float(0x7fc00000u);
+  }
+  const float s = __fdiv_rn(__uint_as_float(amax_bits), 127.f);
+  if (s < 1.17549435e-38f) {
+    *inv = 0.f;
+    return 0.f;
+  }
+  *inv = __frcp_rn(s);
+  return s;
+}
+
+template <int kLanes> __host__ __device__ constexpr int threads_for() { return kLanes <= 32 ? 256 : kLanes; }
+// Rows a thread has in flight: 32 to 64 bytes of each tensor.
+template <int kVecs, int kLanes> __host__ __device__ constexpr int rows_for() { return kLanes <= 32 && kVecs == 1 ? 2 : 1; }
+
+// kLanes threads share a row, kVecs pieces of V elements each.  CTAs walk over the rows, the next rows' loads ahead of this
+// one's sums, so that weight and bias are fetched once per CTA.
+template <class T, int V, int kVecs, int kLanes, bool kNorm, bool kQuant>
+__global__ void __launch_bounds__(threads_for<kLanes>())
+norm_kernel(const NormArgs a) {
+  constexpr int kThreads = threads_for<kLanes>(), kGroups = kThreads / kLanes, kRows = rows_for<kVecs, kLanes>();
+  using P = Pack<T, V>;
+  __shared__ uint32_t scratch[kLanes > 32 ? 2 * kRows * (kLanes / 32) : 1];
+  int turn = 0;
+  const int lane = threadIdx.x % kLanes, group = threadIdx.x / kLanes;
+  const int channels = a.channels;
+  const int64_t rows = live_rows(a.rows, a.num_rows);
+  float w[kVecs][V], b[kVecs][V];
+  if (kNorm) {
+#pragma unroll
+    for (int k = 0; k < kVecs; ++k)
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        const int c = (k * kLanes + lane) * V + e;
+        w[k][e] = c < channels ? (a.weight ? __ldg(a.weight + c) : 1.f) : 0.f;
+        b[k][e] = c < channels && a.bias ? __ldg(a.bias + c) : 0.f;
+      }
+  }
+  const float inv_n = 1.f / (float)channels;
+  const bool sum = kNorm && a.residual != nullptr;
+  P next[kRows][kVecs], next_r[kRows][kVecs];
+  auto load = [&](int64_t base) {
+#pragma unroll
+    for (int i = 0; i < kRows; ++i) {
+      const int64_t row = base + i * kGroups + group;
+#pragma unroll
+      for (int k = 0; k < kVecs; ++k) {
+        const int c = (k * kLanes + lane) * V;
+        if (row < rows && c < channels) {
+          next[i][k] = *reinterpret_cast<const P*>((const T*)a.x + row * a.x_ld + c);
+          if (sum) next_r[i][k] = *reinterpret_cast<const P*>((const T*)a.residual + row * a.residual_ld + c);
+        } else {
+#pragma unroll
+          for (int e = 0; e < V; ++e) next[i][k].v[e] = next_r[i][k].v[e] = from_f32<T>(0.f);
+        }
+      }
+    }
+  };
+  const int64_t stride = (int64_t)gridDim.x * kGroups * kRows;
+  int64_t base = (int64_t)blockIdx.x * kGroups * kRows;
+  if (base < rows) load(base);
+  for (; base < rows; base += stride) {
+    float y[kRows][kVecs * V];
+#pragma unroll
+    for (int i = 0; i < kRows; ++i)
+#pragma unroll
+      for (int k = 0; k < kVecs; ++k) {
+        if (sum) {
+          const int64_t row = base + i * kGroups + group;
+          const int c = (k * kLanes + lane) * V;
+          P t;
+#pragma unroll
+          for (int e = 0; e < V; ++e) t.v[e] = from_f32<T>(to_f32(next[i][k].v[e]) + to_f32(next_r[i][k].v[e]));
+          if (row < rows && c < channels) *reinterpret_cast<P*>((T*)a.total + row * channels + c) = t;
+          next[i][k] = t;  // the norm is that of the rounded sum, which is what the backward pass will see
+        }
+#pragma unroll
+        for (int e = 0; e < V; ++e) y[i][k * V + e] = to_f32(next[i][k].v[e]);
+      }
+    if (base + stride < rows) load(base + stride);
+    if (kNorm) {
+      float mean[kRows], var[kRows];
+#pragma unroll
+      for (int i = 0; i < kRows; ++i) {
+        mean[i] = 0.f;
+#pragma unroll
+        for (int j = 0; j < kVecs * V; ++j) mean[i] += y[i][j];
+      }
+      row_reduce<kLanes>(mean, Add(), scratch, turn);
+#pragma unroll
+      for (int i = 0; i < kRows; ++i) {
+        mean[i] *= inv_n;
+        var[i] = 0.f;
+#pragma unroll
+        for (int k = 0; k < kVecs; ++k)
+          if ((k * kLanes + lane) * V < channels)
+#pragma unroll
+            for (int e = 0; e < V; ++e) {
+              y[i][k * V + e] -= mean[i];
+              var[i] += y[i][k * V + e] * y[i][k * V + e];
+            }
+      }
+      row_reduce<kLanes>(var, Add(), scratch, turn);
+#pragma unroll
+      for (int i = 0; i < kRows; ++i) {
+        const float rstd = 1.f / sqrtf(var[i] * inv_n + a.eps);
+        const int64_t row = base + i * kGroups + group;
+        if (lane == 0 && row < rows && a.mean) a.mean[row] = mean[i], a.rstd[row] = rstd;
+#pragma unroll
+        for (int k = 0; k < kVecs; ++k)
+#pragma unroll
+          for (int e = 0; e < V; ++e) y[i][k * V + e] = y[i][k * V + e] * rstd * w[k][e] + b[k][e];
+      }
+    }
+    uint32_t amax[kRows];
+    if (kQuant) {
+#pragma unroll
+      for (int i = 0; i < kRows; ++i) {
+        amax[i] = 0u;
+#pragma unroll
+        for (int j = 0; j < kVecs * V; ++j) amax[i] = MaxBits()(amax[i], __float_as_uint(y[i][j]) & 0x7fffffffu);
+      }
+      row_reduce<kLanes>(amax, MaxBits(), scratch, turn);
+    }
+#pragma unroll
+    for (int i = 0; i < kRows; ++i) {
+      const int64_t row = base + i * kGroups + group;
+      if (row >= rows) continue;
+      float inv = 0.f, scale = 0.f;
+      if (kQuant) {
+        scale = step_of(amax[i], &inv);
+        if (lane == 0) a.scales[row] = scale;
+      }
+#pragma unroll
+      for (int k = 0; k < kVecs; ++k) {
+        const int c = (k * kLanes + lane) * V;
+        if (c >= channels) continue;
+        if (kQuant) {
+          Pack<int8_t, V> q;
+#pragma unroll
+          for (int e = 0; e < V; ++e) q.v[e] = inv == 0.f ? 0 : (int8_t)nearest_step(y[i][k * V + e], scale, inv);
+          *reinterpret_cast<Pack<int8_t, V>*>(a.q + row * a.q_ld + c) = q;
+        } else {
+          P o;
+#pragma unroll
+          for (int e = 0; e < V; ++e) o.v[e] = from_f32<T>(y[i][k * V + e]);
+          *reinterpret_cast<P*>((T*)a.out + row * channels + c) = o;
+        }
+      }
+    }
+  }
+}
+
+struct NormBackwardArgs {
+  const void *grad, *x, *grad_total;
+  int64_t grad_ld, x_ld, grad_total_ld;
+  const float *weight, *mean, *rstd;
+  int64_t rows;
+  int channels;
+  const int32_t* num_rows;
+  void* grad_x;
+  float* partial;  // [CTAs][2][channels]
+  float *grad_weight, *grad_bias;
+};
+
+// As above; a thread adds up the weight's and the bias's gradient of its columns over all its rows, the CTA adds its
+// threads' sums in a fixed order.
+template <class T, int V, int kVecs, int kLanes>
+__global__ void __launch_bounds__(threads_for<kLanes>())
+norm_backward_kernel(const NormBackwardArgs a) {
+  constexpr int kThreads = threads_for<kLanes>(), kGroups = kThreads / kLanes, kRows = rows_for<kVecs, kLanes>();
+  using P = Pack<T, V>;
+  __shared__ uint32_t scratch[kLanes > 32 ? 4 * kRows * (kLanes / 32) : 1];
+  extern __shared__ float sums[];  // [2][channels] where several rows share the CTA
+  int turn = 0;
+  const int lane = threadIdx.x % kLanes, group = threadIdx.x / kLanes;
+  const int channels = a.channels;
+  const int64_t rows = live_rows(a.rows, a.num_rows);
+  float w[kVecs][V], dw[kVecs][V], db[kVecs][V];
+#pragma unroll
+  for (int k = 0; k < kVecs; ++k)
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+      const int c = (k * kLanes + lane) * V + e;
+      w[k][e] = c < channels ? (a.weight ? __ldg(a.weight + c) : 1.f) : 0.f;
+      dw[k][e] = db[k][e] = 0.f;
+    }
+  const float inv_n = 1.f / (float)channels;
+  P next_x[kRows][kVecs], next_g[kRows][kVecs];
+  float next_mean[kRows], next_rstd[kRows];
+  auto load = [&](int64_t base) {
+#pragma unroll
+    for (int i = 0; i < kRows; ++i) {
+      const int64_t row = base + i * kGroups + group;
+      next_mean[i] = row < rows ? __ldg(a.mean + row) : 0.f;
+      next_rstd[i] = row < rows ? __ldg(a.rstd + row) : 0.f;
+#pragma unroll
+      for (int k = 0; k < kVecs; ++k) {
+        const int c = (k * kLanes + lane) * V;
+        if (row < rows && c < channels) {
+          next_x[i][k] = *reinterpret_cast<const P*>((const T*)a.x + row * a.x_ld + c);
+          next_g[i][k] = *reinterpret_cast<const P*>((const T*)a.grad + row * a.grad_ld + c);
+        } else {
+#pragma unroll
+          for (int e = 0; e < V; ++e) next_x[i][k].v[e] = next_g[i][k].v[e] = from_f32<T>(0.f);
+        }
+      }
+    }
+  };
+  const int64_t stride = (int64_t)gridDim.x * kGroups * kRows;
+  int64_t base = (int64_t)blockIdx.x * kGroups * kRows;
+  if (base < rows) load(base);
+  for (; base < rows; base += stride) {
+    P x[kRows][kVecs], g[kRows][kVecs];
+    float mean[kRows], rstd[kRows], dot[2 * kRows];
+#pragma unroll
+    for (int i = 0; i < kRows; ++i) {
+      mean[i] = next_mean[i], rstd[i] = next_rstd[i];
+#pragma unroll
+      for (int k = 0; k < kVecs; ++k) x[i][k] = next_x[i][k], g[i][k] = next_g[i][k];
+    }
+    if (base + stride < rows) load(base + stride);
+#pragma unroll
+    for (int i = 0; i < kRows; ++i) {
+      dot[2 * i] = dot[2 * i + 1] = 0.f;
+#pragma unroll
+      for (int k = 0; k < kVecs; ++k)
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+          // beyond the last channel gradient and weight are zeros, so xhat may be anything finite there
+          const float hat = (to_f32(x[i][k].v[e]) - mean[i]) * rstd[i], dy = to_f32(g[i][k].v[e]), gw = dy * w[k][e];
+          dot[2 * i] += gw;
+          dot[2 * i + 1] += gw * hat;
+          dw[k][e] += dy * hat;
+          db[k][e] += dy;
+        }
+    }
+    row_reduce<kLanes>(dot, Add(), scratch, turn);
+#pragma unroll
+    for (int i = 0; i < kRows; ++i) {
+      const int64_t row = base + i * kGroups + group;
+      if (row >= rows) continue;
+      const float m1 = dot[2 * i] * inv_n, m2 = dot[2 * i + 1] * inv_n;
+#pragma unroll
+      for (int k = 0; k < kVecs; ++k) {
+        const int c = (k * kLanes + lane) * V;
+        if (c >= channels) continue;
+        P o, t;
+        if (a.grad_total) t = *reinterpret_cast<const P*>((const T*)a.grad_total + row * a.grad_total_ld + c);
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+          const float hat = (to_f32(x[i][k].v[e]) - mean[i]) * rstd[i], gw = to_f32(g[i][k].v[e]) * w[k][e];
+          float d = rstd[i] * (gw - m1 - hat * m2);
+          if (a.grad_total) d += to_f32(t.v[e]);
+          o.v[e] = from_f32<T>(d);
+        }
+        *reinterpret_cast<P*>((T*)a.grad_x + row * channels + c) = o;
+      }
+    }
+  }
+  float* mine = a.partial + (int64_t)blockIdx.x * 2 * channels;
+  if (kGroups > 1) {
+#pragma unroll
+    for (int d = 16; d >= kLanes; d >>= 1)
+#pragma unroll
+      for (int k = 0; k < kVecs; ++k)
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+          dw[k][e] += __shfl_xor_sync(0xffffffffu, dw[k][e], d);
+          db[k][e] += __shfl_xor_sync(0xffffffffu, db[k][e], d);
+        }
+    for (int turn_of = 0; turn_of < kThreads / 32; ++turn_of) {
+      if ((int)(threadIdx.x >> 5) == turn_of && lane_id() < kLanes)
+#pragma unroll
+        for (int k = 0; k < kVecs; ++k)
+#pragma unroll
+          for (int e = 0; e < V; ++e) {
+            const int c = (k * kLanes + lane) * V + e;
+            if (c >= channels) continue;
+            sums[c] = turn_of ? sums[c] + dw[k][e] : dw[k][e];
+            sums[channels + c] = turn_of ? sums[channels + c] + db[k][e] : db[k][e];
+          }
+      __syncthreads();
+    }
+    for (int c = threadIdx.x; c < 2 * channels; c += kThreads) mine[c] = sums[c];
+  } else {
+#pragma unroll
+    for (int k = 0; k < kVecs; ++k)
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        const int c = (k * kLanes + lane) * V + e;
+        if (c < channels) mine[c] = dw[k][e], mine[channels + c] = db[k][e];
+      }
+  }
+}
+
+// Sums the CTAs' partial gradients in a fixed order: 32 columns to a CTA, eight warps take the partials in turn.
+__global__ void __launch_bounds__(256)
+norm_columns_kernel(const float* __restrict__ partial, int parts, int channels, float* __restrict__ grad_weight,
+                    float* __restrict__ grad_bias) {
+  __shared__ float s[8][33];
+  pdl_wait();
+  const int lane = lane_id(), warp = threadIdx.x >> 5, c = blockIdx.x * 32 + lane;
+  float sum = 0.f;
+  if (c < 2 * channels)
+#pragma unroll 8
+    for (int p = warp; p < parts; p += 8) sum += __ldg(partial + (int64_t)p * 2 * channels + c);
+  s[warp][lane] = sum;
+  __syncthreads();
+  if (warp == 0 && c < 2 * channels) {
+    float t = s[0][lane];
+#pragma unroll
+    for (int w = 1; w < 8; ++w) t += s[w][lane];
+    if (c < channels) {
+      if (grad_weight) grad_weight[c] = t;
+    } else if (grad_bias) grad_bias[c - channels] = t;
+  }
+}
+
+constexpr int kMaxChannels = 8192;
+
+// f(vector length, pieces, threads of a row) for the shape that covers `pieces` pieces; each returned value is a launch.
+#define D3D_NORM_SHAPE(V, K, L) return f(std::integral_constant<int, V>(), std::integral_constant<int, K>(), std::integral_constant<int, L>())
+template <int V, class F> int by_shape(int channels, F f) {
+  const int n = (channels + V - 1) / V;
+  if constexpr (V > 1) {
+    if (n <= 2) D3D_NORM_SHAPE(V, 1, 2);
+    if (n <= 4) D3D_NORM_SHAPE(V, 1, 4);
+    if (n <= 8) D3D_NORM_SHAPE(V, 1, 8);
+    if (n <= 16) D3D_NORM_SHAPE(V, 1, 16);
+    if (n <= 32) D3D_NORM_SHAPE(V, 1, 32);
+    if (n <= 64) D3D_NORM_SHAPE(V, 2, 32);
+    if (n <= 128) D3D_NORM_SHAPE(V, 2, 64);
+    if (n <= 256) D3D_NORM_SHAPE(V, 2, 128);
+    if (n <= 512) D3D_NORM_SHAPE(V, 2, 256);
+    if (n <= 1024) D3D_NORM_SHAPE(V, 2, 512);
+    D3D_NORM_SHAPE(V, 4, 512);
+  } else {
+  if (n <= 8) D3D_NORM_SHAPE(1, 1, 8);
+  if (n <= 32) D3D_NORM_SHAPE(1, 4, 8);
+  if (n <= 128) D3D_NORM_SHAPE(1, 4, 32);
+  if (n <= 512) D3D_NORM_SHAPE(1, 8, 64);
+  if (n <= 2048) D3D_NORM_SHAPE(1, 8, 256);
+  D3D_NORM_SHAPE(1, 16, 512);
+  }
+}
+#undef D3D_NORM_SHAPE
+
+template <class T, class F> int by_alignment(bool wide, int channels, F f) {
+  return wide ? by_shape<16 / (int)sizeof(T)>(channels, f) : by_shape<1>(channels, f);
+}
+template <class F> int by_type(int dtype, F f) {
+  switch (dtype) {
+    case D3D_FLOAT: return f(float());
+    case D3D_HALF: return f(__half());
+    case D3D_BF16: return f(__nv_bfloat16());
+    default: return D3D_ERR_UNSUPPORTED_DTYPE;
+  }
+}
+
+// Whether rows of `ld` elements from `p` on can be read in 16-byte pieces.
+bool rows_wide(const void* p, int64_t ld, int esize) {
+  return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld * esize % 16 == 0;
+}
+bool rows_aligned(const void* p, int esize) { return reinterpret_cast<uintptr_t>(p) % esize == 0; }
+
+// CTAs of `kernel` that fill the GPU once.
+template <class K> int resident(K kernel, int threads, size_t smem) {
+  int n = 0;
+  if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, threads, smem) != cudaSuccess || n < 1) n = 1;
+  return n * kNumSMs;
+}
+
+template <bool kNorm, bool kQuant> int launch_norm(int dtype, bool wide, const NormArgs& a, cudaStream_t st) {
+  return by_type(dtype, [&](auto t) -> int {
+    using T = decltype(t);
+    return by_alignment<T>(wide, a.channels, [&](auto v, auto k, auto l) -> int {
+      constexpr int V = decltype(v)::value, K = decltype(k)::value, L = decltype(l)::value;
+      constexpr int per_cta = threads_for<L>() / L * rows_for<K, L>();
+      auto kernel = norm_kernel<T, V, K, L, kNorm, kQuant>;
+      static const int most = resident(kernel, threads_for<L>(), 0);
+      const int64_t need = ceil_div(a.rows, per_cta);
+      kernel<<<(int)(need < most ? need : most), threads_for<L>(), 0, st>>>(a);
+      D3D_CHECK_LAUNCH();
+      return D3D_OK;
+    });
+  });
+}
+
+// The backward pass keeps its sums per CTA, so that their number decides how large the workspace is.
+int backward_ctas(int64_t rows, int per_cta) {
+  const int64_t need = ceil_div(rows > 0 ? rows : 1, per_cta), most = 2 * kNumSMs;
+  return (int)(need < most ? need : most);
+}
+
+}  // namespace
+}  // namespace d3d
+
+using namespace d3d;
+
+extern "C" int d3d_layer_norm(int dtype, const void* x, int64_t x_ld, const void* residual, int64_t residual_ld,
+                              const float* weight, const float* bias, float eps, int64_t rows, int channels,
+                              const int32_t* num_rows, void* total, void* out, float* mean, float* rstd, void* stream) {
+  D3D_NVTX_RANGE("d3d_layer_norm");
+  const int esize = (int)dtype_size(dtype);
+  D3D_REQUIRE(dtype == D3D_FLOAT || dtype == D3D_HALF || dtype == D3D_BF16, D3D_ERR_UNSUPPORTED_DTYPE);
+  D3D_REQUIRE(rows >= 0 && channels >= 1 && eps >= 0.f && x_ld >= channels && (!residual || residual_ld >= channels) &&
+                  !residual == !total && !mean == !rstd,
+              D3D_ERR_INVALID_ARGUMENT);
+  D3D_REQUIRE(channels <= kMaxChannels, D3D_ERR_TOO_LARGE);
+  if (rows == 0) return D3D_OK;
+  D3D_REQUIRE(x && out && rows_aligned(x, esize) && rows_aligned(residual, esize) && rows_aligned(out, esize) &&
+                  rows_aligned(total, esize),
+              D3D_ERR_INVALID_ARGUMENT);
+  NormArgs a = {};
+  a.x = x, a.x_ld = x_ld, a.residual = residual, a.residual_ld = residual_ld, a.weight = weight, a.bias = bias, a.eps = eps;
+  a.rows = rows, a.channels = channels, a.num_rows = num_rows, a.total = total, a.out = out, a.mean = mean, a.rstd = rstd;
+  const bool wide = channels * esize % 16 == 0 && rows_wide(x, x_ld, esize) && (!residual || rows_wide(residual, residual_ld, esize)) &&
+                    rows_wide(out, channels, esize) && rows_wide(total, channels, esize);
+  return launch_norm<true, false>(dtype, wide, a, reinterpret_cast<cudaStream_t>(stream));
+}
+
+extern "C" int d3d_layer_norm_int8(int dtype, const void* x, int64_t x_ld, const void* residual, int64_t residual_ld,
+                                   const float* weight, const float* bias, float eps, int64_t rows, int channels,
+                                   const int32_t* num_rows, void* total, int8_t* q, int64_t q_ld, float* scales,
+                                   void* stream) {
+  D3D_NVTX_RANGE("d3d_layer_norm_int8");
+  const int esize = (int)dtype_size(dtype);
+  D3D_REQUIRE(dtype == D3D_FLOAT || dtype == D3D_HALF || dtype == D3D_BF16, D3D_ERR_UNSUPPORTED_DTYPE);
+  D3D_REQUIRE(rows >= 0 && channels >= 1 && eps >= 0.f && x_ld >= channels && (!residual || residual_ld >= channels) &&
+                  !residual == !total && q_ld >= channels,
+              D3D_ERR_INVALID_ARGUMENT);
+  D3D_REQUIRE(channels <= kMaxChannels, D3D_ERR_TOO_LARGE);
+  if (rows == 0) return D3D_OK;
+  D3D_REQUIRE(x && q && scales && rows_aligned(x, esize) && rows_aligned(residual, esize) && rows_aligned(total, esize),
+              D3D_ERR_INVALID_ARGUMENT);
+  NormArgs a = {};
+  a.x = x, a.x_ld = x_ld, a.residual = residual, a.residual_ld = residual_ld, a.weight = weight, a.bias = bias, a.eps = eps;
+  a.rows = rows, a.channels = channels, a.num_rows = num_rows, a.total = total, a.q = q, a.q_ld = q_ld, a.scales = scales;
+  const bool wide = channels * esize % 16 == 0 && rows_wide(x, x_ld, esize) && (!residual || rows_wide(residual, residual_ld, esize)) &&
+                    rows_wide(total, channels, esize) && reinterpret_cast<uintptr_t>(q) % 8 == 0 && q_ld % 8 == 0;
+  return launch_norm<true, true>(dtype, wide, a, reinterpret_cast<cudaStream_t>(stream));
+}
+
+extern "C" int d3d_quantize_rows(int dtype, const void* x, int64_t x_ld, int64_t rows, int channels, const int32_t* num_rows,
+                                 int8_t* q, int64_t q_ld, float* scales, void* stream) {
+  D3D_NVTX_RANGE("d3d_quantize_rows");
+  const int esize = (int)dtype_size(dtype);
+  D3D_REQUIRE(dtype == D3D_FLOAT || dtype == D3D_HALF || dtype == D3D_BF16, D3D_ERR_UNSUPPORTED_DTYPE);
+  D3D_REQUIRE(rows >= 0 && channels >= 1 && x_ld >= channels && q_ld >= channels, D3D_ERR_INVALID_ARGUMENT);
+  D3D_REQUIRE(channels <= kMaxChannels, D3D_ERR_TOO_LARGE);
+  if (rows == 0) return D3D_OK;
+  D3D_REQUIRE(x && q && scales && rows_aligned(x, esize), D3D_ERR_INVALID_ARGUMENT);
+  NormArgs a = {};
+  a.x = x, a.x_ld = x_ld, a.rows = rows, a.channels = channels, a.num_rows = num_rows, a.q = q, a.q_ld = q_ld, a.scales = scales;
+  const bool wide = channels * esize % 16 == 0 && rows_wide(x, x_ld, esize) && reinterpret_cast<uintptr_t>(q) % 8 == 0 && q_ld % 8 == 0;
+  return launch_norm<false, true>(dtype, wide, a, reinterpret_cast<cudaStream_t>(stream));
+}
+
+extern "C" size_t d3d_layer_norm_backward_workspace(int64_t rows, int channels) {
+  if (rows < 0 || channels < 1) return 0;
+  return (size_t)backward_ctas(rows, 1) * 2 * channels * sizeof(float);
+}
+
+extern "C" int d3d_layer_norm_backward(int dtype, const void* grad, int64_t grad_ld, const void* x, int64_t x_ld,
+                                       const void* grad_total, int64_t grad_total_ld, const float* weight, const float* mean,
+                                       const float* rstd, int64_t rows, int channels, const int32_t* num_rows, void* grad_x,
+                                       float* grad_weight, float* grad_bias, void* workspace, size_t workspace_bytes,
+                                       void* stream) {
+  D3D_NVTX_RANGE("d3d_layer_norm_backward");
+  const int esize = (int)dtype_size(dtype);
+  D3D_REQUIRE(dtype == D3D_FLOAT || dtype == D3D_HALF || dtype == D3D_BF16, D3D_ERR_UNSUPPORTED_DTYPE);
+  D3D_REQUIRE(rows >= 0 && channels >= 1 && x_ld >= channels && grad_ld >= channels && (!grad_total || grad_total_ld >= channels),
+              D3D_ERR_INVALID_ARGUMENT);
+  D3D_REQUIRE(channels <= kMaxChannels, D3D_ERR_TOO_LARGE);
+  D3D_REQUIRE(rows == 0 || (x && grad && mean && rstd && grad_x), D3D_ERR_INVALID_ARGUMENT);
+  D3D_REQUIRE(rows_aligned(x, esize) && rows_aligned(grad, esize) && rows_aligned(grad_total, esize) && rows_aligned(grad_x, esize),
+              D3D_ERR_INVALID_ARGUMENT);
+  D3D_REQUIRE(workspace && reinterpret_cast<uintptr_t>(workspace) % 4 == 0, D3D_ERR_INVALID_ARGUMENT);
+  D3D_REQUIRE(workspace_bytes >= d3d_layer_norm_backward_workspace(rows, channels), D3D_ERR_WORKSPACE_TOO_SMALL);
+  NormBackwardArgs a = {};
+  a.grad = grad, a.grad_ld = grad_ld, a.x = x, a.x_ld = x_ld, a.grad_total = grad_total, a.grad_total_ld = grad_total_ld;
+  a.weight = weight, a.mean = mean, a.rstd = rstd, a.rows = rows, a.channels = channels, a.num_rows = num_rows, a.grad_x = grad_x;
+  a.partial = reinterpret_cast<float*>(workspace);
+  const bool wide = channels * esize % 16 == 0 && rows_wide(x, x_ld, esize) && rows_wide(grad, grad_ld, esize) &&
+                    (!grad_total || rows_wide(grad_total, grad_total_ld, esize)) && rows_wide(grad_x, channels, esize);
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  return by_type(dtype, [&](auto t) -> int {
+    using T = decltype(t);
+    return by_alignment<T>(wide, channels, [&](auto v, auto k, auto l) -> int {
+      constexpr int V = decltype(v)::value, K = decltype(k)::value, L = decltype(l)::value;
+      constexpr int per_cta = threads_for<L>() / L * rows_for<K, L>();
+      const int ctas = backward_ctas(rows, per_cta);
+      const size_t smem = L <= 32 ? (size_t)2 * channels * sizeof(float) : 0;
+      norm_backward_kernel<T, V, K, L><<<ctas, threads_for<L>(), smem, st>>>(a);
+      D3D_CHECK_LAUNCH();
+      D3D_LAUNCH(true, norm_columns_kernel, (unsigned)ceil_div(2 * channels, 32), 256, 0, st, a.partial, ctas, channels, grad_weight,
+                 grad_bias);
+      return D3D_OK;
+    });
+  });
+}

@@ -481,6 +481,59 @@ int d3d_yolox3d_decode_enqueue(const d3d_yolox3d_decode_params* p, const d3d_ten
                                const d3d_tensor_desc* out, int n_out, const void* const* inputs, void* const* outputs,
                                void* workspace, size_t workspace_bytes, void* stream);
 
+/* ---------------------------------------------------------------------------------------------
+ * Operators of voxel-sequence networks (no reference counterpart): blocks that mix the active voxels of a sparse tensor
+ * along an order of theirs instead of through a kernel neighbourhood.  Features are rows x channels as everywhere in this
+ * library, dtype float | half | bf16; parameters, states and scales are float.  `*_ld`: elements from one row to the next
+ * (at least the row's own), so that inputs may be columns of a wider tensor; outputs without one are dense.  Rows that start
+ * on 16 bytes and are multiples of 16 bytes apart are read in 16-byte pieces, any others element by element.
+ * `num_rows`: the live rows, int32 [1] on the device, or NULL for all of them; rows behind are neither read nor written.
+ * ------------------------------------------------------------------------------------------- */
+/* out = (t - mean) * rstd * weight + bias over the channels, t = x, or the sum x + residual rounded to the type, which is then
+ * written to `total` (given exactly when `residual` is).  weight, bias: [channels] or NULL (1, 0).  mean and rstd, [rows], both
+ * or neither: what the backward pass needs.  channels <= 8192. */
+int d3d_layer_norm(int dtype, const void* x, int64_t x_ld, const void* residual, int64_t residual_ld, const float* weight,
+                   const float* bias, float eps, int64_t rows, int channels, const int32_t* num_rows, void* total, void* out,
+                   float* mean, float* rstd, void* stream);
+/* Gradients of the above: grad_x [rows][channels] (with grad_total, the gradient of `total`, added: then it is that of x and of
+ * residual alike), grad_weight and grad_bias [channels] (either may be NULL).  `x`: what was normed, so `total` where there was
+ * a residual.  The sums over rows are made in a fixed order. */
+size_t d3d_layer_norm_backward_workspace(int64_t rows, int channels);
+int d3d_layer_norm_backward(int dtype, const void* grad, int64_t grad_ld, const void* x, int64_t x_ld, const void* grad_total,
+                            int64_t grad_total_ld, const float* weight, const float* mean, const float* rstd, int64_t rows,
+                            int channels, const int32_t* num_rows, void* grad_x, float* grad_weight, float* grad_bias,
+                            void* workspace, size_t workspace_bytes, void* stream);
+/* Rows in 8-bit integers: scales[row] = max |x| / 127, q = x / scales[row] to the nearest integer, ties to even, the quotient as
+ * if exact.  A row whose largest magnitude is below 127 times the smallest normal float gets q = 0 and scale 0, a row that
+ * is not finite q = 0 and scale NaN, so that products with it are NaN.  _int8 of layer norm: the normed rows so. */
+int d3d_quantize_rows(int dtype, const void* x, int64_t x_ld, int64_t rows, int channels, const int32_t* num_rows, int8_t* q,
+                      int64_t q_ld, float* scales, void* stream);
+int d3d_layer_norm_int8(int dtype, const void* x, int64_t x_ld, const void* residual, int64_t residual_ld,
+                        const float* weight, const float* bias, float eps, int64_t rows, int channels,
+                        const int32_t* num_rows, void* total, int8_t* q, int64_t q_ld, float* scales, void* stream);
+/* Gated linear recurrence over sequences: h[t] = f[t] h[t-1] + (1 - f[t]) x[t] per channel, f = sigmoid(gates), out = h.
+ * Sequence s are the rows offsets[s] .. offsets[s+1]-1 (int32 [seqs+1] on the device, ascending; equal ones are a sequence
+ * without rows), walked upwards or, with `reverse`, downwards.  initial [seqs][channels]: h in front of the first row walked
+ * (NULL: zeros); final_state [seqs][channels] (or NULL): h of the last one, initial where there is none.  Rows outside all
+ * sequences are neither read nor written.  h is held in float; sequences do not touch each other, whatever their values.
+ * states: NULL, or [d3d_gated_recurrence_state_rows(rows)][channels], what the backward pass needs. */
+int64_t d3d_gated_recurrence_state_rows(int64_t rows);
+size_t d3d_gated_recurrence_workspace(int64_t rows, int channels);
+int d3d_gated_recurrence(int dtype, const void* x, int64_t x_ld, const void* gates, int64_t gates_ld, const int32_t* offsets,
+                         int seqs, int64_t rows, int channels, int reverse, const float* initial, void* out,
+                         float* final_state, float* states, void* workspace, size_t workspace_bytes, void* stream);
+/* Gradients of the above for those of `out` and of final_state (grad_final, NULL: zeros): grad_x, grad_gates [rows][channels]
+ * and grad_initial [seqs][channels] (or NULL). */
+int d3d_gated_recurrence_backward(int dtype, const void* grad, int64_t grad_ld, const void* x, int64_t x_ld, const void* gates,
+                                  int64_t gates_ld, const int32_t* offsets, int seqs, int64_t rows, int channels, int reverse,
+                                  const float* states, const float* initial, const float* grad_final, void* grad_x,
+                                  void* grad_gates, float* grad_initial, void* workspace, size_t workspace_bytes,
+                                  void* stream);
+/* The recurrence for one new row of each of `rows` sequences: state_out = f state + (1 - f) x, out = state_out in the type of x.
+ * state_out may be state. */
+int d3d_gated_recurrence_step(int dtype, const void* x, int64_t x_ld, const void* gates, int64_t gates_ld, const float* state,
+                              float* state_out, void* out, int64_t rows, int channels, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,382 @@
+"""The voxel-sequence operators against their definitions in 64 bits (tests/_sequence.py says where the bounds come from)."""
+import numpy as np
+import pytest
+import torch
+
+from tests import _sequence as ref
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+TYPES = [torch.float32, torch.float16, torch.bfloat16]
+EPS = 1e-5
+
+
+def normal(seed, *shape):
+    return torch.randn(shape, generator=torch.Generator(device=DEV).manual_seed(seed), device=DEV)
+
+
+def features(seed, rows, channels, dtype, layout="dense"):
+    """Rows of different scale.  layout: "columns" of a wider tensor with 16-byte rows, "odd": rows two elements apart from them."""
+    x = (normal(seed, rows, channels) * torch.exp(normal(seed + 1, rows, 1))).to(dtype)
+    if layout == "dense":
+        return x
+    wide = torch.full((rows, channels + (16 if layout == "columns" else 3)), float("nan"), device=DEV, dtype=dtype)
+    at = 8 if layout == "columns" else 1
+    wide[:, at:at + channels] = x
+    return wide[:, at:at + channels]
+
+
+def live(n):
+    return torch.tensor([n], dtype=torch.int32, device=DEV)
+
+
+# ---- layer norm -----------------------------------------------------------------------------------------------------
+def check_norm(x, weight, bias, y, mean=None, rstd=None):
+    w = ref.as64(weight) if weight is not None else np.ones(x.shape[1])
+    b = ref.as64(bias) if bias is not None else np.zeros(x.shape[1])
+    want, limit, m, r, _ = ref.norm(ref.as64(x), w, b, EPS)
+    ref.assert_within(y, want, limit + ref.half_step(y.dtype) * (np.abs(want) + limit) + ref.smallest(y.dtype), "norm")
+    if mean is not None:
+        ref.assert_within(mean, m, ref.U32 * ref.DEPTH * np.abs(ref.as64(x)).mean(1), "mean")
+        ref.assert_within(rstd, r, ref.U32 * ref.DEPTH * r * (1 + (np.abs(ref.as64(x)).mean(1) * r) ** 2), "rstd")
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,channels", [(0, 16), (1, 1), (1, 16), (257, 3), (300, 24), (1000, 64), (77, 96), (513, 131),
+                                           (33, 256), (65, 520), (9, 1000), (5, 1025), (6, 4096), (3, 8191), (2, 8192)])
+def test_norm_and_backward(d3d, dtype, rows, channels):
+    x, grad = features(1, rows, channels, dtype), normal(3, rows, channels).to(dtype)
+    weight, bias = 1 + 0.2 * normal(4, channels), 0.1 * normal(5, channels)
+    y, mean, rstd = d3d.layer_norm(x, weight, bias, EPS, with_stats=True)
+    dx, dw, db = d3d.layer_norm_backward(grad, x, weight, mean, rstd)
+    if rows == 0:
+        assert y.shape == x.shape and (dw == 0).all() and (db == 0).all()
+        return
+    check_norm(x, weight, bias, y, mean, rstd)
+    want = ref.norm_backward(ref.as64(grad), ref.as64(x), ref.as64(weight), ref.as64(mean), ref.as64(rstd))
+    for got, (w, limit), what in zip((dx, dw, db), want, ("dx", "dweight", "dbias")):
+        ref.assert_within(got, w, limit + ref.half_step(got.dtype) * (np.abs(w) + limit) + ref.smallest(got.dtype), what)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("layout", ["dense", "columns", "odd"])
+@pytest.mark.parametrize("channels", [16, 40, 200])
+def test_norm_of_a_sum(d3d, dtype, layout, channels):
+    rows, n = 211, 150
+    x, r = features(1, rows, channels, dtype, layout), features(7, rows, channels, dtype, layout)
+    grad, more = normal(3, rows, channels).to(dtype), normal(9, rows, channels).to(dtype)
+    out = torch.full((rows, channels), 3.0, device=DEV, dtype=dtype)
+    y, total, mean, rstd = d3d.layer_norm(x, None, None, EPS, residual=r, num_rows=live(n), with_stats=True, out=out)
+    assert y is out and (out[n:] == 3).all()
+    assert torch.equal(total[:n], (x.float() + r.float()).to(dtype)[:n])
+    check_norm(total[:n], None, None, y[:n], mean[:n], rstd[:n])
+    dx, dw, db = d3d.layer_norm_backward(grad, total, None, mean, rstd, num_rows=live(n), grad_total=more)
+    g, t, m, v = (ref.as64(a[:n]) for a in (grad, total, mean, rstd))
+    (wx, lx), (ww, lw), (wb, lb) = ref.norm_backward(g, t, np.ones(channels), m, v)
+    wx, lx = wx + ref.as64(more[:n]), lx + ref.U32 * 2 * (np.abs(wx) + np.abs(ref.as64(more[:n])))
+    ref.assert_within(dx[:n], wx, lx + ref.half_step(dtype) * (np.abs(wx) + lx) + ref.smallest(dtype), "dx")
+    ref.assert_within(dw, ww, lw, "dweight")
+    ref.assert_within(db, wb, lb, "dbias")
+
+
+@pytest.mark.parametrize("count", [-5, 0, 1, 64, 1000])
+def test_norm_counts(d3d, count):
+    rows = 64
+    x, w = features(1, rows, 32, torch.float16), normal(2, 32)
+    out = torch.full((rows, 32), 7.0, device=DEV, dtype=torch.float16)
+    d3d.layer_norm(x, w, None, EPS, num_rows=live(count), out=out)
+    n = max(0, min(rows, count))
+    assert (out[n:] == 7).all()
+    if n:
+        check_norm(x[:n], w, None, out[:n])
+    _, mean, rstd = d3d.layer_norm(x, w, None, EPS, with_stats=True)
+    _, dw, db = d3d.layer_norm_backward(x, x, w, mean, rstd, num_rows=live(count))
+    assert torch.equal(db == 0, torch.full((32,), n == 0, device=DEV)) and (n > 0 or (dw == 0).all())
+
+
+def test_norm_rows_keep_to_themselves(d3d):
+    """A row that is not finite, beside rows that share its warp; a constant row."""
+    for dtype in TYPES:
+        for channels in (8, 24, 64, 5, 1000):
+            x = features(1, 67, channels, dtype)
+            want = d3d.layer_norm(x, None, None, EPS)
+            x[5, 1], x[40, channels - 1], x[66] = float("nan"), float("inf"), 2.5
+            got = d3d.layer_norm(x, None, None, EPS)
+            fine = torch.ones(67, dtype=torch.bool, device=DEV)
+            fine[[5, 40, 66]] = False
+            assert torch.equal(got[fine], want[fine])
+            assert got[5].isnan().all() and got[40].isnan().all() and (got[66] == 0).all()
+
+
+def test_norm_backward_is_the_same_every_time(d3d):
+    x, g = features(1, 20011, 64, torch.bfloat16), features(2, 20011, 64, torch.bfloat16)
+    w = normal(4, 64)
+    _, mean, rstd = d3d.layer_norm(x, w, None, EPS, with_stats=True)
+    first = d3d.layer_norm_backward(g, x, w, mean, rstd)
+    for _ in range(3):
+        assert all(torch.equal(a, b) for a, b in zip(first, d3d.layer_norm_backward(g, x, w, mean, rstd)))
+
+
+# ---- rows in 8-bit integers -----------------------------------------------------------------------------------------
+def check_quantized(x32, q, scale):
+    want, s = ref.quantize(x32.cpu().numpy())
+    assert np.array_equal(scale.cpu().numpy(), s, equal_nan=True)
+    assert np.array_equal(q.cpu().numpy(), want)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("layout", ["dense", "columns", "odd"])
+@pytest.mark.parametrize("rows,channels", [(0, 16), (1, 1), (300, 24), (1000, 64), (513, 131), (6, 4096), (3, 8191)])
+def test_quantize_rows(d3d, dtype, layout, rows, channels):
+    x = features(1, rows, channels, dtype, layout)
+    q, scale = d3d.quantize_rows(x)
+    assert q.shape == x.shape and (rows <= 1 or q.stride(0) % 16 == 0)
+    if rows:
+        check_quantized(x.float(), q, scale)
+
+
+def test_quantize_borders(d3d):
+    """Values half-way between two steps, of rows whose scale is and is not a power of two, as exact fp32 numbers; rows of
+    zeros, of the smallest numbers, of what is not finite."""
+    halves = torch.arange(-126.5, 127.0, 0.5, device=DEV)
+    rows = [halves * s for s in (1.0, 2.0 ** -20, 3.0, 0.7, 1e30, 1e-30)]
+    x = torch.stack([torch.cat([r, r.abs().max()[None] * 127 / 126.5]) for r in rows])
+    neighbours = torch.cat([x, torch.nextafter(x, x + x.abs()), torch.nextafter(x, x - x.abs())])
+    neighbours[:, -1] = x[:, -1].repeat(3)
+    special = torch.zeros((5, x.shape[1]), device=DEV)
+    special[1, 3], special[2, 3], special[3, 3], special[4, 3] = 1e-42, 1.4e-36, float("inf"), float("nan")
+    x = torch.cat([neighbours, special])
+    q, scale = d3d.quantize_rows(x)
+    check_quantized(x, q, scale)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("channels", [24, 131, 256])
+def test_norm_int8(d3d, dtype, channels):
+    """The integers are those of the normed rows, give or take one where a value lies within the norm's bound of a border."""
+    rows, n = 301, 290
+    x, r = features(1, rows, channels, dtype), features(7, rows, channels, dtype)
+    w, b = 1 + 0.2 * normal(4, channels), 0.1 * normal(5, channels)
+    q, scale, total = d3d.layer_norm_int8(x, w, b, EPS, residual=r, num_rows=live(n))
+    q, scale, total = q[:n], scale[:n], total[:n]
+    y, limit, _, _, _ = ref.norm(ref.as64(total), ref.as64(w), ref.as64(b), EPS)
+    amax = np.abs(y).max(1)
+    ref.assert_within(scale, amax / 127, limit.max(1) / 127 + 2 * ref.U32 * amax / 127, "scale")
+    assert (q.abs().max(1).values == 127).all()
+    s = ref.as64(scale)[:, None]
+    assert (np.abs(ref.as64(q) * s - y) <= s / 2 + limit + ref.U32 * 127 * s).all()
+    plain, s2 = d3d.layer_norm_int8(total, w, b, EPS)  # the sum as an input gives the same
+    assert torch.equal(plain, q) and torch.equal(s2, scale)
+
+
+# ---- gated recurrence -----------------------------------------------------------------------------------------------
+def offsets_of(kind, rows):
+    r = np.random.Generator(np.random.PCG64(rows + len(kind)))
+    if kind == "one":
+        return [0, rows]
+    if kind == "singles":
+        return list(range(rows + 1))
+    if kind == "few":
+        return sorted([0, rows] + list(r.integers(0, rows + 1, 3)))
+    if kind == "many":  # short ones, some without rows, single rows at a tile's edges
+        cuts = list(r.integers(0, rows + 1, rows // 9)) + [c for c in (127, 128, 128, 129, 255, 256) if c <= rows]
+        return sorted([0, rows] + cuts)
+    low, high = rows // 5, rows - rows // 7  # "inside": rows in front of the first sequence and behind the last
+    return sorted([low, high] + list(r.integers(low, high + 1, 4)))
+
+
+def gates_like(seed, rows, channels, dtype, layout="dense"):
+    """Memories from one row to thousands."""
+    g = (normal(seed, rows, channels) + torch.linspace(-2, 8, channels, device=DEV)).to(dtype)
+    if layout == "dense":
+        return g
+    wide = features(seed, rows, channels, dtype, layout)
+    wide.copy_(g)
+    return wide
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("reverse", [False, True])
+@pytest.mark.parametrize("kind", ["one", "few", "many", "inside", "singles"])
+@pytest.mark.parametrize("rows,channels", [(1, 1), (5, 16), (128, 8), (129, 40), (300, 3), (700, 72), (1030, 24), (2500, 64)])
+def test_recurrence(d3d, dtype, reverse, kind, rows, channels):
+    layout = ("dense", "columns", "odd")[(rows + channels) % 3]
+    x, g = features(1, rows, channels, dtype, layout), gates_like(3, rows, channels, dtype, layout)
+    offs = offsets_of(kind, rows)
+    seqs = len(offs) - 1
+    offsets = torch.tensor(offs, dtype=torch.int32, device=DEV)
+    initial = normal(5, seqs, channels) if kind != "few" else None
+    grad, grad_final = normal(7, rows, channels).to(dtype), normal(8, seqs, channels) if kind != "inside" else None
+    out = torch.full((rows, channels), 9.0, device=DEV, dtype=dtype)
+    h, final, states = d3d.gated_recurrence(x, g, offsets, initial, reverse=reverse, with_states=True, out=out)
+    assert h is out
+    x64, g64 = ref.as64(x), ref.as64(g)
+    i64 = ref.as64(initial) if initial is not None else None
+    want, off, wfinal, foff, _, _ = ref.recurrence(x64, g64, offs, i64, reverse)
+    inside = ~np.isnan(want[:, 0])
+    assert (ref.as64(out)[~inside] == 9).all()
+    lim = off + ref.half_step(dtype) * (np.abs(want) + off) + ref.smallest(dtype)
+    ref.assert_within(ref.as64(h)[inside], want[inside], lim[inside], "h")
+    ref.assert_within(final, wfinal, foff + ref.U32 * np.abs(wfinal), "final")
+    plain = d3d.gated_recurrence(x, g, offsets, initial, reverse=reverse)
+    assert torch.equal(plain[0][torch.from_numpy(inside).to(DEV)], h[torch.from_numpy(inside).to(DEV)])
+    assert torch.equal(plain[1], final)
+    got = d3d.gated_recurrence_backward(grad, x, g, offsets, states, initial, grad_final, reverse=reverse)
+    back = ref.recurrence_backward(ref.as64(grad), x64, g64, offs, i64,
+                                   ref.as64(grad_final) if grad_final is not None else None, reverse)
+    for t, (w, o), what in zip(got, back, ("dx", "dgates", "dinitial")):
+        t = ref.as64(t)
+        rnd = torch.float32 if what == "dinitial" else dtype
+        lim = o + ref.half_step(rnd) * (np.abs(w) + o) + ref.smallest(rnd)
+        keep = inside if what != "dinitial" else slice(None)
+        ref.assert_within(t[keep], w[keep], lim[keep], what)
+
+
+def test_recurrence_without_rows_or_sequences(d3d):
+    for dtype in TYPES:
+        x = torch.empty((0, 24), dtype=dtype, device=DEV)
+        zero = torch.zeros(4, dtype=torch.int32, device=DEV)
+        initial = normal(1, 3, 24)
+        out, final, states = d3d.gated_recurrence(x, x, zero, initial, with_states=True)
+        assert out.shape == (0, 24) and torch.equal(final, initial)
+        assert (d3d.gated_recurrence(x, x, zero)[1] == 0).all()
+        _, _, di = d3d.gated_recurrence_backward(x, x, x, zero, states, initial, 2 * initial)
+        assert torch.equal(di, 2 * initial)
+        x = features(2, 9, 24, dtype)
+        out = torch.full_like(x, 4.0)
+        _, final = d3d.gated_recurrence(x, x, zero[:1], out=out)
+        assert final.shape == (0, 24) and (out == 4).all()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("channels", [16, 64, 5])
+def test_sequences_do_not_touch_each_other(d3d, dtype, channels):
+    """Sequences that hold NaN, infinities and gates at the type's ends, beside ones that do not: the same bytes."""
+    rows, offs = 900, [0, 130, 256, 256, 300, 700, 900]
+    offsets = torch.tensor(offs, dtype=torch.int32, device=DEV)
+    x, g = features(1, rows, channels, dtype), gates_like(2, rows, channels, dtype)
+    initial, grad, gf = normal(3, 6, channels), normal(4, rows, channels).to(dtype), normal(5, 6, channels)
+
+    def run(reverse):
+        out, final, states = d3d.gated_recurrence(x, g, offsets, initial, reverse=reverse, with_states=True)
+        return (out, final) + d3d.gated_recurrence_backward(grad, x, g, offsets, states, initial, gf, reverse=reverse)
+    want = [[t.clone() for t in run(r)] for r in (False, True)]
+    x[131], g[200], x[310], g[500] = float("nan"), float("nan"), float("inf"), torch.finfo(dtype).min
+    g[600, 0], initial[4, 0], grad[299], gf[1] = torch.finfo(dtype).max, float("-inf"), float("inf"), float("nan")
+    rows_ok = torch.zeros(rows, dtype=torch.bool, device=DEV)
+    rows_ok[:130] = rows_ok[700:] = True
+    seqs_ok = [0, 2, 5]
+    for r in (False, True):
+        for a, b in zip(run(r), want[r]):
+            assert torch.equal(a[rows_ok], b[rows_ok]) if len(a) == rows else torch.equal(a[seqs_ok], b[seqs_ok])
+
+
+def test_recurrence_gates_at_their_ends(d3d):
+    """Gates so large that nothing is added or kept, also in 32 bits: the state passes unchanged or is the row."""
+    x = features(1, 300, 16, torch.float32)
+    offsets = torch.tensor([0, 300], dtype=torch.int32, device=DEV)
+    initial = normal(2, 1, 16)
+    big = torch.full_like(x, 200.0)
+    out, final = d3d.gated_recurrence(x, big, offsets, initial)
+    assert torch.equal(out, initial.expand(300, 16)) and torch.equal(final, initial)
+    out, final = d3d.gated_recurrence(x, -big, offsets, initial)
+    assert torch.equal(out, x) and torch.equal(final, x[-1:])
+    inf = torch.full_like(x, float("inf"))
+    assert torch.equal(d3d.gated_recurrence(x, -inf, offsets, initial)[0], x)
+    assert torch.equal(d3d.gated_recurrence(x, inf, offsets, initial)[0], initial.expand(300, 16))
+
+
+@pytest.mark.parametrize("offs", [[5, 3], [-4, 50], [0, 500], [20, 10, 60, 0, 99], [-9, -3], [400, 600]])
+def test_offsets_out_of_order_stay_inside_the_tensors(d3d, offs):
+    """Nothing is said about the results; rows behind the tensors' own are not touched."""
+    rows = 100
+    buf = torch.full((rows + 64, 16), 5.0, device=DEV)
+    x = features(1, rows, 16, torch.float32)
+    offsets = torch.tensor(offs, dtype=torch.int32, device=DEV)
+    for reverse in (False, True):
+        out, final, states = d3d.gated_recurrence(x, x, offsets, out=buf[32:32 + rows], reverse=reverse, with_states=True)
+        d3d.gated_recurrence_backward(x, x, x, offsets, states, reverse=reverse)
+        torch.cuda.synchronize()
+        assert (buf[:32] == 5).all() and (buf[32 + rows:] == 5).all()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("layout", ["dense", "columns", "odd"])
+@pytest.mark.parametrize("rows,channels", [(0, 8), (1, 1), (77, 24), (512, 131)])
+def test_step_is_the_recurrence_of_one_row(d3d, dtype, layout, rows, channels):
+    x, g = features(1, rows, channels, dtype, layout), gates_like(2, rows, channels, dtype, layout)
+    state = normal(3, rows, channels)
+    out, new = d3d.gated_recurrence_step(x, g, state)
+    offsets = torch.arange(rows + 1, dtype=torch.int32, device=DEV)
+    want, final = d3d.gated_recurrence(x, g, offsets, state)
+    assert torch.equal(out, want) and torch.equal(new, final)
+    again, same = d3d.gated_recurrence_step(x, g, state, state_out=state)
+    assert same is state and torch.equal(state, new) and torch.equal(again, out)
+
+
+def test_gradients_against_differences(d3d):
+    """fp32, along a random direction: (L(p + e d) - L(p - e d)) / 2 e for L = <out, c> against the gradients.  The gates are
+    smooth on a scale of one, so with e = 2^-6 the difference is off by at most e^2 of its terms' sizes, and rounding adds
+    2^-24 / e of the outputs' sizes, summed at random."""
+    rows, channels, e = 333, 16, 2.0 ** -6
+    x, g = (normal(s, rows, channels) for s in (1, 2))
+    offsets = torch.tensor([0, 100, 100, 333], dtype=torch.int32, device=DEV)
+    h0, c, cf = normal(3, 3, channels), normal(4, rows, channels), normal(5, 3, channels)
+    dirs = [normal(s, *t.shape) for s, t in ((6, x), (7, g), (8, h0))]
+
+    def loss(e):
+        out, final = d3d.gated_recurrence(x + e * dirs[0], g + e * dirs[1], offsets, h0 + e * dirs[2])
+        return ((out.double() * c).sum() + (final.double() * cf).sum()).item()
+    _, _, states = d3d.gated_recurrence(x, g, offsets, h0, with_states=True)
+    grads = d3d.gated_recurrence_backward(c, x, g, offsets, states, h0, cf)
+    along = sum((a.double() * b).sum().item() for a, b in zip(grads, dirs))
+    size = sum((a.double() * b).abs().sum().item() for a, b in zip(grads, dirs))
+    assert abs((loss(e) - loss(-e)) / (2 * e) - along) <= 4 * e * e * size
+
+    w, b = 1 + 0.2 * normal(9, channels), normal(10, channels)
+    dirs = [normal(11, rows, channels), normal(12, channels), normal(13, channels)]
+    _, mean, rstd = d3d.layer_norm(x, w, b, EPS, with_stats=True)
+    grads = d3d.layer_norm_backward(c, x, w, mean, rstd)
+    along = sum((p.double() * q).sum().item() for p, q in zip(grads, dirs))
+    size = sum((p.double() * q).abs().sum().item() for p, q in zip(grads, dirs))
+
+    def loss(e):
+        return (d3d.layer_norm(x + e * dirs[0], w + e * dirs[1], b + e * dirs[2], EPS).double() * c).sum().item()
+    assert abs((loss(e) - loss(-e)) / (2 * e) - along) <= 4 * e * e * size
+
+
+# ---- streams, graphs ------------------------------------------------------------------------------------------------
+def test_on_another_stream_and_in_graphs(d3d):
+    """Two graphs captured one after the other and replayed in turn on new inputs, and a call on a stream of its own."""
+    def inputs(seed):
+        return features(seed, 3000, 64, torch.bfloat16), gates_like(seed + 5, 3000, 64, torch.bfloat16)
+    offsets = torch.tensor([0, 700, 700, 3000], dtype=torch.int32, device=DEV)
+    w = normal(3, 64)
+
+    def chain(x, g, reverse):
+        y, mean, rstd = d3d.layer_norm(x, w, None, EPS, with_stats=True)
+        h, final, states = d3d.gated_recurrence(y, g, offsets, reverse=reverse, with_states=True)
+        dy, dg, _ = d3d.gated_recurrence_backward(x, y, g, offsets, states, reverse=reverse)
+        return (h, final, dg) + d3d.layer_norm_backward(dy, x, w, mean, rstd)
+    x, g = inputs(1)
+    want = chain(x, g, False)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = chain(x, g, False)
+    side.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    graphs = []
+    for reverse in (False, True):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs = chain(x, g, reverse)
+        graphs.append((graph, outs))
+    for seed in (11, 12):
+        a, b = inputs(seed)
+        x.copy_(a), g.copy_(b)
+        for (graph, _) in graphs * 2:
+            graph.replay()
+        torch.cuda.synchronize()
+        for (_, outs), reverse in zip(graphs, (False, True)):
+            assert all(torch.equal(p, q) for p, q in zip(outs, chain(a, b, reverse)))
