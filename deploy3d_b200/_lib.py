@@ -187,6 +187,8 @@ SIGNATURES = {
     "d3d_quantize_rows": (ctypes.c_int, [_int, _vp, _i64, _i64, _int, _vp, _vp, _i64, _vp, _vp]),
     "d3d_layer_norm_int8": (ctypes.c_int, [_int, _vp, _i64, _vp, _i64, _vp, _vp, _f32, _i64, _int, _vp, _vp, _vp, _i64, _vp,
                                            _vp]),
+    "d3d_int8_linear_workspace": (_sz, [_vp, _i64, _i64, _vp, _i64, _int, _int]),
+    "d3d_int8_linear": (ctypes.c_int, [_int, _vp, _i64, _vp, _i64, _vp, _vp, _i64, _vp, _vp, _int, _int, _vp, _vp, _sz, _vp]),
     "d3d_gated_recurrence_state_rows": (_i64, [_i64]),
     "d3d_gated_recurrence_workspace": (_sz, [_i64, _int]),
     "d3d_gated_recurrence": (ctypes.c_int, [_int, _vp, _i64, _vp, _i64, _vp, _int, _i64, _int, _int, _vp, _vp, _vp, _vp, _vp,

@@ -197,7 +197,7 @@ scan_kernel(const ScanArgs a) {
     }
   }
   scan_threads<kLanes, V, kWarps, true>(ma, mb, totals);
-  if (kMaps) {
+  if constexpr (kMaps) {
     if ((int)threadIdx.x < kWidth && slab * kWidth + (int)threadIdx.x < a.channels)
       a.maps[(int64_t)tile * a.channels + slab * kWidth + threadIdx.x] = tile_map<kWidth, kWarps, true>(totals, threadIdx.x);
     return;

@@ -1,0 +1,510 @@
+// Product of 8-bit rows and 8-bit weights with a scale per row and per output channel:
+//   out[m][n] = x_scale[m] w_scale[n] sum_k q[m][k] w[n][k] + bias[n]
+// The sum is exact (32-bit integers, |sum| <= 2^14 k), the rest is three 32-bit operations and one rounding.
+//
+// Two kernels.  From kFewRows rows on, tcgen05.mma (kind::i8, K = 32 per instruction) over tiles of 128 or, with two CTAs to a
+// tile, 256 rows by up to 256 output channels: operands by TMA in 128-byte rows (128 channels of the sum a stage), accumulators of
+// two tiles in tensor memory so that the epilogue of one runs beside the products of the next.  Fewer rows: the weights are
+// what is read, once, and four-way dot products keep up with that.
+#include <mutex>
+#include <type_traits>
+
+#include "common.cuh"
+#include "kernel_errors.h"
+#include "tc_ptx.cuh"
+
+namespace d3d {
+namespace {
+
+__device__ int g_int8_error;  // 0 ok; otherwise the code of the first wait that gave up
+
+template <class T, int V> struct alignas(sizeof(T) * V) Pack { T v[V]; };
+
+struct LinearArgs {
+  const int8_t *x, *w;
+  int64_t x_ld, w_ld;
+  const float *x_scale, *w_scale, *bias;
+  void* out;
+  int64_t rows;
+  const int32_t* num_rows;
+  int inputs, outputs;
+};
+
+__device__ __forceinline__ int64_t live_rows(int64_t rows, const int32_t* num_rows) {
+  if (!num_rows) return rows;
+  const int64_t n = __ldg(num_rows);
+  return n < 0 ? 0 : n < rows ? n : rows;
+}
+
+// ---- few rows ---------------------------------------------------------------------------------------------------------
+// A warp per output channel: its weights stream by once, every lane multiplies its pieces with those of kM rows.
+// kBytes: what one load takes (16 where rows start on 16 bytes, else one).
+template <class T, int kM, int kBytes>
+__global__ void __launch_bounds__(256)
+few_rows_kernel(const LinearArgs a) {
+  const int64_t rows = live_rows(a.rows, a.num_rows);
+  const int64_t m0 = (int64_t)blockIdx.y * kM;
+  if (m0 >= rows) return;
+  const int n = blockIdx.x * 8 + (threadIdx.x >> 5), lane = lane_id();
+  if (n >= a.outputs) return;
+  const int8_t* w = a.w + (int64_t)n * a.w_ld;
+  int acc[kM];
+#pragma unroll
+  for (int m = 0; m < kM; ++m) acc[m] = 0;
+  using P = Pack<int8_t, kBytes>;
+#pragma unroll 4
+  for (int k = lane * kBytes; k + kBytes <= a.inputs; k += 32 * kBytes) {
+    const P pw = *reinterpret_cast<const P*>(w + k);
+#pragma unroll
+    for (int m = 0; m < kM; ++m) {
+      const int64_t row = m0 + m < rows ? m0 + m : rows - 1;
+      const P px = *reinterpret_cast<const P*>(a.x + row * a.x_ld + k);
+      if constexpr (kBytes == 16) {
+        const int4 x4 = *reinterpret_cast<const int4*>(&px), w4 = *reinterpret_cast<const int4*>(&pw);
+        acc[m] = __dp4a(x4.x, w4.x, acc[m]), acc[m] = __dp4a(x4.y, w4.y, acc[m]);
+        acc[m] = __dp4a(x4.z, w4.z, acc[m]), acc[m] = __dp4a(x4.w, w4.w, acc[m]);
+      } else {
+        acc[m] += (int)px.v[0] * (int)pw.v[0];
+      }
+    }
+  }
+  if (kBytes > 1)  // what is left of the rows
+    for (int k = a.inputs / kBytes * kBytes + lane; k < a.inputs; k += 32)
+#pragma unroll
+      for (int m = 0; m < kM; ++m) {
+        const int64_t row = m0 + m < rows ? m0 + m : rows - 1;
+        acc[m] += (int)a.x[row * a.x_ld + k] * (int)w[k];
+      }
+  const float ws = __ldg(a.w_scale + n), b = a.bias ? __ldg(a.bias + n) : 0.f;
+#pragma unroll
+  for (int m = 0; m < kM; ++m) {
+    const int sum = __reduce_add_sync(0xffffffffu, acc[m]);
+    if (lane == 0 && m0 + m < rows)
+      ((T*)a.out)[(m0 + m) * a.outputs + n] = from_f32<T>(fmaf((float)sum * ws, __ldg(a.x_scale + m0 + m), b));
+  }
+}
+
+// ---- tensor cores -----------------------------------------------------------------------------------------------------
+constexpr int kTileRows = 128;    // rows of a CTA
+constexpr int kBlockK = 128;      // channels of the sum a stage holds: one 128-byte swizzled row
+constexpr int kMaxStages = 8;
+constexpr int kMaxCols = 256;     // output channels of a tile
+constexpr int kEpilogueWarps = 8;
+constexpr int kThreads = (kEpilogueWarps + 2) * 32;
+constexpr int kStagePitch = 144;  // bytes of a row of the epilogue's staging: 128 and a shift of four banks from row to row
+constexpr uint32_t kABytes = kTileRows * kBlockK;
+
+struct TcArgs {
+  LinearArgs l;
+  int cols;        // output channels of a tile
+  int col_tiles;
+  int stages, k_blocks;
+  uint32_t stage_bytes;
+  uint32_t idesc;
+  int out_wide;    // rows of the output start on 16 bytes
+};
+
+struct Shared {
+  uint64_t full[kMaxStages];   // TMA -> MMA
+  uint64_t empty[kMaxStages];  // MMA -> TMA
+  uint64_t acc_full[2];        // MMA -> epilogue
+  uint64_t acc_empty[2];       // epilogue -> MMA
+  uint64_t drained;            // MMA, where a wait has given up: the products on their way
+  uint32_t tmem;
+  int abort;
+  alignas(16) float scale[2][2][kMaxCols];  // by tile parity: weight scales, bias
+};
+
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+// Address of this CTA's `p` in CTA 0 of the cluster.
+__device__ __forceinline__ uint32_t in_leader(const void* p) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(r) : "r"(smem_u32(p)));
+  return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+template <int kCta> __device__ __forceinline__ void arrive_leader(uint64_t* bar) {
+  if (kCta == 1) mbar_arrive(bar);
+  else asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(in_leader(bar)) : "memory");
+}
+// A box of the tensor into this CTA's shared memory; with two CTAs to a tile its bytes count on the leader's barrier.
+template <int kCta> __device__ __forceinline__ void load_box(const CUtensorMap* map, uint64_t* bar, void* dst, int x, int y) {
+  if (kCta == 1)
+    tma_load_2d(map, bar, dst, x, y);
+  else
+    asm volatile(
+        "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
+        ::"r"(smem_u32(dst)), "l"((uint64_t)map), "r"(in_leader(bar)), "r"(x), "r"(y) : "memory");
+}
+template <int kCta> __device__ __forceinline__ void mma_i8(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  if (kCta == 1)
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}"
+                 ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+  else
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n\t}"
+                 ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+}
+// The barrier, in both CTAs of a pair, learns that all products issued so far are done.
+template <int kCta> __device__ __forceinline__ void commit(uint64_t* bar) {
+  if (kCta == 1)
+    umma_commit(bar);
+  else
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
+                 ::"r"(smem_u32(bar)), "h"((uint16_t)3) : "memory");
+}
+template <int kCta> __device__ __forceinline__ void alloc_tmem(uint32_t* dst) {
+  if (kCta == 1) {
+    tmem_alloc(dst, 512);
+  } else {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(dst)) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  }
+}
+template <int kCta> __device__ __forceinline__ void free_tmem(uint32_t addr) {
+  if (kCta == 1) tmem_dealloc(addr, 512);
+  else asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 512;" ::"r"(addr) : "memory");
+}
+// K-major operand, 128-byte swizzle: groups of eight rows 1024 bytes apart; 32 channels further is 32 bytes further.
+__device__ __forceinline__ uint64_t operand(uint32_t smem_addr) {
+  return (uint64_t)((smem_addr & 0x3FFFFu) >> 4) | (1ull << 16) | (64ull << 32) | (1ull << 46) | (2ull << 61);
+}
+
+struct Tiles {
+  int first, step, count;  // this CTA's (pair's) tiles: first, first + step, ... below count
+};
+
+// kCta CTAs share a tile of kCta * 128 rows: each holds its rows and its share of the weight rows, CTA 0 issues the products.
+template <int kCta, class T>
+__global__ void __launch_bounds__(kThreads, 1)
+linear_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w, const TcArgs p) {
+  extern __shared__ __align__(1024) unsigned char smem_raw[];
+  unsigned char* ring = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  unsigned char* staging = ring + p.stages * p.stage_bytes;
+  Shared* sh = reinterpret_cast<Shared*>(staging + kEpilogueWarps * 32 * kStagePitch);
+  const int warp = threadIdx.x >> 5, lane = lane_id();
+  const uint32_t rank = kCta == 1 ? 0 : cluster_rank();
+  const int64_t rows = live_rows(p.l.rows, p.l.num_rows);
+  const Tiles tiles = {(int)(blockIdx.x / kCta), (int)(gridDim.x / kCta),
+                       (int)((rows + kCta * kTileRows - 1) / (kCta * kTileRows)) * p.col_tiles};
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kMaxStages; ++s) mbar_init(&sh->full[s], 1), mbar_init(&sh->empty[s], 1);
+    for (int b = 0; b < 2; ++b) mbar_init(&sh->acc_full[b], 1), mbar_init(&sh->acc_empty[b], kCta * kEpilogueWarps);
+    mbar_init(&sh->drained, 1);
+    sh->abort = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == kEpilogueWarps + 1) alloc_tmem<kCta>(&sh->tmem);
+  tc_fence_before();
+  __syncthreads();
+  if (kCta == 2) cluster_sync();
+  tc_fence_after();
+  const uint32_t tmem = sh->tmem;
+  volatile int* abort_flag = &sh->abort;
+
+  if (warp == kEpilogueWarps) {
+    if (lane == 0) {
+      int stage = 0, phase = 0;
+      bool ok = true;
+      for (int t = tiles.first; ok && t < tiles.count; t += tiles.step) {
+        const int m0 = (t / p.col_tiles * kCta + (int)rank) * kTileRows;
+        const int n0 = t % p.col_tiles * p.cols + (int)rank * (p.cols / kCta);
+        for (int k = 0; k < p.k_blocks; ++k) {
+          ok = mbar_wait(&sh->empty[stage], phase ^ 1, abort_flag, 1, kWaitLimitCycles);
+          if (!ok) break;
+          unsigned char* a = ring + stage * p.stage_bytes;
+          if (rank == 0) mbar_arrive_expect_tx(&sh->full[stage], kCta * p.stage_bytes);
+          load_box<kCta>(&map_x, &sh->full[stage], a, k * kBlockK, m0);
+          load_box<kCta>(&map_w, &sh->full[stage], a + kABytes, k * kBlockK, n0);
+          if (++stage == p.stages) stage = 0, phase ^= 1;
+        }
+      }
+      // The CTAs do not end with copies on their way, whoever has given up (those of both count here).
+      if (rank == 0)
+        for (int s = 0; s < p.stages; ++s) mbar_drain(&sh->full[s], s < stage ? phase : phase ^ 1);
+    }
+  } else if (warp == kEpilogueWarps + 1) {
+    if (lane == 0 && rank == 0) {
+      int stage = 0, phase = 0, buf = 0, acc_phase = 0;
+      bool ok = true;
+      const int last = (p.l.inputs - (p.k_blocks - 1) * kBlockK + 31) / 32;  // products of the last stage
+      for (int t = tiles.first; ok && t < tiles.count; t += tiles.step) {
+        ok = mbar_wait(&sh->acc_empty[buf], acc_phase ^ 1, abort_flag, 2, kWaitLimitCycles);
+        if (!ok) break;
+        tc_fence_after();
+        const uint32_t d = tmem + buf * kMaxCols;
+        for (int k = 0; k < p.k_blocks; ++k) {
+          ok = mbar_wait(&sh->full[stage], phase, abort_flag, 3, kWaitLimitCycles);
+          if (!ok) break;
+          tc_fence_after();
+          const uint32_t at = smem_u32(ring + stage * p.stage_bytes);
+          const uint64_t da = operand(at), db = operand(at + kABytes);
+          const int n = k == p.k_blocks - 1 ? last : 4;
+          for (int i = 0; i < n; ++i) mma_i8<kCta>(d, da + 2 * i, db + 2 * i, p.idesc, k > 0 || i > 0);
+          commit<kCta>(&sh->empty[stage]);
+          if (++stage == p.stages) stage = 0, phase ^= 1;
+        }
+        if (!ok) break;
+        commit<kCta>(&sh->acc_full[buf]);
+        if (++buf == 2) buf = 0, acc_phase ^= 1;
+      }
+      if (!ok) {
+        commit<kCta>(&sh->drained);
+        mbar_drain(&sh->drained, 0);
+      }
+    }
+  } else {
+    // Two sets of four warps; a warp reads its quarter of the accumulator's lanes, the sets take turns in the columns.
+    constexpr int kCols = 128 / (int)sizeof(T);  // columns of a 128-byte piece
+    constexpr int kVec = 16 / (int)sizeof(T);
+    const int quarter = warp & 3, set = warp >> 2;
+    unsigned char* mine = staging + warp * 32 * kStagePitch;
+    int buf = 0, acc_phase = 0;
+    bool ok = true;
+    for (int t = tiles.first; t < tiles.count; t += tiles.step) {
+      const int64_t m0 = ((int64_t)(t / p.col_tiles) * kCta + rank) * kTileRows + quarter * 32;
+      const int n0 = t % p.col_tiles * p.cols;
+      float* scale = sh->scale[buf][0];
+      for (int c = threadIdx.x; c < p.cols; c += kEpilogueWarps * 32) {
+        const bool in = n0 + c < p.l.outputs;
+        scale[c] = in ? __ldg(p.l.w_scale + n0 + c) : 0.f;
+        scale[kMaxCols + c] = in && p.l.bias ? __ldg(p.l.bias + n0 + c) : 0.f;
+      }
+      const float xs = m0 + lane < rows ? __ldg(p.l.x_scale + m0 + lane) : 0.f;
+      asm volatile("bar.sync 1, %0;" ::"n"(kEpilogueWarps * 32) : "memory");
+      // a warp whose wait gave up still comes to the barriers of the others
+      if (ok) ok = mbar_wait(&sh->acc_full[buf], acc_phase, abort_flag, 4, kWaitLimitCycles);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) continue;
+      tc_fence_after();
+      const uint32_t acc = tmem + buf * kMaxCols + ((uint32_t)(quarter * 32) << 16);
+      for (int c0 = set * kCols; c0 < p.cols; c0 += 2 * kCols) {
+#pragma unroll
+        for (int h = 0; h < kCols; h += 16) {
+          if (c0 + h >= p.cols) break;
+          uint32_t r[16];
+          tmem_ld16(acc + c0 + h, r);
+          tmem_ld_wait(r);
+          const float4* ws = reinterpret_cast<const float4*>(scale + c0 + h);
+          const float4* bs = reinterpret_cast<const float4*>(scale + kMaxCols + c0 + h);
+          alignas(16) T v[16];
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const float4 w4 = ws[q], b4 = bs[q];
+            v[4 * q] = from_f32<T>(fmaf((float)(int)r[4 * q] * w4.x, xs, b4.x));
+            v[4 * q + 1] = from_f32<T>(fmaf((float)(int)r[4 * q + 1] * w4.y, xs, b4.y));
+            v[4 * q + 2] = from_f32<T>(fmaf((float)(int)r[4 * q + 2] * w4.z, xs, b4.z));
+            v[4 * q + 3] = from_f32<T>(fmaf((float)(int)r[4 * q + 3] * w4.w, xs, b4.w));
+          }
+          uint4* to = reinterpret_cast<uint4*>(mine + lane * kStagePitch + h * sizeof(T));
+#pragma unroll
+          for (int q = 0; q < (int)sizeof(T); ++q) to[q] = reinterpret_cast<const uint4*>(v)[q];
+        }
+        __syncwarp();
+        const int n = n0 + c0;
+        if (p.out_wide) {  // eight lanes to a row
+          const int c = n + lane % 8 * kVec;
+          if (c0 + lane % 8 * kVec < p.cols && c < p.l.outputs)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              const int row = 4 * i + lane / 8;
+              if (m0 + row < rows)
+                *reinterpret_cast<uint4*>((T*)p.l.out + (m0 + row) * p.l.outputs + c) =
+                    *reinterpret_cast<const uint4*>(mine + row * kStagePitch + lane % 8 * 16);
+            }
+        } else {
+          for (int row = 0; row < 32 && m0 + row < rows; ++row)
+#pragma unroll
+            for (int h = 0; h < kCols; h += 32)
+              if (c0 + h + lane < p.cols && n + h + lane < p.l.outputs)
+                ((T*)p.l.out)[(m0 + row) * p.l.outputs + n + h + lane] =
+                    reinterpret_cast<const T*>(mine + row * kStagePitch)[h + lane];
+        }
+        __syncwarp();
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) arrive_leader<kCta>(&sh->acc_empty[buf]);
+      if (++buf == 2) buf = 0, acc_phase ^= 1;
+    }
+  }
+  __syncwarp();
+  tc_fence_before();
+  __syncthreads();
+  if (kCta == 2) cluster_sync();
+  if (threadIdx.x == 0 && sh->abort) atomicCAS(&g_int8_error, 0, 100 + sh->abort);
+  if (warp == kEpilogueWarps + 1) free_tmem<kCta>(tmem);
+}
+
+// Rows of bytes that do not start on 16 bytes: copied so that they do.
+__global__ void __launch_bounds__(256)
+repitch_kernel(const int8_t* __restrict__ from, int64_t from_ld, int8_t* __restrict__ to, int64_t to_ld, int64_t rows, int channels,
+               const int32_t* num_rows) {
+  rows = live_rows(rows, num_rows);
+  const int words = (int)(to_ld / 4);
+  const int64_t n = rows * words, nth = (int64_t)gridDim.x * blockDim.x;
+  for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += nth) {
+    const int64_t row = i / words;
+    const int c = (int)(i - row * words) * 4;
+    const int8_t* s = from + row * from_ld + c;
+    char4 v;
+    v.x = c < channels ? s[0] : 0, v.y = c + 1 < channels ? s[1] : 0, v.z = c + 2 < channels ? s[2] : 0, v.w = c + 3 < channels ? s[3] : 0;
+    *reinterpret_cast<char4*>(to + row * to_ld + c) = v;
+  }
+}
+
+constexpr int kFewRows = 8;
+constexpr int kMaxInputs = 65536, kMaxOutputs = 65536;
+
+bool aligned_rows(const void* p, int64_t ld) { return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld % 16 == 0; }
+
+bool byte_map(CUtensorMap* map, const void* base, uint64_t cols, uint64_t rows, uint64_t pitch, uint32_t box_rows) {
+  EncodeTiledFn fn = encode_fn();
+  if (!fn) return false;
+  cuuint64_t dims[2] = {cols, rows}, strides[1] = {pitch};
+  cuuint32_t box[2] = {kBlockK, box_rows}, elem[2] = {1, 1};
+  return fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
+            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <class T> int launch_few(const LinearArgs& a, cudaStream_t st) {
+  const bool wide = aligned_rows(a.x, a.x_ld) && aligned_rows(a.w, a.w_ld);
+  const unsigned gx = (unsigned)ceil_div(a.outputs, 8);
+#define D3D_FEW(M)                                                                                                 \
+  do {                                                                                                             \
+    const dim3 grid(gx, (unsigned)ceil_div(a.rows, M));                                                            \
+    if (wide) few_rows_kernel<T, M, 16><<<grid, 256, 0, st>>>(a);                                                  \
+    else few_rows_kernel<T, M, 1><<<grid, 256, 0, st>>>(a);                                                        \
+  } while (0)
+  if (a.rows == 1) D3D_FEW(1);
+  else if (a.rows == 2) D3D_FEW(2);
+  else if (a.rows <= 4) D3D_FEW(4);
+  else D3D_FEW(8);
+#undef D3D_FEW
+  D3D_CHECK_LAUNCH();
+  return D3D_OK;
+}
+
+template <int kCta, class T> int launch_tiles(const LinearArgs& a, int cols, cudaStream_t st) {
+  TcArgs p;
+  p.l = a;
+  p.cols = cols;
+  p.col_tiles = (int)ceil_div(a.outputs, cols);
+  p.k_blocks = (int)ceil_div(a.inputs, kBlockK);
+  p.stage_bytes = kABytes + (uint32_t)(cols / kCta) * kBlockK;
+  const size_t fixed = 1024 + kEpilogueWarps * 32 * kStagePitch + sizeof(Shared);
+  p.stages = (int)((227 * 1024 - fixed) / p.stage_bytes);
+  if (p.stages > kMaxStages) p.stages = kMaxStages;
+  // D 32-bit integers, A and B signed
+  p.idesc = (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(cols >> 3) << 17) | ((uint32_t)(kCta * kTileRows >> 4) << 24);
+  p.out_wide = reinterpret_cast<uintptr_t>(a.out) % 16 == 0 && (int64_t)a.outputs * sizeof(T) % 16 == 0;
+  CUtensorMap map_x, map_w;
+  if (!byte_map(&map_x, a.x, a.inputs, a.rows, a.x_ld, kTileRows) || !byte_map(&map_w, a.w, a.inputs, a.outputs, a.w_ld, cols / kCta))
+    return D3D_ERR_CUDA;
+  auto kernel = linear_kernel<kCta, T>;
+  {
+    static std::mutex lock;
+    static bool set[64] = {};
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return D3D_ERR_CUDA;
+    std::lock_guard<std::mutex> guard(lock);
+    if (!set[dev]) {
+      if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024) != cudaSuccess) return D3D_ERR_CUDA;
+      set[dev] = true;
+    }
+  }
+  const int64_t tiles = ceil_div(a.rows, kCta * kTileRows) * p.col_tiles;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(kCta * (tiles < kNumSMs / kCta ? tiles : kNumSMs / kCta))), cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = fixed + p.stages * p.stage_bytes, cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = kCta, attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr, cfg.numAttrs = 1;
+  if (cudaLaunchKernelEx(&cfg, kernel, map_x, map_w, p) != cudaSuccess) return D3D_ERR_CUDA;
+  D3D_CHECK_LAUNCH();
+  return D3D_OK;
+}
+
+// Output channels of a tile: as many as fill the tiles evenly, fewer where the GPU would not be filled.
+int tile_cols(int64_t row_tiles, int outputs, int unit, int units) {
+  const int64_t want = ceil_div(units, row_tiles);          // column tiles that occupy everything
+  int64_t n = ceil_div(outputs, kMaxCols);
+  if (n < want) n = want;
+  const int cols = (int)(ceil_div(ceil_div(outputs, n), unit) * unit);
+  return cols < unit ? unit : cols;
+}
+
+template <class T> int launch_linear(const LinearArgs& a, cudaStream_t st) {
+  const int64_t pairs = ceil_div(a.rows, 2 * kTileRows) * ceil_div(a.outputs, kMaxCols);
+  if (pairs >= kNumSMs / 2) return launch_tiles<2, T>(a, tile_cols(ceil_div(a.rows, 2 * kTileRows), a.outputs, 32, kNumSMs / 2), st);
+  return launch_tiles<1, T>(a, tile_cols(ceil_div(a.rows, kTileRows), a.outputs, 16, kNumSMs), st);
+}
+
+size_t repitched(const void* p, int64_t ld, int64_t rows, int channels) {
+  return aligned_rows(p, ld) ? 0 : align_up((size_t)rows * align_up(channels, 16), 256);
+}
+
+}  // namespace
+
+int take_int8_linear_error(int* code) {
+  const int zero = 0;
+  if (cudaMemcpyFromSymbol(code, g_int8_error, sizeof(int)) != cudaSuccess) return D3D_ERR_CUDA;
+  if (cudaMemcpyToSymbol(g_int8_error, &zero, sizeof(int)) != cudaSuccess) return D3D_ERR_CUDA;
+  return D3D_OK;
+}
+
+}  // namespace d3d
+
+using namespace d3d;
+
+extern "C" size_t d3d_int8_linear_workspace(const int8_t* x, int64_t x_ld, int64_t rows, const int8_t* weight, int64_t weight_ld,
+                                            int inputs, int outputs) {
+  if (rows <= kFewRows || inputs < 1 || outputs < 1) return 0;
+  return repitched(x, x_ld, rows, inputs) + repitched(weight, weight_ld, outputs, inputs);
+}
+
+extern "C" int d3d_int8_linear(int dtype, const int8_t* x, int64_t x_ld, const float* x_scales, int64_t rows, const int32_t* num_rows,
+                               const int8_t* weight, int64_t weight_ld, const float* weight_scales, const float* bias, int inputs,
+                               int outputs, void* out, void* workspace, size_t workspace_bytes, void* stream) {
+  D3D_NVTX_RANGE("d3d_int8_linear");
+  const int esize = (int)dtype_size(dtype);
+  D3D_REQUIRE(dtype == D3D_FLOAT || dtype == D3D_HALF || dtype == D3D_BF16, D3D_ERR_UNSUPPORTED_DTYPE);
+  D3D_REQUIRE(rows >= 0 && inputs >= 1 && outputs >= 1 && x_ld >= inputs && weight_ld >= inputs, D3D_ERR_INVALID_ARGUMENT);
+  D3D_REQUIRE(inputs <= kMaxInputs && outputs <= kMaxOutputs && rows <= (1ll << 31) - 1024 &&
+                  ceil_div(rows, kTileRows) * ceil_div(outputs, 16) < (1ll << 30),
+              D3D_ERR_TOO_LARGE);
+  if (rows == 0) return D3D_OK;
+  D3D_REQUIRE(x && x_scales && weight && weight_scales && out && reinterpret_cast<uintptr_t>(out) % esize == 0,
+              D3D_ERR_INVALID_ARGUMENT);
+  const size_t need = d3d_int8_linear_workspace(x, x_ld, rows, weight, weight_ld, inputs, outputs);
+  D3D_REQUIRE(need == 0 || (workspace && reinterpret_cast<uintptr_t>(workspace) % 256 == 0), D3D_ERR_INVALID_ARGUMENT);
+  D3D_REQUIRE(workspace_bytes >= need, D3D_ERR_WORKSPACE_TOO_SMALL);
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  LinearArgs a = {x, weight, x_ld, weight_ld, x_scales, weight_scales, bias, out, rows, num_rows, inputs, outputs};
+  if (rows > kFewRows) {
+    uint8_t* ws = reinterpret_cast<uint8_t*>(workspace);
+    const int64_t pitch = (int64_t)align_up(inputs, 16);
+    if (!aligned_rows(x, x_ld)) {
+      repitch_kernel<<<stream_grid(rows * (pitch / 4), 256), 256, 0, st>>>(x, x_ld, (int8_t*)ws, pitch, rows, inputs, num_rows);
+      a.x = (const int8_t*)ws, a.x_ld = pitch;
+      ws += repitched(x, x_ld, rows, inputs);
+    }
+    if (!aligned_rows(weight, weight_ld)) {
+      repitch_kernel<<<stream_grid(outputs * (pitch / 4), 256), 256, 0, st>>>(weight, weight_ld, (int8_t*)ws, pitch, outputs, inputs, nullptr);
+      a.w = (const int8_t*)ws, a.w_ld = pitch;
+    }
+    D3D_CHECK_LAUNCH();
+  }
+  const bool few = rows <= kFewRows;
+  switch (dtype) {
+    case D3D_FLOAT: return few ? launch_few<float>(a, st) : launch_linear<float>(a, st);
+    case D3D_HALF: return few ? launch_few<__half>(a, st) : launch_linear<__half>(a, st);
+    default: return few ? launch_few<__nv_bfloat16>(a, st) : launch_linear<__nv_bfloat16>(a, st);
+  }
+}

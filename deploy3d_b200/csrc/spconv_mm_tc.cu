@@ -59,6 +59,7 @@
 #include <type_traits>
 
 #include "common.cuh"
+#include "kernel_errors.h"
 #include "spconv_mm_internal.h"
 #include "tc_ptx.cuh"
 
@@ -1170,7 +1171,10 @@ extern "C" int d3d_debug_take_kernel_error(int* code) {
   if (cudaDeviceSynchronize() != cudaSuccess) return D3D_ERR_CUDA;
   if (cudaMemcpyFromSymbol(code, d3d::g_tc_error, sizeof(int)) != cudaSuccess) return D3D_ERR_CUDA;
   if (cudaMemcpyToSymbol(d3d::g_tc_error, &zero, sizeof(int)) != cudaSuccess) return D3D_ERR_CUDA;
-  return D3D_OK;
+  int other = 0;
+  const int rc = d3d::take_int8_linear_error(&other);
+  if (*code == 0) *code = other;
+  return rc;
 }
 
 // Debug aid without a reference counterpart: after how many cycles a bounded wait of the tensor-core kernel gives up, for every

@@ -13,11 +13,11 @@ from .spconv import (bev_densify, data_s_bev_densify, data_s_spconv_index, data_
 from .voxel_encoder import (cylinder_encoder, data_s_voxel_encoder, simple_mean_encoder)
 from .point_voxel_mapping import (data_s_gather_back, data_s_scatter_to, gather_back, scatter_to)
 from .decoder import data_s_yolox3d_decode, nms3d, yolox3d_decode
-from .sequence import (gated_recurrence, gated_recurrence_backward, gated_recurrence_step, layer_norm,
+from .sequence import (gated_recurrence, gated_recurrence_backward, gated_recurrence_step, int8_linear, layer_norm,
                        layer_norm_backward, layer_norm_int8, quantize_rows)
 
 __all__ = ["spconv_index", "spconv_mm", "bev_densify", "simple_mean_encoder", "cylinder_encoder", "scatter_to",
            "gather_back", "nms3d", "yolox3d_decode", "data_s_yolox3d_decode", "data_s_spconv_index", "data_s_spconv_mm", "data_s_bev_densify",
            "data_s_voxel_encoder", "data_s_scatter_to", "data_s_gather_back",
-           "layer_norm", "layer_norm_backward", "layer_norm_int8", "quantize_rows", "gated_recurrence",
+           "layer_norm", "layer_norm_backward", "layer_norm_int8", "quantize_rows", "int8_linear", "gated_recurrence",
            "gated_recurrence_backward", "gated_recurrence_step"]

@@ -153,6 +153,45 @@ def quantize_rows(feats, num_rows=None):
     return q, scales
 
 
+def _bytes(t, what):
+    """(tensor, bytes between its rows) of a matrix of 8-bit integers."""
+    if t.dim() != 2 or not t.is_cuda or t.dtype != torch.int8 or t.shape[1] == 0:
+        raise ValueError("%s: an int8 CUDA tensor [rows, channels] is needed" % what)
+    rows, channels = t.shape
+    ld = t.stride(0) if rows > 1 else (channels + 15) // 16 * 16  # nothing lies behind a single row
+    if (t.stride(1) != 1 and channels > 1) or ld < channels:
+        t, ld = t.contiguous(), channels
+    return t, ld
+
+
+def int8_linear(feats, scales, weight, weight_scales, bias=None, dtype=torch.float16, num_rows=None, out=None):
+    """scales[m] * weight_scales[n] * sum_k feats[m, k] weight[n, k] + bias[n] in `dtype` [rows, outputs].
+
+    feats int8 [rows, inputs] and scales float32 [rows], as quantize_rows and layer_norm_int8 give them; weight int8 [outputs,
+    inputs], weight_scales and bias (or None) float32 [outputs].  The sum is exact.  Rows and weights that start on 16 bytes
+    and lie multiples of 16 bytes apart are read as they are, others are copied first, on every call.  At most 65536
+    inputs and outputs."""
+    feats, ld = _bytes(feats, "feats")
+    weight, weight_ld = _bytes(weight, "weight")
+    device, (rows, inputs), outputs = feats.device, feats.shape, weight.shape[0]
+    if weight.shape[1] != inputs or weight.device != device or outputs == 0:
+        raise ValueError("weight: [outputs, %d] on %s is needed" % (inputs, device))
+    if dtype not in _FEATURES:
+        raise TypeError("unsupported tensor dtype %s" % dtype)
+    if scales is None or weight_scales is None:
+        raise ValueError("scales of the rows and of the output channels are needed")
+    s, ws, b = (_dense(t, (n,), torch.float32, device, what) for t, n, what in (
+        (scales, rows, "scales"), (weight_scales, outputs, "weight_scales"), (bias, outputs, "bias")))
+    if out is None:
+        out = torch.empty((rows, outputs), dtype=dtype, device=device)
+    _dense(out, (rows, outputs), dtype, device, "out")
+    nbytes = _lib.lib().d3d_int8_linear_workspace(feats.data_ptr(), ld, rows, weight.data_ptr(), weight_ld, inputs, outputs)
+    workspace = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+    _call("d3d_int8_linear", device, _TORCH2D3D[dtype], feats.data_ptr(), ld, s, rows, _count(num_rows, device), weight.data_ptr(),
+          weight_ld, ws, b, inputs, outputs, out.data_ptr(), workspace.data_ptr() if nbytes else None, nbytes)
+    return out
+
+
 def _sequences(offsets, device):
     if offsets.dim() != 1 or offsets.shape[0] < 1 or offsets.dtype != torch.int32 or offsets.device != device:
         raise ValueError("seq_offsets: an int32 tensor [sequences + 1] on %s is needed" % device)

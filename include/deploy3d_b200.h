@@ -511,6 +511,15 @@ int d3d_quantize_rows(int dtype, const void* x, int64_t x_ld, int64_t rows, int 
 int d3d_layer_norm_int8(int dtype, const void* x, int64_t x_ld, const void* residual, int64_t residual_ld,
                         const float* weight, const float* bias, float eps, int64_t rows, int channels,
                         const int32_t* num_rows, void* total, int8_t* q, int64_t q_ld, float* scales, void* stream);
+/* Product of 8-bit rows and 8-bit weights: out[m][n] = x_scales[m] * weight_scales[n] * sum_k x[m][k] weight[n][k] + bias[n], the
+ * sum in 32-bit integers, out [rows][outputs] of `dtype` (float | half | bf16), bias [outputs] or NULL.  Rows of x and weight that
+ * start on 16 bytes and are multiples of 16 bytes apart are read where they are; others are copied into the workspace first
+ * (more than eight rows; its size depends on the addresses' alignment).  inputs, outputs <= 65536. */
+size_t d3d_int8_linear_workspace(const int8_t* x, int64_t x_ld, int64_t rows, const int8_t* weight, int64_t weight_ld, int inputs,
+                                 int outputs);
+int d3d_int8_linear(int dtype, const int8_t* x, int64_t x_ld, const float* x_scales, int64_t rows, const int32_t* num_rows,
+                    const int8_t* weight, int64_t weight_ld, const float* weight_scales, const float* bias, int inputs,
+                    int outputs, void* out, void* workspace, size_t workspace_bytes, void* stream);
 /* Gated linear recurrence over sequences: h[t] = f[t] h[t-1] + (1 - f[t]) x[t] per channel, f = sigmoid(gates), out = h.
  * Sequence s are the rows offsets[s] .. offsets[s+1]-1 (int32 [seqs+1] on the device, ascending; equal ones are a sequence
  * without rows), walked upwards or, with `reverse`, downwards.  initial [seqs][channels]: h in front of the first row walked

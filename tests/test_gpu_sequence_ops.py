@@ -380,3 +380,80 @@ def test_on_another_stream_and_in_graphs(d3d):
         torch.cuda.synchronize()
         for (_, outs), reverse in zip(graphs, (False, True)):
             assert all(torch.equal(p, q) for p, q in zip(outs, chain(a, b, reverse)))
+
+
+# ---- product of 8-bit rows ------------------------------------------------------------------------------------------
+def int8(seed, rows, channels, layout="dense"):
+    """Any bytes, -128 among them.  layout: "columns" 16 bytes into wider rows, "odd" one byte into them."""
+    gen = torch.Generator(device=DEV).manual_seed(seed)
+    x = torch.randint(-128, 128, (rows, channels), generator=gen, device=DEV, dtype=torch.int8)
+    if layout == "dense":
+        return x
+    pitch, at = ((channels + 47) // 16 * 16, 16) if layout == "columns" else (channels + 3, 1)
+    wide = torch.full((rows, pitch), 77, dtype=torch.int8, device=DEV)
+    wide[:, at:at + channels] = x
+    return wide[:, at:at + channels]
+
+
+def check_linear(x, s, w, ws, b, y):
+    """The sum is exact; then (float) sum, times the channel's scale, times the row's plus the bias in one rounding: three half
+    units of 32 bits, and half a step of the type."""
+    acc = (x.double() @ w.double().T).cpu().numpy()
+    scaled = acc * ref.as64(ws) * ref.as64(s)[:, None]
+    want = scaled + (ref.as64(b) if b is not None else 0.0)
+    limit = 3 * ref.U32 * (np.abs(scaled) + np.abs(want))
+    ref.assert_within(y, want, limit + ref.half_step(y.dtype) * (np.abs(want) + limit) + ref.smallest(y.dtype), "linear")
+
+
+@pytest.mark.parametrize("layout", ["dense", "columns", "odd"])
+@pytest.mark.parametrize("rows", [0, 1, 2, 3, 5, 8])
+@pytest.mark.parametrize("inputs,outputs", [(1, 1), (16, 16), (40, 9), (131, 387), (1000, 70), (4096, 33)])
+def test_linear_of_few_rows(d3d, layout, rows, inputs, outputs):
+    dtype = TYPES[(rows + inputs) % 3]
+    x, w = int8(1, rows, inputs, layout), int8(2, outputs, inputs, layout)
+    s, ws, b = 0.01 * normal(3, rows).abs(), 0.01 * normal(4, outputs), normal(5, outputs) if rows != 2 else None
+    y = d3d.int8_linear(x, s, w, ws, b, dtype=dtype)
+    assert y.shape == (rows, outputs) and y.dtype == dtype
+    check_linear(x, s, w, ws, b, y)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("layout", ["dense", "columns", "odd"])
+@pytest.mark.parametrize("rows,inputs,outputs", [
+    (9, 16, 16), (9, 1, 1), (127, 128, 64), (128, 96, 32), (129, 131, 40), (300, 64, 192), (257, 1000, 387), (40, 4096, 520),
+    (1000, 32, 1030), (20000, 48, 24), (20000, 144, 300), (9500, 640, 515)])
+def test_linear(d3d, dtype, layout, rows, inputs, outputs):
+    """One and two CTAs to a tile, one tile and several to a CTA, ends of every kind."""
+    x, w = int8(1, rows, inputs, layout), int8(2, outputs, inputs, layout)
+    s, ws, b = 0.01 * normal(3, rows).abs(), 0.01 * normal(4, outputs), normal(5, outputs)
+    check_linear(x, s, w, ws, b, d3d.int8_linear(x, s, w, ws, b, dtype=dtype))
+
+
+@pytest.mark.parametrize("rows,count", [(8, 5), (8, 0), (300, 200), (300, 0), (300, -3), (20000, 19001), (20000, 40000)])
+def test_linear_counts(d3d, rows, count):
+    x, w = int8(1, rows, 64), int8(2, 136, 64)
+    s, ws = 0.01 * normal(3, rows).abs(), 0.01 * normal(4, 136)
+    out = torch.full((rows, 136), 7.0, device=DEV, dtype=torch.float16)
+    d3d.int8_linear(x, s, w, ws, num_rows=live(count), out=out)
+    n = max(0, min(rows, count))
+    assert (out[n:] == 7).all()
+    if n:
+        check_linear(x[:n], s[:n], w, ws, None, out[:n])
+
+
+def test_linear_of_rows_that_are_not_finite(d3d):
+    """A row with a NaN in it is NaN behind the product, and no other is."""
+    for rows in (4, 200):
+        x = features(1, rows, 64, torch.float16)
+        x[2, 5] = float("inf")
+        q, s = d3d.quantize_rows(x)
+        y = d3d.int8_linear(q, s, int8(2, 48, 64), normal(3, 48))
+        assert y[2].isnan().all() and int(y.isnan().any(1).sum()) == 1
+
+
+def test_no_wait_gave_up(d3d):
+    import ctypes
+    from deploy3d_b200 import _lib
+    code = ctypes.c_int(0)
+    _lib.check("d3d_debug_take_kernel_error", _lib.lib().d3d_debug_take_kernel_error(ctypes.byref(code)))
+    assert code.value == 0
