@@ -1,4 +1,4 @@
-"""Loads ``libs/_d3d_host.so`` (csrc/host/dispatch.cpp), the native path of a plugin's ``enqueue``.
+"""Loads ``libs/_d3d_host.so`` (csrc/host), the native path of a plugin's ``enqueue`` and of the operators without a plugin.
 
 The module gets the addresses of the C-ABI entry points from the library that ``_lib`` has loaded, so that the checked
 and the tuning builds go through the same path.  There is no interpreted fallback: a missing module is an error.
@@ -37,3 +37,20 @@ def call(name, prefix):
     """Native enqueue of the plugin `name` whose C-ABI functions start with `prefix`."""
     return module().Call(name, prefix, _address(prefix + "_output_desc"), _address(prefix + "_workspace"),
                          _address(prefix + "_enqueue"))
+
+
+_SEQUENCE = ("d3d_layer_norm", "d3d_layer_norm_int8", "d3d_layer_norm_backward", "d3d_layer_norm_backward_workspace",
+             "d3d_quantize_rows", "d3d_int8_linear", "d3d_int8_linear_workspace", "d3d_gated_recurrence",
+             "d3d_gated_recurrence_backward", "d3d_gated_recurrence_step", "d3d_gated_recurrence_state_rows",
+             "d3d_gated_recurrence_workspace")  # in the order of csrc/host/sequence.cpp
+_BOUND = False
+
+
+def sequence():
+    """The module with the voxel-sequence operators' entry points in place."""
+    global _BOUND
+    mod = module()
+    if not _BOUND:
+        mod.bind_sequence(tuple(_address(name) for name in _SEQUENCE))
+        _BOUND = True
+    return mod

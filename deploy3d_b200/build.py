@@ -53,25 +53,26 @@ def _digest(path, flags):
 
 
 def build_host():
-    """Compile ``csrc/host/dispatch.cpp`` against the installed torch; returns the module's path."""
+    """Compile ``csrc/host`` against the installed torch; returns the module's path."""
     import sysconfig
 
     import torch
-    src, out = os.path.join(CSRC, "host", "dispatch.cpp"), os.path.join(HERE, "libs", "_d3d_host.so")
+    host, out = os.path.join(CSRC, "host"), os.path.join(HERE, "libs", "_d3d_host.so")
+    files = [os.path.join(host, f) for f in sorted(os.listdir(host)) if f.endswith((".cpp", ".h"))]
+    src = [f for f in files if f.endswith(".cpp")]
     root = os.path.dirname(torch.__file__)
     cuda = os.path.join(os.path.dirname(os.path.dirname(os.path.realpath(_nvcc()))), "include")
     cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-pthread", "-Wall", "-Wno-unused-function",
            "-D_GLIBCXX_USE_CXX11_ABI=%d" % int(torch._C._GLIBCXX_USE_CXX11_ABI), "-I" + os.path.join(root, "include"),
            "-I" + os.path.join(root, "include", "torch", "csrc", "api", "include"),
-           "-I" + sysconfig.get_paths()["include"], "-I" + cuda, src, "-o", out, "-L" + os.path.join(root, "lib"),
+           "-I" + sysconfig.get_paths()["include"], "-I" + cuda, *src, "-o", out, "-L" + os.path.join(root, "lib"),
            "-ltorch_python", "-ltorch_cpu", "-lc10", "-lc10_cuda"]
-    with open(src) as f:
-        want = _digest(src, cmd + [torch.__version__, f.read()])
+    want = _digest(out, cmd + [torch.__version__] + [open(f).read() for f in files])
     stamp = os.path.join(OBJ, "link_host.stamp")
     if not (os.path.exists(out) and os.path.exists(stamp) and open(stamp).read() == want):
         r = subprocess.run(cmd, capture_output=True, text=True)
         if r.returncode != 0:
-            raise RuntimeError("g++ failed for %s:\n%s\n%s" % (src, " ".join(cmd), r.stderr))
+            raise RuntimeError("g++ failed for %s:\n%s\n%s" % (host, " ".join(cmd), r.stderr))
         with open(stamp, "w") as f:
             f.write(want)
     return out

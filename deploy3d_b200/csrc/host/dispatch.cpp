@@ -8,10 +8,8 @@
 //
 // The library's entry points arrive as addresses (the package decides which build of the library is loaded), so this
 // module links against torch only.
-#define PY_SSIZE_T_CLEAN
-#include <Python.h>
+#include "host.h"
 
-#include <ATen/core/Tensor.h>
 #include <ATen/ops/empty.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
@@ -28,7 +26,19 @@
 #include <thread>
 #include <vector>
 
-#include "../../../include/deploy3d_b200.h"
+PyObject* g_check = nullptr;
+
+int dtype_of(const at::Tensor& t) {
+  switch (t.scalar_type()) {
+    case at::kFloat: return D3D_FLOAT;
+    case at::kHalf: return D3D_HALF;
+    case at::kInt: return D3D_INT32;
+    case at::kBFloat16: return D3D_BF16;
+    case at::kChar: return D3D_INT8;
+    case at::kBool: return D3D_BOOL;
+    default: return -1;
+  }
+}
 
 namespace {
 
@@ -57,20 +67,8 @@ struct Call {
   size_t oldest;
 };
 
-PyObject* g_check = nullptr;      // check(function name, status): raises
 PyObject* g_workspace = nullptr;  // interned "_workspace"
 
-int dtype_of(const at::Tensor& t) {
-  switch (t.scalar_type()) {
-    case at::kFloat: return D3D_FLOAT;
-    case at::kHalf: return D3D_HALF;
-    case at::kInt: return D3D_INT32;
-    case at::kBFloat16: return D3D_BF16;
-    case at::kChar: return D3D_INT8;
-    case at::kBool: return D3D_BOOL;
-    default: return -1;
-  }
-}
 at::ScalarType scalar_of(int dtype) {
   switch (dtype) {
     case D3D_FLOAT: return at::kFloat;
@@ -473,6 +471,7 @@ PyMODINIT_FUNC PyInit__d3d_host() {
   PyObject* m = PyModule_Create(&module_def);
   if (!m) return nullptr;
   Py_INCREF(&call_type);
+  if (PyModule_AddFunctions(m, sequence_methods) < 0) return nullptr;
   if (PyModule_AddObject(m, "Call", reinterpret_cast<PyObject*>(&call_type)) < 0) return nullptr;
   return m;
 }
