@@ -2,12 +2,11 @@
 //   h[t] = f[t] h[t-1] + (1 - f[t]) x[t],  f = sigmoid(gate);  h in front of a sequence is initial[s] (zeros without)
 //   delta[t] = grad[t] + f[t+1] delta[t+1]  (+ grad_final[s] at the last row),  dx = delta (1 - f),
 //   dgate = delta (h[t-1] - x) f (1 - f),  dinitial[s] = f delta at the first row
-// A step is the map c -> a c + b.  Maps compose: (a2, b2) after (a1, b1) is (a2 a1, a2 b1 + b2), so a tile of rows is one map
-// per channel, and tiles can be worked on side by side.  A row that starts a sequence is the map c -> b whatever c is, also
-// where c is not finite: its a is -0, and the sign says that what came before is not looked at (products keep it, f is never
-// negative).
-// Everything is held in 32 bits; 1 - f is computed as sigmoid(-gate), not as a difference, and f as 1 - (1 - f) where it is
-// the larger one, so that neither loses digits at long memories.
+// A row is the map c -> a c + b.  Maps compose: (a2, b2) after (a1, b1) is (a2 a1, a2 b1 + b2), so a tile of rows is one map per
+// channel, and tiles can be worked on side by side: one kernel leaves the tiles' maps, one chains them, one goes over the rows
+// again with what comes into each tile.  No kernel waits for another CTA, and every sum is made in one order.  A row that
+// starts a sequence is the map c -> b whatever c is, also where c is not finite: its a is -0, and the sign says that what came
+// before is not looked at (products keep it, f is never negative).
 #include <type_traits>
 
 #include "common.cuh"
@@ -17,9 +16,61 @@ namespace {
 
 template <class T, int V> struct alignas(sizeof(T) * V) Pack { T v[V]; };
 
-// Rows of a tile, whatever the types: the states the forward pass leaves at their starts are those of the backward pass.
-constexpr int kTile = 128;
-__host__ __device__ constexpr int backward_threads(int lanes) { return lanes >= 8 ? 512 : 256; }
+// The channels of a thread; two at a time are worked on by packed instructions.
+template <int V> struct Vec { float v[V]; };
+template <int V> __device__ __forceinline__ Vec<V> all(float x) {
+  Vec<V> r;
+#pragma unroll
+  for (int e = 0; e < V; ++e) r.v[e] = x;
+  return r;
+}
+template <int V> __device__ __forceinline__ float2 pair(const Vec<V>& a, int e) { return make_float2(a.v[e], a.v[e + 1]); }
+template <int V> __device__ __forceinline__ Vec<V> fma(const Vec<V>& a, const Vec<V>& b, const Vec<V>& c) {
+  Vec<V> r;
+#pragma unroll
+  for (int e = 0; e + 1 < V; e += 2) {
+    const float2 t = __ffma2_rn(pair(a, e), pair(b, e), pair(c, e));
+    r.v[e] = t.x, r.v[e + 1] = t.y;
+  }
+  if constexpr (V % 2) r.v[V - 1] = fmaf(a.v[V - 1], b.v[V - 1], c.v[V - 1]);
+  return r;
+}
+template <int V> __device__ __forceinline__ Vec<V> mul(const Vec<V>& a, const Vec<V>& b) {
+  Vec<V> r;
+#pragma unroll
+  for (int e = 0; e + 1 < V; e += 2) {
+    const float2 t = __fmul2_rn(pair(a, e), pair(b, e));
+    r.v[e] = t.x, r.v[e + 1] = t.y;
+  }
+  if constexpr (V % 2) r.v[V - 1] = a.v[V - 1] * b.v[V - 1];
+  return r;
+}
+template <int V> __device__ __forceinline__ Vec<V> add(const Vec<V>& a, const Vec<V>& b) {
+  Vec<V> r;
+#pragma unroll
+  for (int e = 0; e + 1 < V; e += 2) {
+    const float2 t = __fadd2_rn(pair(a, e), pair(b, e));
+    r.v[e] = t.x, r.v[e + 1] = t.y;
+  }
+  if constexpr (V % 2) r.v[V - 1] = a.v[V - 1] + b.v[V - 1];
+  return r;
+}
+template <class T, int V> __device__ __forceinline__ Vec<V> widen(const Pack<T, V>& p) {
+  Vec<V> r;
+#pragma unroll
+  for (int e = 0; e < V; ++e) r.v[e] = to_f32(p.v[e]);
+  return r;
+}
+template <class T, int V> __device__ __forceinline__ Pack<T, V> narrow(const Vec<V>& x) {
+  Pack<T, V> r;
+#pragma unroll
+  for (int e = 0; e < V; ++e) r.v[e] = from_f32<T>(x.v[e]);
+  return r;
+}
+
+constexpr int kTile = 128;     // rows of a tile
+constexpr int kThreads = 512;  // of a CTA
+constexpr int kWarps = kThreads / 32;
 
 struct ScanArgs {
   const void *x, *gates;
@@ -47,12 +98,41 @@ struct ScanArgs {
 
 __device__ __forceinline__ bool is_reset(float a) { return __float_as_int(a) < 0; }
 __device__ __forceinline__ float reset_mark() { return __int_as_float((int)0x80000000u); }
+// The map (a, b) at h.
+__device__ __forceinline__ float apply(float a, float b, float h) { return is_reset(a) ? b : fmaf(a, h, b); }
+// (a, b) after (pa, pb).
+__device__ __forceinline__ void after(float& a, float& b, float pa, float pb) {
+  if (!is_reset(a)) b = fmaf(a, pb, b), a *= pa;
+}
 
-// f and 1 - f
-__device__ __forceinline__ void gate_of(float g, float* f, float* add) {
-  const float e = expf(-fabsf(g)), small = e * __fdividef(1.f, 1.f + e), large = 1.f - small;
-  *f = fabsf(g >= 0.f ? large : small);  // NaN without a sign: the sign of a map means a reset
-  *add = g >= 0.f ? small : large;
+// f = sigmoid(gate) and 1 - f, each without the cancellation that a difference to the other one would be where that is near
+// one.  Features of 32 bits: exponential and quotient to two units of the last place.  Of 16 bits: the hardware's base-two
+// exponential, whose argument is rounded to |gate| 2^-24 (so that 1 - f is off by that much, relatively; the gate itself came
+// rounded to 2^-9 or 2^-12 of it), a third of the instructions.
+template <class T, int V> __device__ __forceinline__ void gate_of(const Pack<T, V>& g, Vec<V>& f, Vec<V>& rest) {
+  if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+      const float x = to_f32(g.v[e]), t = expf(-fabsf(x)), small = t * __fdividef(1.f, 1.f + t), large = 1.f - small;
+      f.v[e] = fabsf(x >= 0.f ? large : small);  // NaN without a sign: the sign of a map means a reset
+      rest.v[e] = x >= 0.f ? small : large;
+    }
+  } else {
+    Vec<V> t, r;
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+      float x;  // from below -80 on f is below 2^-115: nothing is left of any state
+      asm("max.NaN.f32 %0, %1, 0fC2A00000;" : "=f"(x) : "f"(to_f32(g.v[e])));
+      t.v[e] = __expf(-x);
+    }
+    const Vec<V> d = add(t, all<V>(1.f));
+#pragma unroll
+    for (int e = 0; e < V; ++e) asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r.v[e]) : "f"(d.v[e]));
+    rest = mul(t, r);
+    const Vec<V> large = fma(rest, all<V>(-1.f), all<V>(1.f));
+#pragma unroll
+    for (int e = 0; e < V; ++e) f.v[e] = fabsf(t.v[e] < 1.f ? large.v[e] : r.v[e]);
+  }
 }
 
 // The rows the sequences cover, clamped to the tensor.
@@ -68,306 +148,354 @@ __device__ __forceinline__ Span span_of(const ScanArgs& a) {
 __device__ __forceinline__ int64_t row_at(const ScanArgs& a, const Span& s, int64_t p) {
   return a.reverse ? s.begin + s.count - 1 - p : s.begin + p;
 }
-// The sequence row t belongs to: the last one that starts at or before it.
-__device__ __forceinline__ int seq_of(const ScanArgs& a, int64_t t) {
-  int lo = 0, hi = a.seqs;
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (__ldg(a.offsets + mid) <= t) lo = mid;
-    else hi = mid;
+
+// Where in a tile sequences start and end, in the order the rows are walked in: a bit per row, and whose row it is.
+struct Marks {
+  uint32_t first_bits[4], last_bits[4];
+  int first[kTile], last[kTile];  // where the bit is set
+  int range[2];                   // sequences of the tile's lowest and highest row
+};
+
+// The last sequence that starts at or before row t, by a whole warp: 32 probes a step.
+__device__ __forceinline__ int sequence_of(const ScanArgs& a, int64_t t) {
+  int lo = 0, n = a.seqs;
+  while (n > 1) {
+    const int step = (n + 31) / 32, at = lo + lane_id() * step;
+    const unsigned before = __ballot_sync(0xffffffffu, at < lo + n && __ldg(a.offsets + at) <= t);
+    const int k = before ? __popc(before) - 1 : 0, end = lo + n;
+    lo += k * step;
+    if (lo > end - 1) lo = end - 1;  // offsets out of order
+    n = end - lo < step ? end - lo : step;
   }
   return lo;
 }
 
-// For the rows of a tile, in the order they are walked in: the sequence that starts / ends there, or -1.
-template <int kThreads>
-__device__ __forceinline__ void mark_ends(const ScanArgs& a, const Span& span, int tile, int* first, int* last) {
-  for (int i = threadIdx.x; i < kTile; i += kThreads) {
-    const int64_t p = (int64_t)tile * kTile + i;
-    int f = -1, l = -1;
-    if (p < span.count) {
-      const int64_t t = row_at(a, span, p);
-      const int s = seq_of(a, t);
-      const bool at_low = t == __ldg(a.offsets + s), at_high = t + 1 == __ldg(a.offsets + s + 1);
-      f = (a.reverse ? at_high : at_low) ? s : -1;
-      l = (a.reverse ? at_low : at_high) ? s : -1;
+// Fills `m` for the tile; the caller's barrier in front of its use of it.  Two barriers inside.
+__device__ __forceinline__ void mark_ends(const ScanArgs& a, const Span& span, int tile, Marks* m) {
+  const int64_t p0 = (int64_t)tile * kTile, n = span.count - p0 < kTile ? span.count - p0 : kTile;
+  if (n <= 0) {
+    if (threadIdx.x < 4) m->first_bits[threadIdx.x] = m->last_bits[threadIdx.x] = 0u;
+    return;  // the whole CTA
+  }
+  const int64_t low = a.reverse ? row_at(a, span, p0 + n - 1) : row_at(a, span, p0);
+  const int warp = threadIdx.x >> 5;
+  if (threadIdx.x < 4) m->first_bits[threadIdx.x] = m->last_bits[threadIdx.x] = 0u;
+  if (warp < 2) {
+    const int s = sequence_of(a, warp ? low + n - 1 : low);
+    if (lane_id() == 0) m->range[warp] = s;
+  }
+  __syncthreads();
+  const int s1 = m->range[1];
+  for (int s = m->range[0] + (int)threadIdx.x; s <= s1; s += kThreads) {
+    const int64_t b = (int64_t)__ldg(a.offsets + s) - low, e = (int64_t)__ldg(a.offsets + s + 1) - 1 - low;
+    if (e < b) continue;
+    if (b >= 0 && b < n) {
+      const int i = (int)(a.reverse ? n - 1 - b : b);
+      (a.reverse ? m->last : m->first)[i] = s;
+      atomicOr(&(a.reverse ? m->last_bits : m->first_bits)[i >> 5], 1u << (i & 31));
     }
-    first[i] = f, last[i] = l;
+    if (e >= 0 && e < n) {
+      const int i = (int)(a.reverse ? n - 1 - e : e);
+      (a.reverse ? m->first : m->last)[i] = s;
+      atomicOr(&(a.reverse ? m->first_bits : m->last_bits)[i >> 5], 1u << (i & 31));
+    }
   }
 }
 
-// Every thread has a map per channel; afterwards it has that of all threads in front of it (kUp) or behind it.  kLanes lanes
-// of a warp stand side by side along the channels.  totals: [2][kWarps][kLanes * V], left with the warps' maps.
-template <int kLanes, int V, int kWarps, bool kUp>
-__device__ __forceinline__ void scan_threads(float (&a)[V], float (&b)[V], float* totals) {
-  const int lane = lane_id(), warp = threadIdx.x >> 5, at = lane % kLanes * V;
-  constexpr int kWidth = kLanes * V;
-#pragma unroll
-  for (int d = kLanes; d < 32; d <<= 1)
-#pragma unroll
-    for (int e = 0; e < V; ++e) {
-      const float pa = kUp ? __shfl_up_sync(0xffffffffu, a[e], d) : __shfl_down_sync(0xffffffffu, a[e], d);
-      const float pb = kUp ? __shfl_up_sync(0xffffffffu, b[e], d) : __shfl_down_sync(0xffffffffu, b[e], d);
-      if ((kUp ? lane >= d : lane + d < 32) && !is_reset(a[e])) b[e] = fmaf(a[e], pb, b[e]), a[e] *= pa;
-    }
-  if (kUp ? lane >= 32 - kLanes : lane < kLanes)
-#pragma unroll
-    for (int e = 0; e < V; ++e) totals[warp * kWidth + at + e] = a[e], totals[(kWarps + warp) * kWidth + at + e] = b[e];
-#pragma unroll
-  for (int e = 0; e < V; ++e) {
-    const float pa = kUp ? __shfl_up_sync(0xffffffffu, a[e], kLanes & 31) : __shfl_down_sync(0xffffffffu, a[e], kLanes & 31);
-    const float pb = kUp ? __shfl_up_sync(0xffffffffu, b[e], kLanes & 31) : __shfl_down_sync(0xffffffffu, b[e], kLanes & 31);
-    const bool has = kLanes < 32 && (kUp ? lane >= kLanes : lane + kLanes < 32);
-    a[e] = has ? pa : 1.f, b[e] = has ? pb : 0.f;
+// A thread's place: kLanes threads stand side by side along the channels, V channels each; the groups of them follow the rows,
+// kRows each.
+template <int V, int kLanes> struct Place {
+  static constexpr int kRows = kTile * kLanes / kThreads, kWidth = V * kLanes;
+  int tile, slab, lane, group, c, rows;  // rows: of this thread that there are
+  int64_t t0, step;                      // its first row, and to the next one
+  __device__ __forceinline__ Place(const ScanArgs& a, const Span& span) {
+    const int slabs = (a.channels + kWidth - 1) / kWidth;
+    slab = blockIdx.x % slabs, tile = blockIdx.x / slabs;
+    lane = threadIdx.x % kLanes, group = threadIdx.x / kLanes, c = slab * kWidth + lane * V;
+    const int64_t p = (int64_t)tile * kTile + group * kRows, left = span.count - p;
+    rows = c >= a.channels || left <= 0 ? 0 : left < kRows ? (int)left : kRows;
+    t0 = row_at(a, span, p), step = a.reverse ? -1 : 1;
   }
-  __syncthreads();
-  float pa[V], pb[V];
-#pragma unroll
-  for (int e = 0; e < V; ++e) pa[e] = 1.f, pb[e] = 0.f;
-  for (int i = 0; i < (kUp ? warp : kWarps - 1 - warp); ++i) {
-    const int w = kUp ? i : kWarps - 1 - i;
-#pragma unroll
-    for (int e = 0; e < V; ++e) {
-      const float wa = totals[w * kWidth + at + e], wb = totals[(kWarps + w) * kWidth + at + e];
-      if (is_reset(wa)) pa[e] = wa, pb[e] = wb;
-      else pb[e] = fmaf(wa, pb[e], wb), pa[e] *= wa;
-    }
+  __device__ __forceinline__ uint32_t bits(const uint32_t* of_tile) const {
+    const int at = group * kRows;
+    return of_tile[at >> 5] >> (at & 31) & ((1u << kRows) - 1);
   }
+};
+
+template <class T, int V, int kLanes>
+__device__ __forceinline__ void load_rows(Pack<T, V> (&to)[Place<V, kLanes>::kRows], const Place<V, kLanes>& at, const void* p, int64_t ld) {
+  const T* src = (const T*)p + at.t0 * ld + at.c;
+  const int64_t step = at.step * ld;
 #pragma unroll
-  for (int e = 0; e < V; ++e)
-    if (!is_reset(a[e])) b[e] = fmaf(a[e], pb[e], b[e]), a[e] *= pa[e];
+  for (int r = 0; r < Place<V, kLanes>::kRows; ++r)
+    if (r < at.rows) to[r] = *reinterpret_cast<const Pack<T, V>*>(src + r * step);
 }
-// The tile's map of the channel at `c` of its slab, from the warps' maps.
-template <int kWidth, int kWarps, bool kUp> __device__ __forceinline__ float2 tile_map(const float* totals, int c) {
-  float a = 1.f, b = 0.f;
-  for (int i = 0; i < kWarps; ++i) {
-    const int w = kUp ? i : kWarps - 1 - i;
-    const float wa = totals[w * kWidth + c], wb = totals[(kWarps + w) * kWidth + c];
-    if (is_reset(wa)) a = wa, b = wb;
-    else b = fmaf(wa, b, wb), a *= wa;
-  }
-  return make_float2(a, b);
+template <int V> __device__ __forceinline__ Vec<V> load_state(const float* p, int64_t s, int channels, int c) {
+  Vec<V> r = all<V>(0.f);
+  if (p)
+#pragma unroll
+    for (int e = 0; e < V; ++e) r.v[e] = __ldg(p + s * channels + c + e);
+  return r;
+}
+template <int V> __device__ __forceinline__ void store_state(float* p, int64_t s, int channels, int c, const Vec<V>& h) {
+  if (p)
+#pragma unroll
+    for (int e = 0; e < V; ++e) p[s * channels + c + e] = h.v[e];
 }
 
-// A tile is kTile rows by kLanes * V channels; a thread has kRows rows of V channels in its registers.
-// kMaps: the first pass, which leaves the tile's map.
-template <class T, int V, int kLanes, bool kMaps>
-__global__ void __launch_bounds__(256)
-scan_kernel(const ScanArgs a) {
-  constexpr int kThreads = 256, kRows = kTile * kLanes / kThreads, kWidth = kLanes * V, kWarps = kThreads / 32;
-  using P = Pack<T, V>;
-  __shared__ int first[kTile], last[kTile];
-  __shared__ float totals[2 * kWarps * kWidth];
-  const int slabs = (a.channels + kWidth - 1) / kWidth, slab = blockIdx.x % slabs, tile = blockIdx.x / slabs;
-  const int lane = threadIdx.x % kLanes, group = threadIdx.x / kLanes, c = slab * kWidth + lane * V;
-  const bool live = c < a.channels;
-  const Span span = span_of(a);
-  P x[kRows], g[kRows];
+// Every thread brings the map of its rows; the tile's is left in `map` (by the threads of the first kWidth channels), and
+// where `into` is given every thread gets what `into` (one value per channel of the slab, or 0) becomes in front of its rows
+// (kUp) or behind them.  Two barriers.  The channels' chains over the warps are walked by one thread each: a product per warp.
+template <int V, int kLanes, bool kUp> struct Chain {
+  float2 totals[kWarps][V * kLanes];
+  float into[kWarps][V * kLanes];
+
+  __device__ __forceinline__ Vec<V> run(Vec<V> ma, Vec<V> mb, const float* carry, float2* map, const Place<V, kLanes>& at, int channels) {
+    const int lane = lane_id(), warp = threadIdx.x >> 5, col = at.lane * V;
+    if constexpr (kLanes < 32)
 #pragma unroll
-  for (int r = 0; r < kRows; ++r) {
-    const int64_t p = (int64_t)tile * kTile + group * kRows + r, t = row_at(a, span, p);
-    if (live && p < span.count) {
-      x[r] = *reinterpret_cast<const P*>((const T*)a.x + t * a.x_ld + c);
-      g[r] = *reinterpret_cast<const P*>((const T*)a.gates + t * a.gates_ld + c);
-    }
-  }
-  mark_ends<kThreads>(a, span, tile, first, last);
-  __syncthreads();
-  float f[kRows][V], u[kRows][V], ma[V], mb[V];
+      for (int d = kLanes; d < 32; d <<= 1)
 #pragma unroll
-  for (int e = 0; e < V; ++e) ma[e] = 1.f, mb[e] = 0.f;
+        for (int e = 0; e < V; ++e) {
+          const float pa = kUp ? __shfl_up_sync(0xffffffffu, ma.v[e], d) : __shfl_down_sync(0xffffffffu, ma.v[e], d);
+          const float pb = kUp ? __shfl_up_sync(0xffffffffu, mb.v[e], d) : __shfl_down_sync(0xffffffffu, mb.v[e], d);
+          if (kUp ? lane >= d : lane + d < 32) after(ma.v[e], mb.v[e], pa, pb);
+        }
+    if (kUp ? lane >= 32 - kLanes : lane < kLanes)
 #pragma unroll
-  for (int r = 0; r < kRows; ++r) {
-    const bool in = live && (int64_t)tile * kTile + group * kRows + r < span.count;
-    const int s = first[group * kRows + r];
+      for (int e = 0; e < V; ++e) totals[warp][col + e] = make_float2(ma.v[e], mb.v[e]);
+    __syncthreads();
+    const int t = threadIdx.x, c = at.slab * V * kLanes + t;
+    if (t < V * kLanes && c < channels) {
+      if (map) {
+        float a = 1.f, b = 0.f;
 #pragma unroll
-    for (int e = 0; e < V; ++e) {
-      float add;
-      f[r][e] = 1.f, u[r][e] = 0.f;
-      if (in) {
-        gate_of(to_f32(g[r].v[e]), &f[r][e], &add);
-        u[r][e] = add * to_f32(x[r].v[e]);
-        if (s >= 0) {
-          if (a.initial) u[r][e] = fmaf(f[r][e], __ldg(a.initial + (int64_t)s * a.channels + c + e), u[r][e]);
-          f[r][e] = reset_mark();
+        for (int i = 0; i < kWarps; ++i) {
+          float2 m = totals[kUp ? i : kWarps - 1 - i][t];
+          after(m.x, m.y, a, b);
+          a = m.x, b = m.y;
+        }
+        map[(int64_t)at.tile * channels + c] = make_float2(a, b);
+      } else {
+        float h = carry ? __ldg(carry + (int64_t)at.tile * channels + c) : 0.f;
+#pragma unroll
+        for (int i = 0; i < kWarps; ++i) {
+          const int w = kUp ? i : kWarps - 1 - i;
+          into[w][t] = h;
+          const float2 m = totals[w][t];
+          h = apply(m.x, m.y, h);
         }
       }
-      if (is_reset(f[r][e])) ma[e] = f[r][e], mb[e] = u[r][e];
-      else mb[e] = fmaf(f[r][e], mb[e], u[r][e]), ma[e] *= f[r][e];
     }
-  }
-  scan_threads<kLanes, V, kWarps, true>(ma, mb, totals);
-  if constexpr (kMaps) {
-    if ((int)threadIdx.x < kWidth && slab * kWidth + (int)threadIdx.x < a.channels)
-      a.maps[(int64_t)tile * a.channels + slab * kWidth + threadIdx.x] = tile_map<kWidth, kWarps, true>(totals, threadIdx.x);
-    return;
-  }
-  float h[V];
-#pragma unroll
-  for (int e = 0; e < V; ++e) {
-    const float before = live && a.states ? __ldg(a.states + (int64_t)tile * a.channels + c + e) : 0.f;
-    h[e] = is_reset(ma[e]) ? mb[e] : fmaf(ma[e], before, mb[e]);
-  }
-#pragma unroll
-  for (int r = 0; r < kRows; ++r) {
-    const int64_t p = (int64_t)tile * kTile + group * kRows + r, t = row_at(a, span, p);
-    if (!live || p >= span.count) continue;
-    const int s = last[group * kRows + r];
-    P o;
+    if (map) return all<V>(0.f);
+    __syncthreads();
+    Vec<V> h;
 #pragma unroll
     for (int e = 0; e < V; ++e) {
-      h[e] = is_reset(f[r][e]) ? u[r][e] : fmaf(f[r][e], h[e], u[r][e]);
-      o.v[e] = from_f32<T>(h[e]);
-      if (s >= 0 && a.final_state) a.final_state[(int64_t)s * a.channels + c + e] = h[e];
+      h.v[e] = into[warp][col + e];
+      if constexpr (kLanes < 32) {
+        const float pa = kUp ? __shfl_up_sync(0xffffffffu, ma.v[e], kLanes) : __shfl_down_sync(0xffffffffu, ma.v[e], kLanes);
+        const float pb = kUp ? __shfl_up_sync(0xffffffffu, mb.v[e], kLanes) : __shfl_down_sync(0xffffffffu, mb.v[e], kLanes);
+        if (kUp ? lane >= kLanes : lane + kLanes < 32) h.v[e] = apply(pa, pb, h.v[e]);
+      }
     }
-    *reinterpret_cast<P*>((T*)a.out + t * a.channels + c) = o;
+    return h;
   }
+};
+
+// Sequences without rows: their last state is the one they start with.
+template <int V, int kLanes>
+__device__ __forceinline__ void pass_empty(const ScanArgs& a, const Place<V, kLanes>& at, const float* from, float* to) {
+  if (!to) return;
+  const int tiles = a.tiles > 0 ? a.tiles : 1, low = at.slab * V * kLanes;
+  const int high = low + V * kLanes < a.channels ? low + V * kLanes : a.channels;
+  for (int64_t s = (int64_t)at.tile * kThreads + threadIdx.x; s < a.seqs; s += (int64_t)tiles * kThreads)
+    if (__ldg(a.offsets + s + 1) <= __ldg(a.offsets + s))
+      for (int c = low; c < high; ++c) to[s * a.channels + c] = from ? __ldg(from + s * a.channels + c) : 0.f;
 }
 
-// The tiles' maps one after the other, a thread per channel: what comes into each tile.
-__global__ void __launch_bounds__(128) carry_kernel(const float2* maps, float* into, int tiles, int channels, int backward) {
-  const int c = blockIdx.x * blockDim.x + threadIdx.x;
-  if (c >= channels) return;
-  float h = 0.f;
-  for (int i = 0; i < tiles; ++i) {
-    const int64_t at = (int64_t)(backward ? tiles - 1 - i : i) * channels + c;
-    into[at] = h;
-    const float2 m = __ldg(maps + at);
-    h = is_reset(m.x) ? m.y : fmaf(m.x, h, m.y);
+// kMaps: the first pass, which leaves the tile's map.
+template <class T, int V, int kLanes, bool kMaps>
+__global__ void __launch_bounds__(kThreads, 2)
+scan_kernel(const ScanArgs a) {
+  constexpr int kRows = Place<V, kLanes>::kRows;
+  using P = Pack<T, V>;
+  __shared__ Marks marks;
+  __shared__ Chain<V, kLanes, true> chain;
+  const Span span = span_of(a);
+  const Place<V, kLanes> at(a, span);
+  if (kMaps) pdl_release();
+  P x[kRows], g[kRows];
+  load_rows<T, V, kLanes>(x, at, a.x, a.x_ld);
+  load_rows<T, V, kLanes>(g, at, a.gates, a.gates_ld);
+  mark_ends(a, span, at.tile, &marks);
+  __syncthreads();
+  const uint32_t starts = at.bits(marks.first_bits);
+  Vec<V> f[kRows], u[kRows], ma = all<V>(1.f), mb = all<V>(0.f);
+#pragma unroll
+  for (int r = 0; r < kRows; ++r) {
+    f[r] = all<V>(1.f), u[r] = all<V>(0.f);
+    if (r < at.rows) {
+      Vec<V> rest;
+      gate_of<T, V>(g[r], f[r], rest);
+      u[r] = mul(rest, widen<T, V>(x[r]));
+      if (starts >> r & 1) {
+        u[r] = fma(f[r], load_state<V>(a.initial, marks.first[at.group * kRows + r], a.channels, at.c), u[r]);
+        f[r] = ma = all<V>(reset_mark()), mb = u[r];
+      } else {
+        mb = fma(f[r], mb, u[r]), ma = mul(ma, f[r]);
+      }
+    }
   }
+  if (!kMaps) pdl_wait();
+  Vec<V> h = chain.run(ma, mb, a.states, kMaps ? a.maps : nullptr, at, a.channels);
+  if (kMaps) return;
+  const uint32_t ends = at.bits(marks.last_bits);
+  T* out = (T*)a.out + at.t0 * a.channels + at.c;
+  const int64_t step = at.step * a.channels;
+#pragma unroll
+  for (int r = 0; r < kRows; ++r)
+    if (r < at.rows) {
+      h = starts >> r & 1 ? u[r] : fma(f[r], h, u[r]);
+      *reinterpret_cast<P*>(out + r * step) = narrow<T, V>(h);
+      if (ends >> r & 1) store_state<V>(a.final_state, marks.last[at.group * kRows + r], a.channels, at.c, h);
+    }
+  pass_empty<V, kLanes>(a, at, a.initial, a.final_state);
 }
 
-// Sequences without rows end as they start.
-__global__ void __launch_bounds__(256) empty_kernel(const ScanArgs a, const float* from, float* to) {
-  const int64_t n = (int64_t)a.seqs * a.channels, nth = (int64_t)gridDim.x * blockDim.x;
-  for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += nth) {
-    const int64_t s = i / a.channels;
-    if (__ldg(a.offsets + s + 1) <= __ldg(a.offsets + s)) to[i] = from ? __ldg(from + i) : 0.f;
+// What comes into each tile: the tiles' maps one after the other, from the first (or, backwards, the last) on.  Eight channels to
+// a CTA; 128 threads of each take kHeld tiles into registers, chain them, and are chained by shuffles and through shared memory.
+constexpr int kHeld = 8, kCarryThreads = 1024, kCarryChannels = 8;
+__global__ void __launch_bounds__(kCarryThreads)
+carry_kernel(const float2* __restrict__ maps, float* __restrict__ into, int tiles, int channels, int backward) {
+  __shared__ float2 totals[32][kCarryChannels];
+  __shared__ float starts[32][kCarryChannels];
+  const int lane = lane_id(), warp = threadIdx.x >> 5, ch = threadIdx.x % kCarryChannels, c = blockIdx.x * kCarryChannels + ch;
+  const int segment = threadIdx.x / kCarryChannels;
+  pdl_release();
+  pdl_wait();
+  float carry = 0.f;  // of channel `warp` of this CTA, in the warps that chain
+  constexpr int kTurn = kCarryThreads / kCarryChannels * kHeld;
+  for (int t0 = 0; t0 < tiles; t0 += kTurn) {
+    float2 m[kHeld];
+    float a = 1.f, b = 0.f;
+#pragma unroll
+    for (int i = 0; i < kHeld; ++i) {
+      const int t = t0 + segment * kHeld + i;
+      m[i] = make_float2(1.f, 0.f);
+      if (t < tiles && c < channels) m[i] = __ldg(maps + (int64_t)(backward ? tiles - 1 - t : t) * channels + c);
+    }
+#pragma unroll
+    for (int i = 0; i < kHeld; ++i) {
+      float na = m[i].x, nb = m[i].y;
+      after(na, nb, a, b);
+      a = na, b = nb;
+    }
+#pragma unroll
+    for (int d = kCarryChannels; d < 32; d <<= 1) {
+      const float pa = __shfl_up_sync(0xffffffffu, a, d), pb = __shfl_up_sync(0xffffffffu, b, d);
+      if (lane >= d) after(a, b, pa, pb);
+    }
+    if (lane >= 32 - kCarryChannels) totals[warp][ch] = make_float2(a, b);
+    __syncthreads();
+    if (warp < kCarryChannels) {  // a warp per channel, a lane per warp's total
+      float2 w = totals[lane][warp];
+#pragma unroll
+      for (int d = 1; d < 32; d <<= 1) {
+        const float pa = __shfl_up_sync(0xffffffffu, w.x, d), pb = __shfl_up_sync(0xffffffffu, w.y, d);
+        if (lane >= d) after(w.x, w.y, pa, pb);
+      }
+      const float end = apply(w.x, w.y, carry), before = __shfl_up_sync(0xffffffffu, end, 1);
+      starts[lane][warp] = lane ? before : carry;
+      carry = __shfl_sync(0xffffffffu, end, 31);
+    }
+    __syncthreads();
+    float h = starts[warp][ch];
+    const float pa = __shfl_up_sync(0xffffffffu, a, kCarryChannels), pb = __shfl_up_sync(0xffffffffu, b, kCarryChannels);
+    if (lane >= kCarryChannels) h = apply(pa, pb, h);
+#pragma unroll
+    for (int i = 0; i < kHeld; ++i) {
+      const int t = t0 + segment * kHeld + i;
+      if (t < tiles && c < channels) into[(int64_t)(backward ? tiles - 1 - t : t) * channels + c] = h;
+      h = apply(m[i].x, m[i].y, h);
+    }
   }
 }
 
 // Backward: the rows of a tile forward once more from the state in front of it, which gives h[t-1], and the gradients from its
 // end.  The map of a row is c -> f (grad + c): c comes in from the row behind and goes out to the row in front.
 template <class T, int V, int kLanes, bool kMaps>
-__global__ void __launch_bounds__(backward_threads(kLanes))
+__global__ void __launch_bounds__(kThreads, kMaps ? 2 : 1)
 scan_backward_kernel(const ScanArgs a) {
-  constexpr int kThreads = backward_threads(kLanes), kRows = kTile * kLanes / kThreads, kWidth = kLanes * V, kWarps = kThreads / 32;
+  constexpr int kRows = Place<V, kLanes>::kRows;
   using P = Pack<T, V>;
-  __shared__ int first[kTile], last[kTile];
-  __shared__ float totals[2 * kWarps * kWidth];
-  const int slabs = (a.channels + kWidth - 1) / kWidth, slab = blockIdx.x % slabs, tile = blockIdx.x / slabs;
-  const int lane = threadIdx.x % kLanes, group = threadIdx.x / kLanes, c = slab * kWidth + lane * V;
-  const bool live = c < a.channels;
+  __shared__ Marks marks;
+  __shared__ Chain<V, kLanes, true> ahead;
+  __shared__ Chain<V, kLanes, false> back;
   const Span span = span_of(a);
+  const Place<V, kLanes> at(a, span);
+  if (kMaps) pdl_release();
   P x[kRows], g[kRows], d[kRows];
-#pragma unroll
-  for (int r = 0; r < kRows; ++r) {
-    const int64_t p = (int64_t)tile * kTile + group * kRows + r, t = row_at(a, span, p);
-    if (live && p < span.count) {
-      if (!kMaps) x[r] = *reinterpret_cast<const P*>((const T*)a.x + t * a.x_ld + c);
-      g[r] = *reinterpret_cast<const P*>((const T*)a.gates + t * a.gates_ld + c);
-      d[r] = *reinterpret_cast<const P*>((const T*)a.grad + t * a.grad_ld + c);
-    }
-  }
-  mark_ends<kThreads>(a, span, tile, first, last);
+  if (!kMaps) load_rows<T, V, kLanes>(x, at, a.x, a.x_ld);
+  load_rows<T, V, kLanes>(g, at, a.gates, a.gates_ld);
+  load_rows<T, V, kLanes>(d, at, a.grad, a.grad_ld);
+  mark_ends(a, span, at.tile, &marks);
   __syncthreads();
-  float f[kRows][V], add[kRows][V], ma[V], mb[V];
-  bool in[kRows];
+  const uint32_t starts = at.bits(marks.first_bits), ends = at.bits(marks.last_bits);
+  const int* first = marks.first + at.group * kRows;
+  const int* last = marks.last + at.group * kRows;
+  Vec<V> f[kRows], rest[kRows], before[kRows], ma, mb;
 #pragma unroll
-  for (int r = 0; r < kRows; ++r) {
-    in[r] = live && (int64_t)tile * kTile + group * kRows + r < span.count;
-#pragma unroll
-    for (int e = 0; e < V; ++e) {
-      f[r][e] = 1.f, add[r][e] = 0.f;
-      if (in[r]) gate_of(to_f32(g[r].v[e]), &f[r][e], &add[r][e]);
-    }
-  }
-  float before[kRows][V];  // h[t-1]
+  for (int r = 0; r < kRows; ++r)
+    if (r < at.rows) gate_of<T, V>(g[r], f[r], rest[r]);
   if (!kMaps) {
+    ma = all<V>(1.f), mb = all<V>(0.f);
 #pragma unroll
-    for (int e = 0; e < V; ++e) ma[e] = 1.f, mb[e] = 0.f;
-#pragma unroll
-    for (int r = 0; r < kRows; ++r) {
-      if (!in[r]) continue;
-      const int s = first[group * kRows + r];
-#pragma unroll
-      for (int e = 0; e < V; ++e) {
-        const float u = add[r][e] * to_f32(x[r].v[e]);
-        if (s >= 0) {
-          const float h0 = a.initial ? __ldg(a.initial + (int64_t)s * a.channels + c + e) : 0.f;
-          ma[e] = reset_mark(), mb[e] = fmaf(f[r][e], h0, u);
+    for (int r = 0; r < kRows; ++r)
+      if (r < at.rows) {
+        const Vec<V> u = mul(rest[r], widen<T, V>(x[r]));
+        if (starts >> r & 1) {
+          ma = all<V>(reset_mark()), mb = fma(f[r], load_state<V>(a.initial, first[r], a.channels, at.c), u);
         } else {
-          mb[e] = fmaf(f[r][e], mb[e], u), ma[e] *= f[r][e];
+          mb = fma(f[r], mb, u), ma = mul(ma, f[r]);
         }
       }
-    }
-    scan_threads<kLanes, V, kWarps, true>(ma, mb, totals);
-    __syncthreads();
-    float h[V];
+    Vec<V> h = ahead.run(ma, mb, a.states, nullptr, at, a.channels);
 #pragma unroll
-    for (int e = 0; e < V; ++e) {
-      const float h0 = live ? __ldg(a.states + (int64_t)tile * a.channels + c + e) : 0.f;
-      h[e] = is_reset(ma[e]) ? mb[e] : fmaf(ma[e], h0, mb[e]);
-    }
-#pragma unroll
-    for (int r = 0; r < kRows; ++r) {
-      if (!in[r]) continue;
-      const int s = first[group * kRows + r];
-#pragma unroll
-      for (int e = 0; e < V; ++e) {
-        if (s >= 0) h[e] = a.initial ? __ldg(a.initial + (int64_t)s * a.channels + c + e) : 0.f;
-        before[r][e] = h[e];
-        h[e] = fmaf(f[r][e], h[e], add[r][e] * to_f32(x[r].v[e]));
+    for (int r = 0; r < kRows; ++r)
+      if (r < at.rows) {
+        if (starts >> r & 1) h = load_state<V>(a.initial, first[r], a.channels, at.c);
+        before[r] = h;
+        h = fma(f[r], h, mul(rest[r], widen<T, V>(x[r])));
       }
-    }
   }
+  ma = all<V>(1.f), mb = all<V>(0.f);
 #pragma unroll
-  for (int e = 0; e < V; ++e) ma[e] = 1.f, mb[e] = 0.f;
-#pragma unroll
-  for (int r = kRows - 1; r >= 0; --r) {
-    if (!in[r]) continue;
-    const int s = last[group * kRows + r];
-#pragma unroll
-    for (int e = 0; e < V; ++e) {
-      const float dy = to_f32(d[r].v[e]);
-      if (s >= 0) {
-        const float dl = a.grad_final ? __ldg(a.grad_final + (int64_t)s * a.channels + c + e) : 0.f;
-        ma[e] = reset_mark(), mb[e] = f[r][e] * (dy + dl);
+  for (int r = kRows - 1; r >= 0; --r)
+    if (r < at.rows) {
+      const Vec<V> dy = widen<T, V>(d[r]);
+      if (ends >> r & 1) {
+        ma = all<V>(reset_mark()), mb = mul(f[r], add(dy, load_state<V>(a.grad_final, last[r], a.channels, at.c)));
       } else {
-        mb[e] = f[r][e] * (dy + mb[e]), ma[e] *= f[r][e];
+        mb = mul(f[r], add(dy, mb)), ma = mul(ma, f[r]);
       }
     }
-  }
-  scan_threads<kLanes, V, kWarps, false>(ma, mb, totals);
-  if (kMaps) {
-    if ((int)threadIdx.x < kWidth && slab * kWidth + (int)threadIdx.x < a.channels)
-      a.maps[(int64_t)tile * a.channels + slab * kWidth + threadIdx.x] = tile_map<kWidth, kWarps, false>(totals, threadIdx.x);
-    return;
-  }
-  float q[V];
+  if (!kMaps) pdl_wait();
+  Vec<V> q = back.run(ma, mb, a.carry, kMaps ? a.maps : nullptr, at, a.channels);
+  if (kMaps) return;
+  const int64_t from = at.t0 * a.channels + at.c, step = at.step * a.channels;
 #pragma unroll
-  for (int e = 0; e < V; ++e) {
-    const float behind = live ? __ldg(a.carry + (int64_t)tile * a.channels + c + e) : 0.f;
-    q[e] = is_reset(ma[e]) ? mb[e] : fmaf(ma[e], behind, mb[e]);
-  }
-#pragma unroll
-  for (int r = kRows - 1; r >= 0; --r) {
-    if (!in[r]) continue;
-    const int64_t t = row_at(a, span, (int64_t)tile * kTile + group * kRows + r);
-    const int s = last[group * kRows + r], s0 = first[group * kRows + r];
-    P dx, dg;
-#pragma unroll
-    for (int e = 0; e < V; ++e) {
-      if (s >= 0) q[e] = a.grad_final ? __ldg(a.grad_final + (int64_t)s * a.channels + c + e) : 0.f;
-      const float delta = to_f32(d[r].v[e]) + q[e];
-      q[e] = f[r][e] * delta;
-      dx.v[e] = from_f32<T>(delta * add[r][e]);
-      dg.v[e] = from_f32<T>(q[e] * add[r][e] * (before[r][e] - to_f32(x[r].v[e])));
-      if (s0 >= 0 && a.grad_initial) a.grad_initial[(int64_t)s0 * a.channels + c + e] = q[e];
+  for (int r = kRows - 1; r >= 0; --r)
+    if (r < at.rows) {
+      if (ends >> r & 1) q = load_state<V>(a.grad_final, last[r], a.channels, at.c);
+      const Vec<V> delta = add(widen<T, V>(d[r]), q);
+      q = mul(f[r], delta);
+      const Vec<V> away = fma(widen<T, V>(x[r]), all<V>(-1.f), before[r]);
+      *reinterpret_cast<P*>((T*)a.grad_x + from + r * step) = narrow<T, V>(mul(delta, rest[r]));
+      *reinterpret_cast<P*>((T*)a.grad_gates + from + r * step) = narrow<T, V>(mul(mul(q, rest[r]), away));
+      if (starts >> r & 1) store_state<V>(a.grad_initial, first[r], a.channels, at.c, q);
     }
-    *reinterpret_cast<P*>((T*)a.grad_x + t * a.channels + c) = dx;
-    *reinterpret_cast<P*>((T*)a.grad_gates + t * a.channels + c) = dg;
-  }
+  pass_empty<V, kLanes>(a, at, a.grad_final, a.grad_initial);
 }
 
 // One row a sequence: the state is read, moved on and written; state_out may be state.
@@ -382,31 +510,27 @@ step_kernel(const T* __restrict__ x, int64_t x_ld, const T* __restrict__ gates, 
     const int64_t row = i / per_row, at = i * V;
     const int c = (int)(i - row * per_row) * V;
     const P px = *reinterpret_cast<const P*>(x + row * x_ld + c), pg = *reinterpret_cast<const P*>(gates + row * gates_ld + c);
-    P o;
-    Pack<float, V> h;
+    Pack<float, V> h = *reinterpret_cast<const Pack<float, V>*>(state + at);
+    Vec<V> f, rest, v;
 #pragma unroll
-    for (int e = 0; e < V; ++e) h.v[e] = state[at + e];
+    for (int e = 0; e < V; ++e) v.v[e] = h.v[e];
+    gate_of<T, V>(pg, f, rest);
+    v = fma(f, v, mul(rest, widen<T, V>(px)));
 #pragma unroll
-    for (int e = 0; e < V; ++e) {
-      float f, add;
-      gate_of(to_f32(pg.v[e]), &f, &add);
-      h.v[e] = fmaf(f, h.v[e], add * to_f32(px.v[e]));
-      o.v[e] = from_f32<T>(h.v[e]);
-    }
-#pragma unroll
-    for (int e = 0; e < V; ++e) state_out[at + e] = h.v[e];
-    *reinterpret_cast<P*>(out + at) = o;
+    for (int e = 0; e < V; ++e) h.v[e] = v.v[e];
+    *reinterpret_cast<Pack<float, V>*>(state_out + at) = h;
+    *reinterpret_cast<P*>(out + at) = narrow<T, V>(v);
   }
 }
 
-// f(V, lanes) for the tile shape of this many channels.  Rows that cannot be read in 16-byte pieces: a channel a thread.
-template <class T, class F> int by_shape(bool wide, int channels, F f) {
-  constexpr int V = 16 / (int)sizeof(T);
+// f(V, lanes) for the tile shape of this many channels: two channels a thread where rows can be read so, and as few threads side
+// by side as cover the channels.
+template <class F> int by_shape(bool pairs, int channels, F f) {
 #define D3D_SCAN_SHAPE(V, L) return f(std::integral_constant<int, V>(), std::integral_constant<int, L>())
-  if (!wide) D3D_SCAN_SHAPE(1, 32);
-  if (channels <= 2 * V) D3D_SCAN_SHAPE(V, 2);
-  if (channels <= 4 * V) D3D_SCAN_SHAPE(V, 4);
-  D3D_SCAN_SHAPE(V, 8);
+  if (!pairs) D3D_SCAN_SHAPE(1, 32);
+  if (channels <= 16) D3D_SCAN_SHAPE(2, 8);
+  if (channels <= 32) D3D_SCAN_SHAPE(2, 16);
+  D3D_SCAN_SHAPE(2, 32);
 #undef D3D_SCAN_SHAPE
 }
 template <class F> int by_type(int dtype, F f) {
@@ -418,14 +542,8 @@ template <class F> int by_type(int dtype, F f) {
   }
 }
 
-bool rows_wide(const void* p, int64_t ld, int esize) { return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld * esize % 16 == 0; }
-
-int fill_empty(const ScanArgs& a, const float* from, float* to, cudaStream_t st) {
-  if (!to || a.seqs == 0) return D3D_OK;
-  empty_kernel<<<stream_grid((int64_t)a.seqs * a.channels, 256), 256, 0, st>>>(a, from, to);
-  D3D_CHECK_LAUNCH();
-  return D3D_OK;
-}
+// Whether rows of `ld` elements from `p` on can be read in pairs.
+bool rows_paired(const void* p, int64_t ld, int esize) { return reinterpret_cast<uintptr_t>(p) % (2 * esize) == 0 && ld % 2 == 0; }
 
 int check_scan(int dtype, const ScanArgs& a) {
   D3D_REQUIRE(dtype == D3D_FLOAT || dtype == D3D_HALF || dtype == D3D_BF16, D3D_ERR_UNSUPPORTED_DTYPE);
@@ -472,19 +590,25 @@ extern "C" int d3d_gated_recurrence(int dtype, const void* x, int64_t x_ld, cons
   a.states = states ? states : w.take<float>((size_t)d3d_gated_recurrence_state_rows(rows) * channels);
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   const int esize = (int)dtype_size(dtype);
-  const bool wide = channels * esize % 16 == 0 && rows_wide(x, x_ld, esize) && rows_wide(gates, gates_ld, esize) && rows_wide(out, channels, esize);
+  const bool pairs = channels % 2 == 0 && rows_paired(x, x_ld, esize) && rows_paired(gates, gates_ld, esize) && rows_paired(out, channels, esize);
   if (seqs == 0) return D3D_OK;
-  const int rc2 = fill_empty(a, initial, final_state, st);
-  if (rc2 != D3D_OK || rows == 0) return rc2;
   return by_type(dtype, [&](auto t) -> int {
     using T = decltype(t);
-    return by_shape<T>(wide, channels, [&](auto v, auto l) -> int {
+    return by_shape(pairs, channels, [&](auto v, auto l) -> int {
       constexpr int V = decltype(v)::value, L = decltype(l)::value;
       a.tiles = (int)ceil_div(rows, kTile);
-      const unsigned grid = (unsigned)(a.tiles * ceil_div(channels, L * V));
-      scan_kernel<T, V, L, true><<<grid, 256, 0, st>>>(a);
-      carry_kernel<<<(unsigned)ceil_div(channels, 128), 128, 0, st>>>(a.maps, a.states, a.tiles, channels, 0);
-      scan_kernel<T, V, L, false><<<grid, 256, 0, st>>>(a);
+      const unsigned grid = (unsigned)((a.tiles > 0 ? a.tiles : 1) * ceil_div(channels, V * L));
+      if (a.tiles > 1) {
+        scan_kernel<T, V, L, true><<<grid, kThreads, 0, st>>>(a);
+        D3D_CHECK_LAUNCH();
+        D3D_LAUNCH(true, carry_kernel, (unsigned)ceil_div(channels, kCarryChannels), kCarryThreads, 0, st, a.maps, a.states, a.tiles,
+                   channels, 0);
+      } else if (states) {  // nothing lies in front of the only tile
+        if (cudaMemsetAsync(states, 0, channels * sizeof(float), st) != cudaSuccess) return D3D_ERR_CUDA;
+      } else {
+        a.states = nullptr;
+      }
+      D3D_LAUNCH(a.tiles > 1, (scan_kernel<T, V, L, false>), grid, kThreads, 0, st, a);
       D3D_CHECK_LAUNCH();
       return D3D_OK;
     });
@@ -514,20 +638,24 @@ extern "C" int d3d_gated_recurrence_backward(int dtype, const void* grad, int64_
   a.states = const_cast<float*>(states);
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   const int esize = (int)dtype_size(dtype);
-  const bool wide = channels * esize % 16 == 0 && rows_wide(x, x_ld, esize) && rows_wide(gates, gates_ld, esize) &&
-                    rows_wide(grad, grad_ld, esize) && rows_wide(grad_x, channels, esize) && rows_wide(grad_gates, channels, esize);
+  const bool pairs = channels % 2 == 0 && rows_paired(x, x_ld, esize) && rows_paired(gates, gates_ld, esize) &&
+                     rows_paired(grad, grad_ld, esize) && rows_paired(grad_x, channels, esize) && rows_paired(grad_gates, channels, esize);
   if (seqs == 0) return D3D_OK;
-  const int rc2 = fill_empty(a, grad_final, grad_initial, st);
-  if (rc2 != D3D_OK || rows == 0) return rc2;
   return by_type(dtype, [&](auto t) -> int {
     using T = decltype(t);
-    return by_shape<T>(wide, channels, [&](auto v, auto l) -> int {
+    return by_shape(pairs, channels, [&](auto v, auto l) -> int {
       constexpr int V = decltype(v)::value, L = decltype(l)::value;
       a.tiles = (int)ceil_div(rows, kTile);
-      const unsigned grid = (unsigned)(a.tiles * ceil_div(channels, L * V));
-      scan_backward_kernel<T, V, L, true><<<grid, backward_threads(L), 0, st>>>(a);
-      carry_kernel<<<(unsigned)ceil_div(channels, 128), 128, 0, st>>>(a.maps, a.carry, a.tiles, channels, 1);
-      scan_backward_kernel<T, V, L, false><<<grid, backward_threads(L), 0, st>>>(a);
+      const unsigned grid = (unsigned)((a.tiles > 0 ? a.tiles : 1) * ceil_div(channels, V * L));
+      if (a.tiles > 1) {
+        scan_backward_kernel<T, V, L, true><<<grid, kThreads, 0, st>>>(a);
+        D3D_CHECK_LAUNCH();
+        D3D_LAUNCH(true, carry_kernel, (unsigned)ceil_div(channels, kCarryChannels), kCarryThreads, 0, st, a.maps, a.carry, a.tiles,
+                   channels, 1);
+      } else {
+        a.carry = nullptr;  // nothing lies behind the only tile
+      }
+      D3D_LAUNCH(a.tiles > 1, (scan_backward_kernel<T, V, L, false>), grid, kThreads, 0, st, a);
       D3D_CHECK_LAUNCH();
       return D3D_OK;
     });
@@ -546,9 +674,9 @@ extern "C" int d3d_gated_recurrence_step(int dtype, const void* x, int64_t x_ld,
                   reinterpret_cast<uintptr_t>(gates) % esize == 0 && reinterpret_cast<uintptr_t>(out) % esize == 0,
               D3D_ERR_INVALID_ARGUMENT);
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  const bool wide = channels * esize % 16 == 0 && rows_wide(x, x_ld, esize) && rows_wide(gates, gates_ld, esize) &&
-                    rows_wide(out, channels, esize) && reinterpret_cast<uintptr_t>(state) % 16 == 0 &&
-                    reinterpret_cast<uintptr_t>(state_out) % 16 == 0;
+  auto wide_rows = [esize](const void* p, int64_t ld) { return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld * esize % 16 == 0; };
+  const bool wide = channels * esize % 16 == 0 && wide_rows(x, x_ld) && wide_rows(gates, gates_ld) && wide_rows(out, channels) && reinterpret_cast<uintptr_t>(state) % 32 == 0 &&
+                    reinterpret_cast<uintptr_t>(state_out) % 32 == 0;
   return by_type(dtype, [&](auto t) -> int {
     using T = decltype(t);
     constexpr int V = 16 / (int)sizeof(T);

@@ -8,6 +8,10 @@ import torch
 
 U32 = 2.0 ** -24
 K = 16          # half units per step of a recurrence: exp 4, quotient 4, products, sums and the composition of maps 8
+# 16-bit gates g: 1 - f = t / (1 + t), t = 2^y by the hardware's exponential, y = -g log2(e) in 32 bits.  log2(e) is rounded to
+# half a unit and so is y, each at most |y| U32, which moves t by ln 2 as much relatively: 2 |g| log2(e) ln 2 = 2 |g| half units
+# on top of the 4 of the exponential itself.
+PER_GATE = 2.0
 DEPTH = 64      # half units of a sum over channels: up to 32 terms in a thread, a tree behind it, the operations around it
 
 
@@ -79,10 +83,15 @@ def sigmoid(g):
         return np.where(g >= 0, 1 / (1 + np.exp(-np.abs(g))), np.exp(-np.abs(g)) / (1 + np.exp(-np.abs(g))))
 
 
-def recurrence(x, gates, offsets, initial, reverse):
+def half_units(gates, dtype):
+    """Half units that a step of the recurrence may be off, by gate."""
+    return K + (PER_GATE * np.abs(gates) if dtype != torch.float32 else 0.0 * gates)
+
+
+def recurrence(x, gates, offsets, initial, reverse, dtype=torch.float32):
     """h, its bound, final, its bound, h in front of every row, its bound.  Rows outside the sequences stay NaN."""
     seqs, channels = len(offsets) - 1, x.shape[1]
-    f, add = sigmoid(gates), sigmoid(-gates)
+    f, add, k = sigmoid(gates), sigmoid(-gates), half_units(gates, dtype)
     h, off, before, before_off = (np.full(x.shape, np.nan) for _ in range(4))
     final, final_off = np.zeros((seqs, channels)), np.zeros((seqs, channels))
     for s in range(seqs):
@@ -93,17 +102,17 @@ def recurrence(x, gates, offsets, initial, reverse):
             before[t], before_off[t] = c, e
             c = f[t] * c + add[t] * x[t]
             size = f[t] * size + add[t] * np.abs(x[t])
-            e = f[t] * e + U32 * K * size
+            e = f[t] * e + U32 * k[t] * size
             h[t], off[t] = c, e
         final[s], final_off[s] = c, e
     return h, off, final, final_off, before, before_off
 
 
-def recurrence_backward(grad, x, gates, offsets, initial, grad_final, reverse):
+def recurrence_backward(grad, x, gates, offsets, initial, grad_final, reverse, dtype=torch.float32):
     """(dx, bound), (dgates, bound), (dinitial, bound)."""
     seqs, channels = len(offsets) - 1, x.shape[1]
-    f, add = sigmoid(gates), sigmoid(-gates)
-    _, _, _, _, before, before_off = recurrence(x, gates, offsets, initial, reverse)
+    f, add, k = sigmoid(gates), sigmoid(-gates), half_units(gates, dtype)
+    _, _, _, _, before, before_off = recurrence(x, gates, offsets, initial, reverse, dtype)
     dx, dg, dx_off, dg_off = (np.full(x.shape, np.nan) for _ in range(4))
     di, di_off = np.zeros((seqs, channels)), np.zeros((seqs, channels))
     for s in range(seqs):
@@ -114,11 +123,11 @@ def recurrence_backward(grad, x, gates, offsets, initial, grad_final, reverse):
             delta, dsize = grad[t] + q, np.abs(grad[t]) + size
             doff = e + U32 * dsize
             dx[t] = delta * add[t]
-            dx_off[t] = add[t] * (doff + U32 * K * dsize)
+            dx_off[t] = add[t] * (doff + U32 * k[t] * dsize)
             dg[t] = delta * (before[t] - x[t]) * f[t] * add[t]
             dg_off[t] = f[t] * add[t] * (doff * np.abs(before[t] - x[t]) + dsize * before_off[t] +
-                                         U32 * K * dsize * (np.abs(before[t]) + np.abs(x[t])))
+                                         U32 * k[t] * dsize * (np.abs(before[t]) + np.abs(x[t])))
             q, size = f[t] * delta, f[t] * dsize
-            e = f[t] * doff + U32 * K * size
+            e = f[t] * doff + U32 * k[t] * size
         di[s], di_off[s] = q, e
     return (dx, dx_off), (dg, dg_off), (di, di_off)

@@ -212,7 +212,7 @@ def test_recurrence(d3d, dtype, reverse, kind, rows, channels):
     assert h is out
     x64, g64 = ref.as64(x), ref.as64(g)
     i64 = ref.as64(initial) if initial is not None else None
-    want, off, wfinal, foff, _, _ = ref.recurrence(x64, g64, offs, i64, reverse)
+    want, off, wfinal, foff, _, _ = ref.recurrence(x64, g64, offs, i64, reverse, dtype)
     inside = ~np.isnan(want[:, 0])
     assert (ref.as64(out)[~inside] == 9).all()
     lim = off + ref.half_step(dtype) * (np.abs(want) + off) + ref.smallest(dtype)
@@ -223,7 +223,7 @@ def test_recurrence(d3d, dtype, reverse, kind, rows, channels):
     assert torch.equal(plain[1], final)
     got = d3d.gated_recurrence_backward(grad, x, g, offsets, states, initial, grad_final, reverse=reverse)
     back = ref.recurrence_backward(ref.as64(grad), x64, g64, offs, i64,
-                                   ref.as64(grad_final) if grad_final is not None else None, reverse)
+                                   ref.as64(grad_final) if grad_final is not None else None, reverse, dtype)
     for t, (w, o), what in zip(got, back, ("dx", "dgates", "dinitial")):
         t = ref.as64(t)
         rnd = torch.float32 if what == "dinitial" else dtype
