@@ -57,20 +57,39 @@ template <int V> __device__ __forceinline__ Vec<V> add(const Vec<V>& a, const Ve
 }
 template <class T, int V> __device__ __forceinline__ Vec<V> widen(const Pack<T, V>& p) {
   Vec<V> r;
+  if constexpr (V == 2 && std::is_same<T, __nv_bfloat16>::value) {
+    const uint32_t w = *reinterpret_cast<const uint32_t*>(&p);
+    r.v[0] = __uint_as_float(w << 16), r.v[1] = __uint_as_float(w & 0xffff0000u);
+    return r;
+  }
+  if constexpr (V == 2 && std::is_same<T, __half>::value) {
+    const float2 t = __half22float2(*reinterpret_cast<const __half2*>(&p));
+    r.v[0] = t.x, r.v[1] = t.y;
+    return r;
+  }
 #pragma unroll
   for (int e = 0; e < V; ++e) r.v[e] = to_f32(p.v[e]);
   return r;
 }
 template <class T, int V> __device__ __forceinline__ Pack<T, V> narrow(const Vec<V>& x) {
   Pack<T, V> r;
+  if constexpr (V == 2 && std::is_same<T, __nv_bfloat16>::value) {
+    *reinterpret_cast<__nv_bfloat162*>(&r) = __float22bfloat162_rn(make_float2(x.v[0], x.v[1]));
+    return r;
+  }
+  if constexpr (V == 2 && std::is_same<T, __half>::value) {
+    *reinterpret_cast<__half2*>(&r) = __float22half2_rn(make_float2(x.v[0], x.v[1]));
+    return r;
+  }
 #pragma unroll
   for (int e = 0; e < V; ++e) r.v[e] = from_f32<T>(x.v[e]);
   return r;
 }
 
 constexpr int kTile = 128;     // rows of a tile
-constexpr int kThreads = 512;  // of a CTA
+constexpr int kThreads = 256;  // of a CTA
 constexpr int kWarps = kThreads / 32;
+constexpr int kTilesY = 32768;  // grid: slabs of channels, tiles, thousands of tiles
 
 struct ScanArgs {
   const void *x, *gates;
@@ -105,33 +124,50 @@ __device__ __forceinline__ void after(float& a, float& b, float pa, float pb) {
   if (!is_reset(a)) b = fmaf(a, pb, b), a *= pa;
 }
 
-// f = sigmoid(gate) and 1 - f, each without the cancellation that a difference to the other one would be where that is near
-// one.  Features of 32 bits: exponential and quotient to two units of the last place.  Of 16 bits: the hardware's base-two
-// exponential, whose argument is rounded to |gate| 2^-24 (so that 1 - f is off by that much, relatively; the gate itself came
-// rounded to 2^-9 or 2^-12 of it), a third of the instructions.
-template <class T, int V> __device__ __forceinline__ void gate_of(const Pack<T, V>& g, Vec<V>& f, Vec<V>& rest) {
+// f = sigmoid(gate) and 1 - f: the smaller one is t / (1 + t), t = exp(-|gate|), the other one a difference that loses nothing.
+// Neither has a sign, NaN included: the sign of a map means a reset.
+// Features of 32 bits: exponential and quotient to two units of the last place.  Of 16 bits: the hardware's base-two exponential,
+// whose argument is rounded to |gate| 2^-24 (so that 1 - f is off by that much, relatively; the gate itself came rounded to 2^-9
+// or 2^-12 of it), a third of the instructions.
+template <class T, int V> __device__ __forceinline__ Vec<V> small_of(const Vec<V>& g) {
+  Vec<V> t, r;
   if constexpr (sizeof(T) == 4) {
 #pragma unroll
-    for (int e = 0; e < V; ++e) {
-      const float x = to_f32(g.v[e]), t = expf(-fabsf(x)), small = t * __fdividef(1.f, 1.f + t), large = 1.f - small;
-      f.v[e] = fabsf(x >= 0.f ? large : small);  // NaN without a sign: the sign of a map means a reset
-      rest.v[e] = x >= 0.f ? small : large;
-    }
+    for (int e = 0; e < V; ++e) t.v[e] = expf(-fabsf(g.v[e]));
   } else {
-    Vec<V> t, r;
+    Vec<V> y;
 #pragma unroll
-    for (int e = 0; e < V; ++e) {
-      float x;  // from below -80 on f is below 2^-115: nothing is left of any state
-      asm("max.NaN.f32 %0, %1, 0fC2A00000;" : "=f"(x) : "f"(to_f32(g.v[e])));
-      t.v[e] = __expf(-x);
-    }
-    const Vec<V> d = add(t, all<V>(1.f));
+    for (int e = 0; e < V; ++e) y.v[e] = fabsf(g.v[e]);
+    y = mul(y, all<V>(-1.44269504f));
 #pragma unroll
-    for (int e = 0; e < V; ++e) asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r.v[e]) : "f"(d.v[e]));
-    rest = mul(t, r);
-    const Vec<V> large = fma(rest, all<V>(-1.f), all<V>(1.f));
+    for (int e = 0; e < V; ++e) asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(t.v[e]) : "f"(y.v[e]));
+  }
+  const Vec<V> d = add(t, all<V>(1.f));
 #pragma unroll
-    for (int e = 0; e < V; ++e) f.v[e] = fabsf(t.v[e] < 1.f ? large.v[e] : r.v[e]);
+  for (int e = 0; e < V; ++e) {
+    if constexpr (sizeof(T) == 4) r.v[e] = __fdividef(1.f, d.v[e]);
+    else asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r.v[e]) : "f"(d.v[e]));
+  }
+  return mul(t, r);
+}
+template <class T, int V> __device__ __forceinline__ void gate_of(const Vec<V>& g, Vec<V>& f, Vec<V>& rest) {
+  const Vec<V> small = small_of<T, V>(g), large = fma(small, all<V>(-1.f), all<V>(1.f));
+#pragma unroll
+  for (int e = 0; e < V; ++e) f.v[e] = g.v[e] >= 0.f ? large.v[e] : small.v[e], rest.v[e] = g.v[e] >= 0.f ? small.v[e] : large.v[e];
+}
+// Both in one number: the smaller one, with a sign where that is f.
+template <class T, int V> __device__ __forceinline__ Vec<V> folded_gate(const Vec<V>& g) {
+  Vec<V> small = small_of<T, V>(g);
+#pragma unroll
+  for (int e = 0; e < V; ++e) small.v[e] = copysignf(small.v[e], g.v[e]);
+  return small;
+}
+template <int V> __device__ __forceinline__ void open_gate(const Vec<V>& gate, Vec<V>& f, Vec<V>& rest) {
+#pragma unroll
+  for (int e = 0; e < V; ++e) {
+    const bool keeps = __float_as_int(gate.v[e]) >= 0;
+    const float small = fabsf(gate.v[e]), large = 1.f - small;
+    f.v[e] = keeps ? large : small, rest.v[e] = keeps ? small : large;
   }
 }
 
@@ -207,14 +243,18 @@ __device__ __forceinline__ void mark_ends(const ScanArgs& a, const Span& span, i
 template <int V, int kLanes> struct Place {
   static constexpr int kRows = kTile * kLanes / kThreads, kWidth = V * kLanes;
   int tile, slab, lane, group, c, rows;  // rows: of this thread that there are
-  int64_t t0, step;                      // its first row, and to the next one
+  int64_t first;                         // row of the tensors that the tile's first one would be, walked upwards
   __device__ __forceinline__ Place(const ScanArgs& a, const Span& span) {
-    const int slabs = (a.channels + kWidth - 1) / kWidth;
-    slab = blockIdx.x % slabs, tile = blockIdx.x / slabs;
+    slab = blockIdx.x, tile = blockIdx.z * kTilesY + blockIdx.y;
     lane = threadIdx.x % kLanes, group = threadIdx.x / kLanes, c = slab * kWidth + lane * V;
-    const int64_t p = (int64_t)tile * kTile + group * kRows, left = span.count - p;
+    const int64_t p = (int64_t)tile * kTile, left = span.count - p - group * kRows;
     rows = c >= a.channels || left <= 0 ? 0 : left < kRows ? (int)left : kRows;
-    t0 = row_at(a, span, p), step = a.reverse ? -1 : 1;
+    first = a.reverse ? span.begin + span.count - p - kTile : span.begin + p;
+  }
+  // Element of the thread's row r in rows `ld` apart, as an address that is the same for all threads and a distance from it.
+  template <class T> __device__ __forceinline__ T* row(T* base, int64_t ld, int r, bool reverse) const {
+    const uint32_t mine = (uint32_t)(reverse ? kTile - kRows - group * kRows : group * kRows) * (uint32_t)ld + (uint32_t)(lane * V);
+    return base + (first + (reverse ? kRows - 1 - r : r)) * ld + slab * kWidth + mine;
   }
   __device__ __forceinline__ uint32_t bits(const uint32_t* of_tile) const {
     const int at = group * kRows;
@@ -223,12 +263,10 @@ template <int V, int kLanes> struct Place {
 };
 
 template <class T, int V, int kLanes>
-__device__ __forceinline__ void load_rows(Pack<T, V> (&to)[Place<V, kLanes>::kRows], const Place<V, kLanes>& at, const void* p, int64_t ld) {
-  const T* src = (const T*)p + at.t0 * ld + at.c;
-  const int64_t step = at.step * ld;
+__device__ __forceinline__ void load_rows(Pack<T, V> (&to)[Place<V, kLanes>::kRows], const Place<V, kLanes>& at, const void* p, int64_t ld, bool reverse) {
 #pragma unroll
   for (int r = 0; r < Place<V, kLanes>::kRows; ++r)
-    if (r < at.rows) to[r] = *reinterpret_cast<const Pack<T, V>*>(src + r * step);
+    if (r < at.rows) to[r] = *reinterpret_cast<const Pack<T, V>*>(at.row((const T*)p, ld, r, reverse));
 }
 template <int V> __device__ __forceinline__ Vec<V> load_state(const float* p, int64_t s, int channels, int c) {
   Vec<V> r = all<V>(0.f);
@@ -243,14 +281,16 @@ template <int V> __device__ __forceinline__ void store_state(float* p, int64_t s
     for (int e = 0; e < V; ++e) p[s * channels + c + e] = h.v[e];
 }
 
-// Every thread brings the map of its rows; the tile's is left in `map` (by the threads of the first kWidth channels), and
-// where `into` is given every thread gets what `into` (one value per channel of the slab, or 0) becomes in front of its rows
-// (kUp) or behind them.  Two barriers.  The channels' chains over the warps are walked by one thread each: a product per warp.
-template <int V, int kLanes, bool kUp> struct Chain {
-  float2 totals[kWarps][V * kLanes];
-  float into[kWarps][V * kLanes];
+// From the maps of the threads' rows to what comes in front of them (kUp) or behind them, in three steps with a barrier after
+// each: every thread brings its map, the channels' chains over the warps are walked by a thread each (a product a warp), every
+// thread takes what comes in.  Two of them side by side: the backward pass goes both ways.
+template <int V, int kLanes, int kChains = 1> struct Chain {
+  static constexpr int kWidth = V * kLanes;
+  float2 totals[kChains][kWarps][kWidth];
+  float into[kChains][kWarps][kWidth];
 
-  __device__ __forceinline__ Vec<V> run(Vec<V> ma, Vec<V> mb, const float* carry, float2* map, const Place<V, kLanes>& at, int channels) {
+  // Afterwards the thread's map is that of its group and of those of its warp on the way to it.
+  template <bool kUp> __device__ __forceinline__ void bring_unsynced(int i, Vec<V>& ma, Vec<V>& mb, const Place<V, kLanes>& at) {
     const int lane = lane_id(), warp = threadIdx.x >> 5, col = at.lane * V;
     if constexpr (kLanes < 32)
 #pragma unroll
@@ -263,36 +303,44 @@ template <int V, int kLanes, bool kUp> struct Chain {
         }
     if (kUp ? lane >= 32 - kLanes : lane < kLanes)
 #pragma unroll
-      for (int e = 0; e < V; ++e) totals[warp][col + e] = make_float2(ma.v[e], mb.v[e]);
+      for (int e = 0; e < V; ++e) totals[i][warp][col + e] = make_float2(ma.v[e], mb.v[e]);
+  }
+  template <bool kUp> __device__ __forceinline__ void bring(int i, Vec<V>& ma, Vec<V>& mb, const Place<V, kLanes>& at) {
+    bring_unsynced<kUp>(i, ma, mb, at);
     __syncthreads();
-    const int t = threadIdx.x, c = at.slab * V * kLanes + t;
-    if (t < V * kLanes && c < channels) {
-      if (map) {
-        float a = 1.f, b = 0.f;
+  }
+  // The tile's map.
+  template <bool kUp> __device__ __forceinline__ void map(int i, float2* maps, const Place<V, kLanes>& at, int channels) const {
+    const int t = threadIdx.x, c = at.slab * kWidth + t;
+    if (t >= kWidth || c >= channels) return;
+    float a = 1.f, b = 0.f;
 #pragma unroll
-        for (int i = 0; i < kWarps; ++i) {
-          float2 m = totals[kUp ? i : kWarps - 1 - i][t];
-          after(m.x, m.y, a, b);
-          a = m.x, b = m.y;
-        }
-        map[(int64_t)at.tile * channels + c] = make_float2(a, b);
-      } else {
-        float h = carry ? __ldg(carry + (int64_t)at.tile * channels + c) : 0.f;
-#pragma unroll
-        for (int i = 0; i < kWarps; ++i) {
-          const int w = kUp ? i : kWarps - 1 - i;
-          into[w][t] = h;
-          const float2 m = totals[w][t];
-          h = apply(m.x, m.y, h);
-        }
-      }
+    for (int w = 0; w < kWarps; ++w) {
+      float2 m = totals[i][kUp ? w : kWarps - 1 - w][t];
+      after(m.x, m.y, a, b);
+      a = m.x, b = m.y;
     }
-    if (map) return all<V>(0.f);
-    __syncthreads();
+    maps[(int64_t)at.tile * channels + c] = make_float2(a, b);
+  }
+  // carry: [tiles][channels] what comes into the tile, or null for zeros.  Chain i has the threads from i * kWidth on.
+  template <bool kUp> __device__ __forceinline__ void walk(int i, const float* carry, const Place<V, kLanes>& at, int channels) {
+    const int t = (int)threadIdx.x - i * kWidth, c = at.slab * kWidth + t;
+    if (t < 0 || t >= kWidth || c >= channels) return;
+    float h = carry ? __ldg(carry + (int64_t)at.tile * channels + c) : 0.f;
+#pragma unroll
+    for (int k = 0; k < kWarps; ++k) {
+      const int w = kUp ? k : kWarps - 1 - k;
+      into[i][w][t] = h;
+      const float2 m = totals[i][w][t];
+      h = apply(m.x, m.y, h);
+    }
+  }
+  template <bool kUp> __device__ __forceinline__ Vec<V> take(int i, const Vec<V>& ma, const Vec<V>& mb, const Place<V, kLanes>& at) const {
+    const int lane = lane_id(), warp = threadIdx.x >> 5, col = at.lane * V;
     Vec<V> h;
 #pragma unroll
     for (int e = 0; e < V; ++e) {
-      h.v[e] = into[warp][col + e];
+      h.v[e] = into[i][warp][col + e];
       if constexpr (kLanes < 32) {
         const float pa = kUp ? __shfl_up_sync(0xffffffffu, ma.v[e], kLanes) : __shfl_down_sync(0xffffffffu, ma.v[e], kLanes);
         const float pb = kUp ? __shfl_up_sync(0xffffffffu, mb.v[e], kLanes) : __shfl_down_sync(0xffffffffu, mb.v[e], kLanes);
@@ -314,52 +362,69 @@ __device__ __forceinline__ void pass_empty(const ScanArgs& a, const Place<V, kLa
       for (int c = low; c < high; ++c) to[s * a.channels + c] = from ? __ldg(from + s * a.channels + c) : 0.f;
 }
 
-// kMaps: the first pass, which leaves the tile's map.
+// kMaps: the first pass, which leaves the tile's map.  Rows between two ends of sequences, all but a few, take a path without
+// the tests.
 template <class T, int V, int kLanes, bool kMaps>
-__global__ void __launch_bounds__(kThreads, 2)
+__global__ void __launch_bounds__(kThreads, kMaps ? 3 : 2)
 scan_kernel(const ScanArgs a) {
   constexpr int kRows = Place<V, kLanes>::kRows;
   using P = Pack<T, V>;
   __shared__ Marks marks;
-  __shared__ Chain<V, kLanes, true> chain;
+  __shared__ Chain<V, kLanes> chain;
   const Span span = span_of(a);
   const Place<V, kLanes> at(a, span);
+  const bool reverse = a.reverse != 0;
+  if (at.tile >= a.tiles && at.tile > 0) return;  // the last thousands of tiles are not all there
   if (kMaps) pdl_release();
   P x[kRows], g[kRows];
-  load_rows<T, V, kLanes>(x, at, a.x, a.x_ld);
-  load_rows<T, V, kLanes>(g, at, a.gates, a.gates_ld);
+  load_rows<T, V, kLanes>(x, at, a.x, a.x_ld, reverse);
+  load_rows<T, V, kLanes>(g, at, a.gates, a.gates_ld, reverse);
   mark_ends(a, span, at.tile, &marks);
   __syncthreads();
-  const uint32_t starts = at.bits(marks.first_bits);
+  const uint32_t starts = at.bits(marks.first_bits), ends = at.bits(marks.last_bits);
+  const int* first = marks.first + at.group * kRows;
+  const int* last = marks.last + at.group * kRows;
   Vec<V> f[kRows], u[kRows], ma = all<V>(1.f), mb = all<V>(0.f);
+  auto enter = [&](auto is_plain) {
+    constexpr bool kPlain = decltype(is_plain)::value;
 #pragma unroll
-  for (int r = 0; r < kRows; ++r) {
-    f[r] = all<V>(1.f), u[r] = all<V>(0.f);
-    if (r < at.rows) {
-      Vec<V> rest;
-      gate_of<T, V>(g[r], f[r], rest);
-      u[r] = mul(rest, widen<T, V>(x[r]));
-      if (starts >> r & 1) {
-        u[r] = fma(f[r], load_state<V>(a.initial, marks.first[at.group * kRows + r], a.channels, at.c), u[r]);
-        f[r] = ma = all<V>(reset_mark()), mb = u[r];
-      } else {
-        mb = fma(f[r], mb, u[r]), ma = mul(ma, f[r]);
+    for (int r = 0; r < kRows; ++r)
+      if (kPlain || r < at.rows) {
+        Vec<V> rest;
+        gate_of<T, V>(widen<T, V>(g[r]), f[r], rest);
+        u[r] = mul(rest, widen<T, V>(x[r]));
+        if (!kPlain && (starts >> r & 1)) {
+          u[r] = fma(f[r], load_state<V>(a.initial, first[r], a.channels, at.c), u[r]);
+          f[r] = ma = all<V>(reset_mark()), mb = u[r];
+        } else {
+          mb = fma(f[r], mb, u[r]), ma = mul(ma, f[r]);
+        }
       }
-    }
-  }
+  };
+  const bool plain = at.rows == kRows && starts == 0;
+  if (plain) enter(std::true_type());
+  else enter(std::false_type());
   if (!kMaps) pdl_wait();
-  Vec<V> h = chain.run(ma, mb, a.states, kMaps ? a.maps : nullptr, at, a.channels);
-  if (kMaps) return;
-  const uint32_t ends = at.bits(marks.last_bits);
-  T* out = (T*)a.out + at.t0 * a.channels + at.c;
-  const int64_t step = at.step * a.channels;
+  chain.template bring<true>(0, ma, mb, at);
+  if (kMaps) {
+    chain.template map<true>(0, a.maps, at, a.channels);
+    return;
+  }
+  chain.template walk<true>(0, a.states, at, a.channels);
+  __syncthreads();
+  Vec<V> h = chain.template take<true>(0, ma, mb, at);
+  auto leave = [&](auto is_plain) {
+    constexpr bool kPlain = decltype(is_plain)::value;
 #pragma unroll
-  for (int r = 0; r < kRows; ++r)
-    if (r < at.rows) {
-      h = starts >> r & 1 ? u[r] : fma(f[r], h, u[r]);
-      *reinterpret_cast<P*>(out + r * step) = narrow<T, V>(h);
-      if (ends >> r & 1) store_state<V>(a.final_state, marks.last[at.group * kRows + r], a.channels, at.c, h);
-    }
+    for (int r = 0; r < kRows; ++r)
+      if (kPlain || r < at.rows) {
+        h = !kPlain && (starts >> r & 1) ? u[r] : fma(f[r], h, u[r]);
+        *reinterpret_cast<P*>(at.row((T*)a.out, a.channels, r, reverse)) = narrow<T, V>(h);
+        if (!kPlain && (ends >> r & 1)) store_state<V>(a.final_state, last[r], a.channels, at.c, h);
+      }
+  };
+  if (plain && ends == 0) leave(std::true_type());
+  else leave(std::false_type());
   pass_empty<V, kLanes>(a, at, a.initial, a.final_state);
 }
 
@@ -423,78 +488,97 @@ carry_kernel(const float2* __restrict__ maps, float* __restrict__ into, int tile
 }
 
 // Backward: the rows of a tile forward once more from the state in front of it, which gives h[t-1], and the gradients from its
-// end.  The map of a row is c -> f (grad + c): c comes in from the row behind and goes out to the row in front.
+// end.  The map of a row is c -> f (grad + c): c comes in from the row behind and goes out to the row in front.  Between the
+// passes a thread holds its gates (the smaller halves), h[t-1] - x and the gradients as they came.
 template <class T, int V, int kLanes, bool kMaps>
-__global__ void __launch_bounds__(kThreads, kMaps ? 2 : 1)
+__global__ void __launch_bounds__(kThreads, kMaps ? 3 : 2)
 scan_backward_kernel(const ScanArgs a) {
   constexpr int kRows = Place<V, kLanes>::kRows;
   using P = Pack<T, V>;
   __shared__ Marks marks;
-  __shared__ Chain<V, kLanes, true> ahead;
-  __shared__ Chain<V, kLanes, false> back;
+  __shared__ Chain<V, kLanes, 2> chain;
   const Span span = span_of(a);
   const Place<V, kLanes> at(a, span);
+  const bool reverse = a.reverse != 0;
+  if (at.tile >= a.tiles && at.tile > 0) return;  // the last thousands of tiles are not all there
   if (kMaps) pdl_release();
   P x[kRows], g[kRows], d[kRows];
-  if (!kMaps) load_rows<T, V, kLanes>(x, at, a.x, a.x_ld);
-  load_rows<T, V, kLanes>(g, at, a.gates, a.gates_ld);
-  load_rows<T, V, kLanes>(d, at, a.grad, a.grad_ld);
+  if (!kMaps) load_rows<T, V, kLanes>(x, at, a.x, a.x_ld, reverse);
+  load_rows<T, V, kLanes>(g, at, a.gates, a.gates_ld, reverse);
+  load_rows<T, V, kLanes>(d, at, a.grad, a.grad_ld, reverse);
   mark_ends(a, span, at.tile, &marks);
   __syncthreads();
   const uint32_t starts = at.bits(marks.first_bits), ends = at.bits(marks.last_bits);
   const int* first = marks.first + at.group * kRows;
   const int* last = marks.last + at.group * kRows;
-  Vec<V> f[kRows], rest[kRows], before[kRows], ma, mb;
-#pragma unroll
-  for (int r = 0; r < kRows; ++r)
-    if (r < at.rows) gate_of<T, V>(g[r], f[r], rest[r]);
-  if (!kMaps) {
-    ma = all<V>(1.f), mb = all<V>(0.f);
+  const bool plain = at.rows == kRows && starts == 0 && ends == 0;
+  Vec<V> gate[kRows], away[kRows];
+  Vec<V> ma = all<V>(1.f), mb = all<V>(0.f), na = all<V>(1.f), nb = all<V>(0.f);  // forward; from the end
+  auto enter = [&](auto is_plain) {
+    constexpr bool kPlain = decltype(is_plain)::value;
 #pragma unroll
     for (int r = 0; r < kRows; ++r)
-      if (r < at.rows) {
-        const Vec<V> u = mul(rest[r], widen<T, V>(x[r]));
-        if (starts >> r & 1) {
-          ma = all<V>(reset_mark()), mb = fma(f[r], load_state<V>(a.initial, first[r], a.channels, at.c), u);
-        } else {
-          mb = fma(f[r], mb, u), ma = mul(ma, f[r]);
+      if (kPlain || r < at.rows) {
+        gate[r] = folded_gate<T, V>(widen<T, V>(g[r]));
+        Vec<V> f, rest;
+        open_gate<V>(gate[r], f, rest);
+        if (!kMaps) {
+          const Vec<V> u = mul(rest, widen<T, V>(x[r]));
+          if (!kPlain && (starts >> r & 1))
+            ma = all<V>(reset_mark()), mb = fma(f, load_state<V>(a.initial, first[r], a.channels, at.c), u);
+          else
+            mb = fma(f, mb, u), ma = mul(ma, f);
+        }
+        // the rows so far after this one: its end is what comes in
+        if (kPlain || !is_reset(na.v[0])) {
+          Vec<V> dy = widen<T, V>(d[r]);
+          const bool end = !kPlain && (ends >> r & 1);
+          if (end) dy = add(dy, load_state<V>(a.grad_final, last[r], a.channels, at.c));
+          nb = fma(mul(na, f), dy, nb);
+          na = end ? all<V>(reset_mark()) : mul(na, f);
         }
       }
-    Vec<V> h = ahead.run(ma, mb, a.states, nullptr, at, a.channels);
+  };
+  if (plain) enter(std::true_type());
+  else enter(std::false_type());
+  if (!kMaps) pdl_wait();
+  if (!kMaps) chain.template bring_unsynced<true>(0, ma, mb, at);
+  chain.template bring<false>(1, na, nb, at);
+  if (kMaps) {
+    chain.template map<false>(1, a.maps, at, a.channels);
+    return;
+  }
+  chain.template walk<true>(0, a.states, at, a.channels);
+  chain.template walk<false>(1, a.carry, at, a.channels);
+  __syncthreads();
+  Vec<V> h = chain.template take<true>(0, ma, mb, at), q = chain.template take<false>(1, na, nb, at);
+  auto leave = [&](auto is_plain) {
+    constexpr bool kPlain = decltype(is_plain)::value;
 #pragma unroll
     for (int r = 0; r < kRows; ++r)
-      if (r < at.rows) {
-        if (starts >> r & 1) h = load_state<V>(a.initial, first[r], a.channels, at.c);
-        before[r] = h;
-        h = fma(f[r], h, mul(rest[r], widen<T, V>(x[r])));
+      if (kPlain || r < at.rows) {
+        Vec<V> f, rest;
+        open_gate<V>(gate[r], f, rest);
+        if (!kPlain && (starts >> r & 1)) h = load_state<V>(a.initial, first[r], a.channels, at.c);
+        const Vec<V> in = widen<T, V>(x[r]);
+        away[r] = fma(in, all<V>(-1.f), h);
+        h = fma(f, h, mul(rest, in));
       }
-  }
-  ma = all<V>(1.f), mb = all<V>(0.f);
 #pragma unroll
-  for (int r = kRows - 1; r >= 0; --r)
-    if (r < at.rows) {
-      const Vec<V> dy = widen<T, V>(d[r]);
-      if (ends >> r & 1) {
-        ma = all<V>(reset_mark()), mb = mul(f[r], add(dy, load_state<V>(a.grad_final, last[r], a.channels, at.c)));
-      } else {
-        mb = mul(f[r], add(dy, mb)), ma = mul(ma, f[r]);
+    for (int r = kRows - 1; r >= 0; --r)
+      if (kPlain || r < at.rows) {
+        Vec<V> f, rest;
+        open_gate<V>(gate[r], f, rest);
+        if (!kPlain && (ends >> r & 1)) q = load_state<V>(a.grad_final, last[r], a.channels, at.c);
+        const Vec<V> delta = add(widen<T, V>(d[r]), q), dx = mul(delta, rest);
+        q = mul(f, delta);
+        *reinterpret_cast<P*>(at.row((T*)a.grad_x, a.channels, r, reverse)) = narrow<T, V>(dx);
+        *reinterpret_cast<P*>(at.row((T*)a.grad_gates, a.channels, r, reverse)) = narrow<T, V>(mul(mul(q, rest), away[r]));
+        if (!kPlain && (starts >> r & 1)) store_state<V>(a.grad_initial, first[r], a.channels, at.c, q);
       }
-    }
-  if (!kMaps) pdl_wait();
-  Vec<V> q = back.run(ma, mb, a.carry, kMaps ? a.maps : nullptr, at, a.channels);
-  if (kMaps) return;
-  const int64_t from = at.t0 * a.channels + at.c, step = at.step * a.channels;
-#pragma unroll
-  for (int r = kRows - 1; r >= 0; --r)
-    if (r < at.rows) {
-      if (ends >> r & 1) q = load_state<V>(a.grad_final, last[r], a.channels, at.c);
-      const Vec<V> delta = add(widen<T, V>(d[r]), q);
-      q = mul(f[r], delta);
-      const Vec<V> away = fma(widen<T, V>(x[r]), all<V>(-1.f), before[r]);
-      *reinterpret_cast<P*>((T*)a.grad_x + from + r * step) = narrow<T, V>(mul(delta, rest[r]));
-      *reinterpret_cast<P*>((T*)a.grad_gates + from + r * step) = narrow<T, V>(mul(mul(q, rest[r]), away));
-      if (starts >> r & 1) store_state<V>(a.grad_initial, first[r], a.channels, at.c, q);
-    }
+  };
+  if (plain) leave(std::true_type());
+  else leave(std::false_type());
   pass_empty<V, kLanes>(a, at, a.grad_final, a.grad_initial);
 }
 
@@ -514,7 +598,7 @@ step_kernel(const T* __restrict__ x, int64_t x_ld, const T* __restrict__ gates, 
     Vec<V> f, rest, v;
 #pragma unroll
     for (int e = 0; e < V; ++e) v.v[e] = h.v[e];
-    gate_of<T, V>(pg, f, rest);
+    gate_of<T, V>(widen<T, V>(pg), f, rest);
     v = fma(f, v, mul(rest, widen<T, V>(px)));
 #pragma unroll
     for (int e = 0; e < V; ++e) h.v[e] = v.v[e];
@@ -542,6 +626,13 @@ template <class F> int by_type(int dtype, F f) {
   }
 }
 
+constexpr int64_t kMaxPitch = 1 << 24;  // elements between rows: distances inside a tile are 32 bits
+
+dim3 grid_of(int tiles, int64_t slabs) {
+  const int n = tiles > 0 ? tiles : 1;
+  return dim3((unsigned)slabs, (unsigned)(n < kTilesY ? n : kTilesY), (unsigned)ceil_div(n, kTilesY));
+}
+
 // Whether rows of `ld` elements from `p` on can be read in pairs.
 bool rows_paired(const void* p, int64_t ld, int esize) { return reinterpret_cast<uintptr_t>(p) % (2 * esize) == 0 && ld % 2 == 0; }
 
@@ -549,6 +640,7 @@ int check_scan(int dtype, const ScanArgs& a) {
   D3D_REQUIRE(dtype == D3D_FLOAT || dtype == D3D_HALF || dtype == D3D_BF16, D3D_ERR_UNSUPPORTED_DTYPE);
   D3D_REQUIRE(a.rows >= 0 && a.channels >= 1 && a.seqs >= 0 && a.x_ld >= a.channels && a.gates_ld >= a.channels && a.offsets,
               D3D_ERR_INVALID_ARGUMENT);
+  D3D_REQUIRE(a.x_ld <= kMaxPitch && a.gates_ld <= kMaxPitch && a.grad_ld <= kMaxPitch, D3D_ERR_TOO_LARGE);
   D3D_REQUIRE(a.rows < (1ll << 31) && a.channels <= (1 << 16) &&
                   ceil_div(a.rows, kTile) * ceil_div(a.channels, 32) < (1ll << 30),
               D3D_ERR_TOO_LARGE);
@@ -597,7 +689,7 @@ extern "C" int d3d_gated_recurrence(int dtype, const void* x, int64_t x_ld, cons
     return by_shape(pairs, channels, [&](auto v, auto l) -> int {
       constexpr int V = decltype(v)::value, L = decltype(l)::value;
       a.tiles = (int)ceil_div(rows, kTile);
-      const unsigned grid = (unsigned)((a.tiles > 0 ? a.tiles : 1) * ceil_div(channels, V * L));
+      const dim3 grid = grid_of(a.tiles, ceil_div(channels, V * L));
       if (a.tiles > 1) {
         scan_kernel<T, V, L, true><<<grid, kThreads, 0, st>>>(a);
         D3D_CHECK_LAUNCH();
@@ -646,7 +738,7 @@ extern "C" int d3d_gated_recurrence_backward(int dtype, const void* grad, int64_
     return by_shape(pairs, channels, [&](auto v, auto l) -> int {
       constexpr int V = decltype(v)::value, L = decltype(l)::value;
       a.tiles = (int)ceil_div(rows, kTile);
-      const unsigned grid = (unsigned)((a.tiles > 0 ? a.tiles : 1) * ceil_div(channels, V * L));
+      const dim3 grid = grid_of(a.tiles, ceil_div(channels, V * L));
       if (a.tiles > 1) {
         scan_backward_kernel<T, V, L, true><<<grid, kThreads, 0, st>>>(a);
         D3D_CHECK_LAUNCH();
