@@ -28,7 +28,7 @@ template <int V> __device__ __forceinline__ float2 pair(const Vec<V>& a, int e) 
 template <int V> __device__ __forceinline__ Vec<V> fma(const Vec<V>& a, const Vec<V>& b, const Vec<V>& c) {
   Vec<V> r;
 #pragma unroll
-  for (int e = 0; e + 1 < V; e += 2) {
+  for (int e = 0; e < V / 2 * 2; e += 2) {
     const float2 t = __ffma2_rn(pair(a, e), pair(b, e), pair(c, e));
     r.v[e] = t.x, r.v[e + 1] = t.y;
   }
@@ -38,7 +38,7 @@ template <int V> __device__ __forceinline__ Vec<V> fma(const Vec<V>& a, const Ve
 template <int V> __device__ __forceinline__ Vec<V> mul(const Vec<V>& a, const Vec<V>& b) {
   Vec<V> r;
 #pragma unroll
-  for (int e = 0; e + 1 < V; e += 2) {
+  for (int e = 0; e < V / 2 * 2; e += 2) {
     const float2 t = __fmul2_rn(pair(a, e), pair(b, e));
     r.v[e] = t.x, r.v[e + 1] = t.y;
   }
@@ -48,7 +48,7 @@ template <int V> __device__ __forceinline__ Vec<V> mul(const Vec<V>& a, const Ve
 template <int V> __device__ __forceinline__ Vec<V> add(const Vec<V>& a, const Vec<V>& b) {
   Vec<V> r;
 #pragma unroll
-  for (int e = 0; e + 1 < V; e += 2) {
+  for (int e = 0; e < V / 2 * 2; e += 2) {
     const float2 t = __fadd2_rn(pair(a, e), pair(b, e));
     r.v[e] = t.x, r.v[e + 1] = t.y;
   }
@@ -251,11 +251,11 @@ template <int V, int kLanes> struct Place {
     rows = c >= a.channels || left <= 0 ? 0 : left < kRows ? (int)left : kRows;
     first = a.reverse ? span.begin + span.count - p - kTile : span.begin + p;
   }
-  // Element of the thread's row r in rows `ld` apart, as an address that is the same for all threads and a distance from it.
-  template <class T> __device__ __forceinline__ T* row(T* base, int64_t ld, int r, bool reverse) const {
-    const uint32_t mine = (uint32_t)(reverse ? kTile - kRows - group * kRows : group * kRows) * (uint32_t)ld + (uint32_t)(lane * V);
-    return base + (first + (reverse ? kRows - 1 - r : r)) * ld + slab * kWidth + mine;
+  // The thread's first row walked (of kRows) in rows `ld` elements apart, and the distance to the next one.
+  template <class T> __device__ __forceinline__ T* start(T* base, int64_t ld, bool reverse) const {
+    return base + (first + (reverse ? kTile - 1 - group * kRows : group * kRows)) * ld + c;
   }
+  static __device__ __forceinline__ int64_t step(int64_t ld, bool reverse) { return reverse ? -ld : ld; }
   __device__ __forceinline__ uint32_t bits(const uint32_t* of_tile) const {
     const int at = group * kRows;
     return of_tile[at >> 5] >> (at & 31) & ((1u << kRows) - 1);
@@ -264,9 +264,17 @@ template <int V, int kLanes> struct Place {
 
 template <class T, int V, int kLanes>
 __device__ __forceinline__ void load_rows(Pack<T, V> (&to)[Place<V, kLanes>::kRows], const Place<V, kLanes>& at, const void* p, int64_t ld, bool reverse) {
+  constexpr int kRows = Place<V, kLanes>::kRows;
+  const T* src = at.start((const T*)p, ld, reverse);
+  const int64_t step = at.step(ld, reverse);
+  if (at.rows == kRows) {
 #pragma unroll
-  for (int r = 0; r < Place<V, kLanes>::kRows; ++r)
-    if (r < at.rows) to[r] = *reinterpret_cast<const Pack<T, V>*>(at.row((const T*)p, ld, r, reverse));
+    for (int r = 0; r < kRows; ++r, src += step) to[r] = *reinterpret_cast<const Pack<T, V>*>(src);
+  } else {
+#pragma unroll
+    for (int r = 0; r < kRows; ++r, src += step)
+      if (r < at.rows) to[r] = *reinterpret_cast<const Pack<T, V>*>(src);
+  }
 }
 template <int V> __device__ __forceinline__ Vec<V> load_state(const float* p, int64_t s, int channels, int c) {
   Vec<V> r = all<V>(0.f);
@@ -413,13 +421,15 @@ scan_kernel(const ScanArgs a) {
   chain.template walk<true>(0, a.states, at, a.channels);
   __syncthreads();
   Vec<V> h = chain.template take<true>(0, ma, mb, at);
+  T* out = at.start((T*)a.out, a.channels, reverse);
+  const int64_t step = at.step(a.channels, reverse);
   auto leave = [&](auto is_plain) {
     constexpr bool kPlain = decltype(is_plain)::value;
 #pragma unroll
-    for (int r = 0; r < kRows; ++r)
+    for (int r = 0; r < kRows; ++r, out += step)
       if (kPlain || r < at.rows) {
         h = !kPlain && (starts >> r & 1) ? u[r] : fma(f[r], h, u[r]);
-        *reinterpret_cast<P*>(at.row((T*)a.out, a.channels, r, reverse)) = narrow<T, V>(h);
+        *reinterpret_cast<P*>(out) = narrow<T, V>(h);
         if (!kPlain && (ends >> r & 1)) store_state<V>(a.final_state, last[r], a.channels, at.c, h);
       }
   };
@@ -564,16 +574,19 @@ scan_backward_kernel(const ScanArgs a) {
         away[r] = fma(in, all<V>(-1.f), h);
         h = fma(f, h, mul(rest, in));
       }
+    const int64_t step = at.step(a.channels, reverse);
+    T* dx_at = at.start((T*)a.grad_x, a.channels, reverse) + (kRows - 1) * step;
+    T* dg_at = at.start((T*)a.grad_gates, a.channels, reverse) + (kRows - 1) * step;
 #pragma unroll
-    for (int r = kRows - 1; r >= 0; --r)
+    for (int r = kRows - 1; r >= 0; --r, dx_at -= step, dg_at -= step)
       if (kPlain || r < at.rows) {
         Vec<V> f, rest;
         open_gate<V>(gate[r], f, rest);
         if (!kPlain && (ends >> r & 1)) q = load_state<V>(a.grad_final, last[r], a.channels, at.c);
         const Vec<V> delta = add(widen<T, V>(d[r]), q), dx = mul(delta, rest);
         q = mul(f, delta);
-        *reinterpret_cast<P*>(at.row((T*)a.grad_x, a.channels, r, reverse)) = narrow<T, V>(dx);
-        *reinterpret_cast<P*>(at.row((T*)a.grad_gates, a.channels, r, reverse)) = narrow<T, V>(mul(mul(q, rest), away[r]));
+        *reinterpret_cast<P*>(dx_at) = narrow<T, V>(dx);
+        *reinterpret_cast<P*>(dg_at) = narrow<T, V>(mul(mul(q, rest), away[r]));
         if (!kPlain && (starts >> r & 1)) store_state<V>(a.grad_initial, first[r], a.channels, at.c, q);
       }
   };
@@ -626,8 +639,6 @@ template <class F> int by_type(int dtype, F f) {
   }
 }
 
-constexpr int64_t kMaxPitch = 1 << 24;  // elements between rows: distances inside a tile are 32 bits
-
 dim3 grid_of(int tiles, int64_t slabs) {
   const int n = tiles > 0 ? tiles : 1;
   return dim3((unsigned)slabs, (unsigned)(n < kTilesY ? n : kTilesY), (unsigned)ceil_div(n, kTilesY));
@@ -640,7 +651,6 @@ int check_scan(int dtype, const ScanArgs& a) {
   D3D_REQUIRE(dtype == D3D_FLOAT || dtype == D3D_HALF || dtype == D3D_BF16, D3D_ERR_UNSUPPORTED_DTYPE);
   D3D_REQUIRE(a.rows >= 0 && a.channels >= 1 && a.seqs >= 0 && a.x_ld >= a.channels && a.gates_ld >= a.channels && a.offsets,
               D3D_ERR_INVALID_ARGUMENT);
-  D3D_REQUIRE(a.x_ld <= kMaxPitch && a.gates_ld <= kMaxPitch && a.grad_ld <= kMaxPitch, D3D_ERR_TOO_LARGE);
   D3D_REQUIRE(a.rows < (1ll << 31) && a.channels <= (1 << 16) &&
                   ceil_div(a.rows, kTile) * ceil_div(a.channels, 32) < (1ll << 30),
               D3D_ERR_TOO_LARGE);

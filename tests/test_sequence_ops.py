@@ -37,7 +37,6 @@ def test_entry_points_refuse_bad_arguments(d3d):
     scan = lambda dt=F, x=ONE, g=ONE, ld=16, offs=ONE, seqs=2, rows=200, ch=16, out=ONE, ws=ONE, nb=n: \
         lib.d3d_gated_recurrence(dt, x, ld, g, 16, offs, seqs, rows, ch, 0, None, out, None, None, ws, nb, None)
     assert scan(dt=I8) == -2 and scan(nb=n - 1) == -3 and scan(seqs=0) == 0
-    assert scan(ld=(1 << 24) + 1) == -6
     assert scan(rows=1 << 31) == -6 and scan(ch=1 << 17, ld=1 << 17) == BAD
     for bad in (dict(x=None), dict(g=None), dict(offs=None), dict(ld=3), dict(seqs=-1), dict(rows=-1), dict(ch=0), dict(out=None),
                 dict(ws=None), dict(ws=ctypes.c_void_p(4100)), dict(x=odd)):
