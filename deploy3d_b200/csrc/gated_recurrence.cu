@@ -3,9 +3,9 @@
 //   delta[t] = grad[t] + f[t+1] delta[t+1]  (+ grad_final[s] at the last row),  dx = delta (1 - f),
 //   dgate = delta (h[t-1] - x) f (1 - f),  dinitial[s] = f delta at the first row
 // A row is the map c -> a c + b.  Maps compose: (a2, b2) after (a1, b1) is (a2 a1, a2 b1 + b2), so a tile of rows is one map per
-// channel, and tiles can be worked on side by side: one kernel leaves the tiles' maps, one chains them, one goes over the rows
-// again with what comes into each tile.  No kernel waits for another CTA, and every sum is made in one order.  A row that
-// starts a sequence is the map c -> b whatever c is, also where c is not finite: its a is -0, and the sign says that what came
+// channel, and tiles can be worked on side by side: one kernel leaves the tiles' maps (and, for every sixteen rows, that of the
+// tile's rows in front of them), one chains the tiles, one goes over the rows again, each sixteen on their own.  No thread of
+// it waits for another CTA, and every sum is made in one order.  A row that starts a sequence is the map c -> b whatever c is, also where c is not finite: its a is -0, and the sign says that what came
 // before is not looked at (products keep it, f is never negative).
 #include <type_traits>
 
@@ -27,31 +27,34 @@ template <int V> __device__ __forceinline__ Vec<V> all(float x) {
 template <int V> __device__ __forceinline__ float2 pair(const Vec<V>& a, int e) { return make_float2(a.v[e], a.v[e + 1]); }
 template <int V> __device__ __forceinline__ Vec<V> fma(const Vec<V>& a, const Vec<V>& b, const Vec<V>& c) {
   Vec<V> r;
+  if constexpr (V > 1)
 #pragma unroll
-  for (int e = 0; e < V / 2 * 2; e += 2) {
-    const float2 t = __ffma2_rn(pair(a, e), pair(b, e), pair(c, e));
-    r.v[e] = t.x, r.v[e + 1] = t.y;
-  }
+    for (int e = 0; e < V / 2 * 2; e += 2) {
+      const float2 t = __ffma2_rn(pair(a, e), pair(b, e), pair(c, e));
+      r.v[e] = t.x, r.v[e + 1] = t.y;
+    }
   if constexpr (V % 2) r.v[V - 1] = fmaf(a.v[V - 1], b.v[V - 1], c.v[V - 1]);
   return r;
 }
 template <int V> __device__ __forceinline__ Vec<V> mul(const Vec<V>& a, const Vec<V>& b) {
   Vec<V> r;
+  if constexpr (V > 1)
 #pragma unroll
-  for (int e = 0; e < V / 2 * 2; e += 2) {
-    const float2 t = __fmul2_rn(pair(a, e), pair(b, e));
-    r.v[e] = t.x, r.v[e + 1] = t.y;
-  }
+    for (int e = 0; e < V / 2 * 2; e += 2) {
+      const float2 t = __fmul2_rn(pair(a, e), pair(b, e));
+      r.v[e] = t.x, r.v[e + 1] = t.y;
+    }
   if constexpr (V % 2) r.v[V - 1] = a.v[V - 1] * b.v[V - 1];
   return r;
 }
 template <int V> __device__ __forceinline__ Vec<V> add(const Vec<V>& a, const Vec<V>& b) {
   Vec<V> r;
+  if constexpr (V > 1)
 #pragma unroll
-  for (int e = 0; e < V / 2 * 2; e += 2) {
-    const float2 t = __fadd2_rn(pair(a, e), pair(b, e));
-    r.v[e] = t.x, r.v[e + 1] = t.y;
-  }
+    for (int e = 0; e < V / 2 * 2; e += 2) {
+      const float2 t = __fadd2_rn(pair(a, e), pair(b, e));
+      r.v[e] = t.x, r.v[e + 1] = t.y;
+    }
   if constexpr (V % 2) r.v[V - 1] = a.v[V - 1] + b.v[V - 1];
   return r;
 }
@@ -86,7 +89,7 @@ template <class T, int V> __device__ __forceinline__ Pack<T, V> narrow(const Vec
   return r;
 }
 
-constexpr int kTile = 128;     // rows of a tile
+constexpr int kRows = 16;      // rows of a thread
 constexpr int kThreads = 256;  // of a CTA
 constexpr int kWarps = kThreads / 32;
 constexpr int kTilesY = 32768;  // grid: slabs of channels, tiles, thousands of tiles
@@ -108,10 +111,12 @@ struct ScanArgs {
   const float* grad_final;
   void *grad_x, *grad_gates;
   float* grad_initial;
-  // between the passes
-  float2* maps;   // [tiles][channels] the tile's map
-  float* states;  // [tiles][channels] h in front of the tile's first row
-  float* carry;   // [tiles][channels] backward: f delta of the row behind the tile
+  // between the kernels; a group are the kRows rows of a thread
+  float2* prefix;   // [groups][channels] map of the tile's rows in front of the group, or behind it
+  float2* maps;     // [tiles][channels] the tile's map
+  float* carry;     // [tiles][channels] what comes into the tile
+  uint4* marks;     // [groups] Marks
+  float* states;    // [rows / kRows][channels] h in front of the group, from the forward pass to the backward pass
   int tiles;
 };
 
@@ -171,110 +176,43 @@ template <int V> __device__ __forceinline__ void open_gate(const Vec<V>& gate, V
   }
 }
 
-// The rows the sequences cover, clamped to the tensor.
-struct Span {
-  int64_t begin, count;
-};
-__device__ __forceinline__ Span span_of(const ScanArgs& a) {
-  int64_t b = __ldg(a.offsets), e = __ldg(a.offsets + a.seqs);
-  b = b < 0 ? 0 : b < a.rows ? b : a.rows;
-  e = e < b ? b : e < a.rows ? e : a.rows;
-  return {b, a.seqs > 0 ? e - b : 0};
-}
-__device__ __forceinline__ int64_t row_at(const ScanArgs& a, const Span& s, int64_t p) {
-  return a.reverse ? s.begin + s.count - 1 - p : s.begin + p;
-}
-
-// Where in a tile sequences start and end, in the order the rows are walked in: a bit per row, and whose row it is.
-struct Marks {
-  uint32_t first_bits[4], last_bits[4];
-  int first[kTile], last[kTile];  // where the bit is set
-  int range[2];                   // sequences of the tile's lowest and highest row
-};
-
-// The last sequence that starts at or before row t, by a whole warp: 32 probes a step.
-__device__ __forceinline__ int sequence_of(const ScanArgs& a, int64_t t) {
-  int lo = 0, n = a.seqs;
-  while (n > 1) {
-    const int step = (n + 31) / 32, at = lo + lane_id() * step;
-    const unsigned before = __ballot_sync(0xffffffffu, at < lo + n && __ldg(a.offsets + at) <= t);
-    const int k = before ? __popc(before) - 1 : 0, end = lo + n;
-    lo += k * step;
-    if (lo > end - 1) lo = end - 1;  // offsets out of order
-    n = end - lo < step ? end - lo : step;
-  }
-  return lo;
-}
-
-// Fills `m` for the tile; the caller's barrier in front of its use of it.  Two barriers inside.
-__device__ __forceinline__ void mark_ends(const ScanArgs& a, const Span& span, int tile, Marks* m) {
-  const int64_t p0 = (int64_t)tile * kTile, n = span.count - p0 < kTile ? span.count - p0 : kTile;
-  if (n <= 0) {
-    if (threadIdx.x < 4) m->first_bits[threadIdx.x] = m->last_bits[threadIdx.x] = 0u;
-    return;  // the whole CTA
-  }
-  const int64_t low = a.reverse ? row_at(a, span, p0 + n - 1) : row_at(a, span, p0);
-  const int warp = threadIdx.x >> 5;
-  if (threadIdx.x < 4) m->first_bits[threadIdx.x] = m->last_bits[threadIdx.x] = 0u;
-  if (warp < 2) {
-    const int s = sequence_of(a, warp ? low + n - 1 : low);
-    if (lane_id() == 0) m->range[warp] = s;
-  }
-  __syncthreads();
-  const int s1 = m->range[1];
-  for (int s = m->range[0] + (int)threadIdx.x; s <= s1; s += kThreads) {
-    const int64_t b = (int64_t)__ldg(a.offsets + s) - low, e = (int64_t)__ldg(a.offsets + s + 1) - 1 - low;
-    if (e < b) continue;
-    if (b >= 0 && b < n) {
-      const int i = (int)(a.reverse ? n - 1 - b : b);
-      (a.reverse ? m->last : m->first)[i] = s;
-      atomicOr(&(a.reverse ? m->last_bits : m->first_bits)[i >> 5], 1u << (i & 31));
-    }
-    if (e >= 0 && e < n) {
-      const int i = (int)(a.reverse ? n - 1 - e : e);
-      (a.reverse ? m->first : m->last)[i] = s;
-      atomicOr(&(a.reverse ? m->first_bits : m->last_bits)[i >> 5], 1u << (i & 31));
-    }
-  }
-}
-
 // A thread's place: kLanes threads stand side by side along the channels, V channels each; the groups of them follow the rows,
-// kRows each.
+// kRows each.  Tiles lie where they lie in the tensors, whatever the sequences cover, so that nothing has to be read before the
+// rows are; walking down, they are counted from the end.
 template <int V, int kLanes> struct Place {
-  static constexpr int kRows = kTile * kLanes / kThreads, kWidth = V * kLanes;
-  int tile, slab, lane, group, c, rows;  // rows: of this thread that there are
-  int64_t first;                         // row of the tensors that the tile's first one would be, walked upwards
-  __device__ __forceinline__ Place(const ScanArgs& a, const Span& span) {
-    slab = blockIdx.x, tile = blockIdx.z * kTilesY + blockIdx.y;
+  static constexpr int kWidth = V * kLanes, kGroups = kThreads / kLanes, kTile = kGroups * kRows;
+  int tile, slab, lane, group, c, there;  // there: rows of the thread that the tensors have, a bit each
+  int64_t low;                            // the tile's lowest row
+  bool reverse;
+  __device__ __forceinline__ explicit Place(const ScanArgs& a) {
+    slab = blockIdx.x, tile = blockIdx.z * kTilesY + blockIdx.y, reverse = a.reverse != 0;
     lane = threadIdx.x % kLanes, group = threadIdx.x / kLanes, c = slab * kWidth + lane * V;
-    const int64_t p = (int64_t)tile * kTile, left = span.count - p - group * kRows;
-    rows = c >= a.channels || left <= 0 ? 0 : left < kRows ? (int)left : kRows;
-    first = a.reverse ? span.begin + span.count - p - kTile : span.begin + p;
+    low = (int64_t)(reverse ? a.tiles - 1 - tile : tile) * kTile;
+    there = c < a.channels && tile < a.tiles ? (int)span(low_row(), 0, a.rows) : 0;
   }
-  // The thread's first row walked (of kRows) in rows `ld` elements apart, and the distance to the next one.
-  template <class T> __device__ __forceinline__ T* start(T* base, int64_t ld, bool reverse) const {
-    return base + (first + (reverse ? kTile - 1 - group * kRows : group * kRows)) * ld + c;
+  __device__ __forceinline__ int64_t low_row() const { return low + (reverse ? kTile - kRows - group * kRows : group * kRows); }
+  // Of the sixteen rows from `from` on those in [begin, end), a bit each, in the order they are walked in.
+  __device__ __forceinline__ uint32_t span(int64_t from, int64_t begin, int64_t end) const {
+    const int64_t b = begin - from, e = end - from;
+    const int lo = b < 0 ? 0 : b < kRows ? (int)b : kRows, hi = e < 0 ? 0 : e < kRows ? (int)e : kRows;
+    const uint32_t up = hi > lo ? ((1u << hi) - 1) & ~((1u << lo) - 1) : 0u;
+    return reverse ? __brev(up) >> (32 - kRows) : up;
   }
-  static __device__ __forceinline__ int64_t step(int64_t ld, bool reverse) { return reverse ? -ld : ld; }
-  __device__ __forceinline__ uint32_t bits(const uint32_t* of_tile) const {
-    const int at = group * kRows;
-    return of_tile[at >> 5] >> (at & 31) & ((1u << kRows) - 1);
-  }
+  // The thread's first row walked and its address in rows `ld` elements apart, with the distance to the next one.
+  __device__ __forceinline__ int64_t first_row() const { return low_row() + (reverse ? kRows - 1 : 0); }
+  template <class T> __device__ __forceinline__ T* start(T* base, int64_t ld) const { return base + first_row() * ld + c; }
+  __device__ __forceinline__ int64_t step(int64_t ld) const { return reverse ? -ld : ld; }
+  __device__ __forceinline__ int64_t group_id() const { return (int64_t)tile * kGroups + group; }
+  __device__ __forceinline__ int64_t state_row() const { return low_row() / kRows; }  // the same for tiles of any shape
 };
 
 template <class T, int V, int kLanes>
-__device__ __forceinline__ void load_rows(Pack<T, V> (&to)[Place<V, kLanes>::kRows], const Place<V, kLanes>& at, const void* p, int64_t ld, bool reverse) {
-  constexpr int kRows = Place<V, kLanes>::kRows;
-  const T* src = at.start((const T*)p, ld, reverse);
-  const int64_t step = at.step(ld, reverse);
-  if (at.rows == kRows) {
+__device__ __forceinline__ void load_rows(Pack<T, V> (&to)[kRows], const Place<V, kLanes>& at, const void* p, int64_t ld) {
+  const T* src = at.start((const T*)p, ld);
+  const int64_t step = at.step(ld);
 #pragma unroll
-    for (int r = 0; r < kRows; ++r, src += step) to[r] = *reinterpret_cast<const Pack<T, V>*>(src);
-  } else {
-#pragma unroll
-    for (int r = 0; r < kRows; ++r, src += step)
-      if (r < at.rows) to[r] = *reinterpret_cast<const Pack<T, V>*>(src);
-  }
+  for (int r = 0; r < kRows; ++r, src += step)
+    if (at.there >> r & 1) to[r] = *reinterpret_cast<const Pack<T, V>*>(src);
 }
 template <int V> __device__ __forceinline__ Vec<V> load_state(const float* p, int64_t s, int channels, int c) {
   Vec<V> r = all<V>(0.f);
@@ -289,16 +227,79 @@ template <int V> __device__ __forceinline__ void store_state(float* p, int64_t s
     for (int e = 0; e < V; ++e) p[s * channels + c + e] = h.v[e];
 }
 
-// From the maps of the threads' rows to what comes in front of them (kUp) or behind them, in three steps with a barrier after
-// each: every thread brings its map, the channels' chains over the warps are walked by a thread each (a product a warp), every
-// thread takes what comes in.  Two of them side by side: the backward pass goes both ways.
-template <int V, int kLanes, int kChains = 1> struct Chain {
-  static constexpr int kWidth = V * kLanes;
-  float2 totals[kChains][kWarps][kWidth];
-  float into[kChains][kWarps][kWidth];
+// The last sequence that starts at or before row t, by a whole warp: 32 probes a step.
+__device__ __forceinline__ int sequence_of(const ScanArgs& a, int64_t t) {
+  int lo = 0, n = a.seqs;
+  while (n > 1) {
+    const int step = (n + 31) / 32, at = lo + lane_id() * step;
+    const unsigned before = __ballot_sync(0xffffffffu, at < lo + n && __ldg(a.offsets + at) <= t);
+    const int k = before ? __popc(before) - 1 : 0, end = lo + n;
+    lo += k * step;
+    if (lo > end - 1) lo = end - 1;  // offsets out of order
+    n = end - lo < step ? end - lo : step;
+  }
+  return lo;
+}
+// Of the marked rows of a thread, one after the other in the order they are walked in: whose they are.  s: the sequence of the
+// lowest row around.
+struct Finder {
+  int s;
+  __device__ __forceinline__ int of(const ScanArgs& a, int64_t t) {
+    while (s + 1 < a.seqs && __ldg(a.offsets + s + 1) <= t) ++s;
+    while (s > 0 && __ldg(a.offsets + s) > t) --s;
+    return s;
+  }
+};
 
-  // Afterwards the thread's map is that of its group and of those of its warp on the way to it.
-  template <bool kUp> __device__ __forceinline__ void bring_unsynced(int i, Vec<V>& ma, Vec<V>& mb, const Place<V, kLanes>& at) {
+// Which rows of a thread sequences have, and where they start and end, in the order they are walked in: a bit per row.
+struct Marks {
+  uint32_t live;  // those of the tensors that a sequence has
+  uint32_t ends;  // starts in the low half, ends in the high one
+  int owner;      // sequence of the lowest row of the warp
+  __device__ __forceinline__ bool plain(uint32_t which) const { return live == (1u << kRows) - 1 && (ends & which) == 0; }
+};
+// By every warp for its own rows, which follow one another: the sequences from that of the lowest row on, a lane each.
+template <int V, int kLanes>
+__device__ __forceinline__ Marks mark_ends(const ScanArgs& a, const Place<V, kLanes>& at) {
+  constexpr int kSpan = kRows * (32 / kLanes), kTile = Place<V, kLanes>::kTile;  // rows of a warp: 16, 32 or 64
+  const int front = (int)(threadIdx.x >> 5) * kSpan;
+  const int64_t low = at.low + (at.reverse ? kTile - front - kSpan : front);
+  const int owner = sequence_of(a, low);
+  uint32_t first[kSpan > 32 ? 2 : 1] = {}, last[kSpan > 32 ? 2 : 1] = {};
+  for (int base = owner; base < a.seqs; base += 32) {
+    const int s = base + lane_id();
+    const bool in = s < a.seqs;
+    const int64_t b = in ? (int64_t)__ldg(a.offsets + s) - low : kSpan, e = in ? (int64_t)__ldg(a.offsets + s + 1) - 1 - low : kSpan;
+    if (b <= e) {
+      if (b >= 0 && b < kSpan) first[kSpan > 32 ? (int)b >> 5 : 0] |= 1u << ((int)b & 31);
+      if (e >= 0 && e < kSpan) last[kSpan > 32 ? (int)e >> 5 : 0] |= 1u << ((int)e & 31);
+    }
+    if (__any_sync(0xffffffffu, b >= kSpan)) break;  // past the highest row
+  }
+  // of the warp's rows, upwards, to the thread's sixteen, as they are walked
+  uint64_t f = 0, l = 0;
+#pragma unroll
+  for (int w = 0; w < (kSpan > 32 ? 2 : 1); ++w) {
+    f |= (uint64_t)__reduce_or_sync(0xffffffffu, first[w]) << (32 * w);
+    l |= (uint64_t)__reduce_or_sync(0xffffffffu, last[w]) << (32 * w);
+  }
+  if (at.reverse) {
+    const uint64_t up = f;  // walking down starts where a sequence ends
+    f = __brevll(l) >> (64 - kSpan), l = __brevll(up) >> (64 - kSpan);
+  }
+  const int shift = lane_id() / kLanes * kRows;
+  const uint32_t live = at.there & at.span(at.low_row(), __ldg(a.offsets), __ldg(a.offsets + a.seqs));
+  const uint32_t starts = (uint32_t)(f >> shift) & live, ends = (uint32_t)(l >> shift) & live;
+  return {live, starts | ends << 16, owner};
+}
+
+// From the maps of the threads' rows to that of the tile and, for every thread, that of the rows of the tile in front of its own
+// (kUp) or behind them; both go to memory, with the marks.  The channels' chains over the warps are walked by a thread each.
+template <int V, int kLanes, bool kUp> struct Chain {
+  static constexpr int kWidth = V * kLanes, kGroups = kThreads / kLanes;
+  float2 totals[kWarps][kWidth];
+
+  __device__ __forceinline__ void finish(const ScanArgs& a, Vec<V> ma, Vec<V> mb, const Place<V, kLanes>& at, const Marks& marks) {
     const int lane = lane_id(), warp = threadIdx.x >> 5, col = at.lane * V;
     if constexpr (kLanes < 32)
 #pragma unroll
@@ -311,53 +312,50 @@ template <int V, int kLanes, int kChains = 1> struct Chain {
         }
     if (kUp ? lane >= 32 - kLanes : lane < kLanes)
 #pragma unroll
-      for (int e = 0; e < V; ++e) totals[i][warp][col + e] = make_float2(ma.v[e], mb.v[e]);
-  }
-  template <bool kUp> __device__ __forceinline__ void bring(int i, Vec<V>& ma, Vec<V>& mb, const Place<V, kLanes>& at) {
-    bring_unsynced<kUp>(i, ma, mb, at);
+      for (int e = 0; e < V; ++e) totals[warp][col + e] = make_float2(ma.v[e], mb.v[e]);
+    if (at.slab == 0 && at.lane == 0) a.marks[at.group_id()] = make_uint4(marks.live, marks.ends, (uint32_t)marks.owner, 0u);
     __syncthreads();
-  }
-  // The tile's map.
-  template <bool kUp> __device__ __forceinline__ void map(int i, float2* maps, const Place<V, kLanes>& at, int channels) const {
     const int t = threadIdx.x, c = at.slab * kWidth + t;
-    if (t >= kWidth || c >= channels) return;
-    float a = 1.f, b = 0.f;
+    if (t < kWidth && c < a.channels) {
+      float pa = 1.f, pb = 0.f;
+      float2* to = a.prefix + (int64_t)at.tile * kGroups * a.channels + c;
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
-      float2 m = totals[i][kUp ? w : kWarps - 1 - w][t];
-      after(m.x, m.y, a, b);
-      a = m.x, b = m.y;
+      for (int i = 0; i < kWarps; ++i) {
+        const int w = kUp ? i : kWarps - 1 - i;
+        float2 m = totals[w][t];
+        if constexpr (kLanes == 32) to[w * a.channels] = make_float2(pa, pb);
+        else totals[w][t] = make_float2(pa, pb);
+        after(m.x, m.y, pa, pb);
+        pa = m.x, pb = m.y;
+      }
+      a.maps[(int64_t)at.tile * a.channels + c] = make_float2(pa, pb);
     }
-    maps[(int64_t)at.tile * channels + c] = make_float2(a, b);
-  }
-  // carry: [tiles][channels] what comes into the tile, or null for zeros.  Chain i has the threads from i * kWidth on.
-  template <bool kUp> __device__ __forceinline__ void walk(int i, const float* carry, const Place<V, kLanes>& at, int channels) {
-    const int t = (int)threadIdx.x - i * kWidth, c = at.slab * kWidth + t;
-    if (t < 0 || t >= kWidth || c >= channels) return;
-    float h = carry ? __ldg(carry + (int64_t)at.tile * channels + c) : 0.f;
+    if constexpr (kLanes < 32) {  // several groups in a warp
+      __syncthreads();
 #pragma unroll
-    for (int k = 0; k < kWarps; ++k) {
-      const int w = kUp ? k : kWarps - 1 - k;
-      into[i][w][t] = h;
-      const float2 m = totals[i][w][t];
-      h = apply(m.x, m.y, h);
-    }
-  }
-  template <bool kUp> __device__ __forceinline__ Vec<V> take(int i, const Vec<V>& ma, const Vec<V>& mb, const Place<V, kLanes>& at) const {
-    const int lane = lane_id(), warp = threadIdx.x >> 5, col = at.lane * V;
-    Vec<V> h;
-#pragma unroll
-    for (int e = 0; e < V; ++e) {
-      h.v[e] = into[i][warp][col + e];
-      if constexpr (kLanes < 32) {
-        const float pa = kUp ? __shfl_up_sync(0xffffffffu, ma.v[e], kLanes) : __shfl_down_sync(0xffffffffu, ma.v[e], kLanes);
-        const float pb = kUp ? __shfl_up_sync(0xffffffffu, mb.v[e], kLanes) : __shfl_down_sync(0xffffffffu, mb.v[e], kLanes);
-        if (kUp ? lane >= kLanes : lane + kLanes < 32) h.v[e] = apply(pa, pb, h.v[e]);
+      for (int e = 0; e < V; ++e) {
+        float pa = kUp ? __shfl_up_sync(0xffffffffu, ma.v[e], kLanes) : __shfl_down_sync(0xffffffffu, ma.v[e], kLanes);
+        float pb = kUp ? __shfl_up_sync(0xffffffffu, mb.v[e], kLanes) : __shfl_down_sync(0xffffffffu, mb.v[e], kLanes);
+        const float2 front = totals[warp][col + e];
+        if (kUp ? lane >= kLanes : lane + kLanes < 32) after(pa, pb, front.x, front.y);
+        else pa = front.x, pb = front.y;
+        if (at.c < a.channels) a.prefix[at.group_id() * a.channels + at.c + e] = make_float2(pa, pb);
       }
     }
-    return h;
   }
 };
+
+// What comes into the thread's rows: the tile's rows on the way, after what comes into the tile.
+template <int V, int kLanes>
+__device__ __forceinline__ Vec<V> incoming(const ScanArgs& a, const Place<V, kLanes>& at) {
+  Vec<V> h = all<V>(0.f);
+#pragma unroll
+  for (int e = 0; e < V; ++e) {
+    const float2 m = __ldcg(a.prefix + at.group_id() * a.channels + at.c + e);
+    h.v[e] = apply(m.x, m.y, a.carry ? __ldcg(a.carry + (int64_t)at.tile * a.channels + at.c + e) : 0.f);
+  }
+  return h;
+}
 
 // Sequences without rows: their last state is the one they start with.
 template <int V, int kLanes>
@@ -370,96 +368,71 @@ __device__ __forceinline__ void pass_empty(const ScanArgs& a, const Place<V, kLa
       for (int c = low; c < high; ++c) to[s * a.channels + c] = from ? __ldg(from + s * a.channels + c) : 0.f;
 }
 
-// kMaps: the first pass, which leaves the tile's map.  Rows between two ends of sequences, all but a few, take a path without
-// the tests.
-template <class T, int V, int kLanes, bool kMaps>
-__global__ void __launch_bounds__(kThreads, kMaps ? 3 : 2)
-scan_kernel(const ScanArgs a) {
-  constexpr int kRows = Place<V, kLanes>::kRows;
-  using P = Pack<T, V>;
-  __shared__ Marks marks;
-  __shared__ Chain<V, kLanes> chain;
-  const Span span = span_of(a);
-  const Place<V, kLanes> at(a, span);
-  const bool reverse = a.reverse != 0;
-  if (at.tile >= a.tiles && at.tile > 0) return;  // the last thousands of tiles are not all there
-  if (kMaps) pdl_release();
-  P x[kRows], g[kRows];
-  load_rows<T, V, kLanes>(x, at, a.x, a.x_ld, reverse);
-  load_rows<T, V, kLanes>(g, at, a.gates, a.gates_ld, reverse);
-  mark_ends(a, span, at.tile, &marks);
-  __syncthreads();
-  const uint32_t starts = at.bits(marks.first_bits), ends = at.bits(marks.last_bits);
-  const int* first = marks.first + at.group * kRows;
-  const int* last = marks.last + at.group * kRows;
-  Vec<V> f[kRows], u[kRows], ma = all<V>(1.f), mb = all<V>(0.f);
+// First kernel: maps.  Rows between two ends of sequences, all but a few, take a path without the tests, here and below.
+template <class T, int V, int kLanes>
+__global__ void __launch_bounds__(kThreads, 4)
+scan_maps_kernel(const ScanArgs a) {
+  __shared__ Chain<V, kLanes, true> chain;
+  const Place<V, kLanes> at(a);
+  if (at.tile >= a.tiles) return;  // the last thousands of tiles are not all there
+  pdl_release();
+  Pack<T, V> x[kRows], g[kRows];
+  load_rows<T, V, kLanes>(x, at, a.x, a.x_ld);
+  load_rows<T, V, kLanes>(g, at, a.gates, a.gates_ld);
+  const Marks marks = mark_ends(a, at);
+  Vec<V> ma = all<V>(1.f), mb = all<V>(0.f);
   auto enter = [&](auto is_plain) {
     constexpr bool kPlain = decltype(is_plain)::value;
+    Finder find = {marks.owner};
+    const int64_t t = at.first_row(), step = at.step(1);
 #pragma unroll
     for (int r = 0; r < kRows; ++r)
-      if (kPlain || r < at.rows) {
-        Vec<V> rest;
-        gate_of<T, V>(widen<T, V>(g[r]), f[r], rest);
-        u[r] = mul(rest, widen<T, V>(x[r]));
-        if (!kPlain && (starts >> r & 1)) {
-          u[r] = fma(f[r], load_state<V>(a.initial, first[r], a.channels, at.c), u[r]);
-          f[r] = ma = all<V>(reset_mark()), mb = u[r];
+      if (kPlain || (marks.live >> r & 1)) {
+        Vec<V> f, rest;
+        gate_of<T, V>(widen<T, V>(g[r]), f, rest);
+        const Vec<V> u = mul(rest, widen<T, V>(x[r]));
+        if (!kPlain && (marks.ends >> r & 1)) {
+          mb = fma(f, load_state<V>(a.initial, find.of(a, t + r * step), a.channels, at.c), u);
+          ma = all<V>(reset_mark());
         } else {
-          mb = fma(f[r], mb, u[r]), ma = mul(ma, f[r]);
+          mb = fma(f, mb, u), ma = mul(ma, f);
         }
       }
   };
-  const bool plain = at.rows == kRows && starts == 0;
-  if (plain) enter(std::true_type());
+  if (marks.plain(0xffffu)) enter(std::true_type());
   else enter(std::false_type());
-  if (!kMaps) pdl_wait();
-  chain.template bring<true>(0, ma, mb, at);
-  if (kMaps) {
-    chain.template map<true>(0, a.maps, at, a.channels);
-    return;
-  }
-  chain.template walk<true>(0, a.states, at, a.channels);
-  __syncthreads();
-  Vec<V> h = chain.template take<true>(0, ma, mb, at);
-  T* out = at.start((T*)a.out, a.channels, reverse);
-  const int64_t step = at.step(a.channels, reverse);
-  auto leave = [&](auto is_plain) {
-    constexpr bool kPlain = decltype(is_plain)::value;
-#pragma unroll
-    for (int r = 0; r < kRows; ++r, out += step)
-      if (kPlain || r < at.rows) {
-        h = !kPlain && (starts >> r & 1) ? u[r] : fma(f[r], h, u[r]);
-        *reinterpret_cast<P*>(out) = narrow<T, V>(h);
-        if (!kPlain && (ends >> r & 1)) store_state<V>(a.final_state, last[r], a.channels, at.c, h);
-      }
-  };
-  if (plain && ends == 0) leave(std::true_type());
-  else leave(std::false_type());
-  pass_empty<V, kLanes>(a, at, a.initial, a.final_state);
+  chain.finish(a, ma, mb, at, marks);
 }
 
-// What comes into each tile: the tiles' maps one after the other, from the first (or, backwards, the last) on.  Eight channels to
-// a CTA; 128 threads of each take kHeld tiles into registers, chain them, and are chained by shuffles and through shared memory.
-constexpr int kHeld = 8, kCarryThreads = 1024, kCarryChannels = 8;
+// What comes into each tile: the tiles' maps one after the other, from the first (or, backwards, the last) on.  Two channels to a
+// CTA; 256 threads of each take kHeld tiles into registers, chain them, and are chained by shuffles and through shared memory.
+constexpr int kHeld = 16, kCarryThreads = 512, kCarryChannels = 2, kCarryWarps = kCarryThreads / 32;
 __global__ void __launch_bounds__(kCarryThreads)
 carry_kernel(const float2* __restrict__ maps, float* __restrict__ into, int tiles, int channels, int backward) {
-  __shared__ float2 totals[32][kCarryChannels];
-  __shared__ float starts[32][kCarryChannels];
+  __shared__ float2 totals[kCarryWarps][kCarryChannels];
+  __shared__ float starts[kCarryWarps][kCarryChannels];
   const int lane = lane_id(), warp = threadIdx.x >> 5, ch = threadIdx.x % kCarryChannels, c = blockIdx.x * kCarryChannels + ch;
   const int segment = threadIdx.x / kCarryChannels;
   pdl_release();
   pdl_wait();
   float carry = 0.f;  // of channel `warp` of this CTA, in the warps that chain
   constexpr int kTurn = kCarryThreads / kCarryChannels * kHeld;
+  float2 next[kHeld];
+  auto load = [&](int t0) {
+#pragma unroll
+    for (int i = 0; i < kHeld; ++i) {
+      const int t = t0 + segment * kHeld + i;
+      next[i] = make_float2(1.f, 0.f);
+      if (t < tiles && c < channels) next[i] = __ldcg(maps + (int64_t)(backward ? tiles - 1 - t : t) * channels + c);
+    }
+  };
+  load(0);
   for (int t0 = 0; t0 < tiles; t0 += kTurn) {
     float2 m[kHeld];
     float a = 1.f, b = 0.f;
 #pragma unroll
-    for (int i = 0; i < kHeld; ++i) {
-      const int t = t0 + segment * kHeld + i;
-      m[i] = make_float2(1.f, 0.f);
-      if (t < tiles && c < channels) m[i] = __ldg(maps + (int64_t)(backward ? tiles - 1 - t : t) * channels + c);
-    }
+    for (int i = 0; i < kHeld; ++i) m[i] = next[i];
+    if (t0 + kTurn < tiles) load(t0 + kTurn);
 #pragma unroll
     for (int i = 0; i < kHeld; ++i) {
       float na = m[i].x, nb = m[i].y;
@@ -474,15 +447,15 @@ carry_kernel(const float2* __restrict__ maps, float* __restrict__ into, int tile
     if (lane >= 32 - kCarryChannels) totals[warp][ch] = make_float2(a, b);
     __syncthreads();
     if (warp < kCarryChannels) {  // a warp per channel, a lane per warp's total
-      float2 w = totals[lane][warp];
+      float2 w = lane < kCarryWarps ? totals[lane][warp] : make_float2(1.f, 0.f);
 #pragma unroll
-      for (int d = 1; d < 32; d <<= 1) {
+      for (int d = 1; d < kCarryWarps; d <<= 1) {
         const float pa = __shfl_up_sync(0xffffffffu, w.x, d), pb = __shfl_up_sync(0xffffffffu, w.y, d);
         if (lane >= d) after(w.x, w.y, pa, pb);
       }
       const float end = apply(w.x, w.y, carry), before = __shfl_up_sync(0xffffffffu, end, 1);
-      starts[lane][warp] = lane ? before : carry;
-      carry = __shfl_sync(0xffffffffu, end, 31);
+      if (lane < kCarryWarps) starts[lane][warp] = lane ? before : carry;
+      carry = __shfl_sync(0xffffffffu, end, kCarryWarps - 1);
     }
     __syncthreads();
     float h = starts[warp][ch];
@@ -497,101 +470,129 @@ carry_kernel(const float2* __restrict__ maps, float* __restrict__ into, int tile
   }
 }
 
-// Backward: the rows of a tile forward once more from the state in front of it, which gives h[t-1], and the gradients from its
-// end.  The map of a row is c -> f (grad + c): c comes in from the row behind and goes out to the row in front.  Between the
-// passes a thread holds its gates (the smaller halves), h[t-1] - x and the gradients as they came.
-template <class T, int V, int kLanes, bool kMaps>
-__global__ void __launch_bounds__(kThreads, kMaps ? 3 : 2)
-scan_backward_kernel(const ScanArgs a) {
-  constexpr int kRows = Place<V, kLanes>::kRows;
-  using P = Pack<T, V>;
-  __shared__ Marks marks;
-  __shared__ Chain<V, kLanes, 2> chain;
-  const Span span = span_of(a);
-  const Place<V, kLanes> at(a, span);
-  const bool reverse = a.reverse != 0;
-  if (at.tile >= a.tiles && at.tile > 0) return;  // the last thousands of tiles are not all there
-  if (kMaps) pdl_release();
-  P x[kRows], g[kRows], d[kRows];
-  if (!kMaps) load_rows<T, V, kLanes>(x, at, a.x, a.x_ld, reverse);
-  load_rows<T, V, kLanes>(g, at, a.gates, a.gates_ld, reverse);
-  load_rows<T, V, kLanes>(d, at, a.grad, a.grad_ld, reverse);
-  mark_ends(a, span, at.tile, &marks);
-  __syncthreads();
-  const uint32_t starts = at.bits(marks.first_bits), ends = at.bits(marks.last_bits);
-  const int* first = marks.first + at.group * kRows;
-  const int* last = marks.last + at.group * kRows;
-  const bool plain = at.rows == kRows && starts == 0 && ends == 0;
-  Vec<V> gate[kRows], away[kRows];
-  Vec<V> ma = all<V>(1.f), mb = all<V>(0.f), na = all<V>(1.f), nb = all<V>(0.f);  // forward; from the end
+// Last kernel: the rows, each thread its own from what comes into them.  No thread waits for another.
+template <class T, int V, int kLanes>
+__global__ void __launch_bounds__(kThreads, 4)
+scan_rows_kernel(const ScanArgs a) {
+  const Place<V, kLanes> at(a);
+  Pack<T, V> x[kRows], g[kRows];
+  load_rows<T, V, kLanes>(x, at, a.x, a.x_ld);
+  load_rows<T, V, kLanes>(g, at, a.gates, a.gates_ld);
+  pdl_wait();
+  if (at.there) {
+    const uint4 word = __ldcg(a.marks + at.group_id());
+    const Marks marks = {word.x & (uint32_t)at.there, word.y, (int)word.z};
+    Vec<V> h = incoming<V, kLanes>(a, at);
+    store_state<V>(a.states, at.state_row(), a.channels, at.c, h);
+    T* out = at.start((T*)a.out, a.channels);
+    const int64_t step = at.step(a.channels);
+    auto walk = [&](auto is_plain) {
+      constexpr bool kPlain = decltype(is_plain)::value;
+      Finder find = {marks.owner};
+      const int64_t t = at.first_row(), next = at.step(1);
+#pragma unroll
+      for (int r = 0; r < kRows; ++r, out += step)
+        if (kPlain || (marks.live >> r & 1)) {
+          if (!kPlain && (marks.ends >> r & 1)) h = load_state<V>(a.initial, find.of(a, t + r * next), a.channels, at.c);
+          Vec<V> f, rest;
+          gate_of<T, V>(widen<T, V>(g[r]), f, rest);
+          h = fma(f, h, mul(rest, widen<T, V>(x[r])));
+          *reinterpret_cast<Pack<T, V>*>(out) = narrow<T, V>(h);
+          if (!kPlain && (marks.ends >> (r + 16) & 1)) store_state<V>(a.final_state, find.of(a, t + r * next), a.channels, at.c, h);
+        }
+    };
+    if (marks.plain(~0u)) walk(std::true_type());
+    else walk(std::false_type());
+  }
+  pass_empty<V, kLanes>(a, at, a.initial, a.final_state);
+}
+
+// Backward: gradients are carried from the end.  The map of a row is c -> f (grad + c): c comes in from the row behind and goes out
+// to the row in front.
+template <class T, int V, int kLanes>
+__global__ void __launch_bounds__(kThreads, 4)
+scan_backward_maps_kernel(const ScanArgs a) {
+  __shared__ Chain<V, kLanes, false> chain;
+  const Place<V, kLanes> at(a);
+  if (at.tile >= a.tiles) return;
+  pdl_release();
+  Pack<T, V> g[kRows], d[kRows];
+  load_rows<T, V, kLanes>(g, at, a.gates, a.gates_ld);
+  load_rows<T, V, kLanes>(d, at, a.grad, a.grad_ld);
+  const Marks marks = mark_ends(a, at);
+  Vec<V> ma = all<V>(1.f), mb = all<V>(0.f);
   auto enter = [&](auto is_plain) {
     constexpr bool kPlain = decltype(is_plain)::value;
+    Finder find = {marks.owner};
+    const int64_t t = at.first_row(), step = at.step(1);
 #pragma unroll
-    for (int r = 0; r < kRows; ++r)
-      if (kPlain || r < at.rows) {
-        gate[r] = folded_gate<T, V>(widen<T, V>(g[r]));
+    for (int r = kRows - 1; r >= 0; --r)
+      if (kPlain || (marks.live >> r & 1)) {
         Vec<V> f, rest;
-        open_gate<V>(gate[r], f, rest);
-        if (!kMaps) {
-          const Vec<V> u = mul(rest, widen<T, V>(x[r]));
-          if (!kPlain && (starts >> r & 1))
-            ma = all<V>(reset_mark()), mb = fma(f, load_state<V>(a.initial, first[r], a.channels, at.c), u);
-          else
-            mb = fma(f, mb, u), ma = mul(ma, f);
-        }
-        // the rows so far after this one: its end is what comes in
-        if (kPlain || !is_reset(na.v[0])) {
-          Vec<V> dy = widen<T, V>(d[r]);
-          const bool end = !kPlain && (ends >> r & 1);
-          if (end) dy = add(dy, load_state<V>(a.grad_final, last[r], a.channels, at.c));
-          nb = fma(mul(na, f), dy, nb);
-          na = end ? all<V>(reset_mark()) : mul(na, f);
+        gate_of<T, V>(widen<T, V>(g[r]), f, rest);
+        const Vec<V> dy = widen<T, V>(d[r]);
+        if (!kPlain && (marks.ends >> (r + 16) & 1)) {
+          mb = mul(f, add(dy, load_state<V>(a.grad_final, find.of(a, t + r * step), a.channels, at.c)));
+          ma = all<V>(reset_mark());
+        } else {
+          mb = mul(f, add(dy, mb)), ma = mul(ma, f);
         }
       }
   };
-  if (plain) enter(std::true_type());
+  if (marks.plain(0xffff0000u)) enter(std::true_type());
   else enter(std::false_type());
-  if (!kMaps) pdl_wait();
-  if (!kMaps) chain.template bring_unsynced<true>(0, ma, mb, at);
-  chain.template bring<false>(1, na, nb, at);
-  if (kMaps) {
-    chain.template map<false>(1, a.maps, at, a.channels);
-    return;
+  chain.finish(a, ma, mb, at, marks);
+}
+
+// The rows forward once more from the state in front of them, which gives h[t-1] - x, then back with the gradients.
+template <class T, int V, int kLanes>
+__global__ void __launch_bounds__(kThreads, 2)
+scan_backward_rows_kernel(const ScanArgs a) {
+  const Place<V, kLanes> at(a);
+  Pack<T, V> x[kRows], g[kRows], d[kRows];
+  load_rows<T, V, kLanes>(x, at, a.x, a.x_ld);
+  load_rows<T, V, kLanes>(g, at, a.gates, a.gates_ld);
+  load_rows<T, V, kLanes>(d, at, a.grad, a.grad_ld);
+  pdl_wait();
+  if (at.there) {
+    const uint4 word = __ldcg(a.marks + at.group_id());
+    const Marks marks = {word.x & (uint32_t)at.there, word.y, (int)word.z};
+    Vec<V> q = incoming<V, kLanes>(a, at), h = load_state<V>(a.states, at.state_row(), a.channels, at.c);
+    const int64_t step = at.step(a.channels);
+    T* dx_at = at.start((T*)a.grad_x, a.channels) + (kRows - 1) * step;
+    T* dg_at = at.start((T*)a.grad_gates, a.channels) + (kRows - 1) * step;
+    auto walk = [&](auto is_plain) {
+      constexpr bool kPlain = decltype(is_plain)::value;
+      Finder find = {marks.owner};
+      const int64_t t = at.first_row(), next = at.step(1);
+      Vec<V> gate[kRows], away[kRows];
+#pragma unroll
+      for (int r = 0; r < kRows; ++r)
+        if (kPlain || (marks.live >> r & 1)) {
+          gate[r] = folded_gate<T, V>(widen<T, V>(g[r]));
+          Vec<V> f, rest;
+          open_gate<V>(gate[r], f, rest);
+          if (!kPlain && (marks.ends >> r & 1)) h = load_state<V>(a.initial, find.of(a, t + r * next), a.channels, at.c);
+          const Vec<V> in = widen<T, V>(x[r]);
+          away[r] = fma(in, all<V>(-1.f), h);
+          h = fma(f, h, mul(rest, in));
+        }
+#pragma unroll
+      for (int r = kRows - 1; r >= 0; --r, dx_at -= step, dg_at -= step)
+        if (kPlain || (marks.live >> r & 1)) {
+          Vec<V> f, rest;
+          open_gate<V>(gate[r], f, rest);
+          if (!kPlain && (marks.ends >> (r + 16) & 1)) q = load_state<V>(a.grad_final, find.of(a, t + r * next), a.channels, at.c);
+          const Vec<V> delta = add(widen<T, V>(d[r]), q), dx = mul(delta, rest);
+          q = mul(f, delta);
+          *reinterpret_cast<Pack<T, V>*>(dx_at) = narrow<T, V>(dx);
+          *reinterpret_cast<Pack<T, V>*>(dg_at) = narrow<T, V>(mul(mul(q, rest), away[r]));
+          if (!kPlain && (marks.ends >> r & 1)) store_state<V>(a.grad_initial, find.of(a, t + r * next), a.channels, at.c, q);
+        }
+    };
+    if (marks.plain(~0u)) walk(std::true_type());
+    else walk(std::false_type());
   }
-  chain.template walk<true>(0, a.states, at, a.channels);
-  chain.template walk<false>(1, a.carry, at, a.channels);
-  __syncthreads();
-  Vec<V> h = chain.template take<true>(0, ma, mb, at), q = chain.template take<false>(1, na, nb, at);
-  auto leave = [&](auto is_plain) {
-    constexpr bool kPlain = decltype(is_plain)::value;
-#pragma unroll
-    for (int r = 0; r < kRows; ++r)
-      if (kPlain || r < at.rows) {
-        Vec<V> f, rest;
-        open_gate<V>(gate[r], f, rest);
-        if (!kPlain && (starts >> r & 1)) h = load_state<V>(a.initial, first[r], a.channels, at.c);
-        const Vec<V> in = widen<T, V>(x[r]);
-        away[r] = fma(in, all<V>(-1.f), h);
-        h = fma(f, h, mul(rest, in));
-      }
-    const int64_t step = at.step(a.channels, reverse);
-    T* dx_at = at.start((T*)a.grad_x, a.channels, reverse) + (kRows - 1) * step;
-    T* dg_at = at.start((T*)a.grad_gates, a.channels, reverse) + (kRows - 1) * step;
-#pragma unroll
-    for (int r = kRows - 1; r >= 0; --r, dx_at -= step, dg_at -= step)
-      if (kPlain || r < at.rows) {
-        Vec<V> f, rest;
-        open_gate<V>(gate[r], f, rest);
-        if (!kPlain && (ends >> r & 1)) q = load_state<V>(a.grad_final, last[r], a.channels, at.c);
-        const Vec<V> delta = add(widen<T, V>(d[r]), q), dx = mul(delta, rest);
-        q = mul(f, delta);
-        *reinterpret_cast<P*>(dx_at) = narrow<T, V>(dx);
-        *reinterpret_cast<P*>(dg_at) = narrow<T, V>(mul(mul(q, rest), away[r]));
-        if (!kPlain && (starts >> r & 1)) store_state<V>(a.grad_initial, first[r], a.channels, at.c, q);
-      }
-  };
-  if (plain) leave(std::true_type());
-  else leave(std::false_type());
   pass_empty<V, kLanes>(a, at, a.grad_final, a.grad_initial);
 }
 
@@ -620,14 +621,20 @@ step_kernel(const T* __restrict__ x, int64_t x_ld, const T* __restrict__ gates, 
   }
 }
 
-// f(V, lanes) for the tile shape of this many channels: two channels a thread where rows can be read so, and as few threads side
-// by side as cover the channels.
-template <class F> int by_shape(bool pairs, int channels, F f) {
+// f(V, lanes) for the tile shape: of 16-bit features two channels a thread where rows can be read so, else one, and as few threads
+// side by side as cover the channels.
+template <class T, class F> int by_shape(bool pairs, int channels, F f) {
 #define D3D_SCAN_SHAPE(V, L) return f(std::integral_constant<int, V>(), std::integral_constant<int, L>())
-  if (!pairs) D3D_SCAN_SHAPE(1, 32);
-  if (channels <= 16) D3D_SCAN_SHAPE(2, 8);
-  if (channels <= 32) D3D_SCAN_SHAPE(2, 16);
-  D3D_SCAN_SHAPE(2, 32);
+  if constexpr (sizeof(T) == 2) {
+    if (pairs) {
+      if (channels <= 16) D3D_SCAN_SHAPE(2, 8);
+      if (channels <= 32) D3D_SCAN_SHAPE(2, 16);
+      D3D_SCAN_SHAPE(2, 32);
+    }
+  }
+  if (channels <= 8) D3D_SCAN_SHAPE(1, 8);
+  if (channels <= 16) D3D_SCAN_SHAPE(1, 16);
+  D3D_SCAN_SHAPE(1, 32);
 #undef D3D_SCAN_SHAPE
 }
 template <class F> int by_type(int dtype, F f) {
@@ -651,13 +658,38 @@ int check_scan(int dtype, const ScanArgs& a) {
   D3D_REQUIRE(dtype == D3D_FLOAT || dtype == D3D_HALF || dtype == D3D_BF16, D3D_ERR_UNSUPPORTED_DTYPE);
   D3D_REQUIRE(a.rows >= 0 && a.channels >= 1 && a.seqs >= 0 && a.x_ld >= a.channels && a.gates_ld >= a.channels && a.offsets,
               D3D_ERR_INVALID_ARGUMENT);
-  D3D_REQUIRE(a.rows < (1ll << 31) && a.channels <= (1 << 16) &&
-                  ceil_div(a.rows, kTile) * ceil_div(a.channels, 32) < (1ll << 30),
-              D3D_ERR_TOO_LARGE);
+  D3D_REQUIRE(a.rows < (1ll << 31) && a.channels <= (1 << 16), D3D_ERR_TOO_LARGE);
   const int esize = (int)dtype_size(dtype);
   D3D_REQUIRE(reinterpret_cast<uintptr_t>(a.x) % esize == 0 && reinterpret_cast<uintptr_t>(a.gates) % esize == 0 &&
                   reinterpret_cast<uintptr_t>(a.grad) % esize == 0,
               D3D_ERR_INVALID_ARGUMENT);
+  return D3D_OK;
+}
+
+// Between the kernels, sized for the smallest tiles and for whole ones of any shape.
+constexpr int kSmallTile = kWarps * kRows, kMostGroups = kThreads / 8;
+void carve(ScanArgs& a, Carver& w) {
+  const size_t groups = (size_t)ceil_div(a.rows, kRows) + kMostGroups, tiles = (size_t)ceil_div(a.rows, kSmallTile) + 1;
+  a.prefix = w.take<float2>(groups * a.channels);
+  a.maps = w.take<float2>(tiles * a.channels);
+  a.carry = w.take<float>(tiles * a.channels);
+  a.marks = w.take<uint4>(groups);
+}
+
+// The three kernels of a pass.  One tile: nothing comes into it.
+template <class Maps, class Rows> int launch_pass(ScanArgs a, int tile, int width, Maps maps, Rows rows, int backward, cudaStream_t st) {
+  a.tiles = (int)ceil_div(a.rows, tile);
+  const dim3 grid = grid_of(a.tiles, ceil_div(a.channels, width));
+  if (a.tiles > 0) {
+    maps<<<grid, kThreads, 0, st>>>(a);
+    D3D_CHECK_LAUNCH();
+  }
+  if (a.tiles > 1)
+    D3D_LAUNCH(true, carry_kernel, (unsigned)ceil_div(a.channels, kCarryChannels), kCarryThreads, 0, st, a.maps, a.carry, a.tiles,
+               a.channels, backward);
+  else
+    a.carry = nullptr;
+  D3D_LAUNCH(a.tiles > 0, rows, grid, kThreads, 0, st, a);
   return D3D_OK;
 }
 
@@ -666,12 +698,15 @@ int check_scan(int dtype, const ScanArgs& a) {
 
 using namespace d3d;
 
-extern "C" int64_t d3d_gated_recurrence_state_rows(int64_t rows) { return rows < 0 ? 0 : ceil_div(rows > 0 ? rows : 1, kTile); }
+extern "C" int64_t d3d_gated_recurrence_state_rows(int64_t rows) { return rows < 0 ? 0 : ceil_div(rows > 0 ? rows : 1, kRows); }
 
 extern "C" size_t d3d_gated_recurrence_workspace(int64_t rows, int channels) {
   if (rows < 0 || channels < 1) return 0;
-  const size_t n = (size_t)d3d_gated_recurrence_state_rows(rows) * channels;
-  return align_up(n * sizeof(float2), 256) + align_up(n * sizeof(float), 256);
+  ScanArgs a = {};
+  a.rows = rows, a.channels = channels;
+  Carver w(nullptr);
+  carve(a, w);
+  return w.off;
 }
 
 extern "C" int d3d_gated_recurrence(int dtype, const void* x, int64_t x_ld, const void* gates, int64_t gates_ld,
@@ -681,38 +716,23 @@ extern "C" int d3d_gated_recurrence(int dtype, const void* x, int64_t x_ld, cons
   D3D_NVTX_RANGE("d3d_gated_recurrence");
   ScanArgs a = {};
   a.x = x, a.x_ld = x_ld, a.gates = gates, a.gates_ld = gates_ld, a.offsets = offsets, a.seqs = seqs, a.rows = rows;
-  a.channels = channels, a.reverse = reverse != 0, a.initial = initial, a.out = out, a.final_state = final_state;
+  a.channels = channels, a.reverse = reverse != 0, a.initial = initial, a.out = out, a.final_state = final_state, a.states = states;
   const int rc = check_scan(dtype, a);
   D3D_REQUIRE(rc == D3D_OK, rc);
   D3D_REQUIRE(rows == 0 || (x && gates && out), D3D_ERR_INVALID_ARGUMENT);
   D3D_REQUIRE(workspace && reinterpret_cast<uintptr_t>(workspace) % 256 == 0, D3D_ERR_INVALID_ARGUMENT);
   D3D_REQUIRE(workspace_bytes >= d3d_gated_recurrence_workspace(rows, channels), D3D_ERR_WORKSPACE_TOO_SMALL);
   Carver w(workspace);
-  a.maps = w.take<float2>((size_t)d3d_gated_recurrence_state_rows(rows) * channels);
-  a.states = states ? states : w.take<float>((size_t)d3d_gated_recurrence_state_rows(rows) * channels);
-  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  carve(a, w);
+  if (seqs == 0) return D3D_OK;
   const int esize = (int)dtype_size(dtype);
   const bool pairs = channels % 2 == 0 && rows_paired(x, x_ld, esize) && rows_paired(gates, gates_ld, esize) && rows_paired(out, channels, esize);
-  if (seqs == 0) return D3D_OK;
   return by_type(dtype, [&](auto t) -> int {
     using T = decltype(t);
-    return by_shape(pairs, channels, [&](auto v, auto l) -> int {
+    return by_shape<T>(pairs, channels, [&](auto v, auto l) -> int {
       constexpr int V = decltype(v)::value, L = decltype(l)::value;
-      a.tiles = (int)ceil_div(rows, kTile);
-      const dim3 grid = grid_of(a.tiles, ceil_div(channels, V * L));
-      if (a.tiles > 1) {
-        scan_kernel<T, V, L, true><<<grid, kThreads, 0, st>>>(a);
-        D3D_CHECK_LAUNCH();
-        D3D_LAUNCH(true, carry_kernel, (unsigned)ceil_div(channels, kCarryChannels), kCarryThreads, 0, st, a.maps, a.states, a.tiles,
-                   channels, 0);
-      } else if (states) {  // nothing lies in front of the only tile
-        if (cudaMemsetAsync(states, 0, channels * sizeof(float), st) != cudaSuccess) return D3D_ERR_CUDA;
-      } else {
-        a.states = nullptr;
-      }
-      D3D_LAUNCH(a.tiles > 1, (scan_kernel<T, V, L, false>), grid, kThreads, 0, st, a);
-      D3D_CHECK_LAUNCH();
-      return D3D_OK;
+      return launch_pass(a, Place<V, L>::kTile, V * L, scan_maps_kernel<T, V, L>, scan_rows_kernel<T, V, L>, 0,
+                         reinterpret_cast<cudaStream_t>(stream));
     });
   });
 }
@@ -728,6 +748,7 @@ extern "C" int d3d_gated_recurrence_backward(int dtype, const void* grad, int64_
   a.x = x, a.x_ld = x_ld, a.gates = gates, a.gates_ld = gates_ld, a.offsets = offsets, a.seqs = seqs, a.rows = rows;
   a.channels = channels, a.reverse = reverse != 0, a.initial = initial, a.grad = grad, a.grad_ld = grad_ld;
   a.grad_final = grad_final, a.grad_x = grad_x, a.grad_gates = grad_gates, a.grad_initial = grad_initial;
+  a.states = const_cast<float*>(states);
   const int rc = check_scan(dtype, a);
   D3D_REQUIRE(rc == D3D_OK, rc);
   D3D_REQUIRE(grad_ld >= channels && (rows == 0 || (x && gates && grad && states && grad_x && grad_gates)),
@@ -735,31 +756,17 @@ extern "C" int d3d_gated_recurrence_backward(int dtype, const void* grad, int64_
   D3D_REQUIRE(workspace && reinterpret_cast<uintptr_t>(workspace) % 256 == 0, D3D_ERR_INVALID_ARGUMENT);
   D3D_REQUIRE(workspace_bytes >= d3d_gated_recurrence_workspace(rows, channels), D3D_ERR_WORKSPACE_TOO_SMALL);
   Carver w(workspace);
-  a.maps = w.take<float2>((size_t)d3d_gated_recurrence_state_rows(rows) * channels);
-  a.carry = w.take<float>((size_t)d3d_gated_recurrence_state_rows(rows) * channels);
-  a.states = const_cast<float*>(states);
-  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  carve(a, w);
+  if (seqs == 0) return D3D_OK;
   const int esize = (int)dtype_size(dtype);
   const bool pairs = channels % 2 == 0 && rows_paired(x, x_ld, esize) && rows_paired(gates, gates_ld, esize) &&
                      rows_paired(grad, grad_ld, esize) && rows_paired(grad_x, channels, esize) && rows_paired(grad_gates, channels, esize);
-  if (seqs == 0) return D3D_OK;
   return by_type(dtype, [&](auto t) -> int {
     using T = decltype(t);
-    return by_shape(pairs, channels, [&](auto v, auto l) -> int {
+    return by_shape<T>(pairs, channels, [&](auto v, auto l) -> int {
       constexpr int V = decltype(v)::value, L = decltype(l)::value;
-      a.tiles = (int)ceil_div(rows, kTile);
-      const dim3 grid = grid_of(a.tiles, ceil_div(channels, V * L));
-      if (a.tiles > 1) {
-        scan_backward_kernel<T, V, L, true><<<grid, kThreads, 0, st>>>(a);
-        D3D_CHECK_LAUNCH();
-        D3D_LAUNCH(true, carry_kernel, (unsigned)ceil_div(channels, kCarryChannels), kCarryThreads, 0, st, a.maps, a.carry, a.tiles,
-                   channels, 1);
-      } else {
-        a.carry = nullptr;  // nothing lies behind the only tile
-      }
-      D3D_LAUNCH(a.tiles > 1, (scan_backward_kernel<T, V, L, false>), grid, kThreads, 0, st, a);
-      D3D_CHECK_LAUNCH();
-      return D3D_OK;
+      return launch_pass(a, Place<V, L>::kTile, V * L, scan_backward_maps_kernel<T, V, L>, scan_backward_rows_kernel<T, V, L>, 1,
+                         reinterpret_cast<cudaStream_t>(stream));
     });
   });
 }

@@ -314,6 +314,24 @@ def test_step_is_the_recurrence_of_one_row(d3d, dtype, layout, rows, channels):
     assert same is state and torch.equal(state, new) and torch.equal(again, out)
 
 
+@pytest.mark.parametrize("channels", [6, 14, 30, 64])
+@pytest.mark.parametrize("reverse", [False, True])
+def test_states_serve_inputs_of_another_alignment(d3d, channels, reverse):
+    """The forward pass over columns of an odd-pitched tensor, the backward pass over dense copies: the same gradients as from
+    the dense forward pass, whose tiles have another shape."""
+    rows = 777
+    x, g = features(1, rows, channels, torch.float16, "odd"), gates_like(2, rows, channels, torch.float16, "odd")
+    xd, gd, grad = x.contiguous(), g.contiguous(), normal(3, rows, channels).half()
+    offsets = torch.tensor([0, 300, 777], dtype=torch.int32, device=DEV)
+    for args in ((x, g), (xd, gd)):
+        _, _, states = d3d.gated_recurrence(*args, offsets, reverse=reverse, with_states=True)
+        got = d3d.gated_recurrence_backward(grad, xd, gd, offsets, states, reverse=reverse)
+        back = ref.recurrence_backward(ref.as64(grad), ref.as64(x), ref.as64(g), offsets.tolist(), None, None, reverse, torch.float16)
+        for t, (w, o), what in zip(got, back, ("dx", "dgates", "dinitial")):
+            rnd = torch.float32 if what == "dinitial" else torch.float16
+            ref.assert_within(t, w, o + ref.half_step(rnd) * (np.abs(w) + o) + ref.smallest(rnd), what)
+
+
 def test_gradients_against_differences(d3d):
     """fp32, along a random direction: (L(p + e d) - L(p - e d)) / 2 e for L = <out, c> against the gradients.  The gates are
     smooth on a scale of one, so with e = 2^-6 the difference is off by at most e^2 of its terms' sizes, and rounding adds
