@@ -129,43 +129,42 @@ __device__ __forceinline__ void after(float& a, float& b, float pa, float pb) {
   if (!is_reset(a)) b = fmaf(a, pb, b), a *= pa;
 }
 
-// f = sigmoid(gate) and 1 - f: the smaller one is t / (1 + t), t = exp(-|gate|), the other one a difference that loses nothing.
+// f = sigmoid(gate) and 1 - f.  With t = exp(-|gate|) the smaller one is t / (1 + t), the other one a difference that loses
+// nothing; with t = exp(-gate) the same from f = 1 / (1 + t) and 1 - f = t f, where f is taken as the difference while t < 1.
 // Neither has a sign, NaN included: the sign of a map means a reset.
 // Features of 32 bits: exponential and quotient to two units of the last place.  Of 16 bits: the hardware's base-two exponential,
 // whose argument is rounded to |gate| 2^-24 (so that 1 - f is off by that much, relatively; the gate itself came rounded to 2^-9
 // or 2^-12 of it), a third of the instructions.
-template <class T, int V> __device__ __forceinline__ Vec<V> small_of(const Vec<V>& g) {
-  Vec<V> t, r;
+template <class T, int V> __device__ __forceinline__ void gate_of(const Vec<V>& g, Vec<V>& f, Vec<V>& rest) {
   if constexpr (sizeof(T) == 4) {
 #pragma unroll
-    for (int e = 0; e < V; ++e) t.v[e] = expf(-fabsf(g.v[e]));
+    for (int e = 0; e < V; ++e) {
+      const float t = expf(-fabsf(g.v[e])), small = t * __fdividef(1.f, 1.f + t), large = 1.f - small;
+      f.v[e] = g.v[e] >= 0.f ? large : small, rest.v[e] = g.v[e] >= 0.f ? small : large;
+    }
   } else {
-    Vec<V> y;
+    Vec<V> y = mul(g, all<V>(-1.44269504f)), t, r;
 #pragma unroll
-    for (int e = 0; e < V; ++e) y.v[e] = fabsf(g.v[e]);
-    y = mul(y, all<V>(-1.44269504f));
+    for (int e = 0; e < V; ++e) {
+      // 2^100 is as good as infinity: of any 16-bit state nothing is left, and 1 - f is one
+      asm("min.NaN.f32 %0, %0, 0f42C80000;" : "+f"(y.v[e]));
+      asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(t.v[e]) : "f"(y.v[e]));
+    }
+    const Vec<V> d = add(t, all<V>(1.f));
 #pragma unroll
-    for (int e = 0; e < V; ++e) asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(t.v[e]) : "f"(y.v[e]));
+    for (int e = 0; e < V; ++e) asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r.v[e]) : "f"(d.v[e]));
+    rest = mul(t, r);
+    f = fma(rest, all<V>(-1.f), all<V>(1.f));
+#pragma unroll
+    for (int e = 0; e < V; ++e) f.v[e] = t.v[e] < 1.f ? f.v[e] : r.v[e];
   }
-  const Vec<V> d = add(t, all<V>(1.f));
-#pragma unroll
-  for (int e = 0; e < V; ++e) {
-    if constexpr (sizeof(T) == 4) r.v[e] = __fdividef(1.f, d.v[e]);
-    else asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r.v[e]) : "f"(d.v[e]));
-  }
-  return mul(t, r);
-}
-template <class T, int V> __device__ __forceinline__ void gate_of(const Vec<V>& g, Vec<V>& f, Vec<V>& rest) {
-  const Vec<V> small = small_of<T, V>(g), large = fma(small, all<V>(-1.f), all<V>(1.f));
-#pragma unroll
-  for (int e = 0; e < V; ++e) f.v[e] = g.v[e] >= 0.f ? large.v[e] : small.v[e], rest.v[e] = g.v[e] >= 0.f ? small.v[e] : large.v[e];
 }
 // Both in one number: the smaller one, with a sign where that is f.
-template <class T, int V> __device__ __forceinline__ Vec<V> folded_gate(const Vec<V>& g) {
-  Vec<V> small = small_of<T, V>(g);
+template <int V> __device__ __forceinline__ Vec<V> fold_gate(const Vec<V>& f, const Vec<V>& rest) {
+  Vec<V> r;
 #pragma unroll
-  for (int e = 0; e < V; ++e) small.v[e] = copysignf(small.v[e], g.v[e]);
-  return small;
+  for (int e = 0; e < V; ++e) r.v[e] = f.v[e] < rest.v[e] ? -f.v[e] : rest.v[e];
+  return r;
 }
 template <int V> __device__ __forceinline__ void open_gate(const Vec<V>& gate, Vec<V>& f, Vec<V>& rest) {
 #pragma unroll
@@ -210,9 +209,15 @@ template <class T, int V, int kLanes>
 __device__ __forceinline__ void load_rows(Pack<T, V> (&to)[kRows], const Place<V, kLanes>& at, const void* p, int64_t ld) {
   const T* src = at.start((const T*)p, ld);
   const int64_t step = at.step(ld);
+  if (at.there == (1 << kRows) - 1) {
 #pragma unroll
-  for (int r = 0; r < kRows; ++r, src += step)
-    if (at.there >> r & 1) to[r] = *reinterpret_cast<const Pack<T, V>*>(src);
+    for (int r = 0; r < kRows; ++r, src += step) to[r] = *reinterpret_cast<const Pack<T, V>*>(src);
+  } else {
+    asm("" : "+l"(src));  // the addresses are those above, but need not all be there before the branch
+#pragma unroll
+    for (int r = 0; r < kRows; ++r, src += step)
+      if (at.there >> r & 1) to[r] = *reinterpret_cast<const Pack<T, V>*>(src);
+  }
 }
 template <int V> __device__ __forceinline__ Vec<V> load_state(const float* p, int64_t s, int channels, int c) {
   Vec<V> r = all<V>(0.f);
@@ -569,9 +574,9 @@ scan_backward_rows_kernel(const ScanArgs a) {
 #pragma unroll
       for (int r = 0; r < kRows; ++r)
         if (kPlain || (marks.live >> r & 1)) {
-          gate[r] = folded_gate<T, V>(widen<T, V>(g[r]));
           Vec<V> f, rest;
-          open_gate<V>(gate[r], f, rest);
+          gate_of<T, V>(widen<T, V>(g[r]), f, rest);
+          gate[r] = fold_gate<V>(f, rest);
           if (!kPlain && (marks.ends >> r & 1)) h = load_state<V>(a.initial, find.of(a, t + r * next), a.channels, at.c);
           const Vec<V> in = widen<T, V>(x[r]);
           away[r] = fma(in, all<V>(-1.f), h);
