@@ -8,11 +8,10 @@
 #include <type_traits>
 
 #include "common.cuh"
+#include "packed.cuh"
 
 namespace d3d {
 namespace {
-
-template <class T, int V> struct alignas(sizeof(T) * V) Pack { T v[V]; };
 
 struct NormArgs {
   const void *x, *residual;
@@ -96,104 +95,124 @@ __device__ __forceinline__ float step_of(uint32_t amax_bits, float* inv) {
 template <int kLanes> __host__ __device__ constexpr int threads_for() { return kLanes <= 32 ? 256 : kLanes; }
 // Rows a thread has in flight: 32 to 64 bytes of each tensor.
 template <int kVecs, int kLanes> __host__ __device__ constexpr int rows_for() { return kLanes <= 32 && kVecs == 1 ? 2 : 1; }
+// Rows of few pieces are bound by how many of them are on their way: three CTAs of 256 threads to an SM.
+template <int kVecs, int kLanes> constexpr int ctas_for() { return kVecs == 1 ? 3 : kLanes <= 256 ? 512 / threads_for<kLanes>() : 1; }
+template <int kVecs, int kLanes> constexpr int backward_ctas_for() { return kLanes <= 256 ? 512 / threads_for<kLanes>() : 1; }
 
-// kLanes threads share a row, kVecs pieces of V elements each.  CTAs walk over the rows, the next rows' loads ahead of this
-// one's sums, so that weight and bias are fetched once per CTA.
+// A thread's pieces of kRows rows of a tensor, the next rows' ahead of the sums over this one's.  Rows lie `kGroups` apart.
+template <class T, int V, int kVecs, int kLanes> struct Stream {
+  static constexpr int kGroups = threads_for<kLanes>() / kLanes, kRows = rows_for<kVecs, kLanes>();
+  const T* at;
+  int64_t apart, step;
+  Pack<T, V> next[kRows][kVecs];
+  // first: the thread's first row, `stride` rows in front of its next one
+  __device__ __forceinline__ Stream(const void* p, int64_t ld, int64_t first, int64_t stride, int lane)
+      : at((const T*)p + first * ld + lane * V), apart(kGroups * ld), step(stride * ld) {}
+  __device__ __forceinline__ void load(int64_t row, int64_t rows, int lane, int channels) {
+#pragma unroll
+    for (int i = 0; i < kRows; ++i)
+#pragma unroll
+      for (int k = 0; k < kVecs; ++k) {
+        if (row + i * kGroups < rows && (k * kLanes + lane) * V < channels) {
+          next[i][k] = *reinterpret_cast<const Pack<T, V>*>(at + i * apart + k * kLanes * V);
+        } else {
+#pragma unroll
+          for (int e = 0; e < V; ++e) next[i][k].v[e] = from_f32<T>(0.f);
+        }
+      }
+    at += step;
+  }
+};
+template <int V> __device__ __forceinline__ float across(const Vec<V>& x) {
+  float s = x.v[0];
+#pragma unroll
+  for (int e = 1; e < V; ++e) s += x.v[e];
+  return s;
+}
+// Parameters of a thread's columns; zeros behind the last one.
+template <int V, int kVecs, int kLanes>
+__device__ __forceinline__ void load_columns(Vec<V> (&to)[kVecs], const float* p, float without, int lane, int channels) {
+#pragma unroll
+  for (int k = 0; k < kVecs; ++k)
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+      const int c = (k * kLanes + lane) * V + e;
+      to[k].v[e] = c >= channels ? 0.f : p ? __ldg(p + c) : without;
+    }
+}
+
+// kLanes threads share a row, kVecs pieces of V elements each.  CTAs walk over the rows, so that weight and bias are fetched once
+// per CTA.
 template <class T, int V, int kVecs, int kLanes, bool kNorm, bool kQuant>
-__global__ void __launch_bounds__(threads_for<kLanes>())
+__global__ void __launch_bounds__(threads_for<kLanes>(), ctas_for<kVecs, kLanes>())
 norm_kernel(const NormArgs a) {
-  constexpr int kThreads = threads_for<kLanes>(), kGroups = kThreads / kLanes, kRows = rows_for<kVecs, kLanes>();
+  constexpr int kGroups = threads_for<kLanes>() / kLanes, kRows = rows_for<kVecs, kLanes>();
   using P = Pack<T, V>;
   __shared__ uint32_t scratch[kLanes > 32 ? 2 * kRows * (kLanes / 32) : 1];
   int turn = 0;
   const int lane = threadIdx.x % kLanes, group = threadIdx.x / kLanes;
   const int channels = a.channels;
   const int64_t rows = live_rows(a.rows, a.num_rows);
-  float w[kVecs][V], b[kVecs][V];
-  if (kNorm) {
-#pragma unroll
-    for (int k = 0; k < kVecs; ++k)
-#pragma unroll
-      for (int e = 0; e < V; ++e) {
-        const int c = (k * kLanes + lane) * V + e;
-        w[k][e] = c < channels ? (a.weight ? __ldg(a.weight + c) : 1.f) : 0.f;
-        b[k][e] = c < channels && a.bias ? __ldg(a.bias + c) : 0.f;
-      }
-  }
   const float inv_n = 1.f / (float)channels;
   const bool sum = kNorm && a.residual != nullptr;
-  P next[kRows][kVecs], next_r[kRows][kVecs];
-  auto load = [&](int64_t base) {
-#pragma unroll
-    for (int i = 0; i < kRows; ++i) {
-      const int64_t row = base + i * kGroups + group;
-#pragma unroll
-      for (int k = 0; k < kVecs; ++k) {
-        const int c = (k * kLanes + lane) * V;
-        if (row < rows && c < channels) {
-          next[i][k] = *reinterpret_cast<const P*>((const T*)a.x + row * a.x_ld + c);
-          if (sum) next_r[i][k] = *reinterpret_cast<const P*>((const T*)a.residual + row * a.residual_ld + c);
-        } else {
-#pragma unroll
-          for (int e = 0; e < V; ++e) next[i][k].v[e] = next_r[i][k].v[e] = from_f32<T>(0.f);
-        }
-      }
-    }
-  };
   const int64_t stride = (int64_t)gridDim.x * kGroups * kRows;
-  int64_t base = (int64_t)blockIdx.x * kGroups * kRows;
-  if (base < rows) load(base);
-  for (; base < rows; base += stride) {
-    float y[kRows][kVecs * V];
+  int64_t row = (int64_t)blockIdx.x * kGroups * kRows + group;  // of the CTA's rows all or none are beyond the last one
+  Stream<T, V, kVecs, kLanes> in(a.x, a.x_ld, row, stride, lane), more(a.residual, a.residual_ld, row, stride, lane);
+  const int64_t over = rows + group;  // row < over: the CTA has rows to do
+  if (row < over) {
+    in.load(row, rows, lane, channels);
+    if (sum) more.load(row, rows, lane, channels);
+  }
+  Vec<V> w[kVecs], b[kVecs];
+  if (kNorm) load_columns<V, kVecs, kLanes>(w, a.weight, 1.f, lane, channels), load_columns<V, kVecs, kLanes>(b, a.bias, 0.f, lane, channels);
+  for (; row < over; row += stride) {
+    Vec<V> y[kRows][kVecs];
 #pragma unroll
     for (int i = 0; i < kRows; ++i)
 #pragma unroll
       for (int k = 0; k < kVecs; ++k) {
+        const int c = (k * kLanes + lane) * V;
         if (sum) {
-          const int64_t row = base + i * kGroups + group;
-          const int c = (k * kLanes + lane) * V;
-          P t;
-#pragma unroll
-          for (int e = 0; e < V; ++e) t.v[e] = from_f32<T>(to_f32(next[i][k].v[e]) + to_f32(next_r[i][k].v[e]));
-          if (row < rows && c < channels) *reinterpret_cast<P*>((T*)a.total + row * channels + c) = t;
-          next[i][k] = t;  // the norm is that of the rounded sum, which is what the backward pass will see
+          const P t = narrow<T, V>(add(widen<T, V>(in.next[i][k]), widen<T, V>(more.next[i][k])));
+          if (row + i * kGroups < rows && c < channels) *reinterpret_cast<P*>((T*)a.total + (row + i * kGroups) * channels + c) = t;
+          y[i][k] = widen<T, V>(t);  // the norm is that of the rounded sum, which is what the backward pass will see
+        } else {
+          y[i][k] = widen<T, V>(in.next[i][k]);
         }
-#pragma unroll
-        for (int e = 0; e < V; ++e) y[i][k * V + e] = to_f32(next[i][k].v[e]);
       }
-    if (base + stride < rows) load(base + stride);
+    if (row + stride < over) {
+      in.load(row + stride, rows, lane, channels);
+      if (sum) more.load(row + stride, rows, lane, channels);
+    }
     if (kNorm) {
       float mean[kRows], var[kRows];
 #pragma unroll
       for (int i = 0; i < kRows; ++i) {
-        mean[i] = 0.f;
+        Vec<V> s = y[i][0];
 #pragma unroll
-        for (int j = 0; j < kVecs * V; ++j) mean[i] += y[i][j];
+        for (int k = 1; k < kVecs; ++k) s = add(s, y[i][k]);
+        mean[i] = across(s);
       }
       row_reduce<kLanes>(mean, Add(), scratch, turn);
 #pragma unroll
       for (int i = 0; i < kRows; ++i) {
         mean[i] *= inv_n;
-        var[i] = 0.f;
+        Vec<V> s = all<V>(0.f);
 #pragma unroll
         for (int k = 0; k < kVecs; ++k)
-          if ((k * kLanes + lane) * V < channels)
-#pragma unroll
-            for (int e = 0; e < V; ++e) {
-              y[i][k * V + e] -= mean[i];
-              var[i] += y[i][k * V + e] * y[i][k * V + e];
-            }
+          if ((k * kLanes + lane) * V < channels) {
+            y[i][k] = add(y[i][k], all<V>(-mean[i]));
+            s = fma(y[i][k], y[i][k], s);
+          }
+        var[i] = across(s);
       }
       row_reduce<kLanes>(var, Add(), scratch, turn);
 #pragma unroll
       for (int i = 0; i < kRows; ++i) {
-        const float rstd = 1.f / sqrtf(var[i] * inv_n + a.eps);
-        const int64_t row = base + i * kGroups + group;
-        if (lane == 0 && row < rows && a.mean) a.mean[row] = mean[i], a.rstd[row] = rstd;
+        const float rstd = rsqrtf(var[i] * inv_n + a.eps);
+        if (lane == 0 && row + i * kGroups < rows && a.mean) a.mean[row + i * kGroups] = mean[i], a.rstd[row + i * kGroups] = rstd;
 #pragma unroll
-        for (int k = 0; k < kVecs; ++k)
-#pragma unroll
-          for (int e = 0; e < V; ++e) y[i][k * V + e] = y[i][k * V + e] * rstd * w[k][e] + b[k][e];
+        for (int k = 0; k < kVecs; ++k) y[i][k] = fma(mul(y[i][k], all<V>(rstd)), w[k], b[k]);
       }
     }
     uint32_t amax[kRows];
@@ -202,18 +221,20 @@ norm_kernel(const NormArgs a) {
       for (int i = 0; i < kRows; ++i) {
         amax[i] = 0u;
 #pragma unroll
-        for (int j = 0; j < kVecs * V; ++j) amax[i] = MaxBits()(amax[i], __float_as_uint(y[i][j]) & 0x7fffffffu);
+        for (int k = 0; k < kVecs; ++k)
+#pragma unroll
+          for (int e = 0; e < V; ++e) amax[i] = MaxBits()(amax[i], __float_as_uint(y[i][k].v[e]) & 0x7fffffffu);
       }
       row_reduce<kLanes>(amax, MaxBits(), scratch, turn);
     }
 #pragma unroll
     for (int i = 0; i < kRows; ++i) {
-      const int64_t row = base + i * kGroups + group;
-      if (row >= rows) continue;
+      const int64_t at = row + i * kGroups;
+      if (at >= rows) continue;
       float inv = 0.f, scale = 0.f;
       if (kQuant) {
         scale = step_of(amax[i], &inv);
-        if (lane == 0) a.scales[row] = scale;
+        if (lane == 0) a.scales[at] = scale;
       }
 #pragma unroll
       for (int k = 0; k < kVecs; ++k) {
@@ -222,13 +243,10 @@ norm_kernel(const NormArgs a) {
         if (kQuant) {
           Pack<int8_t, V> q;
 #pragma unroll
-          for (int e = 0; e < V; ++e) q.v[e] = inv == 0.f ? 0 : (int8_t)nearest_step(y[i][k * V + e], scale, inv);
-          *reinterpret_cast<Pack<int8_t, V>*>(a.q + row * a.q_ld + c) = q;
+          for (int e = 0; e < V; ++e) q.v[e] = inv == 0.f ? 0 : (int8_t)nearest_step(y[i][k].v[e], scale, inv);
+          *reinterpret_cast<Pack<int8_t, V>*>(a.q + at * a.q_ld + c) = q;
         } else {
-          P o;
-#pragma unroll
-          for (int e = 0; e < V; ++e) o.v[e] = from_f32<T>(y[i][k * V + e]);
-          *reinterpret_cast<P*>((T*)a.out + row * channels + c) = o;
+          *reinterpret_cast<P*>((T*)a.out + at * channels + c) = narrow<T, V>(y[i][k]);
         }
       }
     }
@@ -250,7 +268,7 @@ struct NormBackwardArgs {
 // As above; a thread adds up the weight's and the bias's gradient of its columns over all its rows, the CTA adds its
 // threads' sums in a fixed order.
 template <class T, int V, int kVecs, int kLanes>
-__global__ void __launch_bounds__(threads_for<kLanes>())
+__global__ void __launch_bounds__(threads_for<kLanes>(), backward_ctas_for<kVecs, kLanes>())
 norm_backward_kernel(const NormBackwardArgs a) {
   constexpr int kThreads = threads_for<kLanes>(), kGroups = kThreads / kLanes, kRows = rows_for<kVecs, kLanes>();
   using P = Pack<T, V>;
@@ -260,85 +278,64 @@ norm_backward_kernel(const NormBackwardArgs a) {
   const int lane = threadIdx.x % kLanes, group = threadIdx.x / kLanes;
   const int channels = a.channels;
   const int64_t rows = live_rows(a.rows, a.num_rows);
-  float w[kVecs][V], dw[kVecs][V], db[kVecs][V];
-#pragma unroll
-  for (int k = 0; k < kVecs; ++k)
-#pragma unroll
-    for (int e = 0; e < V; ++e) {
-      const int c = (k * kLanes + lane) * V + e;
-      w[k][e] = c < channels ? (a.weight ? __ldg(a.weight + c) : 1.f) : 0.f;
-      dw[k][e] = db[k][e] = 0.f;
-    }
   const float inv_n = 1.f / (float)channels;
-  P next_x[kRows][kVecs], next_g[kRows][kVecs];
+  const int64_t stride = (int64_t)gridDim.x * kGroups * kRows;
+  int64_t row = (int64_t)blockIdx.x * kGroups * kRows + group;
+  const int64_t over = rows + group;
+  Stream<T, V, kVecs, kLanes> in(a.x, a.x_ld, row, stride, lane), grad(a.grad, a.grad_ld, row, stride, lane);
   float next_mean[kRows], next_rstd[kRows];
-  auto load = [&](int64_t base) {
+  auto load = [&](int64_t at) {
+    in.load(at, rows, lane, channels);
+    grad.load(at, rows, lane, channels);
 #pragma unroll
     for (int i = 0; i < kRows; ++i) {
-      const int64_t row = base + i * kGroups + group;
-      next_mean[i] = row < rows ? __ldg(a.mean + row) : 0.f;
-      next_rstd[i] = row < rows ? __ldg(a.rstd + row) : 0.f;
-#pragma unroll
-      for (int k = 0; k < kVecs; ++k) {
-        const int c = (k * kLanes + lane) * V;
-        if (row < rows && c < channels) {
-          next_x[i][k] = *reinterpret_cast<const P*>((const T*)a.x + row * a.x_ld + c);
-          next_g[i][k] = *reinterpret_cast<const P*>((const T*)a.grad + row * a.grad_ld + c);
-        } else {
-#pragma unroll
-          for (int e = 0; e < V; ++e) next_x[i][k].v[e] = next_g[i][k].v[e] = from_f32<T>(0.f);
-        }
-      }
+      const bool has = at + i * kGroups < rows;
+      next_mean[i] = has ? __ldg(a.mean + at + i * kGroups) : 0.f, next_rstd[i] = has ? __ldg(a.rstd + at + i * kGroups) : 0.f;
     }
   };
-  const int64_t stride = (int64_t)gridDim.x * kGroups * kRows;
-  int64_t base = (int64_t)blockIdx.x * kGroups * kRows;
-  if (base < rows) load(base);
-  for (; base < rows; base += stride) {
+  if (row < over) load(row);
+  Vec<V> w[kVecs], dw[kVecs], db[kVecs];
+  load_columns<V, kVecs, kLanes>(w, a.weight, 1.f, lane, channels);
+#pragma unroll
+  for (int k = 0; k < kVecs; ++k) dw[k] = db[k] = all<V>(0.f);
+  for (; row < over; row += stride) {
     P x[kRows][kVecs], g[kRows][kVecs];
-    float mean[kRows], rstd[kRows], dot[2 * kRows];
+    float shift[kRows], rstd[kRows], dot[2 * kRows];
 #pragma unroll
     for (int i = 0; i < kRows; ++i) {
-      mean[i] = next_mean[i], rstd[i] = next_rstd[i];
+      rstd[i] = next_rstd[i], shift[i] = -next_mean[i] * rstd[i];
 #pragma unroll
-      for (int k = 0; k < kVecs; ++k) x[i][k] = next_x[i][k], g[i][k] = next_g[i][k];
+      for (int k = 0; k < kVecs; ++k) x[i][k] = in.next[i][k], g[i][k] = grad.next[i][k];
     }
-    if (base + stride < rows) load(base + stride);
+    if (row + stride < over) load(row + stride);
 #pragma unroll
     for (int i = 0; i < kRows; ++i) {
-      dot[2 * i] = dot[2 * i + 1] = 0.f;
+      Vec<V> s1 = all<V>(0.f), s2 = all<V>(0.f);
 #pragma unroll
-      for (int k = 0; k < kVecs; ++k)
-#pragma unroll
-        for (int e = 0; e < V; ++e) {
-          // beyond the last channel gradient and weight are zeros, so xhat may be anything finite there
-          const float hat = (to_f32(x[i][k].v[e]) - mean[i]) * rstd[i], dy = to_f32(g[i][k].v[e]), gw = dy * w[k][e];
-          dot[2 * i] += gw;
-          dot[2 * i + 1] += gw * hat;
-          dw[k][e] += dy * hat;
-          db[k][e] += dy;
-        }
+      for (int k = 0; k < kVecs; ++k) {
+        // beyond the last channel gradient and weight are zeros, so xhat may be anything finite there
+        const Vec<V> hat = fma(widen<T, V>(x[i][k]), all<V>(rstd[i]), all<V>(shift[i])), dy = widen<T, V>(g[i][k]), gw = mul(dy, w[k]);
+        s1 = add(s1, gw), s2 = fma(gw, hat, s2);
+        dw[k] = fma(dy, hat, dw[k]), db[k] = add(db[k], dy);
+      }
+      dot[2 * i] = across(s1), dot[2 * i + 1] = across(s2);
     }
     row_reduce<kLanes>(dot, Add(), scratch, turn);
 #pragma unroll
     for (int i = 0; i < kRows; ++i) {
-      const int64_t row = base + i * kGroups + group;
-      if (row >= rows) continue;
+      const int64_t at = row + i * kGroups;
+      if (at >= rows) continue;
+      // rstd (g - m1 - hat m2) with hat = x rstd + shift
       const float m1 = dot[2 * i] * inv_n, m2 = dot[2 * i + 1] * inv_n;
 #pragma unroll
       for (int k = 0; k < kVecs; ++k) {
         const int c = (k * kLanes + lane) * V;
         if (c >= channels) continue;
-        P o, t;
-        if (a.grad_total) t = *reinterpret_cast<const P*>((const T*)a.grad_total + row * a.grad_total_ld + c);
-#pragma unroll
-        for (int e = 0; e < V; ++e) {
-          const float hat = (to_f32(x[i][k].v[e]) - mean[i]) * rstd[i], gw = to_f32(g[i][k].v[e]) * w[k][e];
-          float d = rstd[i] * (gw - m1 - hat * m2);
-          if (a.grad_total) d += to_f32(t.v[e]);
-          o.v[e] = from_f32<T>(d);
-        }
-        *reinterpret_cast<P*>((T*)a.grad_x + row * channels + c) = o;
+        const Vec<V> hat = fma(widen<T, V>(x[i][k]), all<V>(rstd[i]), all<V>(shift[i]));
+        Vec<V> d = fma(widen<T, V>(g[i][k]), w[k], fma(hat, all<V>(-m2), all<V>(-m1)));
+        d = mul(d, all<V>(rstd[i]));
+        if (a.grad_total) d = add(d, widen<T, V>(*reinterpret_cast<const P*>((const T*)a.grad_total + at * a.grad_total_ld + c)));
+        *reinterpret_cast<P*>((T*)a.grad_x + at * channels + c) = narrow<T, V>(d);
       }
     }
   }
@@ -350,8 +347,8 @@ norm_backward_kernel(const NormBackwardArgs a) {
       for (int k = 0; k < kVecs; ++k)
 #pragma unroll
         for (int e = 0; e < V; ++e) {
-          dw[k][e] += __shfl_xor_sync(0xffffffffu, dw[k][e], d);
-          db[k][e] += __shfl_xor_sync(0xffffffffu, db[k][e], d);
+          dw[k].v[e] += __shfl_xor_sync(0xffffffffu, dw[k].v[e], d);
+          db[k].v[e] += __shfl_xor_sync(0xffffffffu, db[k].v[e], d);
         }
     for (int turn_of = 0; turn_of < kThreads / 32; ++turn_of) {
       if ((int)(threadIdx.x >> 5) == turn_of && lane_id() < kLanes)
@@ -361,8 +358,8 @@ norm_backward_kernel(const NormBackwardArgs a) {
           for (int e = 0; e < V; ++e) {
             const int c = (k * kLanes + lane) * V + e;
             if (c >= channels) continue;
-            sums[c] = turn_of ? sums[c] + dw[k][e] : dw[k][e];
-            sums[channels + c] = turn_of ? sums[channels + c] + db[k][e] : db[k][e];
+            sums[c] = turn_of ? sums[c] + dw[k].v[e] : dw[k].v[e];
+            sums[channels + c] = turn_of ? sums[channels + c] + db[k].v[e] : db[k].v[e];
           }
       __syncthreads();
     }
@@ -373,28 +370,30 @@ norm_backward_kernel(const NormBackwardArgs a) {
 #pragma unroll
       for (int e = 0; e < V; ++e) {
         const int c = (k * kLanes + lane) * V + e;
-        if (c < channels) mine[c] = dw[k][e], mine[channels + c] = db[k][e];
+        if (c < channels) mine[c] = dw[k].v[e], mine[channels + c] = db[k].v[e];
       }
   }
 }
 
-// Sums the CTAs' partial gradients in a fixed order: 32 columns to a CTA, eight warps take the partials in turn.
-__global__ void __launch_bounds__(256)
+// Sums the CTAs' partial gradients in a fixed order: eight columns to a CTA, 64 threads of each take the partials in turn.
+__global__ void __launch_bounds__(512)
 norm_columns_kernel(const float* __restrict__ partial, int parts, int channels, float* __restrict__ grad_weight,
                     float* __restrict__ grad_bias) {
-  __shared__ float s[8][33];
+  __shared__ float s[16][8];
   pdl_wait();
-  const int lane = lane_id(), warp = threadIdx.x >> 5, c = blockIdx.x * 32 + lane;
+  const int lane = lane_id(), warp = threadIdx.x >> 5, c = blockIdx.x * 8 + lane % 8;
   float sum = 0.f;
   if (c < 2 * channels)
 #pragma unroll 8
-    for (int p = warp; p < parts; p += 8) sum += __ldg(partial + (int64_t)p * 2 * channels + c);
-  s[warp][lane] = sum;
+    for (int p = threadIdx.x / 8; p < parts; p += 64) sum += __ldcg(partial + (int64_t)p * 2 * channels + c);
+  sum += __shfl_xor_sync(0xffffffffu, sum, 8);
+  sum += __shfl_xor_sync(0xffffffffu, sum, 16);
+  if (lane < 8) s[warp][lane] = sum;
   __syncthreads();
-  if (warp == 0 && c < 2 * channels) {
+  if (threadIdx.x < 8 && c < 2 * channels) {
     float t = s[0][lane];
 #pragma unroll
-    for (int w = 1; w < 8; ++w) t += s[w][lane];
+    for (int w = 1; w < 16; ++w) t += s[w][lane];
     if (c < channels) {
       if (grad_weight) grad_weight[c] = t;
     } else if (grad_bias) grad_bias[c - channels] = t;
@@ -413,19 +412,19 @@ template <int V, class F> int by_shape(int channels, F f) {
     if (n <= 8) D3D_NORM_SHAPE(V, 1, 8);
     if (n <= 16) D3D_NORM_SHAPE(V, 1, 16);
     if (n <= 32) D3D_NORM_SHAPE(V, 1, 32);
-    if (n <= 64) D3D_NORM_SHAPE(V, 2, 32);
-    if (n <= 128) D3D_NORM_SHAPE(V, 2, 64);
-    if (n <= 256) D3D_NORM_SHAPE(V, 2, 128);
-    if (n <= 512) D3D_NORM_SHAPE(V, 2, 256);
-    if (n <= 1024) D3D_NORM_SHAPE(V, 2, 512);
-    D3D_NORM_SHAPE(V, 4, 512);
+    constexpr int K = 16 / V;  // 16 elements a thread
+    if (n <= 32 * K) D3D_NORM_SHAPE(V, K, 32);
+    if (n <= 64 * K) D3D_NORM_SHAPE(V, K, 64);
+    if (n <= 128 * K) D3D_NORM_SHAPE(V, K, 128);
+    if (n <= 256 * K) D3D_NORM_SHAPE(V, K, 256);
+    D3D_NORM_SHAPE(V, K, 512);
   } else {
-  if (n <= 8) D3D_NORM_SHAPE(1, 1, 8);
-  if (n <= 32) D3D_NORM_SHAPE(1, 4, 8);
-  if (n <= 128) D3D_NORM_SHAPE(1, 4, 32);
-  if (n <= 512) D3D_NORM_SHAPE(1, 8, 64);
-  if (n <= 2048) D3D_NORM_SHAPE(1, 8, 256);
-  D3D_NORM_SHAPE(1, 16, 512);
+    if (n <= 8) D3D_NORM_SHAPE(1, 1, 8);
+    if (n <= 32) D3D_NORM_SHAPE(1, 4, 8);
+    if (n <= 128) D3D_NORM_SHAPE(1, 4, 32);
+    if (n <= 512) D3D_NORM_SHAPE(1, 8, 64);
+    if (n <= 2048) D3D_NORM_SHAPE(1, 8, 256);
+    D3D_NORM_SHAPE(1, 16, 512);
   }
 }
 #undef D3D_NORM_SHAPE
@@ -473,7 +472,7 @@ template <bool kNorm, bool kQuant> int launch_norm(int dtype, bool wide, const N
 
 // The backward pass keeps its sums per CTA, so that their number decides how large the workspace is.
 int backward_ctas(int64_t rows, int per_cta) {
-  const int64_t need = ceil_div(rows > 0 ? rows : 1, per_cta), most = 2 * kNumSMs;
+  const int64_t need = ceil_div(rows > 0 ? rows : 1, per_cta), most = 3 * kNumSMs;
   return (int)(need < most ? need : most);
 }
 
@@ -578,7 +577,7 @@ extern "C" int d3d_layer_norm_backward(int dtype, const void* grad, int64_t grad
       const size_t smem = L <= 32 ? (size_t)2 * channels * sizeof(float) : 0;
       norm_backward_kernel<T, V, K, L><<<ctas, threads_for<L>(), smem, st>>>(a);
       D3D_CHECK_LAUNCH();
-      D3D_LAUNCH(true, norm_columns_kernel, (unsigned)ceil_div(2 * channels, 32), 256, 0, st, a.partial, ctas, channels, grad_weight,
+      D3D_LAUNCH(true, norm_columns_kernel, (unsigned)ceil_div(2 * channels, 8), 512, 0, st, a.partial, ctas, channels, grad_weight,
                  grad_bias);
       return D3D_OK;
     });
