@@ -37,8 +37,13 @@ __device__ __forceinline__ int64_t live_rows(int64_t rows, const int32_t* num_ro
 struct Add {
   __device__ __forceinline__ float operator()(float a, float b) const { return a + b; }
 };
-struct MaxBits {
-  __device__ __forceinline__ uint32_t operator()(uint32_t a, uint32_t b) const { return a > b ? a : b; }
+// The larger one, NaN where either is NaN.
+struct Max {
+  __device__ __forceinline__ float operator()(float a, float b) const {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+  }
 };
 
 // Combines N values over the kLanes threads that share a row; every thread gets the results.  Within a warp by shuffles, beyond
@@ -66,6 +71,12 @@ __device__ __forceinline__ void row_reduce(T (&v)[N], Op op, uint32_t* scratch, 
   }
 }
 
+template <int kLanes, class T, class Op> __device__ __forceinline__ T row_reduce(T v, Op op, uint32_t* scratch, int& turn) {
+  T one[1] = {v};
+  row_reduce<kLanes>(one, op, scratch, turn);
+  return one[0];
+}
+
 // The integer nearest to v / s, ties to even, as if the quotient were exact: the product with 1 / s is at most one step
 // off, and what is left over, v - r s, has no rounding error near the border (s / 2) that decides.
 __device__ __forceinline__ int nearest_step(float v, float s, float inv) {
@@ -76,50 +87,61 @@ __device__ __forceinline__ int nearest_step(float v, float s, float inv) {
   else if (left < -half || (odd && left == -half)) r -= 1.f;
   return (int)fminf(fmaxf(r, -127.f), 127.f);
 }
-// Scale of a row whose largest magnitude has these bits.  A row that is not finite has no scale (NaN, which every product
-// with it becomes), one below 127 times the smallest normal number counts as zeros.
-__device__ __forceinline__ float step_of(uint32_t amax_bits, float* inv) {
-  if (amax_bits >= 0x7f800000u) {
-    *inv = 0.f;
-    return __uint_as_float(0x7fc00000u);
+// V of them.  1.5 2^23 added leaves the nearest integer in the low bits of the sum.  Where what is left over of every value is
+// less than half a step, that is all; values on a border or next to it are looked at one by one.
+template <int V> __device__ __forceinline__ Pack<int8_t, V> steps_of(const Vec<V>& v, float s, float inv) {
+  const Vec<V> magic = all<V>(12582912.f);
+  const Vec<V> sum = fma(v, all<V>(inv), magic), r = add(sum, all<V>(-12582912.f)), left = fma(r, all<V>(-s), v);
+  float most = 0.f;
+#pragma unroll
+  for (int e = 0; e < V; ++e) most = fmaxf(most, fabsf(left.v[e]));
+  Pack<int8_t, V> q;
+  if (most < 0.5f * s) {
+#pragma unroll
+    for (int e = 0; e < V; ++e) q.v[e] = (int8_t)__float_as_int(sum.v[e]);
+  } else {
+#pragma unroll
+    for (int e = 0; e < V; ++e) q.v[e] = inv == 0.f ? (int8_t)0 : (int8_t)nearest_step(v.v[e], s, inv);
   }
-  const float s = __fdiv_rn(__uint_as_float(amax_bits), 127.f);
-  if (s < 1.17549435e-38f) {
-    *inv = 0.f;
-    return 0.f;
-  }
+  return q;
+}
+// Scale of a row with this largest magnitude.  A row that is not finite has no scale (NaN, which every product with it
+// becomes), one below 127 times the smallest normal number counts as zeros; `inv` is 0 for both.
+__device__ __forceinline__ float step_of(float amax, float* inv) {
+  *inv = 0.f;
+  if (!(amax < __uint_as_float(0x7f800000u))) return __uint_as_float(0x7fc00000u);
+  const float s = __fdiv_rn(amax, 127.f);
+  if (s < 1.17549435e-38f) return 0.f;
   *inv = __frcp_rn(s);
   return s;
 }
 
 template <int kLanes> __host__ __device__ constexpr int threads_for() { return kLanes <= 32 ? 256 : kLanes; }
-// Rows a thread has in flight: 32 to 64 bytes of each tensor.
-template <int kVecs, int kLanes> __host__ __device__ constexpr int rows_for() { return kLanes <= 32 && kVecs == 1 ? 2 : 1; }
-// Rows of few pieces are bound by how many of them are on their way: three CTAs of 256 threads to an SM.
-template <int kVecs, int kLanes> constexpr int ctas_for() { return kVecs == 1 ? 3 : kLanes <= 256 ? 512 / threads_for<kLanes>() : 1; }
-template <int kVecs, int kLanes> constexpr int backward_ctas_for() { return kLanes <= 256 ? 512 / threads_for<kLanes>() : 1; }
+// CTAs to an SM.  What counts is how much is on its way: a row of each of 768 threads forward, two of 512 backward, where a
+// thread holds the columns' sums as well; fewer where the parameters are in registers.
+template <int kLanes> constexpr int ctas_for(bool backward) {
+  return backward || kLanes > 32 ? (kLanes <= 256 ? 512 / threads_for<kLanes>() : 1) : 768 / threads_for<kLanes>();
+}
 
-// A thread's pieces of kRows rows of a tensor, the next rows' ahead of the sums over this one's.  Rows lie `kGroups` apart.
+// A thread's pieces of the rows of a tensor that it has part in, the next ones on their way while one is summed up.  The backward
+// pass has two of them in turn, each for every other row.
 template <class T, int V, int kVecs, int kLanes> struct Stream {
-  static constexpr int kGroups = threads_for<kLanes>() / kLanes, kRows = rows_for<kVecs, kLanes>();
   const T* at;
-  int64_t apart, step;
-  Pack<T, V> next[kRows][kVecs];
-  // first: the thread's first row, `stride` rows in front of its next one
+  int64_t step;
+  Pack<T, V> next[kVecs];
+  // first: the first row of these, `stride` rows in front of the next one
   __device__ __forceinline__ Stream(const void* p, int64_t ld, int64_t first, int64_t stride, int lane)
-      : at((const T*)p + first * ld + lane * V), apart(kGroups * ld), step(stride * ld) {}
-  __device__ __forceinline__ void load(int64_t row, int64_t rows, int lane, int channels) {
+      : at((const T*)p + first * ld + lane * V), step(stride * ld) {}
+  __device__ __forceinline__ void load(bool has, int lane, int channels) {
 #pragma unroll
-    for (int i = 0; i < kRows; ++i)
+    for (int k = 0; k < kVecs; ++k) {
+      if (has && (k * kLanes + lane) * V < channels) {
+        next[k] = *reinterpret_cast<const Pack<T, V>*>(at + k * kLanes * V);
+      } else {
 #pragma unroll
-      for (int k = 0; k < kVecs; ++k) {
-        if (row + i * kGroups < rows && (k * kLanes + lane) * V < channels) {
-          next[i][k] = *reinterpret_cast<const Pack<T, V>*>(at + i * apart + k * kLanes * V);
-        } else {
-#pragma unroll
-          for (int e = 0; e < V; ++e) next[i][k].v[e] = from_f32<T>(0.f);
-        }
+        for (int e = 0; e < V; ++e) next[k].v[e] = from_f32<T>(0.f);
       }
+    }
     at += step;
   }
 };
@@ -129,126 +151,125 @@ template <int V> __device__ __forceinline__ float across(const Vec<V>& x) {
   for (int e = 1; e < V; ++e) s += x.v[e];
   return s;
 }
-// Parameters of a thread's columns; zeros behind the last one.
-template <int V, int kVecs, int kLanes>
-__device__ __forceinline__ void load_columns(Vec<V> (&to)[kVecs], const float* p, float without, int lane, int channels) {
+// A parameter of a thread's columns, zeros behind the last one.  Where rows are long the thread has them in registers, where
+// several rows share a warp they are in shared memory: the registers are better spent on rows that are on their way.
+template <int V, int kVecs, int kLanes> struct Columns {
+  static constexpr bool kShared = kLanes <= 32;
+  static constexpr int kWidth = kShared ? V * kVecs * kLanes : 1;
+  using Store = float[kWidth];
+  Vec<V> held[kShared ? 1 : kVecs];
+  const float* store;
+  // The caller's barrier before the first use.
+  __device__ __forceinline__ Columns(Store& shared, const float* p, float without, int lane, int channels) : store(shared) {
+    if constexpr (kShared) {
+      for (int c = threadIdx.x; c < kWidth; c += threads_for<kLanes>()) shared[c] = c >= channels ? 0.f : p ? __ldg(p + c) : without;
+    } else {
 #pragma unroll
-  for (int k = 0; k < kVecs; ++k)
+      for (int k = 0; k < kVecs; ++k)
 #pragma unroll
-    for (int e = 0; e < V; ++e) {
-      const int c = (k * kLanes + lane) * V + e;
-      to[k].v[e] = c >= channels ? 0.f : p ? __ldg(p + c) : without;
+        for (int e = 0; e < V; ++e) {
+          const int c = (k * kLanes + lane) * V + e;
+          held[k].v[e] = c >= channels ? 0.f : p ? __ldg(p + c) : without;
+        }
     }
-}
+  }
+  __device__ __forceinline__ Vec<V> at(int k, int lane) const {
+    if constexpr (kShared) {
+      Vec<V> r;
+      constexpr int kStep = V < 4 ? 1 : 4;
+#pragma unroll
+      for (int e = 0; e < V; e += kStep) {
+        const float* p = store + (k * kLanes + lane) * V + e;
+        if constexpr (kStep == 4) {
+          const float4 t = *reinterpret_cast<const float4*>(p);
+          r.v[e] = t.x, r.v[e + 1] = t.y, r.v[e + 2] = t.z, r.v[e + 3] = t.w;
+        } else {
+          r.v[e] = *p;
+        }
+      }
+      return r;
+    } else {
+      return held[k];
+    }
+  }
+};
 
 // kLanes threads share a row, kVecs pieces of V elements each.  CTAs walk over the rows, so that weight and bias are fetched once
 // per CTA.
 template <class T, int V, int kVecs, int kLanes, bool kNorm, bool kQuant>
-__global__ void __launch_bounds__(threads_for<kLanes>(), ctas_for<kVecs, kLanes>())
+__global__ void __launch_bounds__(threads_for<kLanes>(), ctas_for<kLanes>(false))
 norm_kernel(const NormArgs a) {
-  constexpr int kGroups = threads_for<kLanes>() / kLanes, kRows = rows_for<kVecs, kLanes>();
+  constexpr int kGroups = threads_for<kLanes>() / kLanes;
   using P = Pack<T, V>;
-  __shared__ uint32_t scratch[kLanes > 32 ? 2 * kRows * (kLanes / 32) : 1];
+  __shared__ uint32_t scratch[kLanes > 32 ? 2 * (kLanes / 32) : 1];
   int turn = 0;
   const int lane = threadIdx.x % kLanes, group = threadIdx.x / kLanes;
   const int channels = a.channels;
   const int64_t rows = live_rows(a.rows, a.num_rows);
   const float inv_n = 1.f / (float)channels;
   const bool sum = kNorm && a.residual != nullptr;
-  const int64_t stride = (int64_t)gridDim.x * kGroups * kRows;
-  int64_t row = (int64_t)blockIdx.x * kGroups * kRows + group;  // of the CTA's rows all or none are beyond the last one
+  const int64_t stride = (int64_t)gridDim.x * kGroups;
+  int64_t row = (int64_t)blockIdx.x * kGroups + group;
+  const int64_t over = rows + group;  // row < over: one of the CTA's rows is there
   Stream<T, V, kVecs, kLanes> in(a.x, a.x_ld, row, stride, lane), more(a.residual, a.residual_ld, row, stride, lane);
-  const int64_t over = rows + group;  // row < over: the CTA has rows to do
-  if (row < over) {
-    in.load(row, rows, lane, channels);
-    if (sum) more.load(row, rows, lane, channels);
-  }
-  Vec<V> w[kVecs], b[kVecs];
-  if (kNorm) load_columns<V, kVecs, kLanes>(w, a.weight, 1.f, lane, channels), load_columns<V, kVecs, kLanes>(b, a.bias, 0.f, lane, channels);
+  auto load = [&](int64_t at) {
+    in.load(at < rows, lane, channels);
+    if (sum) more.load(at < rows, lane, channels);
+  };
+  load(row);
+  using Col = Columns<V, kVecs, kLanes>;
+  __shared__ __align__(16) typename Col::Store w_store, b_store;
+  const Col w(w_store, a.weight, 1.f, lane, kNorm ? channels : 0), b(b_store, a.bias, 0.f, lane, kNorm ? channels : 0);
+  if (Col::kShared) __syncthreads();
   for (; row < over; row += stride) {
-    Vec<V> y[kRows][kVecs];
+    const bool has = row < rows;
+    Vec<V> y[kVecs];
 #pragma unroll
-    for (int i = 0; i < kRows; ++i)
-#pragma unroll
-      for (int k = 0; k < kVecs; ++k) {
-        const int c = (k * kLanes + lane) * V;
-        if (sum) {
-          const P t = narrow<T, V>(add(widen<T, V>(in.next[i][k]), widen<T, V>(more.next[i][k])));
-          if (row + i * kGroups < rows && c < channels) *reinterpret_cast<P*>((T*)a.total + (row + i * kGroups) * channels + c) = t;
-          y[i][k] = widen<T, V>(t);  // the norm is that of the rounded sum, which is what the backward pass will see
-        } else {
-          y[i][k] = widen<T, V>(in.next[i][k]);
-        }
+    for (int k = 0; k < kVecs; ++k) {
+      const int c = (k * kLanes + lane) * V;
+      if (sum) {
+        const P t = narrow<T, V>(add(widen<T, V>(in.next[k]), widen<T, V>(more.next[k])));
+        if (has && c < channels) *reinterpret_cast<P*>((T*)a.total + row * channels + c) = t;
+        y[k] = widen<T, V>(t);  // the norm is that of the rounded sum, which is what the backward pass will see
+      } else {
+        y[k] = widen<T, V>(in.next[k]);
       }
-    if (row + stride < over) {
-      in.load(row + stride, rows, lane, channels);
-      if (sum) more.load(row + stride, rows, lane, channels);
     }
+    load(row + stride);
     if (kNorm) {
-      float mean[kRows], var[kRows];
+      Vec<V> s = y[0];
 #pragma unroll
-      for (int i = 0; i < kRows; ++i) {
-        Vec<V> s = y[i][0];
+      for (int k = 1; k < kVecs; ++k) s = add(s, y[k]);
+      const float mean = row_reduce<kLanes>(across(s), Add(), scratch, turn) * inv_n;
+      s = all<V>(0.f);
 #pragma unroll
-        for (int k = 1; k < kVecs; ++k) s = add(s, y[i][k]);
-        mean[i] = across(s);
-      }
-      row_reduce<kLanes>(mean, Add(), scratch, turn);
-#pragma unroll
-      for (int i = 0; i < kRows; ++i) {
-        mean[i] *= inv_n;
-        Vec<V> s = all<V>(0.f);
-#pragma unroll
-        for (int k = 0; k < kVecs; ++k)
-          if ((k * kLanes + lane) * V < channels) {
-            y[i][k] = add(y[i][k], all<V>(-mean[i]));
-            s = fma(y[i][k], y[i][k], s);
-          }
-        var[i] = across(s);
-      }
-      row_reduce<kLanes>(var, Add(), scratch, turn);
-#pragma unroll
-      for (int i = 0; i < kRows; ++i) {
-        const float rstd = rsqrtf(var[i] * inv_n + a.eps);
-        if (lane == 0 && row + i * kGroups < rows && a.mean) a.mean[row + i * kGroups] = mean[i], a.rstd[row + i * kGroups] = rstd;
-#pragma unroll
-        for (int k = 0; k < kVecs; ++k) y[i][k] = fma(mul(y[i][k], all<V>(rstd)), w[k], b[k]);
-      }
-    }
-    uint32_t amax[kRows];
-    if (kQuant) {
-#pragma unroll
-      for (int i = 0; i < kRows; ++i) {
-        amax[i] = 0u;
-#pragma unroll
-        for (int k = 0; k < kVecs; ++k)
-#pragma unroll
-          for (int e = 0; e < V; ++e) amax[i] = MaxBits()(amax[i], __float_as_uint(y[i][k].v[e]) & 0x7fffffffu);
-      }
-      row_reduce<kLanes>(amax, MaxBits(), scratch, turn);
-    }
-#pragma unroll
-    for (int i = 0; i < kRows; ++i) {
-      const int64_t at = row + i * kGroups;
-      if (at >= rows) continue;
-      float inv = 0.f, scale = 0.f;
-      if (kQuant) {
-        scale = step_of(amax[i], &inv);
-        if (lane == 0) a.scales[at] = scale;
-      }
-#pragma unroll
-      for (int k = 0; k < kVecs; ++k) {
-        const int c = (k * kLanes + lane) * V;
-        if (c >= channels) continue;
-        if (kQuant) {
-          Pack<int8_t, V> q;
-#pragma unroll
-          for (int e = 0; e < V; ++e) q.v[e] = inv == 0.f ? 0 : (int8_t)nearest_step(y[i][k].v[e], scale, inv);
-          *reinterpret_cast<Pack<int8_t, V>*>(a.q + at * a.q_ld + c) = q;
-        } else {
-          *reinterpret_cast<P*>((T*)a.out + at * channels + c) = narrow<T, V>(y[i][k]);
+      for (int k = 0; k < kVecs; ++k)
+        if ((k * kLanes + lane) * V < channels) {
+          y[k] = add(y[k], all<V>(-mean));
+          s = fma(y[k], y[k], s);
         }
-      }
+      const float rstd = rsqrtf(row_reduce<kLanes>(across(s), Add(), scratch, turn) * inv_n + a.eps);
+      if (lane == 0 && has && a.mean) a.mean[row] = mean, a.rstd[row] = rstd;
+#pragma unroll
+      for (int k = 0; k < kVecs; ++k) y[k] = fma(mul(y[k], all<V>(rstd)), w.at(k, lane), b.at(k, lane));
+    }
+    float inv = 0.f, scale = 0.f;
+    if (kQuant) {
+      float amax = 0.f;
+#pragma unroll
+      for (int k = 0; k < kVecs; ++k)
+#pragma unroll
+        for (int e = 0; e < V; ++e) amax = Max()(amax, fabsf(y[k].v[e]));
+      scale = step_of(row_reduce<kLanes>(amax, Max(), scratch, turn), &inv);
+      if (lane == 0 && has) a.scales[row] = scale;
+    }
+    if (!has) continue;
+#pragma unroll
+    for (int k = 0; k < kVecs; ++k) {
+      const int c = (k * kLanes + lane) * V;
+      if (c >= channels) continue;
+      if (kQuant) *reinterpret_cast<Pack<int8_t, V>*>(a.q + row * a.q_ld + c) = steps_of<V>(y[k], scale, inv);
+      else *reinterpret_cast<P*>((T*)a.out + row * channels + c) = narrow<T, V>(y[k]);
     }
   }
 }
@@ -268,79 +289,81 @@ struct NormBackwardArgs {
 // As above; a thread adds up the weight's and the bias's gradient of its columns over all its rows, the CTA adds its
 // threads' sums in a fixed order.
 template <class T, int V, int kVecs, int kLanes>
-__global__ void __launch_bounds__(threads_for<kLanes>(), backward_ctas_for<kVecs, kLanes>())
+__global__ void __launch_bounds__(threads_for<kLanes>(), ctas_for<kLanes>(true))
 norm_backward_kernel(const NormBackwardArgs a) {
-  constexpr int kThreads = threads_for<kLanes>(), kGroups = kThreads / kLanes, kRows = rows_for<kVecs, kLanes>();
+  constexpr int kThreads = threads_for<kLanes>(), kGroups = kThreads / kLanes;
   using P = Pack<T, V>;
-  __shared__ uint32_t scratch[kLanes > 32 ? 4 * kRows * (kLanes / 32) : 1];
-  extern __shared__ float sums[];  // [2][channels] where several rows share the CTA
+  __shared__ uint32_t scratch[kLanes > 32 ? 4 * (kLanes / 32) : 1];
+  extern __shared__ float sums[];  // [warps][2][channels] where several rows share the CTA
   int turn = 0;
   const int lane = threadIdx.x % kLanes, group = threadIdx.x / kLanes;
   const int channels = a.channels;
   const int64_t rows = live_rows(a.rows, a.num_rows);
   const float inv_n = 1.f / (float)channels;
-  const int64_t stride = (int64_t)gridDim.x * kGroups * kRows;
-  int64_t row = (int64_t)blockIdx.x * kGroups * kRows + group;
+  const int64_t stride = (int64_t)gridDim.x * kGroups;
+  int64_t row = (int64_t)blockIdx.x * kGroups + group;
   const int64_t over = rows + group;
-  Stream<T, V, kVecs, kLanes> in(a.x, a.x_ld, row, stride, lane), grad(a.grad, a.grad_ld, row, stride, lane);
-  float next_mean[kRows], next_rstd[kRows];
-  auto load = [&](int64_t at) {
-    in.load(at, rows, lane, channels);
-    grad.load(at, rows, lane, channels);
-#pragma unroll
-    for (int i = 0; i < kRows; ++i) {
-      const bool has = at + i * kGroups < rows;
-      next_mean[i] = has ? __ldg(a.mean + at + i * kGroups) : 0.f, next_rstd[i] = has ? __ldg(a.rstd + at + i * kGroups) : 0.f;
-    }
+  using S = Stream<T, V, kVecs, kLanes>;
+  S in[2] = {S(a.x, a.x_ld, row, 2 * stride, lane), S(a.x, a.x_ld, row + stride, 2 * stride, lane)};
+  S grad[2] = {S(a.grad, a.grad_ld, row, 2 * stride, lane), S(a.grad, a.grad_ld, row + stride, 2 * stride, lane)};
+  float next_mean[2], next_rstd[2];
+  auto load = [&](auto which, int64_t at) {
+    constexpr int I = decltype(which)::value;
+    const bool has = at < rows;
+    in[I].load(has, lane, channels);
+    grad[I].load(has, lane, channels);
+    next_mean[I] = has ? __ldg(a.mean + at) : 0.f, next_rstd[I] = has ? __ldg(a.rstd + at) : 0.f;
   };
-  if (row < over) load(row);
-  Vec<V> w[kVecs], dw[kVecs], db[kVecs];
-  load_columns<V, kVecs, kLanes>(w, a.weight, 1.f, lane, channels);
+  load(std::integral_constant<int, 0>(), row);
+  load(std::integral_constant<int, 1>(), row + stride);
+  using Col = Columns<V, kVecs, kLanes>;
+  __shared__ __align__(16) typename Col::Store w_store;
+  const Col w(w_store, a.weight, 1.f, lane, channels);
+  if (Col::kShared) __syncthreads();
+  Vec<V> dw[kVecs], db[kVecs];
 #pragma unroll
   for (int k = 0; k < kVecs; ++k) dw[k] = db[k] = all<V>(0.f);
-  for (; row < over; row += stride) {
-    P x[kRows][kVecs], g[kRows][kVecs];
-    float shift[kRows], rstd[kRows], dot[2 * kRows];
+  auto one = [&](auto which) {
+    constexpr int I = decltype(which)::value;
+    const float rstd = next_rstd[I], shift = -next_mean[I] * rstd;
+    P x[kVecs], g[kVecs];
 #pragma unroll
-    for (int i = 0; i < kRows; ++i) {
-      rstd[i] = next_rstd[i], shift[i] = -next_mean[i] * rstd[i];
+    for (int k = 0; k < kVecs; ++k) x[k] = in[I].next[k], g[k] = grad[I].next[k];
+    load(which, row + 2 * stride);
+    Vec<V> s1 = all<V>(0.f), s2 = all<V>(0.f);
 #pragma unroll
-      for (int k = 0; k < kVecs; ++k) x[i][k] = in.next[i][k], g[i][k] = grad.next[i][k];
+    for (int k = 0; k < kVecs; ++k) {
+      // beyond the last channel gradient and weight are zeros, so xhat may be anything finite there
+      const Vec<V> hat = fma(widen<T, V>(x[k]), all<V>(rstd), all<V>(shift)), dy = widen<T, V>(g[k]), gw = mul(dy, w.at(k, lane));
+      s1 = add(s1, gw), s2 = fma(gw, hat, s2);
+      dw[k] = fma(dy, hat, dw[k]), db[k] = add(db[k], dy);
     }
-    if (row + stride < over) load(row + stride);
-#pragma unroll
-    for (int i = 0; i < kRows; ++i) {
-      Vec<V> s1 = all<V>(0.f), s2 = all<V>(0.f);
-#pragma unroll
-      for (int k = 0; k < kVecs; ++k) {
-        // beyond the last channel gradient and weight are zeros, so xhat may be anything finite there
-        const Vec<V> hat = fma(widen<T, V>(x[i][k]), all<V>(rstd[i]), all<V>(shift[i])), dy = widen<T, V>(g[i][k]), gw = mul(dy, w[k]);
-        s1 = add(s1, gw), s2 = fma(gw, hat, s2);
-        dw[k] = fma(dy, hat, dw[k]), db[k] = add(db[k], dy);
-      }
-      dot[2 * i] = across(s1), dot[2 * i + 1] = across(s2);
-    }
+    float dot[2] = {across(s1), across(s2)};
     row_reduce<kLanes>(dot, Add(), scratch, turn);
+    if (row >= rows) return;
+    // rstd (g - m1 - hat m2) with hat = x rstd + shift
+    const float m1 = dot[0] * inv_n, m2 = dot[1] * inv_n;
 #pragma unroll
-    for (int i = 0; i < kRows; ++i) {
-      const int64_t at = row + i * kGroups;
-      if (at >= rows) continue;
-      // rstd (g - m1 - hat m2) with hat = x rstd + shift
-      const float m1 = dot[2 * i] * inv_n, m2 = dot[2 * i + 1] * inv_n;
-#pragma unroll
-      for (int k = 0; k < kVecs; ++k) {
-        const int c = (k * kLanes + lane) * V;
-        if (c >= channels) continue;
-        const Vec<V> hat = fma(widen<T, V>(x[i][k]), all<V>(rstd[i]), all<V>(shift[i]));
-        Vec<V> d = fma(widen<T, V>(g[i][k]), w[k], fma(hat, all<V>(-m2), all<V>(-m1)));
-        d = mul(d, all<V>(rstd[i]));
-        if (a.grad_total) d = add(d, widen<T, V>(*reinterpret_cast<const P*>((const T*)a.grad_total + at * a.grad_total_ld + c)));
-        *reinterpret_cast<P*>((T*)a.grad_x + at * channels + c) = narrow<T, V>(d);
-      }
+    for (int k = 0; k < kVecs; ++k) {
+      const int c = (k * kLanes + lane) * V;
+      if (c >= channels) continue;
+      const Vec<V> hat = fma(widen<T, V>(x[k]), all<V>(rstd), all<V>(shift));
+      Vec<V> d = fma(widen<T, V>(g[k]), w.at(k, lane), fma(hat, all<V>(-m2), all<V>(-m1)));
+      d = mul(d, all<V>(rstd));
+      if (a.grad_total) d = add(d, widen<T, V>(*reinterpret_cast<const P*>((const T*)a.grad_total + row * a.grad_total_ld + c)));
+      *reinterpret_cast<P*>((T*)a.grad_x + row * channels + c) = narrow<T, V>(d);
     }
+  };
+  while (row < over) {
+    one(std::integral_constant<int, 0>());
+    row += stride;
+    if (row >= over) break;
+    one(std::integral_constant<int, 1>());
+    row += stride;
   }
   float* mine = a.partial + (int64_t)blockIdx.x * 2 * channels;
-  if (kGroups > 1) {
+  if (kGroups > 1) {  // the groups of a warp by shuffles, the warps through shared memory
+    float* of_warp = sums + (threadIdx.x >> 5) * 2 * channels;
 #pragma unroll
     for (int d = 16; d >= kLanes; d >>= 1)
 #pragma unroll
@@ -350,20 +373,21 @@ norm_backward_kernel(const NormBackwardArgs a) {
           dw[k].v[e] += __shfl_xor_sync(0xffffffffu, dw[k].v[e], d);
           db[k].v[e] += __shfl_xor_sync(0xffffffffu, db[k].v[e], d);
         }
-    for (int turn_of = 0; turn_of < kThreads / 32; ++turn_of) {
-      if ((int)(threadIdx.x >> 5) == turn_of && lane_id() < kLanes)
+    if (lane_id() < kLanes)
 #pragma unroll
-        for (int k = 0; k < kVecs; ++k)
+      for (int k = 0; k < kVecs; ++k)
 #pragma unroll
-          for (int e = 0; e < V; ++e) {
-            const int c = (k * kLanes + lane) * V + e;
-            if (c >= channels) continue;
-            sums[c] = turn_of ? sums[c] + dw[k].v[e] : dw[k].v[e];
-            sums[channels + c] = turn_of ? sums[channels + c] + db[k].v[e] : db[k].v[e];
-          }
-      __syncthreads();
+        for (int e = 0; e < V; ++e) {
+          const int c = (k * kLanes + lane) * V + e;
+          if (c < channels) of_warp[c] = dw[k].v[e], of_warp[channels + c] = db[k].v[e];
+        }
+    __syncthreads();
+    for (int c = threadIdx.x; c < 2 * channels; c += kThreads) {
+      float t = sums[c];
+#pragma unroll
+      for (int i = 1; i < kThreads / 32; ++i) t += sums[i * 2 * channels + c];
+      mine[c] = t;
     }
-    for (int c = threadIdx.x; c < 2 * channels; c += kThreads) mine[c] = sums[c];
   } else {
 #pragma unroll
     for (int k = 0; k < kVecs; ++k)
@@ -402,35 +426,40 @@ norm_columns_kernel(const float* __restrict__ partial, int parts, int channels, 
 
 constexpr int kMaxChannels = 8192;
 
-// f(vector length, pieces, threads of a row) for the shape that covers `pieces` pieces; each returned value is a launch.
-#define D3D_NORM_SHAPE(V, K, L) return f(std::integral_constant<int, V>(), std::integral_constant<int, K>(), std::integral_constant<int, L>())
-template <int V, class F> int by_shape(int channels, F f) {
-  const int n = (channels + V - 1) / V;
+// f(elements of a piece, pieces, threads of a row) for the shape that covers the channels: K pieces a thread up to 512 threads.
+template <int V, int K, class F> int by_shape(int channels, F f) {
+#define D3D_NORM_SHAPE(K, L) return f(std::integral_constant<int, V>(), std::integral_constant<int, K>(), std::integral_constant<int, L>())
+  const int n = (channels + V * K - 1) / (V * K);
   if constexpr (V > 1) {
-    if (n <= 2) D3D_NORM_SHAPE(V, 1, 2);
-    if (n <= 4) D3D_NORM_SHAPE(V, 1, 4);
-    if (n <= 8) D3D_NORM_SHAPE(V, 1, 8);
-    if (n <= 16) D3D_NORM_SHAPE(V, 1, 16);
-    if (n <= 32) D3D_NORM_SHAPE(V, 1, 32);
-    constexpr int K = 16 / V;  // 16 elements a thread
-    if (n <= 32 * K) D3D_NORM_SHAPE(V, K, 32);
-    if (n <= 64 * K) D3D_NORM_SHAPE(V, K, 64);
-    if (n <= 128 * K) D3D_NORM_SHAPE(V, K, 128);
-    if (n <= 256 * K) D3D_NORM_SHAPE(V, K, 256);
-    D3D_NORM_SHAPE(V, K, 512);
+    if (n <= 1) D3D_NORM_SHAPE(K, 1);
+    if (n <= 2) D3D_NORM_SHAPE(K, 2);
+    if (n <= 4) D3D_NORM_SHAPE(K, 4);
+    if (n <= 16) {
+      if (n <= 8) D3D_NORM_SHAPE(K, 8);
+      D3D_NORM_SHAPE(K, 16);
+    }
+    if (n <= 32) D3D_NORM_SHAPE(K, 32);
+    if (n <= 64) D3D_NORM_SHAPE(K, 64);
+    if (n <= 128) D3D_NORM_SHAPE(K, 128);
+    if (n <= 256) D3D_NORM_SHAPE(K, 256);
+    if (n <= 512 || V * K >= 16) D3D_NORM_SHAPE(K, 512);
+    D3D_NORM_SHAPE(16 / V, 512);
   } else {
-    if (n <= 8) D3D_NORM_SHAPE(1, 1, 8);
-    if (n <= 32) D3D_NORM_SHAPE(1, 4, 8);
-    if (n <= 128) D3D_NORM_SHAPE(1, 4, 32);
-    if (n <= 512) D3D_NORM_SHAPE(1, 8, 64);
-    if (n <= 2048) D3D_NORM_SHAPE(1, 8, 256);
-    D3D_NORM_SHAPE(1, 16, 512);
+    if (n <= 2) D3D_NORM_SHAPE(K, 2);
+    if (n <= 8) D3D_NORM_SHAPE(K, 8);
+    if (n <= 32) D3D_NORM_SHAPE(K, 32);
+    if (n <= 128) D3D_NORM_SHAPE(K, 128);
+    if (n <= 512) D3D_NORM_SHAPE(K, 512);
+    D3D_NORM_SHAPE(4 * K, 512);
   }
-}
 #undef D3D_NORM_SHAPE
+}
 
-template <class T, class F> int by_alignment(bool wide, int channels, F f) {
-  return wide ? by_shape<16 / (int)sizeof(T)>(channels, f) : by_shape<1>(channels, f);
+// Sixteen elements a thread, which keeps what the sums cost small; eight in the backward pass, where a thread has the columns' sums
+// beside them.  Rows that cannot be read in pieces: one element at a time.
+template <class T, bool kBackward, class F> int by_alignment(bool wide, int channels, F f) {
+  constexpr int V = 16 / (int)sizeof(T), K = (kBackward ? 8 : 16) / V;
+  return wide ? by_shape<V, K>(channels, f) : by_shape<1, 4>(channels, f);
 }
 template <class F> int by_type(int dtype, F f) {
   switch (dtype) {
@@ -457,9 +486,9 @@ template <class K> int resident(K kernel, int threads, size_t smem) {
 template <bool kNorm, bool kQuant> int launch_norm(int dtype, bool wide, const NormArgs& a, cudaStream_t st) {
   return by_type(dtype, [&](auto t) -> int {
     using T = decltype(t);
-    return by_alignment<T>(wide, a.channels, [&](auto v, auto k, auto l) -> int {
+    return by_alignment<T, false>(wide, a.channels, [&](auto v, auto k, auto l) -> int {
       constexpr int V = decltype(v)::value, K = decltype(k)::value, L = decltype(l)::value;
-      constexpr int per_cta = threads_for<L>() / L * rows_for<K, L>();
+      constexpr int per_cta = threads_for<L>() / L;
       auto kernel = norm_kernel<T, V, K, L, kNorm, kQuant>;
       static const int most = resident(kernel, threads_for<L>(), 0);
       const int64_t need = ceil_div(a.rows, per_cta);
@@ -570,11 +599,11 @@ extern "C" int d3d_layer_norm_backward(int dtype, const void* grad, int64_t grad
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   return by_type(dtype, [&](auto t) -> int {
     using T = decltype(t);
-    return by_alignment<T>(wide, channels, [&](auto v, auto k, auto l) -> int {
+    return by_alignment<T, true>(wide, channels, [&](auto v, auto k, auto l) -> int {
       constexpr int V = decltype(v)::value, K = decltype(k)::value, L = decltype(l)::value;
-      constexpr int per_cta = threads_for<L>() / L * rows_for<K, L>();
+      constexpr int per_cta = threads_for<L>() / L;
       const int ctas = backward_ctas(rows, per_cta);
-      const size_t smem = L <= 32 ? (size_t)2 * channels * sizeof(float) : 0;
+      const size_t smem = L <= 32 ? (size_t)(threads_for<L>() / 32) * 2 * channels * sizeof(float) : 0;
       norm_backward_kernel<T, V, K, L><<<ctas, threads_for<L>(), smem, st>>>(a);
       D3D_CHECK_LAUNCH();
       D3D_LAUNCH(true, norm_columns_kernel, (unsigned)ceil_div(2 * channels, 8), 512, 0, st, a.partial, ctas, channels, grad_weight,
