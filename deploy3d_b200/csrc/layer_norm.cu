@@ -46,6 +46,9 @@ struct Max {
   }
 };
 
+// Threads of a CTA: several rows side by side where a row has fewer.
+template <int kLanes> __host__ __device__ constexpr int threads_for() { return kLanes <= 256 ? 256 : kLanes; }
+
 // Combines N values over the kLanes threads that share a row; every thread gets the results.  Within a warp by shuffles, beyond
 // it through `scratch` (two buffers of N words a warp, used in turn: one barrier per call).
 template <int kLanes, int N, class T, class Op>
@@ -55,22 +58,22 @@ __device__ __forceinline__ void row_reduce(T (&v)[N], Op op, uint32_t* scratch, 
 #pragma unroll
     for (int i = 0; i < N; ++i) v[i] = op(v[i], __shfl_xor_sync(0xffffffffu, v[i], d));
   if (kLanes > 32) {
-    constexpr int kWarps = kLanes > 32 ? kLanes / 32 : 1;
+    constexpr int kWarps = threads_for<kLanes>() / 32, kOfRow = kLanes > 32 ? kLanes / 32 : 1;
     T* s = reinterpret_cast<T*>(scratch) + turn * (kWarps * N);
     turn ^= 1;
     if (lane_id() == 0)
 #pragma unroll
       for (int i = 0; i < N; ++i) s[(threadIdx.x >> 5) * N + i] = v[i];
     __syncthreads();
+    s += threadIdx.x / kLanes * kOfRow * N;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       v[i] = s[i];
 #pragma unroll
-      for (int w = 1; w < kWarps; ++w) v[i] = op(v[i], s[w * N + i]);
+      for (int w = 1; w < kOfRow; ++w) v[i] = op(v[i], s[w * N + i]);
     }
   }
 }
-
 template <int kLanes, class T, class Op> __device__ __forceinline__ T row_reduce(T v, Op op, uint32_t* scratch, int& turn) {
   T one[1] = {v};
   row_reduce<kLanes>(one, op, scratch, turn);
@@ -116,12 +119,10 @@ __device__ __forceinline__ float step_of(float amax, float* inv) {
   return s;
 }
 
-template <int kLanes> __host__ __device__ constexpr int threads_for() { return kLanes <= 32 ? 256 : kLanes; }
-// CTAs to an SM.  What counts is how much is on its way: a row of each of 768 threads forward, two of 512 backward, where a
-// thread holds the columns' sums as well; fewer where the parameters are in registers.
-template <int kLanes> constexpr int ctas_for(bool backward) {
-  return backward || kLanes > 32 ? (kLanes <= 256 ? 512 / threads_for<kLanes>() : 1) : 768 / threads_for<kLanes>();
-}
+// CTAs to an SM.  What counts is how much is on its way, so three, and fewer where the registers would not do: forward where the
+// parameters are in them, backward for 32-bit rows (238 k x 64 bf16, backward alone, with two CTAs / three: 30.1 / 27.5 us).
+template <int V, int kLanes> constexpr int ctas_for(bool backward) { return kLanes > 256 ? 1 : (backward ? V == 4 : kLanes > 32) ? 2 : 3; }
+constexpr int kMostBackwardCtas = 3 * kNumSMs;
 
 // A thread's pieces of the rows of a tensor that it has part in, the next ones on their way while one is summed up.  The backward
 // pass has two of them in turn, each for every other row.
@@ -197,11 +198,11 @@ template <int V, int kVecs, int kLanes> struct Columns {
 // kLanes threads share a row, kVecs pieces of V elements each.  CTAs walk over the rows, so that weight and bias are fetched once
 // per CTA.
 template <class T, int V, int kVecs, int kLanes, bool kNorm, bool kQuant>
-__global__ void __launch_bounds__(threads_for<kLanes>(), ctas_for<kLanes>(false))
+__global__ void __launch_bounds__(threads_for<kLanes>(), ctas_for<V, kLanes>(false))
 norm_kernel(const NormArgs a) {
   constexpr int kGroups = threads_for<kLanes>() / kLanes;
   using P = Pack<T, V>;
-  __shared__ uint32_t scratch[kLanes > 32 ? 2 * (kLanes / 32) : 1];
+  __shared__ uint32_t scratch[kLanes > 32 ? 2 * (threads_for<kLanes>() / 32) : 1];
   int turn = 0;
   const int lane = threadIdx.x % kLanes, group = threadIdx.x / kLanes;
   const int channels = a.channels;
@@ -274,6 +275,9 @@ norm_kernel(const NormArgs a) {
   }
 }
 
+// Sums of the columns that a CTA of the backward pass adds up in shared memory: of its warps, or of its rows where those are longer.
+template <int kLanes> __host__ __device__ constexpr int parts_for() { return threads_for<kLanes>() / (kLanes < 32 ? 32 : kLanes); }
+
 struct NormBackwardArgs {
   const void *grad, *x, *grad_total;
   int64_t grad_ld, x_ld, grad_total_ld;
@@ -289,12 +293,12 @@ struct NormBackwardArgs {
 // As above; a thread adds up the weight's and the bias's gradient of its columns over all its rows, the CTA adds its
 // threads' sums in a fixed order.
 template <class T, int V, int kVecs, int kLanes>
-__global__ void __launch_bounds__(threads_for<kLanes>(), ctas_for<kLanes>(true))
+__global__ void __launch_bounds__(threads_for<kLanes>(), ctas_for<V, kLanes>(true))
 norm_backward_kernel(const NormBackwardArgs a) {
   constexpr int kThreads = threads_for<kLanes>(), kGroups = kThreads / kLanes;
   using P = Pack<T, V>;
-  __shared__ uint32_t scratch[kLanes > 32 ? 4 * (kLanes / 32) : 1];
-  extern __shared__ float sums[];  // [warps][2][channels] where several rows share the CTA
+  __shared__ uint32_t scratch[kLanes > 32 ? 4 * (threads_for<kLanes>() / 32) : 1];
+  extern __shared__ float sums[];  // [kParts][2][channels] where several rows share the CTA
   int turn = 0;
   const int lane = threadIdx.x % kLanes, group = threadIdx.x / kLanes;
   const int channels = a.channels;
@@ -362,8 +366,9 @@ norm_backward_kernel(const NormBackwardArgs a) {
     row += stride;
   }
   float* mine = a.partial + (int64_t)blockIdx.x * 2 * channels;
-  if (kGroups > 1) {  // the groups of a warp by shuffles, the warps through shared memory
-    float* of_warp = sums + (threadIdx.x >> 5) * 2 * channels;
+  if (kGroups > 1) {  // the groups of a warp by shuffles, the others through shared memory
+    constexpr int kParts = parts_for<kLanes>();
+    float* part = sums + (kLanes < 32 ? threadIdx.x >> 5 : group) * 2 * channels;
 #pragma unroll
     for (int d = 16; d >= kLanes; d >>= 1)
 #pragma unroll
@@ -373,19 +378,19 @@ norm_backward_kernel(const NormBackwardArgs a) {
           dw[k].v[e] += __shfl_xor_sync(0xffffffffu, dw[k].v[e], d);
           db[k].v[e] += __shfl_xor_sync(0xffffffffu, db[k].v[e], d);
         }
-    if (lane_id() < kLanes)
+    if (kLanes >= 32 || lane_id() < kLanes)
 #pragma unroll
       for (int k = 0; k < kVecs; ++k)
 #pragma unroll
         for (int e = 0; e < V; ++e) {
           const int c = (k * kLanes + lane) * V + e;
-          if (c < channels) of_warp[c] = dw[k].v[e], of_warp[channels + c] = db[k].v[e];
+          if (c < channels) part[c] = dw[k].v[e], part[channels + c] = db[k].v[e];
         }
     __syncthreads();
     for (int c = threadIdx.x; c < 2 * channels; c += kThreads) {
       float t = sums[c];
 #pragma unroll
-      for (int i = 1; i < kThreads / 32; ++i) t += sums[i * 2 * channels + c];
+      for (int i = 1; i < kParts; ++i) t += sums[i * 2 * channels + c];
       mine[c] = t;
     }
   } else {
@@ -499,9 +504,9 @@ template <bool kNorm, bool kQuant> int launch_norm(int dtype, bool wide, const N
   });
 }
 
-// The backward pass keeps its sums per CTA, so that their number decides how large the workspace is.
-int backward_ctas(int64_t rows, int per_cta) {
-  const int64_t need = ceil_div(rows > 0 ? rows : 1, per_cta), most = 3 * kNumSMs;
+// The backward pass keeps its sums per CTA, so that their number decides how large the workspace is: one wave of them.
+int backward_ctas(int64_t rows, int per_cta, int64_t most) {
+  const int64_t need = ceil_div(rows > 0 ? rows : 1, per_cta);
   return (int)(need < most ? need : most);
 }
 
@@ -571,7 +576,7 @@ extern "C" int d3d_quantize_rows(int dtype, const void* x, int64_t x_ld, int64_t
 
 extern "C" size_t d3d_layer_norm_backward_workspace(int64_t rows, int channels) {
   if (rows < 0 || channels < 1) return 0;
-  return (size_t)backward_ctas(rows, 1) * 2 * channels * sizeof(float);
+  return (size_t)backward_ctas(rows, 1, kMostBackwardCtas) * 2 * channels * sizeof(float);
 }
 
 extern "C" int d3d_layer_norm_backward(int dtype, const void* grad, int64_t grad_ld, const void* x, int64_t x_ld,
@@ -602,8 +607,8 @@ extern "C" int d3d_layer_norm_backward(int dtype, const void* grad, int64_t grad
     return by_alignment<T, true>(wide, channels, [&](auto v, auto k, auto l) -> int {
       constexpr int V = decltype(v)::value, K = decltype(k)::value, L = decltype(l)::value;
       constexpr int per_cta = threads_for<L>() / L;
-      const int ctas = backward_ctas(rows, per_cta);
-      const size_t smem = L <= 32 ? (size_t)(threads_for<L>() / 32) * 2 * channels * sizeof(float) : 0;
+      const int ctas = backward_ctas(rows, per_cta, ctas_for<V, L>(true) * kNumSMs);
+      const size_t smem = threads_for<L>() > L ? (size_t)parts_for<L>() * 2 * channels * sizeof(float) : 0;
       norm_backward_kernel<T, V, K, L><<<ctas, threads_for<L>(), smem, st>>>(a);
       D3D_CHECK_LAUNCH();
       D3D_LAUNCH(true, norm_columns_kernel, (unsigned)ceil_div(2 * channels, 8), 512, 0, st, a.partial, ctas, channels, grad_weight,
