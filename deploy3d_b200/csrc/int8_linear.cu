@@ -11,14 +11,13 @@
 
 #include "common.cuh"
 #include "kernel_errors.h"
+#include "packed.cuh"
 #include "tc_ptx.cuh"
 
 namespace d3d {
 namespace {
 
 __device__ int g_int8_error;  // 0 ok; otherwise the code of the first wait that gave up
-
-template <class T, int V> struct alignas(sizeof(T) * V) Pack { T v[V]; };
 
 struct LinearArgs {
   const int8_t *x, *w;
@@ -89,30 +88,34 @@ constexpr int kTileRows = 128;    // rows of a CTA
 constexpr int kBlockK = 128;      // channels of the sum a stage holds: one 128-byte swizzled row
 constexpr int kMaxStages = 8;
 constexpr int kMaxCols = 256;     // output channels of a tile
-constexpr int kEpilogueWarps = 8;
+constexpr int kMaxAcc = 8;        // accumulators in tensor memory, whose 512 columns hold two of the widest tiles
+constexpr int kEpilogueSets = 4;  // of four warps, one for each quarter of an accumulator's lanes
+constexpr int kEpilogueWarps = 4 * kEpilogueSets;
 constexpr int kThreads = (kEpilogueWarps + 2) * 32;
-constexpr int kStagePitch = 144;  // bytes of a row of the epilogue's staging: 128 and a shift of four banks from row to row
+constexpr int kPiece = 64;             // bytes of a row that an epilogue warp puts in order at a time
+constexpr int kStaging = 32 * kPiece;  // of its 32 rows
 constexpr uint32_t kABytes = kTileRows * kBlockK;
 
 struct TcArgs {
   LinearArgs l;
   int cols;        // output channels of a tile
   int col_tiles;
-  int stages, k_blocks;
+  uint64_t inverse;  // of col_tiles, see Tiles
+  int stages, k_blocks, accs;
   uint32_t stage_bytes;
   uint32_t idesc;
-  int out_wide;    // rows of the output start on 16 bytes
+  int out_wide;    // rows of the output start on 16 bytes: it has a map
 };
 
 struct Shared {
   uint64_t full[kMaxStages];   // TMA -> MMA
   uint64_t empty[kMaxStages];  // MMA -> TMA
-  uint64_t acc_full[2];        // MMA -> epilogue
-  uint64_t acc_empty[2];       // epilogue -> MMA
+  uint64_t acc_full[kMaxAcc];   // MMA -> epilogue
+  uint64_t acc_empty[kMaxAcc];  // epilogue -> MMA
   uint64_t drained;            // MMA, where a wait has given up: the products on their way
   uint32_t tmem;
   int abort;
-  alignas(16) float scale[2][2][kMaxCols];  // by tile parity: weight scales, bias
+  alignas(16) float scale[kEpilogueWarps][2][32];  // of a warp's piece: weight scales, bias
 };
 
 __device__ __forceinline__ uint32_t cluster_rank() {
@@ -170,31 +173,44 @@ template <int kCta> __device__ __forceinline__ void free_tmem(uint32_t addr) {
   if (kCta == 1) tmem_dealloc(addr, 512);
   else asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 512;" ::"r"(addr) : "memory");
 }
-// K-major operand, 128-byte swizzle: groups of eight rows 1024 bytes apart; 32 channels further is 32 bytes further.
-__device__ __forceinline__ uint64_t operand(uint32_t smem_addr) {
-  return (uint64_t)((smem_addr & 0x3FFFFu) >> 4) | (1ull << 16) | (64ull << 32) | (1ull << 46) | (2ull << 61);
-}
-
+// This CTA's (pair's) tiles: first, first + step, ... below count.  Eight rows of tiles go side by side, so that what is worked
+// on at a time needs as few rows and weights as can be (8192 x 4096 -> 8192: 74 tiles one row after the other need all
+// weights).
 struct Tiles {
-  int first, step, count;  // this CTA's (pair's) tiles: first, first + step, ... below count
+  int first, step, count, row_tiles, col_tiles;
+  uint64_t inverse;  // 2^40 / col_tiles, rounded up
+  __device__ __forceinline__ int2 at(int t) const {  // row, column
+    if (col_tiles == 1) return make_int2(t, 0);
+    // t / 8 < 2^27 and fewer than 2^13 columns of tiles: the quotient is exact
+    const int b = (int)(((uint64_t)(uint32_t)(t >> 3) * inverse) >> 40), r = t - b * 8 * col_tiles;
+    if (8 * b + 8 <= row_tiles) return make_int2(8 * b + (r & 7), r >> 3);
+    const int high = row_tiles - 8 * b;  // the last rows
+    return make_int2(8 * b + r % high, r / high);
+  }
 };
-
+// A box of this warp's staging to the output.
+__device__ __forceinline__ void store_box(const CUtensorMap* map, const void* src, int x, int y) {
+  asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%2, %3}], [%1];"
+               ::"l"((uint64_t)map), "r"(smem_u32(src)), "r"(x), "r"(y) : "memory");
+  asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+}
 // kCta CTAs share a tile of kCta * 128 rows: each holds its rows and its share of the weight rows, CTA 0 issues the products.
 template <int kCta, class T>
 __global__ void __launch_bounds__(kThreads, 1)
-linear_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w, const TcArgs p) {
+linear_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w,
+              const __grid_constant__ CUtensorMap map_out, const TcArgs p) {
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   unsigned char* ring = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   unsigned char* staging = ring + p.stages * p.stage_bytes;
-  Shared* sh = reinterpret_cast<Shared*>(staging + kEpilogueWarps * 32 * kStagePitch);
+  Shared* sh = reinterpret_cast<Shared*>(staging + kEpilogueWarps * kStaging);
   const int warp = threadIdx.x >> 5, lane = lane_id();
   const uint32_t rank = kCta == 1 ? 0 : cluster_rank();
   const int64_t rows = live_rows(p.l.rows, p.l.num_rows);
-  const Tiles tiles = {(int)(blockIdx.x / kCta), (int)(gridDim.x / kCta),
-                       (int)((rows + kCta * kTileRows - 1) / (kCta * kTileRows)) * p.col_tiles};
+  const int row_tiles = (int)((rows + kCta * kTileRows - 1) / (kCta * kTileRows));
+  const Tiles tiles = {(int)(blockIdx.x / kCta), (int)(gridDim.x / kCta), row_tiles * p.col_tiles, row_tiles, p.col_tiles, p.inverse};
   if (threadIdx.x == 0) {
     for (int s = 0; s < kMaxStages; ++s) mbar_init(&sh->full[s], 1), mbar_init(&sh->empty[s], 1);
-    for (int b = 0; b < 2; ++b) mbar_init(&sh->acc_full[b], 1), mbar_init(&sh->acc_empty[b], kCta * kEpilogueWarps);
+    for (int b = 0; b < kMaxAcc; ++b) mbar_init(&sh->acc_full[b], 1), mbar_init(&sh->acc_empty[b], kCta * kEpilogueWarps);
     mbar_init(&sh->drained, 1);
     sh->abort = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -212,8 +228,8 @@ linear_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__
       int stage = 0, phase = 0;
       bool ok = true;
       for (int t = tiles.first; ok && t < tiles.count; t += tiles.step) {
-        const int m0 = (t / p.col_tiles * kCta + (int)rank) * kTileRows;
-        const int n0 = t % p.col_tiles * p.cols + (int)rank * (p.cols / kCta);
+        const int2 tile = tiles.at(t);
+        const int m0 = (tile.x * kCta + (int)rank) * kTileRows, n0 = tile.y * p.cols + (int)rank * (p.cols / kCta);
         for (int k = 0; k < p.k_blocks; ++k) {
           ok = mbar_wait(&sh->empty[stage], phase ^ 1, abort_flag, 1, kWaitLimitCycles);
           if (!ok) break;
@@ -229,109 +245,146 @@ linear_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__
         for (int s = 0; s < p.stages; ++s) mbar_drain(&sh->full[s], s < stage ? phase : phase ^ 1);
     }
   } else if (warp == kEpilogueWarps + 1) {
-    if (lane == 0 && rank == 0) {
-      int stage = 0, phase = 0, buf = 0, acc_phase = 0;
-      bool ok = true;
+    // The whole warp walks by counters and one lane of it waits and issues: what feeds an MMA has to be the same for all lanes in a
+    // way the compiler can see.  By a loop of one lane four products and a commit took 566 cycles where the tensor cores want
+    // 512, and with the wait in front of them 840.
+    if (rank == 0) {
+      constexpr uint32_t kHigh = 64u | (1u << 14) | (2u << 29);  // rows in groups of eight 1024 bytes apart, 128-byte swizzle
+      const uint32_t low0 = ((smem_u32(ring) & 0x3FFFFu) >> 4) | (1u << 16), low_step = p.stage_bytes >> 4;
       const int last = (p.l.inputs - (p.k_blocks - 1) * kBlockK + 31) / 32;  // products of the last stage
-      for (int t = tiles.first; ok && t < tiles.count; t += tiles.step) {
-        ok = mbar_wait(&sh->acc_empty[buf], acc_phase ^ 1, abort_flag, 2, kWaitLimitCycles);
-        if (!ok) break;
+      int stage = 0, phase = 0, buf = 0, acc_phase = 0;
+      bool bad = false;
+      for (int t = tiles.first; t < tiles.count; t += tiles.step) {
+        if (!bad) bad = !mbar_wait(&sh->acc_empty[buf], acc_phase ^ 1, abort_flag, 2, kWaitLimitCycles);
+        bad = __any_sync(0xffffffffu, bad);
+        if (bad) break;
         tc_fence_after();
-        const uint32_t d = tmem + buf * kMaxCols;
+        const uint32_t d = tmem + buf * p.cols;
         for (int k = 0; k < p.k_blocks; ++k) {
-          ok = mbar_wait(&sh->full[stage], phase, abort_flag, 3, kWaitLimitCycles);
-          if (!ok) break;
-          tc_fence_after();
-          const uint32_t at = smem_u32(ring + stage * p.stage_bytes);
-          const uint64_t da = operand(at), db = operand(at + kABytes);
+          const uint32_t low = low0 + stage * low_step;
+          const uint64_t da = (uint64_t)kHigh << 32 | low, db = (uint64_t)kHigh << 32 | (low + (kABytes >> 4));
           const int n = k == p.k_blocks - 1 ? last : 4;
-          for (int i = 0; i < n; ++i) mma_i8<kCta>(d, da + 2 * i, db + 2 * i, p.idesc, k > 0 || i > 0);
-          commit<kCta>(&sh->empty[stage]);
+          if (elect_one()) {
+            if (!bad) bad = !mbar_wait(&sh->full[stage], phase, abort_flag, 3, kWaitLimitCycles);
+            if (!bad) {
+              tc_fence_after();
+              // 32 channels further is 32 bytes further
+              mma_i8<kCta>(d, da, db, p.idesc, k > 0);
+              if (n > 1) mma_i8<kCta>(d, da + 2, db + 2, p.idesc, 1);
+              if (n > 2) mma_i8<kCta>(d, da + 4, db + 4, p.idesc, 1);
+              if (n > 3) mma_i8<kCta>(d, da + 6, db + 6, p.idesc, 1);
+              commit<kCta>(&sh->empty[stage]);
+              if (k == p.k_blocks - 1) commit<kCta>(&sh->acc_full[buf]);
+            }
+          }
+          __syncwarp();
           if (++stage == p.stages) stage = 0, phase ^= 1;
         }
-        if (!ok) break;
-        commit<kCta>(&sh->acc_full[buf]);
-        if (++buf == 2) buf = 0, acc_phase ^= 1;
+        if (++buf == p.accs) buf = 0, acc_phase ^= 1;
       }
-      if (!ok) {
+      if (__any_sync(0xffffffffu, bad) && elect_one()) {
         commit<kCta>(&sh->drained);
         mbar_drain(&sh->drained, 0);
       }
     }
   } else {
-    // Two sets of four warps; a warp reads its quarter of the accumulator's lanes, the sets take turns in the columns.
-    constexpr int kCols = 128 / (int)sizeof(T);  // columns of a 128-byte piece
+    // Four sets of four warps; a warp reads its quarter of the accumulator's lanes, the sets take turns in pieces of 64 bytes a row,
+    // over the ends of tiles.  What such a piece takes is a chain of trips (tensor memory, scales, shared memory, the store), so it
+    // is warps that count, and nothing that makes them wait for each other: with two sets of 128 bytes and a barrier a tile 238 k
+    // rows of 64 -> 192 took 55 us.  A piece goes through shared memory, 16 bytes of row r at place j ^ (r / 2) of four, which
+    // is what a tensor map with 64-byte swizzle takes out.
+    constexpr int kCols = kPiece / (int)sizeof(T);  // columns of a piece
     constexpr int kVec = 16 / (int)sizeof(T);
-    const int quarter = warp & 3, set = warp >> 2;
-    unsigned char* mine = staging + warp * 32 * kStagePitch;
+    const int quarter = warp & 3, set = warp >> 2, pieces = p.cols / kCols;
+    unsigned char* mine = staging + warp * kStaging;
+    float *ws = sh->scale[warp][0], *bs = sh->scale[warp][1];
+    // the warp's next piece, whose scales, a column and a row a lane, are on their way
+    int next_t = tiles.first, piece = set, of_tile = -1;
+    int m = 0, n_tile = 0;
+    float next_w = 0.f, next_b = 0.f, next_x = 0.f;
+    auto ask = [&] {
+      while (piece >= pieces) piece -= pieces, next_t += tiles.step;
+      if (next_t >= tiles.count) return;
+      if (next_t != of_tile) {
+        const int2 tile = tiles.at(next_t);
+        m = (tile.x * kCta + (int)rank) * kTileRows + quarter * 32, n_tile = tile.y * p.cols, of_tile = next_t;
+        next_x = m + lane < rows ? __ldg(p.l.x_scale + m + lane) : 0.f;
+      }
+      const int n = n_tile + piece * kCols + lane;
+      const bool in = lane < kCols && n < p.l.outputs;
+      next_w = in ? __ldg(p.l.w_scale + n) : 0.f, next_b = in && p.l.bias ? __ldg(p.l.bias + n) : 0.f;
+    };
+    ask();
     int buf = 0, acc_phase = 0;
-    bool ok = true;
     for (int t = tiles.first; t < tiles.count; t += tiles.step) {
-      const int64_t m0 = ((int64_t)(t / p.col_tiles) * kCta + rank) * kTileRows + quarter * 32;
-      const int n0 = t % p.col_tiles * p.cols;
-      float* scale = sh->scale[buf][0];
-      for (int c = threadIdx.x; c < p.cols; c += kEpilogueWarps * 32) {
-        const bool in = n0 + c < p.l.outputs;
-        scale[c] = in ? __ldg(p.l.w_scale + n0 + c) : 0.f;
-        scale[kMaxCols + c] = in && p.l.bias ? __ldg(p.l.bias + n0 + c) : 0.f;
-      }
-      const float xs = m0 + lane < rows ? __ldg(p.l.x_scale + m0 + lane) : 0.f;
-      asm volatile("bar.sync 1, %0;" ::"n"(kEpilogueWarps * 32) : "memory");
-      // a warp whose wait gave up still comes to the barriers of the others
-      if (ok) ok = mbar_wait(&sh->acc_full[buf], acc_phase, abort_flag, 4, kWaitLimitCycles);
-      ok = __all_sync(0xffffffffu, ok);
-      if (!ok) continue;
+      const bool ok = mbar_wait(&sh->acc_full[buf], acc_phase, abort_flag, 4, kWaitLimitCycles);
+      if (!__all_sync(0xffffffffu, ok)) break;
       tc_fence_after();
-      const uint32_t acc = tmem + buf * kMaxCols + ((uint32_t)(quarter * 32) << 16);
-      for (int c0 = set * kCols; c0 < p.cols; c0 += 2 * kCols) {
+      // What the MMA warp waits for is that all have loaded, not that they are done.
+      auto loaded = [&] {
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) arrive_leader<kCta>(&sh->acc_empty[buf]);
+      };
+      if (next_t != t) loaded();
+      while (next_t == t) {
+        const uint32_t acc = tmem + buf * p.cols + ((uint32_t)(quarter * 32) << 16) + piece * kCols;
+        uint32_t r[kCols];
 #pragma unroll
-        for (int h = 0; h < kCols; h += 16) {
-          if (c0 + h >= p.cols) break;
-          uint32_t r[16];
-          tmem_ld16(acc + c0 + h, r);
-          tmem_ld_wait(r);
-          const float4* ws = reinterpret_cast<const float4*>(scale + c0 + h);
-          const float4* bs = reinterpret_cast<const float4*>(scale + kMaxCols + c0 + h);
-          alignas(16) T v[16];
+        for (int h = 0; h < kCols; h += 16) tmem_ld16(acc + h, r + h);
+        const int64_t row0 = m;
+        const int col0 = n_tile + piece * kCols;
+        const float xs = next_x;
+        if (lane < kCols) ws[lane] = next_w, bs[lane] = next_b;
+        if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");  // the piece before has left
+        __syncwarp();
+        piece += kEpilogueSets;
+        ask();
+        asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 #pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            const float4 w4 = ws[q], b4 = bs[q];
-            v[4 * q] = from_f32<T>(fmaf((float)(int)r[4 * q] * w4.x, xs, b4.x));
-            v[4 * q + 1] = from_f32<T>(fmaf((float)(int)r[4 * q + 1] * w4.y, xs, b4.y));
-            v[4 * q + 2] = from_f32<T>(fmaf((float)(int)r[4 * q + 2] * w4.z, xs, b4.z));
-            v[4 * q + 3] = from_f32<T>(fmaf((float)(int)r[4 * q + 3] * w4.w, xs, b4.w));
+        for (int h = 0; h < kCols; ++h) asm volatile("" : "+r"(r[h]));
+        if (next_t != t) loaded();
+#pragma unroll
+        for (int j = 0; j < kPiece / 16; ++j) {
+          Vec<kVec> v, w, b;
+#pragma unroll
+          for (int q = 0; q < kVec; q += 4) {
+            *reinterpret_cast<float4*>(&w.v[q]) = *reinterpret_cast<const float4*>(ws + j * kVec + q);
+            *reinterpret_cast<float4*>(&b.v[q]) = *reinterpret_cast<const float4*>(bs + j * kVec + q);
           }
-          uint4* to = reinterpret_cast<uint4*>(mine + lane * kStagePitch + h * sizeof(T));
 #pragma unroll
-          for (int q = 0; q < (int)sizeof(T); ++q) to[q] = reinterpret_cast<const uint4*>(v)[q];
+          for (int e = 0; e < kVec; ++e) v.v[e] = (float)(int)r[j * kVec + e];
+          v = fma(mul(v, w), all<kVec>(xs), b);
+          *reinterpret_cast<Pack<T, kVec>*>(mine + lane * kPiece + ((j ^ (lane >> 1 & 3)) * 16)) = narrow<T, kVec>(v);
         }
-        __syncwarp();
-        const int n = n0 + c0;
-        if (p.out_wide) {  // eight lanes to a row
-          const int c = n + lane % 8 * kVec;
-          if (c0 + lane % 8 * kVec < p.cols && c < p.l.outputs)
+        if (p.out_wide && row0 + 32 <= rows) {
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+          __syncwarp();
+          if (lane == 0) store_box(&map_out, mine, col0, (int)row0);
+        } else if (p.out_wide) {  // four lanes to a row, up to the last one
+          __syncwarp();
+          const int j = lane % 4, c = col0 + j * kVec;
+          if (c < p.l.outputs)
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              const int row = 4 * i + lane / 8;
-              if (m0 + row < rows)
-                *reinterpret_cast<uint4*>((T*)p.l.out + (m0 + row) * p.l.outputs + c) =
-                    *reinterpret_cast<const uint4*>(mine + row * kStagePitch + lane % 8 * 16);
+            for (int i = 0; i < 4; ++i) {
+              const int row = 8 * i + lane / 4;
+              if (row0 + row < rows)
+                *reinterpret_cast<uint4*>((T*)p.l.out + (row0 + row) * p.l.outputs + c) =
+                    *reinterpret_cast<const uint4*>(mine + row * kPiece + ((j ^ (row >> 1 & 3)) * 16));
             }
-        } else {
-          for (int row = 0; row < 32 && m0 + row < rows; ++row)
-#pragma unroll
-            for (int h = 0; h < kCols; h += 32)
-              if (c0 + h + lane < p.cols && n + h + lane < p.l.outputs)
-                ((T*)p.l.out)[(m0 + row) * p.l.outputs + n + h + lane] =
-                    reinterpret_cast<const T*>(mine + row * kStagePitch)[h + lane];
+        } else {  // an element a lane
+          __syncwarp();
+          const int c = lane % kCols;
+          T* out = (T*)p.l.out + (row0 + lane / kCols) * p.l.outputs + col0 + c;
+#pragma unroll 8
+          for (int row = lane / kCols; row < 32; row += 32 / kCols, out += (int64_t)(32 / kCols) * p.l.outputs)
+            if (row0 + row < rows && col0 + c < p.l.outputs)
+              *out = reinterpret_cast<const T*>(mine + row * kPiece + ((c / kVec ^ (row >> 1 & 3)) * 16))[c % kVec];
         }
-        __syncwarp();
       }
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) arrive_leader<kCta>(&sh->acc_empty[buf]);
-      if (++buf == 2) buf = 0, acc_phase ^= 1;
+      if (++buf == p.accs) buf = 0, acc_phase ^= 1;
     }
+    if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
   }
   __syncwarp();
   tc_fence_before();
@@ -363,13 +416,16 @@ constexpr int kMaxInputs = 65536, kMaxOutputs = 65536;
 
 bool aligned_rows(const void* p, int64_t ld) { return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld % 16 == 0; }
 
-bool byte_map(CUtensorMap* map, const void* base, uint64_t cols, uint64_t rows, uint64_t pitch, uint32_t box_rows) {
+// Map over rows `pitch` bytes apart; boxes of box_bytes (64 or 128) by box_rows, swizzled.
+bool make_map(CUtensorMap* map, CUtensorMapDataType type, int esize, const void* base, uint64_t cols, uint64_t rows, uint64_t pitch,
+              uint32_t box_bytes, uint32_t box_rows) {
   EncodeTiledFn fn = encode_fn();
   if (!fn) return false;
   cuuint64_t dims[2] = {cols, rows}, strides[1] = {pitch};
-  cuuint32_t box[2] = {kBlockK, box_rows}, elem[2] = {1, 1};
-  return fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
-            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+  cuuint32_t box[2] = {box_bytes / esize, box_rows}, elem[2] = {1, 1};
+  return fn(map, type, 2, const_cast<void*>(base), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
+            box_bytes == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 template <class T> int launch_few(const LinearArgs& a, cudaStream_t st) {
@@ -395,16 +451,23 @@ template <int kCta, class T> int launch_tiles(const LinearArgs& a, int cols, cud
   p.l = a;
   p.cols = cols;
   p.col_tiles = (int)ceil_div(a.outputs, cols);
+  p.inverse = ((1ull << 40) + p.col_tiles - 1) / p.col_tiles;
   p.k_blocks = (int)ceil_div(a.inputs, kBlockK);
+  p.accs = 512 / cols < kMaxAcc ? 512 / cols : kMaxAcc;
   p.stage_bytes = kABytes + (uint32_t)(cols / kCta) * kBlockK;
-  const size_t fixed = 1024 + kEpilogueWarps * 32 * kStagePitch + sizeof(Shared);
+  const size_t fixed = 1024 + kEpilogueWarps * kStaging + sizeof(Shared);
   p.stages = (int)((227 * 1024 - fixed) / p.stage_bytes);
   if (p.stages > kMaxStages) p.stages = kMaxStages;
   // D 32-bit integers, A and B signed
   p.idesc = (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(cols >> 3) << 17) | ((uint32_t)(kCta * kTileRows >> 4) << 24);
   p.out_wide = reinterpret_cast<uintptr_t>(a.out) % 16 == 0 && (int64_t)a.outputs * sizeof(T) % 16 == 0;
-  CUtensorMap map_x, map_w;
-  if (!byte_map(&map_x, a.x, a.inputs, a.rows, a.x_ld, kTileRows) || !byte_map(&map_w, a.w, a.inputs, a.outputs, a.w_ld, cols / kCta))
+  CUtensorMap map_x, map_w, map_out = {};
+  constexpr CUtensorMapDataType kType = sizeof(T) == 4                        ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                                        : std::is_same<T, __half>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                                                                         : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+  if (!make_map(&map_x, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, a.x, a.inputs, a.rows, a.x_ld, kBlockK, kTileRows) ||
+      !make_map(&map_w, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, a.w, a.inputs, a.outputs, a.w_ld, kBlockK, cols / kCta) ||
+      (p.out_wide && !make_map(&map_out, kType, sizeof(T), a.out, a.outputs, a.rows, a.outputs * sizeof(T), kPiece, 32)))
     return D3D_ERR_CUDA;
   auto kernel = linear_kernel<kCta, T>;
   {
@@ -426,12 +489,12 @@ template <int kCta, class T> int launch_tiles(const LinearArgs& a, int cols, cud
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = kCta, attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr, cfg.numAttrs = 1;
-  if (cudaLaunchKernelEx(&cfg, kernel, map_x, map_w, p) != cudaSuccess) return D3D_ERR_CUDA;
+  if (cudaLaunchKernelEx(&cfg, kernel, map_x, map_w, map_out, p) != cudaSuccess) return D3D_ERR_CUDA;
   D3D_CHECK_LAUNCH();
   return D3D_OK;
 }
 
-// Output channels of a tile: as many as fill the tiles evenly, fewer where the GPU would not be filled.
+// Output channels of a tile: as many as fill the tiles evenly, fewer where the GPU would not be filled; whole multiples of `unit`.
 int tile_cols(int64_t row_tiles, int outputs, int unit, int units) {
   const int64_t want = ceil_div(units, row_tiles);          // column tiles that occupy everything
   int64_t n = ceil_div(outputs, kMaxCols);
@@ -440,10 +503,17 @@ int tile_cols(int64_t row_tiles, int outputs, int unit, int units) {
   return cols < unit ? unit : cols;
 }
 
+// Two CTAs to a tile, which halves what the weights cost, for long sums over enough tiles; short ones are bound by the epilogue,
+// where a pair waits for the slower one.  us with one / two: 66 k rows, 512 outputs, 512 inputs 26.8 / 34.1, 1024 39.0 / 39.5,
+// 2048 65.9 / 57.2; 16 k rows, 1024 outputs, 1024 inputs 21.0 / 22.7, 2048 32.9 / 30.9; 8192 x 4096 -> 8192 207 / 178.
+// The products want multiples of 16 channels, of 32 with two CTAs, and the output leaves in pieces of 64 bytes a row, which tiles
+// consist of.
 template <class T> int launch_linear(const LinearArgs& a, cudaStream_t st) {
+  constexpr int kCols = kPiece / (int)sizeof(T);
   const int64_t pairs = ceil_div(a.rows, 2 * kTileRows) * ceil_div(a.outputs, kMaxCols);
-  if (pairs >= kNumSMs / 2) return launch_tiles<2, T>(a, tile_cols(ceil_div(a.rows, 2 * kTileRows), a.outputs, 32, kNumSMs / 2), st);
-  return launch_tiles<1, T>(a, tile_cols(ceil_div(a.rows, kTileRows), a.outputs, 16, kNumSMs), st);
+  if (pairs >= kNumSMs / 2 && a.inputs > 1024)
+    return launch_tiles<2, T>(a, tile_cols(ceil_div(a.rows, 2 * kTileRows), a.outputs, 32, kNumSMs / 2), st);
+  return launch_tiles<1, T>(a, tile_cols(ceil_div(a.rows, kTileRows), a.outputs, kCols, kNumSMs), st);
 }
 
 size_t repitched(const void* p, int64_t ld, int64_t rows, int channels) {

@@ -437,26 +437,18 @@ template <int V, int K, class F> int by_shape(int channels, F f) {
   const int n = (channels + V * K - 1) / (V * K);
   if constexpr (V > 1) {
     if (n <= 1) D3D_NORM_SHAPE(K, 1);
-    if (n <= 2) D3D_NORM_SHAPE(K, 2);
-    if (n <= 4) D3D_NORM_SHAPE(K, 4);
-    if (n <= 16) {
-      if (n <= 8) D3D_NORM_SHAPE(K, 8);
-      D3D_NORM_SHAPE(K, 16);
-    }
-    if (n <= 32) D3D_NORM_SHAPE(K, 32);
-    if (n <= 64) D3D_NORM_SHAPE(K, 64);
-    if (n <= 128) D3D_NORM_SHAPE(K, 128);
-    if (n <= 256) D3D_NORM_SHAPE(K, 256);
-    if (n <= 512 || V * K >= 16) D3D_NORM_SHAPE(K, 512);
-    D3D_NORM_SHAPE(16 / V, 512);
-  } else {
-    if (n <= 2) D3D_NORM_SHAPE(K, 2);
-    if (n <= 8) D3D_NORM_SHAPE(K, 8);
-    if (n <= 32) D3D_NORM_SHAPE(K, 32);
-    if (n <= 128) D3D_NORM_SHAPE(K, 128);
-    if (n <= 512) D3D_NORM_SHAPE(K, 512);
-    D3D_NORM_SHAPE(4 * K, 512);
   }
+  if (n <= 2) D3D_NORM_SHAPE(K, 2);
+  if (n <= 4) D3D_NORM_SHAPE(K, 4);
+  if (n <= 8) D3D_NORM_SHAPE(K, 8);
+  if (n <= 16) D3D_NORM_SHAPE(K, 16);
+  if (n <= 32) D3D_NORM_SHAPE(K, 32);
+  if (n <= 64) D3D_NORM_SHAPE(K, 64);
+  if (n <= 128) D3D_NORM_SHAPE(K, 128);
+  if (n <= 256) D3D_NORM_SHAPE(K, 256);
+  if (n <= 512 || V * K >= 16) D3D_NORM_SHAPE(K, 512);
+  if constexpr (V * K < 16) D3D_NORM_SHAPE(16 / V, 512);
+  return D3D_ERR_TOO_LARGE;
 #undef D3D_NORM_SHAPE
 }
 

@@ -10,7 +10,7 @@ namespace {
 template <class T, int V> struct alignas(sizeof(T) * V) Pack { T v[V]; };
 
 // The channels of a thread in 32 bits; two at a time are worked on by packed instructions.
-template <int V> struct Vec { float v[V]; };
+template <int V> struct alignas(V % 4 == 0 ? 16 : V % 2 == 0 ? 8 : 4) Vec { float v[V]; };
 template <int V> __device__ __forceinline__ Vec<V> all(float x) {
   Vec<V> r;
 #pragma unroll

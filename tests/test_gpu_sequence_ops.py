@@ -439,7 +439,7 @@ def test_linear_of_few_rows(d3d, layout, rows, inputs, outputs):
 @pytest.mark.parametrize("layout", ["dense", "columns", "odd"])
 @pytest.mark.parametrize("rows,inputs,outputs", [
     (9, 16, 16), (9, 1, 1), (127, 128, 64), (128, 96, 32), (129, 131, 40), (300, 64, 192), (257, 1000, 387), (40, 4096, 520),
-    (1000, 32, 1030), (20000, 48, 24), (20000, 144, 300), (9500, 640, 515)])
+    (1000, 32, 1030), (20000, 48, 24), (20000, 144, 300), (9500, 640, 515), (9500, 1040, 515), (9500, 2000, 520)])
 def test_linear(d3d, dtype, layout, rows, inputs, outputs):
     """One and two CTAs to a tile, one tile and several to a CTA, ends of every kind."""
     x, w = int8(1, rows, inputs, layout), int8(2, outputs, inputs, layout)
