@@ -2,10 +2,10 @@
 //   out[m][n] = x_scale[m] w_scale[n] sum_k q[m][k] w[n][k] + bias[n]
 // The sum is exact (32-bit integers, |sum| <= 2^14 k), the rest is three 32-bit operations and one rounding.
 //
-// Two kernels.  From kFewRows rows on, tcgen05.mma (kind::i8, K = 32 per instruction) over tiles of 128 or, with two CTAs to a
-// tile, 256 rows by up to 256 output channels: operands by TMA in 128-byte rows (128 channels of the sum a stage), accumulators of
-// two tiles in tensor memory so that the epilogue of one runs beside the products of the next.  Fewer rows: the weights are
-// what is read, once, and four-way dot products keep up with that.
+// tcgen05.mma (kind::i8, K = 32 per instruction) over tiles of 128 or, with two CTAs to a tile, 256 rows by up to 256 output
+// channels: operands by TMA in 128-byte rows (128 channels of the sum a stage), several accumulators in tensor memory so that
+// the epilogue of one tile runs beside the products of the next.  Up to kFewRows rows: the other way round, tiles of 128 output
+// channels by all rows.  Little work is left to the integer units.
 #include <mutex>
 #include <type_traits>
 
@@ -35,29 +35,29 @@ __device__ __forceinline__ int64_t live_rows(int64_t rows, const int32_t* num_ro
   return n < 0 ? 0 : n < rows ? n : rows;
 }
 
-// ---- few rows ---------------------------------------------------------------------------------------------------------
-// A warp per output channel: its weights stream by once, every lane multiplies its pieces with those of kM rows.
-// kBytes: what one load takes (16 where rows start on 16 bytes, else one).
+// ---- little work ------------------------------------------------------------------------------------------------------
+// A warp per output channel: its weights stream by once, eight pieces of a lane on their way, and are multiplied with those of kM
+// rows.  kBytes: what one load takes (16 where rows start on 16 bytes, else one).
 template <class T, int kM, int kBytes>
 __global__ void __launch_bounds__(256)
-few_rows_kernel(const LinearArgs a) {
+dot_kernel(const LinearArgs a) {
   const int64_t rows = live_rows(a.rows, a.num_rows);
   const int64_t m0 = (int64_t)blockIdx.y * kM;
   if (m0 >= rows) return;
   const int n = blockIdx.x * 8 + (threadIdx.x >> 5), lane = lane_id();
   if (n >= a.outputs) return;
   const int8_t* w = a.w + (int64_t)n * a.w_ld;
+  const float ws = __ldg(a.w_scale + n), b = a.bias ? __ldg(a.bias + n) : 0.f;
+  const float xs = lane < kM && m0 + lane < rows ? __ldg(a.x_scale + m0 + lane) : 0.f;
+  const int8_t* x[kM];
   int acc[kM];
 #pragma unroll
-  for (int m = 0; m < kM; ++m) acc[m] = 0;
+  for (int m = 0; m < kM; ++m) x[m] = a.x + (m0 + m < rows ? m0 + m : rows - 1) * a.x_ld, acc[m] = 0;
   using P = Pack<int8_t, kBytes>;
-#pragma unroll 4
-  for (int k = lane * kBytes; k + kBytes <= a.inputs; k += 32 * kBytes) {
-    const P pw = *reinterpret_cast<const P*>(w + k);
+  auto one = [&](const P& pw, int k) {
 #pragma unroll
     for (int m = 0; m < kM; ++m) {
-      const int64_t row = m0 + m < rows ? m0 + m : rows - 1;
-      const P px = *reinterpret_cast<const P*>(a.x + row * a.x_ld + k);
+      const P px = *reinterpret_cast<const P*>(x[m] + k);
       if constexpr (kBytes == 16) {
         const int4 x4 = *reinterpret_cast<const int4*>(&px), w4 = *reinterpret_cast<const int4*>(&pw);
         acc[m] = __dp4a(x4.x, w4.x, acc[m]), acc[m] = __dp4a(x4.y, w4.y, acc[m]);
@@ -66,21 +66,30 @@ few_rows_kernel(const LinearArgs a) {
         acc[m] += (int)px.v[0] * (int)pw.v[0];
       }
     }
-  }
-  if (kBytes > 1)  // what is left of the rows
-    for (int k = a.inputs / kBytes * kBytes + lane; k < a.inputs; k += 32)
+  };
+  constexpr int kAhead = 8;
+  const int whole = a.inputs / kBytes * kBytes;
+  int k = lane * kBytes;
+  for (; k + (kAhead - 1) * 32 * kBytes < whole; k += kAhead * 32 * kBytes) {
+    P pw[kAhead];
 #pragma unroll
-      for (int m = 0; m < kM; ++m) {
-        const int64_t row = m0 + m < rows ? m0 + m : rows - 1;
-        acc[m] += (int)a.x[row * a.x_ld + k] * (int)w[k];
-      }
-  const float ws = __ldg(a.w_scale + n), b = a.bias ? __ldg(a.bias + n) : 0.f;
+    for (int i = 0; i < kAhead; ++i) pw[i] = *reinterpret_cast<const P*>(w + k + i * 32 * kBytes);
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) one(pw[i], k + i * 32 * kBytes);
+  }
+#pragma unroll 2
+  for (; k < whole; k += 32 * kBytes) one(*reinterpret_cast<const P*>(w + k), k);
+  if (kBytes > 1)  // what is left of the rows
+    for (k = whole + lane; k < a.inputs; k += 32)
+#pragma unroll
+      for (int m = 0; m < kM; ++m) acc[m] += (int)x[m][k] * (int)w[k];
+  float mine = 0.f;
 #pragma unroll
   for (int m = 0; m < kM; ++m) {
     const int sum = __reduce_add_sync(0xffffffffu, acc[m]);
-    if (lane == 0 && m0 + m < rows)
-      ((T*)a.out)[(m0 + m) * a.outputs + n] = from_f32<T>(fmaf((float)sum * ws, __ldg(a.x_scale + m0 + m), b));
+    if (lane == m) mine = (float)sum;
   }
+  if (lane < kM && m0 + lane < rows) ((T*)a.out)[(m0 + lane) * a.outputs + n] = from_f32<T>(fmaf(mine * ws, xs, b));
 }
 
 // ---- tensor cores -----------------------------------------------------------------------------------------------------
@@ -394,6 +403,149 @@ linear_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__
   if (warp == kEpilogueWarps + 1) free_tmem<kCta>(tmem);
 }
 
+// ---- few rows ---------------------------------------------------------------------------------------------------------
+// The weights are what is read, so they take the place of the rows: a CTA multiplies 128 of them with all of up to 64 rows.  Where
+// that gives too few CTAs to ask for the weights fast enough, a cluster shares a tile's sum, each CTA some of its channels.  Then
+// each adds up every so many rows' sums, which all of them have put into its shared memory; they are integers, so it does
+// not matter in which order.
+constexpr int kFewRows = 64;
+constexpr int kFewThreads = 6 * 32;  // four warps of the epilogue, one for the copies, one for the products
+
+struct FewArgs {
+  LinearArgs l;
+  int cols;        // rows of the input, rounded up to 16
+  int k_blocks, splits, stages;
+  int share;       // rows whose sums a CTA of a cluster adds up: every splits-th
+  uint32_t stage_bytes, tmem_cols, idesc;
+};
+struct FewShared {
+  uint64_t full[kMaxStages], empty[kMaxStages], done, drained;
+  uint32_t tmem;
+  int abort;
+  float x_scale[kFewRows];
+};
+
+template <class T>
+__global__ void __launch_bounds__(kFewThreads, 1)
+few_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const FewArgs p) {
+  extern __shared__ __align__(1024) unsigned char smem_raw[];
+  unsigned char* ring = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  int* partial = reinterpret_cast<int*>(ring + p.stages * p.stage_bytes);  // [splits][share][128]
+  FewShared* sh = reinterpret_cast<FewShared*>(partial + (p.splits > 1 ? p.splits * p.share * kTileRows : 0));
+  const int warp = threadIdx.x >> 5, lane = lane_id();
+  const int rank = (int)cluster_rank(), n0 = (int)(blockIdx.x / p.splits) * kTileRows;
+  const int rows = (int)live_rows(p.l.rows, p.l.num_rows);
+  // no rows: nothing is copied and nothing waited for
+  const int k0 = p.k_blocks * rank / p.splits, k1 = rows > 0 ? p.k_blocks * (rank + 1) / p.splits : k0;
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kMaxStages; ++s) mbar_init(&sh->full[s], 1), mbar_init(&sh->empty[s], 1);
+    mbar_init(&sh->done, 1), mbar_init(&sh->drained, 1);
+    sh->abort = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 5) tmem_alloc(&sh->tmem, p.tmem_cols);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  // all CTAs of the cluster run before one writes into another: each thread waits for that behind its role
+  if (p.splits > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
+  const uint32_t tmem = sh->tmem;
+  volatile int* abort_flag = &sh->abort;
+  const int n = n0 + warp * 32 + lane;  // of an epilogue thread
+  const bool mine = warp < 4 && n < p.l.outputs;
+  float ws = 0.f, b = 0.f;
+  bool ok = true;
+
+  if (warp == 4) {
+    if (lane == 0) {
+      int stage = 0, phase = 0;
+      for (int k = k0; k < k1; ++k) {
+        if (!mbar_wait(&sh->empty[stage], phase ^ 1, abort_flag, 1, kWaitLimitCycles)) break;
+        unsigned char* a = ring + stage * p.stage_bytes;
+        mbar_arrive_expect_tx(&sh->full[stage], p.stage_bytes);
+        tma_load_2d(&map_w, &sh->full[stage], a, k * kBlockK, n0);
+        tma_load_2d(&map_x, &sh->full[stage], a + kABytes, k * kBlockK, 0);
+        if (++stage == p.stages) stage = 0, phase ^= 1;
+      }
+      for (int s = 0; s < p.stages; ++s) mbar_drain(&sh->full[s], s < stage ? phase : phase ^ 1);
+    }
+  } else if (warp == 5) {
+    constexpr uint32_t kHigh = 64u | (1u << 14) | (2u << 29);
+    const uint32_t low0 = ((smem_u32(ring) & 0x3FFFFu) >> 4) | (1u << 16), low_step = p.stage_bytes >> 4;
+    const int last = (p.l.inputs - (p.k_blocks - 1) * kBlockK + 31) / 32;
+    int stage = 0, phase = 0;
+    bool bad = false;
+    for (int k = k0; k < k1; ++k) {
+      const uint32_t low = low0 + stage * low_step;
+      const uint64_t da = (uint64_t)kHigh << 32 | low, db = (uint64_t)kHigh << 32 | (low + (kABytes >> 4));
+      const int steps = k == p.k_blocks - 1 ? last : 4;
+      if (elect_one()) {
+        if (!bad) bad = !mbar_wait(&sh->full[stage], phase, abort_flag, 3, kWaitLimitCycles);
+        if (!bad) {
+          tc_fence_after();
+          mma_i8<1>(tmem, da, db, p.idesc, k > k0);
+          if (steps > 1) mma_i8<1>(tmem, da + 2, db + 2, p.idesc, 1);
+          if (steps > 2) mma_i8<1>(tmem, da + 4, db + 4, p.idesc, 1);
+          if (steps > 3) mma_i8<1>(tmem, da + 6, db + 6, p.idesc, 1);
+          umma_commit(&sh->empty[stage]);
+          if (k == k1 - 1) umma_commit(&sh->done);
+        }
+      }
+      __syncwarp();
+      if (++stage == p.stages) stage = 0, phase ^= 1;
+    }
+    if (__any_sync(0xffffffffu, bad) && elect_one()) {
+      umma_commit(&sh->drained);
+      mbar_drain(&sh->drained, 0);
+    }
+  } else {
+    if (mine) ws = __ldg(p.l.w_scale + n), b = p.l.bias ? __ldg(p.l.bias + n) : 0.f;
+    if ((int)threadIdx.x < rows) sh->x_scale[threadIdx.x] = __ldg(p.l.x_scale + threadIdx.x);
+    asm volatile("bar.sync 1, 128;" ::: "memory");
+    if (k1 > k0) ok = __all_sync(0xffffffffu, mbar_wait(&sh->done, 0, abort_flag, 4, kWaitLimitCycles));
+    tc_fence_after();
+    __syncwarp();
+    if (p.splits > 1) asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
+    int owner = 0, place = 0;  // of row c + e
+    for (int c = 0; c < rows && ok; c += 16) {
+      uint32_t r[16];
+      tmem_ld16(tmem + ((uint32_t)(warp * 32) << 16) + c, r);
+      tmem_ld_wait(r);
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        if (p.splits > 1) {
+          const int* at = partial + (rank * p.share + place) * kTileRows + threadIdx.x;
+          if (c + e < rows)
+            asm volatile("{\n\t.reg .b32 a;\n\tmapa.shared::cluster.u32 a, %0, %1;\n\tst.shared::cluster.u32 [a], %2;\n\t}"
+                         ::"r"(smem_u32(at)), "r"(owner), "r"(r[e]) : "memory");
+          if (++owner == p.splits) owner = 0, ++place;
+        } else if (c + e < rows && mine) {
+          ((T*)p.l.out)[(int64_t)(c + e) * p.l.outputs + n] = from_f32<T>(fmaf((float)(int)r[e] * ws, sh->x_scale[c + e], b));
+        }
+      }
+    }
+  }
+  __syncwarp();
+  if (warp >= 4 && p.splits > 1) asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
+  if (p.splits > 1) cluster_sync();
+  if (p.splits > 1 && warp < 4 && mine && ok) {
+#pragma unroll 4
+    for (int i = 0; i < p.share; ++i) {
+      const int m = i * p.splits + rank;
+      if (m >= rows) break;
+      int sum = 0;
+#pragma unroll
+      for (int s = 0; s < 8; ++s)
+        if (s < p.splits) sum += partial[(s * p.share + i) * kTileRows + threadIdx.x];
+      ((T*)p.l.out)[(int64_t)m * p.l.outputs + n] = from_f32<T>(fmaf((float)sum * ws, sh->x_scale[m], b));
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (threadIdx.x == 0 && sh->abort) atomicCAS(&g_int8_error, 0, 200 + sh->abort);
+  if (warp == 5) tmem_dealloc(tmem, p.tmem_cols);
+}
+
 // Rows of bytes that do not start on 16 bytes: copied so that they do.
 __global__ void __launch_bounds__(256)
 repitch_kernel(const int8_t* __restrict__ from, int64_t from_ld, int8_t* __restrict__ to, int64_t to_ld, int64_t rows, int channels,
@@ -411,7 +563,6 @@ repitch_kernel(const int8_t* __restrict__ from, int64_t from_ld, int8_t* __restr
   }
 }
 
-constexpr int kFewRows = 8;
 constexpr int kMaxInputs = 65536, kMaxOutputs = 65536;
 
 bool aligned_rows(const void* p, int64_t ld) { return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld % 16 == 0; }
@@ -428,22 +579,72 @@ bool make_map(CUtensorMap* map, CUtensorMapDataType type, int esize, const void*
             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <class T> int launch_few(const LinearArgs& a, cudaStream_t st) {
+// Raises the kernel's limit of shared memory to all there is, once per device.
+template <class K> int allow_smem(K kernel, std::mutex& lock, bool (&set)[64]) {
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return D3D_ERR_CUDA;
+  std::lock_guard<std::mutex> guard(lock);
+  if (!set[dev]) {
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024) != cudaSuccess) return D3D_ERR_CUDA;
+    set[dev] = true;
+  }
+  return D3D_OK;
+}
+
+template <class K, class... A> int launch_cluster(K kernel, int ctas, int cluster, int threads, size_t smem, cudaStream_t st, A... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(ctas), cfg.blockDim = dim3(threads), cfg.dynamicSmemBytes = smem, cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = cluster, attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr, cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, args...) == cudaSuccess ? D3D_OK : D3D_ERR_CUDA;
+}
+
+template <class T> int launch_dot(const LinearArgs& a, cudaStream_t st) {
   const bool wide = aligned_rows(a.x, a.x_ld) && aligned_rows(a.w, a.w_ld);
   const unsigned gx = (unsigned)ceil_div(a.outputs, 8);
-#define D3D_FEW(M)                                                                                                 \
-  do {                                                                                                             \
-    const dim3 grid(gx, (unsigned)ceil_div(a.rows, M));                                                            \
-    if (wide) few_rows_kernel<T, M, 16><<<grid, 256, 0, st>>>(a);                                                  \
-    else few_rows_kernel<T, M, 1><<<grid, 256, 0, st>>>(a);                                                        \
+#define D3D_DOT(M)                                                         \
+  do {                                                                     \
+    const dim3 grid(gx, (unsigned)ceil_div(a.rows, M));                    \
+    if (wide) dot_kernel<T, M, 16><<<grid, 256, 0, st>>>(a);               \
+    else dot_kernel<T, M, 1><<<grid, 256, 0, st>>>(a);                     \
   } while (0)
-  if (a.rows == 1) D3D_FEW(1);
-  else if (a.rows == 2) D3D_FEW(2);
-  else if (a.rows <= 4) D3D_FEW(4);
-  else D3D_FEW(8);
-#undef D3D_FEW
+  if (a.rows == 1) D3D_DOT(1);
+  else if (a.rows == 2) D3D_DOT(2);
+  else if (a.rows <= 4) D3D_DOT(4);
+  else D3D_DOT(8);
+#undef D3D_DOT
   D3D_CHECK_LAUNCH();
   return D3D_OK;
+}
+
+template <class T> int launch_few(const LinearArgs& a, cudaStream_t st) {
+  FewArgs p;
+  p.l = a;
+  p.cols = (int)align_up(a.rows, 16);
+  p.k_blocks = (int)ceil_div(a.inputs, kBlockK);
+  const int tiles = (int)ceil_div(a.outputs, kTileRows);
+  p.splits = kNumSMs / tiles;
+  if (p.splits > 8) p.splits = 8;
+  if (p.splits > p.k_blocks / 2) p.splits = p.k_blocks / 2;
+  if (p.splits < 1) p.splits = 1;
+  p.share = (int)ceil_div(a.rows, p.splits);
+  p.stage_bytes = kABytes + (uint32_t)p.cols * kBlockK;
+  const size_t fixed = 1024 + (p.splits > 1 ? (size_t)p.splits * p.share * kTileRows * 4 : 0) + sizeof(FewShared);
+  p.stages = (int)((227 * 1024 - fixed) / p.stage_bytes);
+  if (p.stages > kMaxStages) p.stages = kMaxStages;
+  p.tmem_cols = p.cols <= 32 ? 32 : 64;
+  p.idesc = (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(p.cols >> 3) << 17) | ((uint32_t)(kTileRows >> 4) << 24);
+  CUtensorMap map_w, map_x;
+  if (!make_map(&map_w, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, a.w, a.inputs, a.outputs, a.w_ld, kBlockK, kTileRows) ||
+      !make_map(&map_x, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, a.x, a.inputs, a.rows, a.x_ld, kBlockK, p.cols))
+    return D3D_ERR_CUDA;
+  static std::mutex lock;
+  static bool set[64] = {};
+  const int rc = allow_smem(few_rows_kernel<T>, lock, set);
+  if (rc != D3D_OK) return rc;
+  return launch_cluster(few_rows_kernel<T>, tiles * p.splits, p.splits, kFewThreads, fixed + p.stages * p.stage_bytes, st, map_w, map_x, p);
 }
 
 template <int kCta, class T> int launch_tiles(const LinearArgs& a, int cols, cudaStream_t st) {
@@ -469,29 +670,13 @@ template <int kCta, class T> int launch_tiles(const LinearArgs& a, int cols, cud
       !make_map(&map_w, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, a.w, a.inputs, a.outputs, a.w_ld, kBlockK, cols / kCta) ||
       (p.out_wide && !make_map(&map_out, kType, sizeof(T), a.out, a.outputs, a.rows, a.outputs * sizeof(T), kPiece, 32)))
     return D3D_ERR_CUDA;
-  auto kernel = linear_kernel<kCta, T>;
-  {
-    static std::mutex lock;
-    static bool set[64] = {};
-    int dev = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return D3D_ERR_CUDA;
-    std::lock_guard<std::mutex> guard(lock);
-    if (!set[dev]) {
-      if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024) != cudaSuccess) return D3D_ERR_CUDA;
-      set[dev] = true;
-    }
-  }
+  static std::mutex lock;
+  static bool set[64] = {};
+  const int rc = allow_smem(linear_kernel<kCta, T>, lock, set);
+  if (rc != D3D_OK) return rc;
   const int64_t tiles = ceil_div(a.rows, kCta * kTileRows) * p.col_tiles;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(kCta * (tiles < kNumSMs / kCta ? tiles : kNumSMs / kCta))), cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = fixed + p.stages * p.stage_bytes, cfg.stream = st;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = kCta, attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-  cfg.attrs = attr, cfg.numAttrs = 1;
-  if (cudaLaunchKernelEx(&cfg, kernel, map_x, map_w, map_out, p) != cudaSuccess) return D3D_ERR_CUDA;
-  D3D_CHECK_LAUNCH();
-  return D3D_OK;
+  return launch_cluster(linear_kernel<kCta, T>, (int)(kCta * (tiles < kNumSMs / kCta ? tiles : kNumSMs / kCta)), kCta, kThreads,
+                        fixed + p.stages * p.stage_bytes, st, map_x, map_w, map_out, p);
 }
 
 // Output channels of a tile: as many as fill the tiles evenly, fewer where the GPU would not be filled; whole multiples of `unit`.
@@ -516,6 +701,14 @@ template <class T> int launch_linear(const LinearArgs& a, cudaStream_t st) {
   return launch_tiles<1, T>(a, tile_cols(ceil_div(a.rows, kTileRows), a.outputs, kCols, kNumSMs), st);
 }
 
+// Whether the integer units' dot products are faster: where there is so little to multiply that setting up the tensor cores takes
+// longer (us, dot products / tensor cores: one row 256 -> 512 4.1 / 6.3, 1024 -> 1024 4.2 / 6.3, 4096 -> 4096 8.5 / 8.3; eight rows
+// 1024 -> 1024 4.4 / 6.3, 4096 -> 4096 22 / 8.3), and for few rows that do not start on 16 bytes, where a copy of all weights to
+// better places would take longer than the product.
+bool little(int64_t rows, int64_t inputs, int64_t outputs, bool aligned) {
+  return (rows <= 64 && rows * inputs * outputs <= (1 << 24)) || (!aligned && rows <= 8);
+}
+
 size_t repitched(const void* p, int64_t ld, int64_t rows, int channels) {
   return aligned_rows(p, ld) ? 0 : align_up((size_t)rows * align_up(channels, 16), 256);
 }
@@ -535,7 +728,7 @@ using namespace d3d;
 
 extern "C" size_t d3d_int8_linear_workspace(const int8_t* x, int64_t x_ld, int64_t rows, const int8_t* weight, int64_t weight_ld,
                                             int inputs, int outputs) {
-  if (rows <= kFewRows || inputs < 1 || outputs < 1) return 0;
+  if (inputs < 1 || outputs < 1 || little(rows, inputs, outputs, aligned_rows(x, x_ld) && aligned_rows(weight, weight_ld))) return 0;
   return repitched(x, x_ld, rows, inputs) + repitched(weight, weight_ld, outputs, inputs);
 }
 
@@ -557,7 +750,9 @@ extern "C" int d3d_int8_linear(int dtype, const int8_t* x, int64_t x_ld, const f
   D3D_REQUIRE(workspace_bytes >= need, D3D_ERR_WORKSPACE_TOO_SMALL);
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   LinearArgs a = {x, weight, x_ld, weight_ld, x_scales, weight_scales, bias, out, rows, num_rows, inputs, outputs};
-  if (rows > kFewRows) {
+  const bool aligned = aligned_rows(x, x_ld) && aligned_rows(weight, weight_ld);
+  const bool dot = little(rows, inputs, outputs, aligned);
+  if (!aligned && !dot) {
     uint8_t* ws = reinterpret_cast<uint8_t*>(workspace);
     const int64_t pitch = (int64_t)align_up(inputs, 16);
     if (!aligned_rows(x, x_ld)) {
@@ -571,10 +766,14 @@ extern "C" int d3d_int8_linear(int dtype, const int8_t* x, int64_t x_ld, const f
     }
     D3D_CHECK_LAUNCH();
   }
-  const bool few = rows <= kFewRows;
+  auto launch = [&](auto t) -> int {
+    using T = decltype(t);
+    if (dot) return launch_dot<T>(a, st);
+    return rows <= kFewRows ? launch_few<T>(a, st) : launch_linear<T>(a, st);
+  };
   switch (dtype) {
-    case D3D_FLOAT: return few ? launch_few<float>(a, st) : launch_linear<float>(a, st);
-    case D3D_HALF: return few ? launch_few<__half>(a, st) : launch_linear<__half>(a, st);
-    default: return few ? launch_few<__nv_bfloat16>(a, st) : launch_linear<__nv_bfloat16>(a, st);
+    case D3D_FLOAT: return launch(float());
+    case D3D_HALF: return launch(__half());
+    default: return launch(__nv_bfloat16());
   }
 }

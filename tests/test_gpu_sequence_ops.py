@@ -424,8 +424,8 @@ def check_linear(x, s, w, ws, b, y):
 
 
 @pytest.mark.parametrize("layout", ["dense", "columns", "odd"])
-@pytest.mark.parametrize("rows", [0, 1, 2, 3, 5, 8])
-@pytest.mark.parametrize("inputs,outputs", [(1, 1), (16, 16), (40, 9), (131, 387), (1000, 70), (4096, 33)])
+@pytest.mark.parametrize("rows", [0, 1, 2, 3, 5, 8, 17, 33, 64])
+@pytest.mark.parametrize("inputs,outputs", [(1, 1), (16, 16), (40, 9), (131, 387), (512, 130), (1000, 70), (4096, 33), (2080, 2500)])
 def test_linear_of_few_rows(d3d, layout, rows, inputs, outputs):
     dtype = TYPES[(rows + inputs) % 3]
     x, w = int8(1, rows, inputs, layout), int8(2, outputs, inputs, layout)
@@ -447,9 +447,10 @@ def test_linear(d3d, dtype, layout, rows, inputs, outputs):
     check_linear(x, s, w, ws, b, d3d.int8_linear(x, s, w, ws, b, dtype=dtype))
 
 
-@pytest.mark.parametrize("rows,count", [(8, 5), (8, 0), (300, 200), (300, 0), (300, -3), (20000, 19001), (20000, 40000)])
+@pytest.mark.parametrize("rows,count", [(8, 5), (8, 0), (50, 33), (50, 0), (300, 200), (300, 0), (300, -3), (20000, 19001), (20000, 40000)])
 def test_linear_counts(d3d, rows, count):
-    x, w = int8(1, rows, 64), int8(2, 136, 64)
+    inputs = 64 if rows > 300 else 512  # few rows: a sum shared by a cluster
+    x, w = int8(1, rows, inputs), int8(2, 136, inputs)
     s, ws = 0.01 * normal(3, rows).abs(), 0.01 * normal(4, 136)
     out = torch.full((rows, 136), 7.0, device=DEV, dtype=torch.float16)
     d3d.int8_linear(x, s, w, ws, num_rows=live(count), out=out)

@@ -41,15 +41,15 @@ def test_entry_points_refuse_bad_arguments(d3d):
     for bad in (dict(x=None), dict(g=None), dict(offs=None), dict(ld=3), dict(seqs=-1), dict(rows=-1), dict(ch=0), dict(out=None),
                 dict(ws=None), dict(ws=ctypes.c_void_p(4100)), dict(x=odd)):
         assert scan(**bad) == BAD, bad
-    lin = lambda dt=F, x=ONE, s=ONE, w=ONE, ld=16, rows=20, k=16, n=16, out=ONE, ws=None, nb=0: \
+    lin = lambda dt=F, x=ONE, s=ONE, w=ONE, ld=16, rows=100, k=16, n=16, out=ONE, ws=None, nb=0: \
         lib.d3d_int8_linear(dt, x, ld, s, rows, None, w, 16, ONE, None, k, n, out, ws, nb, None)
     assert lin(rows=0) == 0 and lin(dt=I8) == -2 and lin(rows=1 << 31) == -6 and lin(n=1 << 17) == -6
     for bad in (dict(x=None), dict(s=None), dict(w=None), dict(ld=15), dict(rows=-1), dict(k=0), dict(n=0), dict(out=None),
                 dict(out=odd), dict(x=odd), dict(w=odd)):  # the last two: rows to be copied, and no workspace for it
         assert lin(**bad) == BAD, bad
-    need = lib.d3d_int8_linear_workspace(odd, 16, 20, ONE, 16, 16, 16)
-    assert need >= 20 * 16 and lin(x=odd, ws=ONE, nb=need - 1) == -3
-    assert lib.d3d_int8_linear_workspace(ONE, 16, 20, ONE, 16, 16, 16) == 0 == lib.d3d_int8_linear_workspace(odd, 17, 8, odd, 17, 16, 16)
+    need = lib.d3d_int8_linear_workspace(odd, 16, 100, ONE, 16, 16, 16)
+    assert need >= 100 * 16 and lin(x=odd, ws=ONE, nb=need - 1) == -3
+    assert lib.d3d_int8_linear_workspace(ONE, 16, 100, ONE, 16, 16, 16) == 0 == lib.d3d_int8_linear_workspace(odd, 17, 8, odd, 17, 16, 16)
     step = lambda dt=F, x=ONE, s=ONE, ld=16, rows=4, out=ONE: \
         lib.d3d_gated_recurrence_step(dt, x, ld, ONE, 16, s, ONE, out, rows, 16, None)
     assert step(rows=0) == 0 and step(dt=I8) == -2
