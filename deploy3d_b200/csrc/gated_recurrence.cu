@@ -306,7 +306,8 @@ scan_maps_kernel(const ScanArgs a) {
   __shared__ Chain<V, kLanes, true> chain;
   const Place<V, kLanes> at(a);
   if (at.tile >= a.tiles) return;  // the last thousands of tiles are not all there
-  pdl_release();
+  pdl_wait();
+  pdl_release();  // behind the wait: the last kernel reads its rows before it waits, relying on this one
   Pack<T, V> x[kRows], g[kRows];
   load_rows<T, V, kLanes>(x, at, a.x, a.x_ld);
   load_rows<T, V, kLanes>(g, at, a.gates, a.gates_ld);
@@ -446,6 +447,7 @@ scan_backward_maps_kernel(const ScanArgs a) {
   __shared__ Chain<V, kLanes, false> chain;
   const Place<V, kLanes> at(a);
   if (at.tile >= a.tiles) return;
+  pdl_wait();
   pdl_release();
   Pack<T, V> g[kRows], d[kRows];
   load_rows<T, V, kLanes>(g, at, a.gates, a.gates_ld);
@@ -533,6 +535,8 @@ __global__ void __launch_bounds__(256)
 step_kernel(const T* __restrict__ x, int64_t x_ld, const T* __restrict__ gates, int64_t gates_ld, const float* state,
             float* state_out, T* __restrict__ out, int64_t rows, int channels) {
   using P = Pack<T, V>;
+  pdl_wait();
+  pdl_release();
   const int per_row = channels / V;
   const int64_t n = rows * per_row, nth = (int64_t)gridDim.x * blockDim.x;
   for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += nth) {
@@ -611,10 +615,7 @@ void carve(ScanArgs& a, Carver& w) {
 template <class Maps, class Rows> int launch_pass(ScanArgs a, int tile, int width, Maps maps, Rows rows, int backward, cudaStream_t st) {
   a.tiles = (int)ceil_div(a.rows, tile);
   const dim3 grid = grid_of(a.tiles, ceil_div(a.channels, width));
-  if (a.tiles > 0) {
-    maps<<<grid, kThreads, 0, st>>>(a);
-    D3D_CHECK_LAUNCH();
-  }
+  if (a.tiles > 0) D3D_LAUNCH(true, maps, grid, kThreads, 0, st, a);
   if (a.tiles > 1)
     D3D_LAUNCH(true, carry_kernel, (unsigned)ceil_div(a.channels, kCarryChannels), kCarryThreads, 0, st, a.maps, a.carry, a.tiles,
                a.channels, backward);
@@ -720,13 +721,10 @@ extern "C" int d3d_gated_recurrence_step(int dtype, const void* x, int64_t x_ld,
   return by_type(dtype, [&](auto t) -> int {
     using T = decltype(t);
     constexpr int V = 16 / (int)sizeof(T);
-    if (wide)
-      step_kernel<T, V><<<stream_grid(rows * (channels / V), 256), 256, 0, st>>>((const T*)x, x_ld, (const T*)gates, gates_ld, state,
-                                                                                state_out, (T*)out, rows, channels);
-    else
-      step_kernel<T, 1><<<stream_grid(rows * channels, 256), 256, 0, st>>>((const T*)x, x_ld, (const T*)gates, gates_ld, state,
-                                                                          state_out, (T*)out, rows, channels);
-    D3D_CHECK_LAUNCH();
+    const int per = wide ? V : 1;
+    auto kernel = wide ? step_kernel<T, V> : step_kernel<T, 1>;
+    D3D_LAUNCH(true, kernel, (unsigned)stream_grid(rows * (channels / per), 256), 256, 0, st, (const T*)x, x_ld, (const T*)gates, gates_ld,
+               state, state_out, (T*)out, rows, channels);
     return D3D_OK;
   });
 }

@@ -55,9 +55,12 @@ dot_kernel(const LinearArgs a) {
   for (int m = 0; m < kM; ++m) x[m] = a.x + (m0 + m < rows ? m0 + m : rows - 1) * a.x_ld, acc[m] = 0;
   using P = Pack<int8_t, kBytes>;
   auto one = [&](const P& pw, int k) {
+    P rows_of[kM];
+#pragma unroll
+    for (int m = 0; m < kM; ++m) rows_of[m] = *reinterpret_cast<const P*>(x[m] + k);
 #pragma unroll
     for (int m = 0; m < kM; ++m) {
-      const P px = *reinterpret_cast<const P*>(x[m] + k);
+      const P px = rows_of[m];
       if constexpr (kBytes == 16) {
         const int4 x4 = *reinterpret_cast<const int4*>(&px), w4 = *reinterpret_cast<const int4*>(&pw);
         acc[m] = __dp4a(x4.x, w4.x, acc[m]), acc[m] = __dp4a(x4.y, w4.y, acc[m]);
@@ -141,6 +144,9 @@ __device__ __forceinline__ uint32_t in_leader(const void* p) {
 __device__ __forceinline__ void cluster_sync() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
+__device__ __forceinline__ void prefetch_map(const CUtensorMap* map) {
+  asm volatile("prefetch.tensormap [%0];" ::"l"((uint64_t)map) : "memory");
+}
 template <int kCta> __device__ __forceinline__ void arrive_leader(uint64_t* bar) {
   if (kCta == 1) mbar_arrive(bar);
   else asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(in_leader(bar)) : "memory");
@@ -214,9 +220,7 @@ linear_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__
   Shared* sh = reinterpret_cast<Shared*>(staging + kEpilogueWarps * kStaging);
   const int warp = threadIdx.x >> 5, lane = lane_id();
   const uint32_t rank = kCta == 1 ? 0 : cluster_rank();
-  const int64_t rows = live_rows(p.l.rows, p.l.num_rows);
-  const int row_tiles = (int)((rows + kCta * kTileRows - 1) / (kCta * kTileRows));
-  const Tiles tiles = {(int)(blockIdx.x / kCta), (int)(gridDim.x / kCta), row_tiles * p.col_tiles, row_tiles, p.col_tiles, p.inverse};
+  if (threadIdx.x == 32) prefetch_map(&map_x), prefetch_map(&map_w), prefetch_map(&map_out);
   if (threadIdx.x == 0) {
     for (int s = 0; s < kMaxStages; ++s) mbar_init(&sh->full[s], 1), mbar_init(&sh->empty[s], 1);
     for (int b = 0; b < kMaxAcc; ++b) mbar_init(&sh->acc_full[b], 1), mbar_init(&sh->acc_empty[b], kCta * kEpilogueWarps);
@@ -231,6 +235,11 @@ linear_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__
   tc_fence_after();
   const uint32_t tmem = sh->tmem;
   volatile int* abort_flag = &sh->abort;
+  pdl_release();
+  pdl_wait();  // so far nothing of the kernels before has been touched
+  const int64_t rows = live_rows(p.l.rows, p.l.num_rows);
+  const int row_tiles = (int)((rows + kCta * kTileRows - 1) / (kCta * kTileRows));
+  const Tiles tiles = {(int)(blockIdx.x / kCta), (int)(gridDim.x / kCta), row_tiles * p.col_tiles, row_tiles, p.col_tiles, p.inverse};
 
   if (warp == kEpilogueWarps) {
     if (lane == 0) {
@@ -404,11 +413,12 @@ linear_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__
 }
 
 // ---- few rows ---------------------------------------------------------------------------------------------------------
-// The weights are what is read, so they take the place of the rows: a CTA multiplies 128 of them with all of up to 64 rows.  Where
+// The weights are what is read, so they take the place of the rows: a CTA multiplies 128 of them with all of up to 32 rows.  Where
 // that gives too few CTAs to ask for the weights fast enough, a cluster shares a tile's sum, each CTA some of its channels.  Then
 // each adds up every so many rows' sums, which all of them have put into its shared memory; they are integers, so it does
 // not matter in which order.
-constexpr int kFewRows = 64;
+constexpr int kFewRows = 32;
+constexpr int kMaxSplits = 4;         // CTAs of a cluster (2048 -> 2048, one row: with eight 7.8 us, four 4.7)
 constexpr int kFewThreads = 6 * 32;  // four warps of the epilogue, one for the copies, one for the products
 
 struct FewArgs {
@@ -434,9 +444,7 @@ few_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
   FewShared* sh = reinterpret_cast<FewShared*>(partial + (p.splits > 1 ? p.splits * p.share * kTileRows : 0));
   const int warp = threadIdx.x >> 5, lane = lane_id();
   const int rank = (int)cluster_rank(), n0 = (int)(blockIdx.x / p.splits) * kTileRows;
-  const int rows = (int)live_rows(p.l.rows, p.l.num_rows);
-  // no rows: nothing is copied and nothing waited for
-  const int k0 = p.k_blocks * rank / p.splits, k1 = rows > 0 ? p.k_blocks * (rank + 1) / p.splits : k0;
+  if (threadIdx.x == 32) prefetch_map(&map_x), prefetch_map(&map_w);
   if (threadIdx.x == 0) {
     for (int s = 0; s < kMaxStages; ++s) mbar_init(&sh->full[s], 1), mbar_init(&sh->empty[s], 1);
     mbar_init(&sh->done, 1), mbar_init(&sh->drained, 1);
@@ -451,6 +459,11 @@ few_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
   if (p.splits > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
   const uint32_t tmem = sh->tmem;
   volatile int* abort_flag = &sh->abort;
+  pdl_release();
+  pdl_wait();
+  const int rows = (int)live_rows(p.l.rows, p.l.num_rows);
+  // no rows: nothing is copied and nothing waited for
+  const int k0 = p.k_blocks * rank / p.splits, k1 = rows > 0 ? p.k_blocks * (rank + 1) / p.splits : k0;
   const int n = n0 + warp * 32 + lane;  // of an epilogue thread
   const bool mine = warp < 4 && n < p.l.outputs;
   float ws = 0.f, b = 0.f;
@@ -535,7 +548,7 @@ few_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
       if (m >= rows) break;
       int sum = 0;
 #pragma unroll
-      for (int s = 0; s < 8; ++s)
+      for (int s = 0; s < kMaxSplits; ++s)
         if (s < p.splits) sum += partial[(s * p.share + i) * kTileRows + threadIdx.x];
       ((T*)p.l.out)[(int64_t)m * p.l.outputs + n] = from_f32<T>(fmaf((float)sum * ws, sh->x_scale[m], b));
     }
@@ -550,6 +563,7 @@ few_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
 __global__ void __launch_bounds__(256)
 repitch_kernel(const int8_t* __restrict__ from, int64_t from_ld, int8_t* __restrict__ to, int64_t to_ld, int64_t rows, int channels,
                const int32_t* num_rows) {
+  pdl_release();
   rows = live_rows(rows, num_rows);
   const int words = (int)(to_ld / 4);
   const int64_t n = rows * words, nth = (int64_t)gridDim.x * blockDim.x;
@@ -591,13 +605,17 @@ template <class K> int allow_smem(K kernel, std::mutex& lock, bool (&set)[64]) {
   return D3D_OK;
 }
 
+// As a programmatic dependent of the kernel before: setting up barriers and tensor memory and fetching the maps takes 2 us, which
+// can be beside its end.
 template <class K, class... A> int launch_cluster(K kernel, int ctas, int cluster, int threads, size_t smem, cudaStream_t st, A... args) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(ctas), cfg.blockDim = dim3(threads), cfg.dynamicSmemBytes = smem, cfg.stream = st;
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = cluster, attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-  cfg.attrs = attr, cfg.numAttrs = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr, cfg.numAttrs = 2;
   return cudaLaunchKernelEx(&cfg, kernel, args...) == cudaSuccess ? D3D_OK : D3D_ERR_CUDA;
 }
 
@@ -626,7 +644,7 @@ template <class T> int launch_few(const LinearArgs& a, cudaStream_t st) {
   p.k_blocks = (int)ceil_div(a.inputs, kBlockK);
   const int tiles = (int)ceil_div(a.outputs, kTileRows);
   p.splits = kNumSMs / tiles;
-  if (p.splits > 8) p.splits = 8;
+  if (p.splits > kMaxSplits) p.splits = kMaxSplits;
   if (p.splits > p.k_blocks / 2) p.splits = p.k_blocks / 2;
   if (p.splits < 1) p.splits = 1;
   p.share = (int)ceil_div(a.rows, p.splits);
@@ -634,7 +652,7 @@ template <class T> int launch_few(const LinearArgs& a, cudaStream_t st) {
   const size_t fixed = 1024 + (p.splits > 1 ? (size_t)p.splits * p.share * kTileRows * 4 : 0) + sizeof(FewShared);
   p.stages = (int)((227 * 1024 - fixed) / p.stage_bytes);
   if (p.stages > kMaxStages) p.stages = kMaxStages;
-  p.tmem_cols = p.cols <= 32 ? 32 : 64;
+  p.tmem_cols = 32;
   p.idesc = (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(p.cols >> 3) << 17) | ((uint32_t)(kTileRows >> 4) << 24);
   CUtensorMap map_w, map_x;
   if (!make_map(&map_w, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, a.w, a.inputs, a.outputs, a.w_ld, kBlockK, kTileRows) ||
@@ -701,12 +719,12 @@ template <class T> int launch_linear(const LinearArgs& a, cudaStream_t st) {
   return launch_tiles<1, T>(a, tile_cols(ceil_div(a.rows, kTileRows), a.outputs, kCols, kNumSMs), st);
 }
 
-// Whether the integer units' dot products are faster: where there is so little to multiply that setting up the tensor cores takes
-// longer (us, dot products / tensor cores: one row 256 -> 512 4.1 / 6.3, 1024 -> 1024 4.2 / 6.3, 4096 -> 4096 8.5 / 8.3; eight rows
-// 1024 -> 1024 4.4 / 6.3, 4096 -> 4096 22 / 8.3), and for few rows that do not start on 16 bytes, where a copy of all weights to
-// better places would take longer than the product.
+// Whether the integer units' dot products are taken: where there is so little to multiply that setting up the tensor cores takes
+// longer (us, dot products / tensor cores, launched on their own: one row 256 -> 512 4.1 / 6.3, 1024 -> 1024 4.2 / 6.3; behind
+// other kernels, where the setting up is hidden, they are equal up to 2048 -> 2048, 5.4 / 4.7, and at 4096 -> 4096 8.2 / 5.6),
+// and for few rows that do not start on 16 bytes, where a copy of all weights to better places would take longer.
 bool little(int64_t rows, int64_t inputs, int64_t outputs, bool aligned) {
-  return (rows <= 64 && rows * inputs * outputs <= (1 << 24)) || (!aligned && rows <= 8);
+  return (rows <= 64 && rows * inputs * outputs <= (1 << 22)) || (!aligned && rows <= 8);
 }
 
 size_t repitched(const void* p, int64_t ld, int64_t rows, int channels) {
