@@ -5,7 +5,7 @@ Features are CUDA tensors ``[rows, channels]`` in float32, float16 or bfloat16 a
 channels side by side); parameters, scales and states are float32.  Everything runs on the current stream of the features'
 device.  ``num_rows``, an int32 tensor of one element on the device, says how many rows are live, as the counts of the voxel
 operators do: rows behind are neither read nor written (in a tensor the call has made itself they hold nothing).  ``out``
-takes the result where given: dense, of the right shape and type.  Backward passes are functions of their own; nothing here
+takes the result where given: dense, of the right shape and type; it may be the (dense) features themselves.  Backward passes are functions of their own; nothing here
 records autograd history.
 """
 import torch
@@ -53,8 +53,8 @@ def int8_linear(feats, scales, weight, weight_scales, bias=None, dtype=torch.flo
 
     feats int8 [rows, inputs] and scales float32 [rows], as quantize_rows and layer_norm_int8 give them; weight int8 [outputs,
     inputs], weight_scales and bias (or None) float32 [outputs].  The sum is exact.  Rows and weights that start on 16 bytes
-    and lie multiples of 16 bytes apart are read as they are, others are copied first, on every call.  At most 65536
-    inputs and outputs."""
+    and lie multiples of 16 bytes apart are read as they are; others, but for few rows, are copied first on every call: keep
+    weights of odd widths as columns of a wider tensor.  At most 65536 inputs and outputs."""
     return (_NATIVE or _native()).int8_linear(feats, scales, weight, weight_scales, bias, dtype, num_rows, out)
 
 
@@ -63,7 +63,7 @@ def gated_recurrence(feats, gates, seq_offsets, initial=None, reverse=False, wit
 
     seq_offsets int32 [sequences + 1] on the device, ascending: sequence s are the rows seq_offsets[s] .. seq_offsets[s+1]-1, walked
     downwards with `reverse`; equal ones are a sequence without rows.  initial float32 [sequences, channels]: h in front of the
-    first row walked (None: zeros).  Rows outside all sequences are neither read nor written.  Returns (h in the type of
+    first row walked (None: zeros).  Rows outside all sequences are not written, and what they hold does not matter.  Returns (h in the type of
     feats, h of the last row walked of every sequence in float32); with `with_states` also what the backward pass needs."""
     return (_NATIVE or _native()).gated_recurrence(feats, gates, seq_offsets, initial, reverse, with_states, out)
 

@@ -68,8 +68,8 @@ const char* d3d_version(void);
 const char* d3d_status_string(int status);
 /* Debug aid (no reference counterpart; the reference only prints CUDA errors, trt/include/common/macros.h:14-34):
  * synchronises the device, returns in *code the error word a kernel of this library raised when one of its bounded
- * waits expired (0 = none) and clears it.  The word is one per process: a wait of the tensor-core SPConvMM kernel
- * gives up after about one second of wall clock (far beyond any hand-over of a running kernel; a context that is
+ * waits expired (0 = none) and clears it.  The word is one per process: a wait of a tensor-core kernel (SPConvMM; the products
+ * of 8-bit rows, whose codes are above 100) gives up after about one second of wall clock (far beyond any hand-over of a running kernel; a context that is
  * time-sliced away for longer would trip it too), the CTA then drains, part of the output stays unwritten, and the
  * asynchronous enqueue that launched it has long returned D3D_OK.  Not thread-safe. */
 int d3d_debug_take_kernel_error(int* code);
@@ -486,12 +486,13 @@ int d3d_yolox3d_decode_enqueue(const d3d_yolox3d_decode_params* p, const d3d_ten
  * along an order of theirs instead of through a kernel neighbourhood.  Features are rows x channels as everywhere in this
  * library, dtype float | half | bf16; parameters, states and scales are float.  `*_ld`: elements from one row to the next
  * (at least the row's own), so that inputs may be columns of a wider tensor; outputs without one are dense.  Rows that start
- * on 16 bytes and are multiples of 16 bytes apart are read in 16-byte pieces, any others element by element.
+ * on 16 bytes and are multiples of 16 bytes apart are read in wider pieces than others.  The kernels are launched as programmatic
+ * dependents: they may start before the kernel in front of them has ended, and wait for it before they touch memory.
  * `num_rows`: the live rows, int32 [1] on the device, or NULL for all of them; rows behind are neither read nor written.
  * ------------------------------------------------------------------------------------------- */
 /* out = (t - mean) * rstd * weight + bias over the channels, t = x, or the sum x + residual rounded to the type, which is then
  * written to `total` (given exactly when `residual` is).  weight, bias: [channels] or NULL (1, 0).  mean and rstd, [rows], both
- * or neither: what the backward pass needs.  channels <= 8192. */
+ * or neither: what the backward pass needs.  out may be x where that is dense.  channels <= 8192. */
 int d3d_layer_norm(int dtype, const void* x, int64_t x_ld, const void* residual, int64_t residual_ld, const float* weight,
                    const float* bias, float eps, int64_t rows, int channels, const int32_t* num_rows, void* total, void* out,
                    float* mean, float* rstd, void* stream);
@@ -513,8 +514,8 @@ int d3d_layer_norm_int8(int dtype, const void* x, int64_t x_ld, const void* resi
                         const int32_t* num_rows, void* total, int8_t* q, int64_t q_ld, float* scales, void* stream);
 /* Product of 8-bit rows and 8-bit weights: out[m][n] = x_scales[m] * weight_scales[n] * sum_k x[m][k] weight[n][k] + bias[n], the
  * sum in 32-bit integers, out [rows][outputs] of `dtype` (float | half | bf16), bias [outputs] or NULL.  Rows of x and weight that
- * start on 16 bytes and are multiples of 16 bytes apart are read where they are; others are copied into the workspace first
- * (more than eight rows; its size depends on the addresses' alignment).  inputs, outputs <= 65536. */
+ * start on 16 bytes and are multiples of 16 bytes apart are read where they are; others are copied into the workspace first,
+ * except for few rows or little work (the size depends on the addresses' alignment).  inputs, outputs <= 65536. */
 size_t d3d_int8_linear_workspace(const int8_t* x, int64_t x_ld, int64_t rows, const int8_t* weight, int64_t weight_ld, int inputs,
                                  int outputs);
 int d3d_int8_linear(int dtype, const int8_t* x, int64_t x_ld, const float* x_scales, int64_t rows, const int32_t* num_rows,
@@ -524,8 +525,9 @@ int d3d_int8_linear(int dtype, const int8_t* x, int64_t x_ld, const float* x_sca
  * Sequence s are the rows offsets[s] .. offsets[s+1]-1 (int32 [seqs+1] on the device, ascending; equal ones are a sequence
  * without rows), walked upwards or, with `reverse`, downwards.  initial [seqs][channels]: h in front of the first row walked
  * (NULL: zeros); final_state [seqs][channels] (or NULL): h of the last one, initial where there is none.  Rows outside all
- * sequences are neither read nor written.  h is held in float; sequences do not touch each other, whatever their values.
- * states: NULL, or [d3d_gated_recurrence_state_rows(rows)][channels], what the backward pass needs. */
+ * sequences are not written, and what they hold does not matter.  h is held in float; sequences do not touch each other,
+ * whatever their values.  out may be x where that is dense.  states: NULL, or [d3d_gated_recurrence_state_rows(rows)][channels],
+ * what the backward pass needs.  rows < 2^31, channels <= 65536. */
 int64_t d3d_gated_recurrence_state_rows(int64_t rows);
 size_t d3d_gated_recurrence_workspace(int64_t rows, int channels);
 int d3d_gated_recurrence(int dtype, const void* x, int64_t x_ld, const void* gates, int64_t gates_ld, const int32_t* offsets,

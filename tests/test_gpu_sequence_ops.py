@@ -470,6 +470,121 @@ def test_linear_of_rows_that_are_not_finite(d3d):
         assert y[2].isnan().all() and int(y.isnan().any(1).sum()) == 1
 
 
+# ---- as a block uses them -------------------------------------------------------------------------------------------
+def test_a_block_over_the_voxels_of_a_scan(d3d):
+    """Encoder, then norm, 8-bit projection to features and gates (columns of one tensor), the recurrence both ways, 8-bit
+    projection back onto a residual: with the live count on the device throughout, captured once and replayed on a second
+    scan of another size.  Every step against its definition, from what the step before left."""
+    most, channels = 4000, 32
+    config = torch.tensor([0, 0, 0, 0.5, 0.5, 0.5], device=DEV)
+    shape = torch.empty((1, 0, 20, 40, 40), dtype=torch.int32, device=DEV)
+    points, batch = torch.zeros((6000, 4), device=DEV), torch.full((6000,), -1, dtype=torch.int32, device=DEV)
+    lift = normal(1, 4, channels).half()
+    w, b = 1 + 0.2 * normal(2, channels), 0.1 * normal(3, channels)
+    q1, s1 = d3d.quantize_rows(normal(4, 2 * channels, channels))
+    q2, s2 = d3d.quantize_rows(normal(5, channels, 2 * channels))
+    b1 = 0.1 * normal(6, 2 * channels)
+    zero = torch.zeros(1, dtype=torch.int32, device=DEV)
+
+    def scan(seed, n):
+        pos = torch.rand((n, 3), generator=torch.Generator(device=DEV).manual_seed(seed), device=DEV) * torch.tensor([20.0, 20, 10], device=DEV)
+        points.zero_(), batch.fill_(-1)
+        points[:n, :3], points[:n, 3], batch[:n] = pos, normal(seed, n), 0
+
+    def block():
+        means, coors, count = d3d.simple_mean_encoder(points, batch, config, shape, most)
+        x = means.half() @ lift
+        q, sx = d3d.layer_norm_int8(x, w, b, EPS, num_rows=count)
+        both = d3d.int8_linear(q, sx, q1, s1, b1, dtype=torch.float16, num_rows=count)
+        offsets = torch.cat([zero, count])
+        feats, gates = both[:, :channels], both[:, channels:]
+        mixed = torch.zeros((most, 2 * channels), device=DEV, dtype=torch.float16)
+        down, _ = d3d.gated_recurrence(feats, gates, offsets)
+        up, _ = d3d.gated_recurrence(feats, gates, offsets, reverse=True)
+        mixed[:, :channels], mixed[:, channels:] = down, up
+        qm, sm = d3d.quantize_rows(mixed, num_rows=count)
+        y = d3d.int8_linear(qm, sm, q2, s2, dtype=torch.float16, num_rows=count)
+        z, total = d3d.layer_norm(y, w, b, EPS, residual=x, num_rows=count)
+        return count, x, q, sx, both, down, up, mixed, qm, sm, y, z, total
+
+    scan(11, 3000)
+    block()
+    graph = torch.cuda.CUDAGraph()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        block()
+    torch.cuda.current_stream().wait_stream(side)
+    with torch.cuda.graph(graph):
+        outs = block()
+    for seed, points_of in ((11, 3000), (12, 5500), (13, 40)):
+        scan(seed, points_of)
+        graph.replay()
+        torch.cuda.synchronize()
+        n = int(outs[0])
+        assert 0 < n <= most
+        x, q, sx, both, down, up, mixed, qm, sm, y, z, total = (t[:n] for t in outs[1:])
+        want, limit, _, _, _ = ref.norm(ref.as64(x), ref.as64(w), ref.as64(b), EPS)
+        step = ref.as64(sx)[:, None]
+        assert (np.abs(ref.as64(q) * step - want) <= step / 2 + limit + ref.U32 * 127 * step).all()
+        check_linear(q, sx, q1, s1, b1, both)
+        for got, reverse in ((down, False), (up, True)):
+            h, off, _, _, _, _ = ref.recurrence(ref.as64(both[:, :channels]), ref.as64(both[:, channels:]), [0, n], None, reverse, torch.float16)
+            ref.assert_within(got, h, off + ref.half_step(got.dtype) * (np.abs(h) + off) + ref.smallest(got.dtype), "h")
+        check_quantized(mixed.float(), qm, sm)
+        check_linear(qm, sm, q2, s2, None, y)
+        assert torch.equal(total, (y.float() + x.float()).half())
+        check_norm(total, w, b, z)
+
+
+def test_results_in_place_of_the_features(d3d):
+    for dtype in TYPES:
+        for channels in (24, 7, 600):
+            x, g = features(1, 1500, channels, dtype), gates_like(2, 1500, channels, dtype)
+            offsets = torch.tensor([0, 700, 1500], dtype=torch.int32, device=DEV)
+            want, again = d3d.layer_norm(x, None, None, EPS), x.clone()
+            assert d3d.layer_norm(again, None, None, EPS, out=again) is again and torch.equal(again, want)
+            for reverse in (False, True):
+                want, again = d3d.gated_recurrence(x, g, offsets, reverse=reverse)[0], x.clone()
+                d3d.gated_recurrence(again, g, offsets, reverse=reverse, out=again)
+                assert torch.equal(again, want)
+
+
+def test_refusals_on_the_gpu(d3d):
+    """Shapes, types and devices that do not fit raise before anything is launched."""
+    x, g = features(1, 8, 16, torch.float16), features(2, 8, 16, torch.float16)
+    w, off = normal(3, 16), torch.tensor([0, 8], dtype=torch.int32, device=DEV)
+    q, s = d3d.quantize_rows(x)
+    _, final, states = d3d.gated_recurrence(x, g, off, with_states=True)
+    stat = normal(4, 8)
+    bad = [
+        (TypeError, lambda: d3d.layer_norm(x.double(), w)), (TypeError, lambda: d3d.layer_norm(None, w)),
+        (ValueError, lambda: d3d.layer_norm(x[0], w)), (ValueError, lambda: d3d.layer_norm(x, w[:8])),
+        (ValueError, lambda: d3d.layer_norm(x, w.half())), (ValueError, lambda: d3d.layer_norm(x, w.cpu())),
+        (ValueError, lambda: d3d.layer_norm(x, w, residual=g[:4])), (ValueError, lambda: d3d.layer_norm(x, w, residual=g.float())),
+        (ValueError, lambda: d3d.layer_norm(x, w, out=torch.empty(8, 32, device=DEV, dtype=torch.float16)[:, :16])),
+        (ValueError, lambda: d3d.layer_norm(x, w, num_rows=torch.tensor([8], device=DEV))),
+        (ValueError, lambda: d3d.layer_norm(x, w, num_rows=torch.tensor([8], dtype=torch.int32))),
+        (ValueError, lambda: d3d.layer_norm(x[:, :0], None)), (TypeError, lambda: d3d.layer_norm_backward(g, x, w, None, stat)),
+        (ValueError, lambda: d3d.layer_norm_backward(g, x, w, stat[:4], stat)),
+        (ValueError, lambda: d3d.quantize_rows(x.cpu())), (TypeError, lambda: d3d.int8_linear(x, s, q, w[:8])),
+        (ValueError, lambda: d3d.int8_linear(q, s, q[:, :8], s)), (ValueError, lambda: d3d.int8_linear(q, s[:4], q, s)),
+        (TypeError, lambda: d3d.int8_linear(q, s, q, s, dtype=torch.int32)), (ValueError, lambda: d3d.int8_linear(q, s, q[:0], s[:0])),
+        (ValueError, lambda: d3d.gated_recurrence(x, g[:, :8], off)), (ValueError, lambda: d3d.gated_recurrence(x, g.float(), off)),
+        (ValueError, lambda: d3d.gated_recurrence(x, g, off.long())), (ValueError, lambda: d3d.gated_recurrence(x, g, off[:0])),
+        (ValueError, lambda: d3d.gated_recurrence(x, g, off, initial=normal(5, 2, 16))),
+        (ValueError, lambda: d3d.gated_recurrence_backward(g, x, g, off, states[:0])),
+        (ValueError, lambda: d3d.gated_recurrence_step(x, g, normal(6, 8, 8))), (TypeError, lambda: d3d.gated_recurrence_step(x, g, None))]
+    for kind, call in bad:
+        with pytest.raises(kind):
+            call()
+    from deploy3d_b200._lib import D3DError
+    with pytest.raises(D3DError):
+        d3d.layer_norm(torch.empty((2, 8193), device=DEV), None)
+    with pytest.raises(D3DError):
+        d3d.layer_norm(x, w, eps=-1.0)
+
+
 def test_no_wait_gave_up(d3d):
     import ctypes
     from deploy3d_b200 import _lib
