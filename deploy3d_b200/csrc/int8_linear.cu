@@ -697,13 +697,18 @@ template <int kCta, class T> int launch_tiles(const LinearArgs& a, int cols, cud
                         fixed + p.stages * p.stage_bytes, st, map_x, map_w, map_out, p);
 }
 
-// Output channels of a tile: as many as fill the tiles evenly, fewer where the GPU would not be filled; whole multiples of `unit`.
+// Output channels of a tile, a multiple of `unit`: such that the rounds of tiles over `units` CTAs (or pairs) take least.  A round
+// lasts as its tile's channels and what does not depend on them, the rows that come in and the hand-overs, about 96 of them (us,
+// as few tiles as fill the GPU / this: 14 k rows 752 -> 592 17.0 / 15.5, 3000 rows 768 -> 2304 10.3 / 8.8, 5000 rows 2048 -> 2048
+// in 32 bits 23.6 / 21.0; 66 k rows 256 -> 512, where both are the same tiles, 19.4).
 int tile_cols(int64_t row_tiles, int outputs, int unit, int units) {
-  const int64_t want = ceil_div(units, row_tiles);          // column tiles that occupy everything
-  int64_t n = ceil_div(outputs, kMaxCols);
-  if (n < want) n = want;
-  const int cols = (int)(ceil_div(ceil_div(outputs, n), unit) * unit);
-  return cols < unit ? unit : cols;
+  int best = unit;
+  int64_t least = INT64_MAX;
+  for (int cols = unit; cols <= kMaxCols; cols += unit) {
+    const int64_t n = ceil_div(outputs, cols), cost = ceil_div(row_tiles * n, units) * (cols + 96);
+    if (cost <= least && (cols == unit || ceil_div(outputs, cols - unit) > n)) least = cost, best = cols;
+  }
+  return best;
 }
 
 // Two CTAs to a tile, which halves what the weights cost, for long sums over enough tiles; short ones are bound by the epilogue,
@@ -722,9 +727,11 @@ template <class T> int launch_linear(const LinearArgs& a, cudaStream_t st) {
 // Whether the integer units' dot products are taken: where there is so little to multiply that setting up the tensor cores takes
 // longer (us, dot products / tensor cores, launched on their own: one row 256 -> 512 4.1 / 6.3, 1024 -> 1024 4.2 / 6.3; behind
 // other kernels, where the setting up is hidden, they are equal up to 2048 -> 2048, 5.4 / 4.7, and at 4096 -> 4096 8.2 / 5.6),
-// and for few rows that do not start on 16 bytes, where a copy of all weights to better places would take longer.
+// and for few rows that do not start on 16 bytes, where a copy of all weights to better places takes longer (dot products / copy and
+// tensor cores, 1001 -> 5000, one row, four, six: 6.5 / 12.5, 10.6 / 16.5, 14.7 / 16.6; 3802 -> 3731: 12.6 / 18.9, 21.5 / 22.8,
+// 33.1 / 22.9).
 bool little(int64_t rows, int64_t inputs, int64_t outputs, bool aligned) {
-  return (rows <= 64 && rows * inputs * outputs <= (1 << 22)) || (!aligned && rows <= 8);
+  return (rows <= 64 && rows * inputs * outputs <= (1 << 22)) || (!aligned && rows <= 4);
 }
 
 size_t repitched(const void* p, int64_t ld, int64_t rows, int channels) {
