@@ -120,8 +120,9 @@ __device__ __forceinline__ float step_of(float amax, float* inv) {
 }
 
 // CTAs to an SM.  What counts is how much is on its way, so three, and fewer where the registers would not do: forward where the
-// parameters are in them, backward for 32-bit rows (238 k x 64 bf16, backward alone, with two CTAs / three: 30.1 / 27.5 us).
-template <int V, int kLanes> constexpr int ctas_for(bool backward) { return kLanes > 256 ? 1 : (backward ? V == 4 : kLanes > 32) ? 2 : 3; }
+// parameters are in them, backward for 32-bit rows (238 k x 64 bf16, backward alone, with two CTAs / three: 30.1 / 27.5 us).  Of the
+// longest rows one, but forward two where they are read an element at a time (3574 x 2377 in 32 bits, one / two: 62 / 41 us).
+template <int V, int kLanes> constexpr int ctas_for(bool backward) { return kLanes > 256 ? (backward || V > 1 ? 1 : 2) : (backward ? V == 4 : kLanes > 32) ? 2 : 3; }
 constexpr int kMostBackwardCtas = 3 * kNumSMs;
 
 // A thread's pieces of the rows of a tensor that it has part in, the next ones on their way while one is summed up.  The backward
@@ -368,6 +369,8 @@ norm_backward_kernel(const NormBackwardArgs a) {
     row += stride;
   }
   float* mine = a.partial + (int64_t)blockIdx.x * 2 * channels;
+  float* mine_b = mine + channels;
+  if (gridDim.x == 1) mine = a.grad_weight, mine_b = a.grad_bias;  // the only CTA's sums are the result
   if (kGroups > 1) {  // the groups of a warp by shuffles, the others through shared memory
     constexpr int kParts = parts_for<kLanes>();
     float* part = sums + (kLanes < 32 ? threadIdx.x >> 5 : group) * 2 * channels;
@@ -393,7 +396,8 @@ norm_backward_kernel(const NormBackwardArgs a) {
       float t = sums[c];
 #pragma unroll
       for (int i = 1; i < kParts; ++i) t += sums[i * 2 * channels + c];
-      mine[c] = t;
+      float* to = c < channels ? mine : mine_b;
+      if (to) to[c < channels ? c : c - channels] = t;
     }
   } else {
 #pragma unroll
@@ -401,7 +405,8 @@ norm_backward_kernel(const NormBackwardArgs a) {
 #pragma unroll
       for (int e = 0; e < V; ++e) {
         const int c = (k * kLanes + lane) * V + e;
-        if (c < channels) mine[c] = dw[k].v[e], mine[channels + c] = db[k].v[e];
+        if (c < channels && mine) mine[c] = dw[k].v[e];
+        if (c < channels && mine_b) mine_b[c] = db[k].v[e];
       }
   }
 }
@@ -593,7 +598,7 @@ extern "C" int d3d_layer_norm_backward(int dtype, const void* grad, int64_t grad
   NormBackwardArgs a = {};
   a.grad = grad, a.grad_ld = grad_ld, a.x = x, a.x_ld = x_ld, a.grad_total = grad_total, a.grad_total_ld = grad_total_ld;
   a.weight = weight, a.mean = mean, a.rstd = rstd, a.rows = rows, a.channels = channels, a.num_rows = num_rows, a.grad_x = grad_x;
-  a.partial = reinterpret_cast<float*>(workspace);
+  a.partial = reinterpret_cast<float*>(workspace), a.grad_weight = grad_weight, a.grad_bias = grad_bias;
   const bool wide = channels * esize % 16 == 0 && rows_wide(x, x_ld, esize) && rows_wide(grad, grad_ld, esize) &&
                     (!grad_total || rows_wide(grad_total, grad_total_ld, esize)) && rows_wide(grad_x, channels, esize);
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
@@ -605,8 +610,9 @@ extern "C" int d3d_layer_norm_backward(int dtype, const void* grad, int64_t grad
       const int ctas = backward_ctas(rows, per_cta, ctas_for<V, L>(true) * kNumSMs);
       const size_t smem = threads_for<L>() > L ? (size_t)parts_for<L>() * 2 * channels * sizeof(float) : 0;
       D3D_LAUNCH(true, (norm_backward_kernel<T, V, K, L>), (unsigned)ctas, threads_for<L>(), smem, st, a);
-      D3D_LAUNCH(true, norm_columns_kernel, (unsigned)ceil_div(2 * channels, 8), 512, 0, st, a.partial, ctas, channels, grad_weight,
-                 grad_bias);
+      if (ctas > 1)
+        D3D_LAUNCH(true, norm_columns_kernel, (unsigned)ceil_div(2 * channels, 8), 512, 0, st, a.partial, ctas, channels, grad_weight,
+                   grad_bias);
       return D3D_OK;
     });
   });
