@@ -230,7 +230,8 @@ template <int V, int kLanes, bool kUp> struct Chain {
   static constexpr int kWidth = V * kLanes, kGroups = kThreads / kLanes;
   float2 totals[kWarps][kWidth];
 
-  __device__ __forceinline__ void finish(const ScanArgs& a, Vec<V> ma, Vec<V> mb, const Place<V, kLanes>& at, const Marks& marks) {
+  // Every thread brings its map; behind a barrier the warps' lie in `totals`.
+  __device__ __forceinline__ void bring(Vec<V>& ma, Vec<V>& mb, const Place<V, kLanes>& at) {
     const int lane = lane_id(), warp = threadIdx.x >> 5, col = at.lane * V;
     if constexpr (kLanes < 32)
 #pragma unroll
@@ -244,35 +245,69 @@ template <int V, int kLanes, bool kUp> struct Chain {
     if (kUp ? lane >= 32 - kLanes : lane < kLanes)
 #pragma unroll
       for (int e = 0; e < V; ++e) totals[warp][col + e] = make_float2(ma.v[e], mb.v[e]);
+  }
+  // The chain of a channel: to(warp, map of the warps on the way to it) for each; the map of all.
+  template <class F> __device__ __forceinline__ float2 walk(int t, F to) {
+    float pa = 1.f, pb = 0.f;
+#pragma unroll
+    for (int i = 0; i < kWarps; ++i) {
+      const int w = kUp ? i : kWarps - 1 - i;
+      float2 m = totals[w][t];
+      to(w, make_float2(pa, pb));
+      after(m.x, m.y, pa, pb);
+      pa = m.x, pb = m.y;
+    }
+    return make_float2(pa, pb);
+  }
+  // Behind a chain that has left its maps in `totals`: that of the rows on the way to the thread's, of its channel `e`.
+  __device__ __forceinline__ float2 own(const Vec<V>& ma, const Vec<V>& mb, const Place<V, kLanes>& at, int e) const {
+    const int lane = lane_id();
+    const float2 front = totals[threadIdx.x >> 5][at.lane * V + e];
+    if constexpr (kLanes < 32) {  // several groups in a warp
+      float pa = kUp ? __shfl_up_sync(0xffffffffu, ma.v[e], kLanes) : __shfl_down_sync(0xffffffffu, ma.v[e], kLanes);
+      float pb = kUp ? __shfl_up_sync(0xffffffffu, mb.v[e], kLanes) : __shfl_down_sync(0xffffffffu, mb.v[e], kLanes);
+      if (kUp ? lane >= kLanes : lane + kLanes < 32) {
+        after(pa, pb, front.x, front.y);
+        return make_float2(pa, pb);
+      }
+    }
+    return front;
+  }
+
+  __device__ __forceinline__ void finish(const ScanArgs& a, Vec<V> ma, Vec<V> mb, const Place<V, kLanes>& at, const Marks& marks) {
+    bring(ma, mb, at);
     if (at.slab == 0 && at.lane == 0) a.marks[at.group_id()] = make_uint4(marks.live, marks.ends, (uint32_t)marks.owner, 0u);
     __syncthreads();
     const int t = threadIdx.x, c = at.slab * kWidth + t;
     if (t < kWidth && c < a.channels) {
-      float pa = 1.f, pb = 0.f;
       float2* to = a.prefix + (int64_t)at.tile * kGroups * a.channels + c;
-#pragma unroll
-      for (int i = 0; i < kWarps; ++i) {
-        const int w = kUp ? i : kWarps - 1 - i;
-        float2 m = totals[w][t];
-        if constexpr (kLanes == 32) to[w * a.channels] = make_float2(pa, pb);
-        else totals[w][t] = make_float2(pa, pb);
-        after(m.x, m.y, pa, pb);
-        pa = m.x, pb = m.y;
-      }
-      a.maps[(int64_t)at.tile * a.channels + c] = make_float2(pa, pb);
+      a.maps[(int64_t)at.tile * a.channels + c] = walk(t, [&](int w, float2 m) {
+        if constexpr (kLanes == 32) to[w * a.channels] = m;
+        else totals[w][t] = m;
+      });
     }
-    if constexpr (kLanes < 32) {  // several groups in a warp
+    if constexpr (kLanes < 32) {
       __syncthreads();
 #pragma unroll
       for (int e = 0; e < V; ++e) {
-        float pa = kUp ? __shfl_up_sync(0xffffffffu, ma.v[e], kLanes) : __shfl_down_sync(0xffffffffu, ma.v[e], kLanes);
-        float pb = kUp ? __shfl_up_sync(0xffffffffu, mb.v[e], kLanes) : __shfl_down_sync(0xffffffffu, mb.v[e], kLanes);
-        const float2 front = totals[warp][col + e];
-        if (kUp ? lane >= kLanes : lane + kLanes < 32) after(pa, pb, front.x, front.y);
-        else pa = front.x, pb = front.y;
-        if (at.c < a.channels) a.prefix[at.group_id() * a.channels + at.c + e] = make_float2(pa, pb);
+        const float2 m = own(ma, mb, at, e);
+        if (at.c < a.channels) a.prefix[at.group_id() * a.channels + at.c + e] = m;
       }
     }
+  }
+  // The same for the only tile, into which nothing comes: what comes into the thread's rows.
+  __device__ __forceinline__ Vec<V> only(Vec<V> ma, Vec<V> mb, const Place<V, kLanes>& at) {
+    bring(ma, mb, at);
+    __syncthreads();
+    if (threadIdx.x < kWidth) walk(threadIdx.x, [&](int w, float2 m) { totals[w][threadIdx.x] = m; });
+    __syncthreads();
+    Vec<V> h;
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+      const float2 m = own(ma, mb, at, e);
+      h.v[e] = apply(m.x, m.y, 0.f);
+    }
+    return h;
   }
 };
 
@@ -283,7 +318,7 @@ __device__ __forceinline__ Vec<V> incoming(const ScanArgs& a, const Place<V, kLa
 #pragma unroll
   for (int e = 0; e < V; ++e) {
     const float2 m = __ldcg(a.prefix + at.group_id() * a.channels + at.c + e);
-    h.v[e] = apply(m.x, m.y, a.carry ? __ldcg(a.carry + (int64_t)at.tile * a.channels + at.c + e) : 0.f);
+    h.v[e] = apply(m.x, m.y, __ldcg(a.carry + (int64_t)at.tile * a.channels + at.c + e));
   }
   return h;
 }
@@ -299,7 +334,36 @@ __device__ __forceinline__ void pass_empty(const ScanArgs& a, const Place<V, kLa
       for (int c = low; c < high; ++c) to[s * a.channels + c] = from ? __ldg(from + s * a.channels + c) : 0.f;
 }
 
-// First kernel: maps.  Rows between two ends of sequences, all but a few, take a path without the tests, here and below.
+// The map of a thread's rows, those from the last start of a sequence on: what was in front of it is gone.  Rows between two ends of
+// sequences, all but a few, take a path without the tests, here and below.
+template <class T, int V, int kLanes>
+__device__ __forceinline__ void map_rows(const ScanArgs& a, const Place<V, kLanes>& at, const Marks& marks, const Pack<T, V> (&x)[kRows],
+                                         const Pack<T, V> (&g)[kRows], Vec<V>& ma, Vec<V>& mb) {
+  ma = all<V>(1.f), mb = all<V>(0.f);
+  auto enter = [&](auto is_plain) {
+    constexpr bool kPlain = decltype(is_plain)::value;
+    Finder find = {marks.owner};
+    const int64_t t = at.first_row(), step = at.step(1);
+    const int from = 31 - __clz((int)(marks.ends & 0xffffu));
+#pragma unroll
+    for (int r = 0; r < kRows; ++r)
+      if (kPlain || (r >= from && (marks.live >> r & 1))) {
+        Vec<V> f, rest;
+        gate_of<T, V>(widen<T, V>(g[r]), f, rest);
+        const Vec<V> u = mul(rest, widen<T, V>(x[r]));
+        if (!kPlain && r == from) {
+          mb = fma(f, load_state<V>(a.initial, find.of(a, t + r * step), a.channels, at.c), u);
+          ma = all<V>(reset_mark());
+        } else {
+          mb = fma(f, mb, u), ma = mul(ma, f);
+        }
+      }
+  };
+  if (marks.plain(0xffffu)) enter(std::true_type());
+  else enter(std::false_type());
+}
+
+// First kernel: maps.
 template <class T, int V, int kLanes>
 __global__ void __launch_bounds__(kThreads, 4)
 scan_maps_kernel(const ScanArgs a) {
@@ -312,27 +376,8 @@ scan_maps_kernel(const ScanArgs a) {
   load_rows<T, V, kLanes>(x, at, a.x, a.x_ld);
   load_rows<T, V, kLanes>(g, at, a.gates, a.gates_ld);
   const Marks marks = mark_ends(a, at);
-  Vec<V> ma = all<V>(1.f), mb = all<V>(0.f);
-  auto enter = [&](auto is_plain) {
-    constexpr bool kPlain = decltype(is_plain)::value;
-    Finder find = {marks.owner};
-    const int64_t t = at.first_row(), step = at.step(1);
-#pragma unroll
-    for (int r = 0; r < kRows; ++r)
-      if (kPlain || (marks.live >> r & 1)) {
-        Vec<V> f, rest;
-        gate_of<T, V>(widen<T, V>(g[r]), f, rest);
-        const Vec<V> u = mul(rest, widen<T, V>(x[r]));
-        if (!kPlain && (marks.ends >> r & 1)) {
-          mb = fma(f, load_state<V>(a.initial, find.of(a, t + r * step), a.channels, at.c), u);
-          ma = all<V>(reset_mark());
-        } else {
-          mb = fma(f, mb, u), ma = mul(ma, f);
-        }
-      }
-  };
-  if (marks.plain(0xffffu)) enter(std::true_type());
-  else enter(std::false_type());
+  Vec<V> ma, mb;
+  map_rows<T, V, kLanes>(a, at, marks, x, g, ma, mb);
   chain.finish(a, ma, mb, at, marks);
 }
 
@@ -402,36 +447,57 @@ carry_kernel(const float2* __restrict__ maps, float* __restrict__ into, int tile
   }
 }
 
-// Last kernel: the rows, each thread its own from what comes into them.  No thread waits for another.
-template <class T, int V, int kLanes>
+// Where sequences are short, their states are fetched for as many rows at once.
+constexpr int kAhead = 4;
+
+// Last kernel: the rows, each thread its own from what comes into them.  No thread waits for another.  kOnly: there is one
+// tile, and this kernel does the others' work as well.
+template <class T, int V, int kLanes, bool kOnly>
 __global__ void __launch_bounds__(kThreads, 4)
 scan_rows_kernel(const ScanArgs a) {
   const Place<V, kLanes> at(a);
+  if (kOnly) pdl_wait();
   Pack<T, V> x[kRows], g[kRows];
   load_rows<T, V, kLanes>(x, at, a.x, a.x_ld);
   load_rows<T, V, kLanes>(g, at, a.gates, a.gates_ld);
-  pdl_wait();
-  if (at.there) {
+  if (!kOnly) pdl_wait();
+  Marks marks = {0u, 0u, 0};
+  Vec<V> h;
+  if constexpr (kOnly) {
+    __shared__ Chain<V, kLanes, true> chain;
+    Vec<V> ma, mb;
+    marks = mark_ends(a, at);
+    map_rows<T, V, kLanes>(a, at, marks, x, g, ma, mb);
+    h = chain.only(ma, mb, at);
+  } else if (at.there) {
     const uint4 word = __ldcg(a.marks + at.group_id());
-    const Marks marks = {word.x & (uint32_t)at.there, word.y, (int)word.z};
-    Vec<V> h = incoming<V, kLanes>(a, at);
+    marks = {word.x & (uint32_t)at.there, word.y, (int)word.z};
+    h = incoming<V, kLanes>(a, at);
+  }
+  if (at.there) {
     store_state<V>(a.states, at.state_row(), a.channels, at.c, h);
     T* out = at.start((T*)a.out, a.channels);
     const int64_t step = at.step(a.channels);
     auto walk = [&](auto is_plain) {
       constexpr bool kPlain = decltype(is_plain)::value;
-      Finder find = {marks.owner};
+      Finder find = {marks.owner}, from = find;
       const int64_t t = at.first_row(), next = at.step(1);
+      Vec<V> start[kAhead];
 #pragma unroll
-      for (int r = 0; r < kRows; ++r, out += step)
+      for (int r = 0; r < kRows; ++r, out += step) {
+        if (!kPlain && r % kAhead == 0)
+#pragma unroll
+          for (int i = r; i < r + kAhead; ++i)
+            if (marks.ends >> i & 1) start[i - r] = load_state<V>(a.initial, from.of(a, t + i * next), a.channels, at.c);
         if (kPlain || (marks.live >> r & 1)) {
-          if (!kPlain && (marks.ends >> r & 1)) h = load_state<V>(a.initial, find.of(a, t + r * next), a.channels, at.c);
+          if (!kPlain && (marks.ends >> r & 1)) h = start[r % kAhead];
           Vec<V> f, rest;
           gate_of<T, V>(widen<T, V>(g[r]), f, rest);
           h = fma(f, h, mul(rest, widen<T, V>(x[r])));
           *reinterpret_cast<Pack<T, V>*>(out) = narrow<T, V>(h);
           if (!kPlain && (marks.ends >> (r + 16) & 1)) store_state<V>(a.final_state, find.of(a, t + r * next), a.channels, at.c, h);
         }
+      }
     };
     if (marks.plain(~0u)) walk(std::true_type());
     else walk(std::false_type());
@@ -441,6 +507,33 @@ scan_rows_kernel(const ScanArgs a) {
 
 // Backward: gradients are carried from the end.  The map of a row is c -> f (grad + c): c comes in from the row behind and goes out
 // to the row in front.
+template <class T, int V, int kLanes>
+__device__ __forceinline__ void map_rows_back(const ScanArgs& a, const Place<V, kLanes>& at, const Marks& marks, const Pack<T, V> (&g)[kRows],
+                                              const Pack<T, V> (&d)[kRows], Vec<V>& ma, Vec<V>& mb) {
+  ma = all<V>(1.f), mb = all<V>(0.f);
+  auto enter = [&](auto is_plain) {
+    constexpr bool kPlain = decltype(is_plain)::value;
+    Finder find = {marks.owner};
+    const int64_t t = at.first_row(), step = at.step(1);
+    const int from = (marks.ends >> 16) ? __ffs((int)(marks.ends >> 16)) - 1 : kRows;
+#pragma unroll
+    for (int r = kRows - 1; r >= 0; --r)
+      if (kPlain || (r <= from && (marks.live >> r & 1))) {
+        Vec<V> f, rest;
+        gate_of<T, V>(widen<T, V>(g[r]), f, rest);
+        const Vec<V> dy = widen<T, V>(d[r]);
+        if (!kPlain && r == from) {
+          mb = mul(f, add(dy, load_state<V>(a.grad_final, find.of(a, t + r * step), a.channels, at.c)));
+          ma = all<V>(reset_mark());
+        } else {
+          mb = mul(f, add(dy, mb)), ma = mul(ma, f);
+        }
+      }
+  };
+  if (marks.plain(0xffff0000u)) enter(std::true_type());
+  else enter(std::false_type());
+}
+
 template <class T, int V, int kLanes>
 __global__ void __launch_bounds__(kThreads, 4)
 scan_backward_maps_kernel(const ScanArgs a) {
@@ -453,44 +546,37 @@ scan_backward_maps_kernel(const ScanArgs a) {
   load_rows<T, V, kLanes>(g, at, a.gates, a.gates_ld);
   load_rows<T, V, kLanes>(d, at, a.grad, a.grad_ld);
   const Marks marks = mark_ends(a, at);
-  Vec<V> ma = all<V>(1.f), mb = all<V>(0.f);
-  auto enter = [&](auto is_plain) {
-    constexpr bool kPlain = decltype(is_plain)::value;
-    Finder find = {marks.owner};
-    const int64_t t = at.first_row(), step = at.step(1);
-#pragma unroll
-    for (int r = kRows - 1; r >= 0; --r)
-      if (kPlain || (marks.live >> r & 1)) {
-        Vec<V> f, rest;
-        gate_of<T, V>(widen<T, V>(g[r]), f, rest);
-        const Vec<V> dy = widen<T, V>(d[r]);
-        if (!kPlain && (marks.ends >> (r + 16) & 1)) {
-          mb = mul(f, add(dy, load_state<V>(a.grad_final, find.of(a, t + r * step), a.channels, at.c)));
-          ma = all<V>(reset_mark());
-        } else {
-          mb = mul(f, add(dy, mb)), ma = mul(ma, f);
-        }
-      }
-  };
-  if (marks.plain(0xffff0000u)) enter(std::true_type());
-  else enter(std::false_type());
+  Vec<V> ma, mb;
+  map_rows_back<T, V, kLanes>(a, at, marks, g, d, ma, mb);
   chain.finish(a, ma, mb, at, marks);
 }
 
 // The rows forward once more from the state in front of them, which gives h[t-1] - x, then back with the gradients.
-template <class T, int V, int kLanes>
+template <class T, int V, int kLanes, bool kOnly>
 __global__ void __launch_bounds__(kThreads, 2)
 scan_backward_rows_kernel(const ScanArgs a) {
   const Place<V, kLanes> at(a);
+  if (kOnly) pdl_wait();
   Pack<T, V> x[kRows], g[kRows], d[kRows];
   load_rows<T, V, kLanes>(x, at, a.x, a.x_ld);
   load_rows<T, V, kLanes>(g, at, a.gates, a.gates_ld);
   load_rows<T, V, kLanes>(d, at, a.grad, a.grad_ld);
-  pdl_wait();
-  if (at.there) {
+  if (!kOnly) pdl_wait();
+  Marks marks = {0u, 0u, 0};
+  Vec<V> q, h = all<V>(0.f);
+  if constexpr (kOnly) {
+    __shared__ Chain<V, kLanes, false> chain;
+    Vec<V> ma, mb;
+    marks = mark_ends(a, at);
+    map_rows_back<T, V, kLanes>(a, at, marks, g, d, ma, mb);
+    q = chain.only(ma, mb, at);
+  } else if (at.there) {
     const uint4 word = __ldcg(a.marks + at.group_id());
-    const Marks marks = {word.x & (uint32_t)at.there, word.y, (int)word.z};
-    Vec<V> q = incoming<V, kLanes>(a, at), h = load_state<V>(a.states, at.state_row(), a.channels, at.c);
+    marks = {word.x & (uint32_t)at.there, word.y, (int)word.z};
+    q = incoming<V, kLanes>(a, at);
+  }
+  if (at.there) {
+    h = load_state<V>(a.states, at.state_row(), a.channels, at.c);
     const int64_t step = at.step(a.channels);
     T* dx_at = at.start((T*)a.grad_x, a.channels) + (kRows - 1) * step;
     T* dg_at = at.start((T*)a.grad_gates, a.channels) + (kRows - 1) * step;
@@ -498,30 +584,41 @@ scan_backward_rows_kernel(const ScanArgs a) {
       constexpr bool kPlain = decltype(is_plain)::value;
       Finder find = {marks.owner};
       const int64_t t = at.first_row(), next = at.step(1);
-      Vec<V> gate[kRows], away[kRows];
+      Vec<V> gate[kRows], away[kRows], start[kAhead];
 #pragma unroll
-      for (int r = 0; r < kRows; ++r)
+      for (int r = 0; r < kRows; ++r) {
+        if (!kPlain && r % kAhead == 0)
+#pragma unroll
+          for (int i = r; i < r + kAhead; ++i)
+            if (marks.ends >> i & 1) start[i - r] = load_state<V>(a.initial, find.of(a, t + i * next), a.channels, at.c);
         if (kPlain || (marks.live >> r & 1)) {
           Vec<V> f, rest;
           gate_of<T, V>(widen<T, V>(g[r]), f, rest);
           gate[r] = fold_gate<V>(f, rest);
-          if (!kPlain && (marks.ends >> r & 1)) h = load_state<V>(a.initial, find.of(a, t + r * next), a.channels, at.c);
+          if (!kPlain && (marks.ends >> r & 1)) h = start[r % kAhead];
           const Vec<V> in = widen<T, V>(x[r]);
           away[r] = fma(in, all<V>(-1.f), h);
           h = fma(f, h, mul(rest, in));
         }
+      }
+      Finder from = find;
 #pragma unroll
-      for (int r = kRows - 1; r >= 0; --r, dx_at -= step, dg_at -= step)
+      for (int r = kRows - 1; r >= 0; --r, dx_at -= step, dg_at -= step) {
+        if (!kPlain && r % kAhead == kAhead - 1)
+#pragma unroll
+          for (int i = r; i > r - kAhead; --i)
+            if (marks.ends >> (i + 16) & 1) start[i % kAhead] = load_state<V>(a.grad_final, from.of(a, t + i * next), a.channels, at.c);
         if (kPlain || (marks.live >> r & 1)) {
           Vec<V> f, rest;
           open_gate<V>(gate[r], f, rest);
-          if (!kPlain && (marks.ends >> (r + 16) & 1)) q = load_state<V>(a.grad_final, find.of(a, t + r * next), a.channels, at.c);
+          if (!kPlain && (marks.ends >> (r + 16) & 1)) q = start[r % kAhead];
           const Vec<V> delta = add(widen<T, V>(d[r]), q), dx = mul(delta, rest);
           q = mul(f, delta);
           *reinterpret_cast<Pack<T, V>*>(dx_at) = narrow<T, V>(dx);
           *reinterpret_cast<Pack<T, V>*>(dg_at) = narrow<T, V>(mul(mul(q, rest), away[r]));
           if (!kPlain && (marks.ends >> r & 1)) store_state<V>(a.grad_initial, find.of(a, t + r * next), a.channels, at.c, q);
         }
+      }
     };
     if (marks.plain(~0u)) walk(std::true_type());
     else walk(std::false_type());
@@ -611,17 +708,19 @@ void carve(ScanArgs& a, Carver& w) {
   a.marks = w.take<uint4>(groups);
 }
 
-// The three kernels of a pass.  One tile: nothing comes into it.
-template <class Maps, class Rows> int launch_pass(ScanArgs a, int tile, int width, Maps maps, Rows rows, int backward, cudaStream_t st) {
+// The three kernels of a pass, or for one tile the last one alone: two launches less where launches are what such a call lasts.
+template <class Maps, class Rows>
+int launch_pass(ScanArgs a, int tile, int width, Maps maps, Rows rows, Rows only, int backward, cudaStream_t st) {
   a.tiles = (int)ceil_div(a.rows, tile);
   const dim3 grid = grid_of(a.tiles, ceil_div(a.channels, width));
-  if (a.tiles > 0) D3D_LAUNCH(true, maps, grid, kThreads, 0, st, a);
-  if (a.tiles > 1)
-    D3D_LAUNCH(true, carry_kernel, (unsigned)ceil_div(a.channels, kCarryChannels), kCarryThreads, 0, st, a.maps, a.carry, a.tiles,
-               a.channels, backward);
-  else
-    a.carry = nullptr;
-  D3D_LAUNCH(a.tiles > 0, rows, grid, kThreads, 0, st, a);
+  if (a.tiles <= 1) {
+    D3D_LAUNCH(true, only, grid, kThreads, 0, st, a);
+    return D3D_OK;
+  }
+  D3D_LAUNCH(true, maps, grid, kThreads, 0, st, a);
+  D3D_LAUNCH(true, carry_kernel, (unsigned)ceil_div(a.channels, kCarryChannels), kCarryThreads, 0, st, a.maps, a.carry, a.tiles,
+             a.channels, backward);
+  D3D_LAUNCH(true, rows, grid, kThreads, 0, st, a);
   return D3D_OK;
 }
 
@@ -633,7 +732,7 @@ using namespace d3d;
 extern "C" int64_t d3d_gated_recurrence_state_rows(int64_t rows) { return rows < 0 ? 0 : ceil_div(rows > 0 ? rows : 1, kRows); }
 
 extern "C" size_t d3d_gated_recurrence_workspace(int64_t rows, int channels) {
-  if (rows < 0 || channels < 1) return 0;
+  if (rows <= kSmallTile || channels < 1) return 0;  // one tile of any shape
   ScanArgs a = {};
   a.rows = rows, a.channels = channels;
   Carver w(nullptr);
@@ -652,8 +751,9 @@ extern "C" int d3d_gated_recurrence(int dtype, const void* x, int64_t x_ld, cons
   const int rc = check_scan(dtype, a);
   D3D_REQUIRE(rc == D3D_OK, rc);
   D3D_REQUIRE(rows == 0 || (x && gates && out), D3D_ERR_INVALID_ARGUMENT);
-  D3D_REQUIRE(workspace && reinterpret_cast<uintptr_t>(workspace) % 256 == 0, D3D_ERR_INVALID_ARGUMENT);
-  D3D_REQUIRE(workspace_bytes >= d3d_gated_recurrence_workspace(rows, channels), D3D_ERR_WORKSPACE_TOO_SMALL);
+  const size_t need = d3d_gated_recurrence_workspace(rows, channels);
+  D3D_REQUIRE(need == 0 || (workspace && reinterpret_cast<uintptr_t>(workspace) % 256 == 0), D3D_ERR_INVALID_ARGUMENT);
+  D3D_REQUIRE(workspace_bytes >= need, D3D_ERR_WORKSPACE_TOO_SMALL);
   Carver w(workspace);
   carve(a, w);
   if (seqs == 0) return D3D_OK;
@@ -663,7 +763,8 @@ extern "C" int d3d_gated_recurrence(int dtype, const void* x, int64_t x_ld, cons
     using T = decltype(t);
     return by_shape<T>(pairs, channels, [&](auto v, auto l) -> int {
       constexpr int V = decltype(v)::value, L = decltype(l)::value;
-      return launch_pass(a, Place<V, L>::kTile, V * L, scan_maps_kernel<T, V, L>, scan_rows_kernel<T, V, L>, 0,
+      return launch_pass(a, Place<V, L>::kTile, V * L, scan_maps_kernel<T, V, L>, scan_rows_kernel<T, V, L, false>,
+                         scan_rows_kernel<T, V, L, true>, 0,
                          reinterpret_cast<cudaStream_t>(stream));
     });
   });
@@ -685,8 +786,9 @@ extern "C" int d3d_gated_recurrence_backward(int dtype, const void* grad, int64_
   D3D_REQUIRE(rc == D3D_OK, rc);
   D3D_REQUIRE(grad_ld >= channels && (rows == 0 || (x && gates && grad && states && grad_x && grad_gates)),
               D3D_ERR_INVALID_ARGUMENT);
-  D3D_REQUIRE(workspace && reinterpret_cast<uintptr_t>(workspace) % 256 == 0, D3D_ERR_INVALID_ARGUMENT);
-  D3D_REQUIRE(workspace_bytes >= d3d_gated_recurrence_workspace(rows, channels), D3D_ERR_WORKSPACE_TOO_SMALL);
+  const size_t need = d3d_gated_recurrence_workspace(rows, channels);
+  D3D_REQUIRE(need == 0 || (workspace && reinterpret_cast<uintptr_t>(workspace) % 256 == 0), D3D_ERR_INVALID_ARGUMENT);
+  D3D_REQUIRE(workspace_bytes >= need, D3D_ERR_WORKSPACE_TOO_SMALL);
   Carver w(workspace);
   carve(a, w);
   if (seqs == 0) return D3D_OK;
@@ -697,7 +799,8 @@ extern "C" int d3d_gated_recurrence_backward(int dtype, const void* grad, int64_
     using T = decltype(t);
     return by_shape<T>(pairs, channels, [&](auto v, auto l) -> int {
       constexpr int V = decltype(v)::value, L = decltype(l)::value;
-      return launch_pass(a, Place<V, L>::kTile, V * L, scan_backward_maps_kernel<T, V, L>, scan_backward_rows_kernel<T, V, L>, 1,
+      return launch_pass(a, Place<V, L>::kTile, V * L, scan_backward_maps_kernel<T, V, L>,
+                         scan_backward_rows_kernel<T, V, L, false>, scan_backward_rows_kernel<T, V, L, true>, 1,
                          reinterpret_cast<cudaStream_t>(stream));
     });
   });

@@ -287,7 +287,8 @@ PyObject* gated_recurrence(Args a, Py_ssize_t n) {
   at::Tensor final_state = made({s.count, x.channels}, at::kFloat, device), states;
   if (truth(a[5])) states = made({f_gated_recurrence_state_rows(x.rows), x.channels}, at::kFloat, device);
   const size_t bytes = f_gated_recurrence_workspace(x.rows, (int)x.channels);
-  at::Tensor ws = made({(int64_t)bytes}, at::kByte, device);
+  at::Tensor ws;
+  if (bytes) ws = made({(int64_t)bytes}, at::kByte, device);
   launch("d3d_gated_recurrence", device, [&](void* stream) {
     return f_gated_recurrence(dtype_of(x.t), x.p(), x.ld, g.p(), g.ld, static_cast<const int32_t*>(s.t.data_ptr()), s.count, x.rows,
                               (int)x.channels, reverse, initial, at_of(out), floats_of(final_state), floats_of(states), at_of(ws),
@@ -310,7 +311,8 @@ PyObject* gated_recurrence_backward(Args a, Py_ssize_t n) {
   at::Tensor dx = made({x.rows, x.channels}, type, device), dg = made({x.rows, x.channels}, type, device);
   at::Tensor di = made({s.count, x.channels}, at::kFloat, device);
   const size_t bytes = f_gated_recurrence_workspace(x.rows, (int)x.channels);
-  at::Tensor ws = made({(int64_t)bytes}, at::kByte, device);
+  at::Tensor ws;
+  if (bytes) ws = made({(int64_t)bytes}, at::kByte, device);
   launch("d3d_gated_recurrence_backward", device, [&](void* stream) {
     return f_gated_recurrence_backward(dtype_of(x.t), d.p(), d.ld, x.p(), x.ld, g.p(), g.ld,
                                        static_cast<const int32_t*>(s.t.data_ptr()), s.count, x.rows, (int)x.channels, reverse, states,
