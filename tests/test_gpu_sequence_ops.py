@@ -94,6 +94,21 @@ def test_norm_counts(d3d, count):
     assert torch.equal(db == 0, torch.full((32,), n == 0, device=DEV)) and (n > 0 or (dw == 0).all())
 
 
+@pytest.mark.parametrize("rows,channels", [(1, 16), (7, 16), (3, 600), (1, 8192)])
+@pytest.mark.parametrize("count", [0, 1, 2, 7])
+def test_norm_backward_of_few_live_rows(d3d, rows, channels, count):
+    """One CTA, whose sums are the parameters' gradients: those of the live rows, to the last bit."""
+    n = min(rows, count)
+    x, dy, w = features(1, rows, channels, torch.float32), normal(2, rows, channels), normal(3, channels)
+    _, mean, rstd = d3d.layer_norm(x, w, None, EPS, with_stats=True)
+    dx, dw, db = d3d.layer_norm_backward(dy, x, w, mean, rstd, num_rows=live(count))
+    assert (n > 0 or not dw.any()) and (n > 0 or not db.any())
+    if n:
+        again = d3d.layer_norm_backward(dy[:n].clone(), x[:n].clone(), w, mean[:n].clone(), rstd[:n].clone())
+        assert torch.equal(dx[:n], again[0]) and torch.equal(dw, again[1]) and torch.equal(db, again[2])
+        ref.assert_within(db, ref.as64(dy[:n]).sum(0), n * ref.U32 * np.abs(ref.as64(dy[:n])).sum(0), "db")
+
+
 def test_norm_rows_keep_to_themselves(d3d):
     """A row that is not finite, beside rows that share its warp; a constant row."""
     for dtype in TYPES:
@@ -363,6 +378,28 @@ def test_gradients_against_differences(d3d):
     assert abs((loss(e) - loss(-e)) / (2 * e) - along) <= 4 * e * e * size
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("kind", ["one", "many", "inside", "singles"])
+@pytest.mark.parametrize("rows", [15, 16, 17, 127, 128, 129, 255, 256, 257, 512, 513])
+@pytest.mark.parametrize("channels", [8, 16, 17, 32, 34, 64, 130])
+def test_recurrence_where_tiles_end(d3d, dtype, kind, rows, channels):
+    """A tile has 128, 256 or 512 rows, by the channels and their type; one tile takes one kernel, two take three."""
+    test_recurrence(d3d, dtype, (rows + channels) % 2 == 0, kind, rows, channels)
+
+
+def test_offsets_out_of_order_over_several_tiles(d3d):
+    rows = 900
+    buf = torch.full((rows + 64, 40), 5.0, device=DEV)
+    x = features(1, rows, 40, torch.float32)
+    for offs in ([500, 3], [-4, 450], [0, 5000], [200, 100, 600, 0, 990], [899, 0, 899, 1, 898]):
+        offsets = torch.tensor(offs, dtype=torch.int32, device=DEV)
+        for reverse in (False, True):
+            out, final, states = d3d.gated_recurrence(x, x, offsets, out=buf[32:32 + rows], reverse=reverse, with_states=True)
+            d3d.gated_recurrence_backward(x, x, x, offsets, states, reverse=reverse)
+            torch.cuda.synchronize()
+            assert (buf[:32] == 5).all() and (buf[32 + rows:] == 5).all()
+
+
 # ---- streams, graphs ------------------------------------------------------------------------------------------------
 def test_on_another_stream_and_in_graphs(d3d):
     """Two graphs captured one after the other and replayed in turn on new inputs, and a call on a stream of its own."""
@@ -398,6 +435,38 @@ def test_on_another_stream_and_in_graphs(d3d):
         torch.cuda.synchronize()
         for (_, outs), reverse in zip(graphs, (False, True)):
             assert all(torch.equal(p, q) for p, q in zip(outs, chain(a, b, reverse)))
+
+
+def test_threads_on_streams_of_their_own(d3d):
+    """Four threads at once, each on its stream, with sizes of several kinds of kernel: what one thread alone gets."""
+    import threading
+
+    def chain(seed):
+        rows, channels = (90, 3000, 700, 20000)[seed], (64, 32, 130, 48)[seed]
+        x, g = features(seed, rows, channels, torch.bfloat16), gates_like(seed + 5, rows, channels, torch.bfloat16)
+        offsets = torch.tensor([0, rows // 3, rows], dtype=torch.int32, device=DEV)
+        w = int8(seed, 96, channels)
+        results = []
+        for _ in range(20):
+            q, s = d3d.layer_norm_int8(x, None)
+            y = d3d.int8_linear(q, s, w, torch.ones(96, device=DEV), dtype=torch.bfloat16)
+            h, final, states = d3d.gated_recurrence(x, g, offsets, with_states=True)
+            results.append((q, y, h, final) + d3d.gated_recurrence_backward(h, x, g, offsets, states))
+        torch.cuda.current_stream().synchronize()
+        return results
+    want, got = [chain(i)[0] for i in range(4)], [None] * 4
+
+    def work(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            got[i] = chain(i)
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    for results, w in zip(got, want):
+        for r in results:
+            assert all(torch.equal(a, b) for a, b in zip(r, w))
 
 
 # ---- product of 8-bit rows ------------------------------------------------------------------------------------------
@@ -445,6 +514,17 @@ def test_linear(d3d, dtype, layout, rows, inputs, outputs):
     x, w = int8(1, rows, inputs, layout), int8(2, outputs, inputs, layout)
     s, ws, b = 0.01 * normal(3, rows).abs(), 0.01 * normal(4, outputs), normal(5, outputs)
     check_linear(x, s, w, ws, b, d3d.int8_linear(x, s, w, ws, b, dtype=dtype))
+
+
+@pytest.mark.parametrize("rows,inputs,outputs", [
+    (4000, 48, n) for n in (130, 208, 272, 336, 387, 464, 528, 592, 656, 720, 784, 848, 912, 976)] + [
+    (9600, 1040, n) for n in (272, 304, 387, 496, 592, 688)])
+def test_linear_by_tiles_of_every_width(d3d, rows, inputs, outputs):
+    """With one CTA to a tile 48 to 256 output channels, by 16, in 32 bits; with two 96 to 256 by 32."""
+    x, w = int8(1, rows, inputs), int8(2, outputs, inputs)
+    s, ws, b = 0.01 * normal(3, rows).abs(), 0.01 * normal(4, outputs), normal(5, outputs)
+    for dtype in (torch.float32, torch.bfloat16):
+        check_linear(x, s, w, ws, b, d3d.int8_linear(x, s, w, ws, b, dtype=dtype))
 
 
 @pytest.mark.parametrize("rows,count", [(8, 5), (8, 0), (50, 33), (50, 0), (300, 200), (300, 0), (300, -3), (20000, 19001), (20000, 40000)])
