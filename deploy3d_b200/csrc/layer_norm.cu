@@ -5,6 +5,9 @@
 // All of them move bytes: every tensor is read and written once, in 16-byte pieces, a row stays in the registers of
 // the threads that share it, and mean, variance and the two means of the backward pass are exact sums over those
 // registers (the variance of differences to the mean, not a difference of two large sums).
+// Measured, of the 6.55 TB/s that a copy gets: a norm with a residual of 120 k x 128 bf16 20.9 us, 5.9 TB/s; norm and backward pass
+// of 238 k x 64 bf16 13.4 + 27.5 + 5.5 us (five passes over the rows, some of them from L2), of 4099 x 4096 in 32 bits 22 + 36 +
+// 7 us; a norm of 66 k x 256 bf16 in 8 bits 25.5 us, 2.0 TB/s, bound by the instructions of norm and rounding.
 #include <type_traits>
 
 #include "common.cuh"
