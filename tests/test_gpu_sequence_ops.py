@@ -617,6 +617,50 @@ def test_a_block_over_the_voxels_of_a_scan(d3d):
         check_norm(total, w, b, z)
 
 
+def test_offsets_past_32_bits(d3d):
+    """Columns of a tensor of 4.4 GB and results of as much: the last rows, a tile and a sequence of their own, are what they are
+    without the rows in front of them."""
+    rows, tail, channels = 512 * 4200, 128, 32
+    wide = torch.zeros((rows, 1040), dtype=torch.bfloat16, device=DEV)
+    wide[-tail:] = features(1, tail, 1040, torch.bfloat16)
+    x, g = wide[:, 16:16 + channels], wide[:, 512:512 + channels]
+    assert rows * 1040 > 2 ** 31
+
+    def alone(t):
+        return t[-tail:].clone()
+    xs, gs, w = alone(x), alone(g), normal(2, channels)
+    y, mean, rstd = d3d.layer_norm(x, w, None, EPS, with_stats=True)
+    for a, b in zip((y, mean, rstd), d3d.layer_norm(xs, w, None, EPS, with_stats=True)):
+        assert torch.equal(a[-tail:], b)
+    dx = d3d.layer_norm_backward(g, x, w, mean, rstd)[0]
+    assert torch.equal(dx[-tail:], d3d.layer_norm_backward(gs, xs, w, alone(mean), alone(rstd))[0])
+    offsets = torch.tensor([0, rows - tail, rows], dtype=torch.int32, device=DEV)
+    short = torch.tensor([0, tail], dtype=torch.int32, device=DEV)
+    for reverse in (False, True):
+        h, final, states = d3d.gated_recurrence(x, g, offsets, reverse=reverse, with_states=True)
+        h2, final2, states2 = d3d.gated_recurrence(xs, gs, short, reverse=reverse, with_states=True)
+        assert torch.equal(h[-tail:], h2) and torch.equal(final[1:], final2)
+        back = d3d.gated_recurrence_backward(g, x, g, offsets, states, reverse=reverse)
+        back2 = d3d.gated_recurrence_backward(gs, xs, gs, short, states2, reverse=reverse)
+        assert all(torch.equal(a[-len(b):], b) for a, b in zip(back, back2))
+    state = torch.zeros((rows, channels), device=DEV)
+    out, _ = d3d.gated_recurrence_step(x, g, state)
+    assert torch.equal(out[-tail:], d3d.gated_recurrence_step(xs, gs, alone(state))[0])
+    y = d3d.layer_norm(wide, None, None, EPS)
+    assert torch.equal(y[-tail:], d3d.layer_norm(alone(wide), None, None, EPS))
+    del y
+    q, s = d3d.quantize_rows(wide)
+    q2, s2 = d3d.quantize_rows(alone(wide))
+    assert torch.equal(q[-tail:], q2) and torch.equal(s[-tail:], s2)
+    ones = torch.ones(1040, device=DEV)
+    for weight in (int8(3, 1040, 1040), int8(3, 1040, 1040, "odd"), int8(3, 1039, 1040)):
+        outs = len(weight)
+        y = d3d.int8_linear(q, s, weight, ones[:outs], dtype=torch.bfloat16)
+        assert torch.equal(y[-tail:], d3d.int8_linear(q2, s2, weight, ones[:outs], dtype=torch.bfloat16))
+    y = d3d.int8_linear(q[:, 1:1001], s, weight[:, :1000].contiguous(), ones[:outs], dtype=torch.bfloat16)
+    assert torch.equal(y[-tail:], d3d.int8_linear(q2[:, 1:1001], s2, weight[:, :1000].contiguous(), ones[:outs], dtype=torch.bfloat16))
+
+
 def test_results_in_place_of_the_features(d3d):
     for dtype in TYPES:
         for channels in (24, 7, 600):
