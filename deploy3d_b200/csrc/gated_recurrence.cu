@@ -13,6 +13,7 @@
 // rows 31 to 41 by what L2 still holds (178 MB of features in and out, floor 27 us); 120 k x 128 fp16 with gradients 107 us, maps 21
 // and 19, chains 5 and 5, rows 21 and 45.  Maps are bound by instructions (23 an element, 2.9 a cycle issued of 4), the rows by
 // their bytes, backward by the 16 warps an SM that 128 registers leave.
+#include <cstring>
 #include <type_traits>
 
 #include "common.cuh"
@@ -137,18 +138,35 @@ template <int V, int kLanes> struct Place {
   __device__ __forceinline__ int64_t state_row() const { return low_row() / kRows; }  // the same for tiles of any shape
 };
 
-template <class T, int V, int kLanes>
+// kPastL1: from L2, for the last kernels, which read their rows before they wait for the ones in front of them (463 k x 64 bf16 73.5 us,
+// waiting first 76.4).  What wrote the rows has ended by then, since the first kernel lets the others start when it has waited for
+// it, but L1 need not know.
+template <class T, int V, bool kPastL1> __device__ __forceinline__ Pack<T, V> load_row(const T* p) {
+  if constexpr (!kPastL1) return *reinterpret_cast<const Pack<T, V>*>(p);
+  Pack<T, V> r;
+  static_assert(sizeof(r) == 4 || sizeof(r) == 2, "one or two channels");
+  if constexpr (sizeof(r) == 4) {
+    const uint32_t bits = __ldcg(reinterpret_cast<const uint32_t*>(p));
+    memcpy(&r, &bits, 4);
+  } else {
+    const uint16_t bits = __ldcg(reinterpret_cast<const unsigned short*>(p));
+    memcpy(&r, &bits, 2);
+  }
+  return r;
+}
+
+template <class T, int V, int kLanes, bool kPastL1 = false>
 __device__ __forceinline__ void load_rows(Pack<T, V> (&to)[kRows], const Place<V, kLanes>& at, const void* p, int64_t ld) {
   const T* src = at.start((const T*)p, ld);
   const int64_t step = at.step(ld);
   if (at.there == (1 << kRows) - 1) {
 #pragma unroll
-    for (int r = 0; r < kRows; ++r, src += step) to[r] = *reinterpret_cast<const Pack<T, V>*>(src);
+    for (int r = 0; r < kRows; ++r, src += step) to[r] = load_row<T, V, kPastL1>(src);
   } else {
     asm("" : "+l"(src));  // the addresses are those above, but need not all be there before the branch
 #pragma unroll
     for (int r = 0; r < kRows; ++r, src += step)
-      if (at.there >> r & 1) to[r] = *reinterpret_cast<const Pack<T, V>*>(src);
+      if (at.there >> r & 1) to[r] = load_row<T, V, kPastL1>(src);
   }
 }
 template <int V> __device__ __forceinline__ Vec<V> load_state(const float* p, int64_t s, int channels, int c) {
@@ -464,8 +482,8 @@ scan_rows_kernel(const ScanArgs a) {
   const Place<V, kLanes> at(a);
   if (kOnly) pdl_wait();
   Pack<T, V> x[kRows], g[kRows];
-  load_rows<T, V, kLanes>(x, at, a.x, a.x_ld);
-  load_rows<T, V, kLanes>(g, at, a.gates, a.gates_ld);
+  load_rows<T, V, kLanes, !kOnly>(x, at, a.x, a.x_ld);
+  load_rows<T, V, kLanes, !kOnly>(g, at, a.gates, a.gates_ld);
   if (!kOnly) pdl_wait();
   Marks marks = {0u, 0u, 0};
   Vec<V> h;
@@ -564,9 +582,9 @@ scan_backward_rows_kernel(const ScanArgs a) {
   const Place<V, kLanes> at(a);
   if (kOnly) pdl_wait();
   Pack<T, V> x[kRows], g[kRows], d[kRows];
-  load_rows<T, V, kLanes>(x, at, a.x, a.x_ld);
-  load_rows<T, V, kLanes>(g, at, a.gates, a.gates_ld);
-  load_rows<T, V, kLanes>(d, at, a.grad, a.grad_ld);
+  load_rows<T, V, kLanes, !kOnly>(x, at, a.x, a.x_ld);
+  load_rows<T, V, kLanes, !kOnly>(g, at, a.gates, a.gates_ld);
+  load_rows<T, V, kLanes, !kOnly>(d, at, a.grad, a.grad_ld);
   if (!kOnly) pdl_wait();
   Marks marks = {0u, 0u, 0};
   Vec<V> q, h = all<V>(0.f);
