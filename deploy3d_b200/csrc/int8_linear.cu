@@ -44,6 +44,8 @@ __device__ __forceinline__ int64_t live_rows(int64_t rows, const int32_t* num_ro
 template <class T, int kM, int kBytes>
 __global__ void __launch_bounds__(256)
 dot_kernel(const LinearArgs a) {
+  pdl_release();
+  pdl_wait();
   const int64_t rows = live_rows(a.rows, a.num_rows);
   const int64_t m0 = (int64_t)blockIdx.y * kM;
   if (m0 >= rows) return;
@@ -567,6 +569,7 @@ __global__ void __launch_bounds__(256)
 repitch_kernel(const int8_t* __restrict__ from, int64_t from_ld, int8_t* __restrict__ to, int64_t to_ld, int64_t rows, int channels,
                const int32_t* num_rows) {
   pdl_release();
+  pdl_wait();
   rows = live_rows(rows, num_rows);
   const int words = (int)(to_ld / 4);
   const int64_t n = rows * words, nth = (int64_t)gridDim.x * blockDim.x;
@@ -628,15 +631,13 @@ template <class T> int launch_dot(const LinearArgs& a, cudaStream_t st) {
 #define D3D_DOT(M)                                                         \
   do {                                                                     \
     const dim3 grid(gx, (unsigned)ceil_div(a.rows, M));                    \
-    if (wide) dot_kernel<T, M, 16><<<grid, 256, 0, st>>>(a);               \
-    else dot_kernel<T, M, 1><<<grid, 256, 0, st>>>(a);                     \
+    D3D_LAUNCH(true, (wide ? dot_kernel<T, M, 16> : dot_kernel<T, M, 1>), grid, 256, 0, st, a); \
   } while (0)
   if (a.rows == 1) D3D_DOT(1);
   else if (a.rows == 2) D3D_DOT(2);
   else if (a.rows <= 4) D3D_DOT(4);
   else D3D_DOT(8);
 #undef D3D_DOT
-  D3D_CHECK_LAUNCH();
   return D3D_OK;
 }
 
@@ -784,15 +785,16 @@ extern "C" int d3d_int8_linear(int dtype, const int8_t* x, int64_t x_ld, const f
     uint8_t* ws = reinterpret_cast<uint8_t*>(workspace);
     const int64_t pitch = (int64_t)align_up(inputs, 16);
     if (!aligned_rows(x, x_ld)) {
-      repitch_kernel<<<stream_grid(rows * (pitch / 4), 256), 256, 0, st>>>(x, x_ld, (int8_t*)ws, pitch, rows, inputs, num_rows);
+      D3D_LAUNCH(true, repitch_kernel, (unsigned)stream_grid(rows * (pitch / 4), 256), 256, 0, st, x, x_ld, (int8_t*)ws, pitch, rows, inputs,
+                 num_rows);
       a.x = (const int8_t*)ws, a.x_ld = pitch;
       ws += repitched(x, x_ld, rows, inputs);
     }
     if (!aligned_rows(weight, weight_ld)) {
-      repitch_kernel<<<stream_grid(outputs * (pitch / 4), 256), 256, 0, st>>>(weight, weight_ld, (int8_t*)ws, pitch, outputs, inputs, nullptr);
+      D3D_LAUNCH(true, repitch_kernel, (unsigned)stream_grid(outputs * (pitch / 4), 256), 256, 0, st, weight, weight_ld, (int8_t*)ws, pitch,
+                 (int64_t)outputs, inputs, (const int32_t*)nullptr);
       a.w = (const int8_t*)ws, a.w_ld = pitch;
     }
-    D3D_CHECK_LAUNCH();
   }
   auto launch = [&](auto t) -> int {
     using T = decltype(t);
