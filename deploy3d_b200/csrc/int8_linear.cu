@@ -121,7 +121,7 @@ struct TcArgs {
   int stages, k_blocks, accs;
   uint32_t stage_bytes;
   uint32_t idesc;
-  int out_wide;    // rows of the output start on 16 bytes: it has a map
+  int out_piece;   // bytes, 16 at most, that the output's rows start on; with 16 it has a map
 };
 
 struct Shared {
@@ -213,6 +213,29 @@ __device__ __forceinline__ void store_box(const CUtensorMap* map, const void* sr
   asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%2, %3}], [%1];"
                ::"l"((uint64_t)map), "r"(smem_u32(src)), "r"(x), "r"(y) : "memory");
   asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+}
+// A warp's 32 rows of staging, rows from row0 and columns from col0 on, to the output by plain stores of kBytes, which the output's
+// rows are multiples of: 64 bytes of a row side by side.
+template <class T, int kBytes>
+__device__ __forceinline__ void store_rows(const unsigned char* mine, T* out, int outputs, int64_t row0, int64_t rows, int col0) {
+  using P = Pack<T, kBytes / (int)sizeof(T)>;
+  constexpr int kLanes = kPiece / kBytes, kAtOnce = 32 / kLanes;
+  const int at = lane_id() % kLanes * kBytes, c = col0 + at / (int)sizeof(T);
+  if (c >= outputs) return;
+  int row = lane_id() / kLanes;
+  out += (row0 + row) * outputs + c;
+#pragma unroll(kLanes < 8 ? kLanes : 8)
+  for (int i = 0; i < kLanes; ++i, row += kAtOnce, out += (int64_t)kAtOnce * outputs)
+    if (row0 + row < rows)
+      *reinterpret_cast<P*>(out) = *reinterpret_cast<const P*>(mine + row * kPiece + ((at >> 4) ^ (row >> 1 & 3)) * 16 + at % 16);
+}
+// The same for 16-bit results in pieces of 8 bytes or 4 (149 k rows 240 -> 188, two bytes / eight: 39.0 / 29.4 us; 30 k rows 128 -> 1004
+// 39.6 / 25.4; of 32-bit results eight bytes were no faster than four).  Not inlined: the epilogue of whole tiles has no registers
+// to spare for it (238 k rows 64 -> 192 fp16, inlined / not: 31.1 / 29.8 us).
+template <class T>
+__device__ __noinline__ void store_rows_in(int bytes, const unsigned char* mine, T* out, int outputs, int64_t row0, int64_t rows, int col0) {
+  if (bytes == 8) store_rows<T, 8>(mine, out, outputs, row0, rows, col0);
+  else store_rows<T, 4>(mine, out, outputs, row0, rows, col0);
 }
 // kCta CTAs share a tile of kCta * 128 rows: each holds its rows and its share of the weight rows, CTA 0 issues the products.
 template <int kCta, class T>
@@ -380,29 +403,19 @@ linear_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__
           v = fma(mul(v, w), all<kVec>(xs), b);
           *reinterpret_cast<Pack<T, kVec>*>(mine + lane * kPiece + ((j ^ (lane >> 1 & 3)) * 16)) = narrow<T, kVec>(v);
         }
-        if (p.out_wide && row0 + 32 <= rows) {
+        if (p.out_piece == 16 && row0 + 32 <= rows) {
           asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
           __syncwarp();
           if (lane == 0) store_box(&map_out, mine, col0, (int)row0);
-        } else if (p.out_wide) {  // four lanes to a row, up to the last one
+        } else if (p.out_piece == 16) {
           __syncwarp();
-          const int j = lane % 4, c = col0 + j * kVec;
-          if (c < p.l.outputs)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const int row = 8 * i + lane / 4;
-              if (row0 + row < rows)
-                *reinterpret_cast<uint4*>((T*)p.l.out + (row0 + row) * p.l.outputs + c) =
-                    *reinterpret_cast<const uint4*>(mine + row * kPiece + ((j ^ (row >> 1 & 3)) * 16));
-            }
-        } else {  // an element a lane
+          store_rows<T, 16>(mine, (T*)p.l.out, p.l.outputs, row0, rows, col0);
+        } else if (sizeof(T) == 4 || p.out_piece == (int)sizeof(T)) {
           __syncwarp();
-          const int c = lane % kCols;
-          T* out = (T*)p.l.out + (row0 + lane / kCols) * p.l.outputs + col0 + c;
-#pragma unroll 8
-          for (int row = lane / kCols; row < 32; row += 32 / kCols, out += (int64_t)(32 / kCols) * p.l.outputs)
-            if (row0 + row < rows && col0 + c < p.l.outputs)
-              *out = reinterpret_cast<const T*>(mine + row * kPiece + ((c / kVec ^ (row >> 1 & 3)) * 16))[c % kVec];
+          store_rows<T, sizeof(T)>(mine, (T*)p.l.out, p.l.outputs, row0, rows, col0);
+        } else {
+          __syncwarp();
+          store_rows_in(p.out_piece, mine, (T*)p.l.out, p.l.outputs, row0, rows, col0);
         }
       }
       if (++buf == p.accs) buf = 0, acc_phase ^= 1;
@@ -683,14 +696,15 @@ template <int kCta, class T> int launch_tiles(const LinearArgs& a, int cols, cud
   if (p.stages > kMaxStages) p.stages = kMaxStages;
   // D 32-bit integers, A and B signed
   p.idesc = (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(cols >> 3) << 17) | ((uint32_t)(kCta * kTileRows >> 4) << 24);
-  p.out_wide = reinterpret_cast<uintptr_t>(a.out) % 16 == 0 && (int64_t)a.outputs * sizeof(T) % 16 == 0;
+  p.out_piece = 16;
+  while ((reinterpret_cast<uintptr_t>(a.out) | (uintptr_t)a.outputs * sizeof(T)) % p.out_piece) p.out_piece /= 2;
   CUtensorMap map_x, map_w, map_out = {};
   constexpr CUtensorMapDataType kType = sizeof(T) == 4                        ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
                                         : std::is_same<T, __half>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
                                                                          : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
   if (!make_map(&map_x, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, a.x, a.inputs, a.rows, a.x_ld, kBlockK, kTileRows) ||
       !make_map(&map_w, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, a.w, a.inputs, a.outputs, a.w_ld, kBlockK, cols / kCta) ||
-      (p.out_wide && !make_map(&map_out, kType, sizeof(T), a.out, a.outputs, a.rows, a.outputs * sizeof(T), kPiece, 32)))
+      (p.out_piece == 16 && !make_map(&map_out, kType, sizeof(T), a.out, a.outputs, a.rows, a.outputs * sizeof(T), kPiece, 32)))
     return D3D_ERR_CUDA;
   static std::mutex lock;
   static bool set[64] = {};

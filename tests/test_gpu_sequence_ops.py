@@ -527,6 +527,25 @@ def test_linear_by_tiles_of_every_width(d3d, rows, inputs, outputs):
         check_linear(x, s, w, ws, b, d3d.int8_linear(x, s, w, ws, b, dtype=dtype))
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("outputs", [24, 20, 18, 17, 264, 260, 258, 257])
+@pytest.mark.parametrize("start", [0, 1, 2, 4, 8])
+def test_linear_into_places_of_every_alignment(d3d, dtype, outputs, start):
+    """Rows of the result that start on 2, 4, 8 or 16 bytes; what lies around it stays as it was."""
+    for rows in (100, 300):
+        x, w = int8(1, rows, 80), int8(2, outputs, 80)
+        s, ws, b = 0.01 * normal(3, rows).abs(), 0.01 * normal(4, outputs), normal(5, outputs)
+        buf = torch.full((rows * outputs + 64,), 7.0, device=DEV, dtype=dtype)
+        out = buf[start:start + rows * outputs].view(rows, outputs)
+        d3d.int8_linear(x, s, w, ws, b, dtype=dtype, out=out)
+        check_linear(x, s, w, ws, b, out)
+        assert (buf[:start] == 7).all() and (buf[start + rows * outputs:] == 7).all()
+        out.fill_(7.0)
+        d3d.int8_linear(x, s, w, ws, b, dtype=dtype, out=out, num_rows=live(90))
+        check_linear(x[:90], s[:90], w, ws, b, out[:90])
+        assert (buf[:start] == 7).all() and (buf[start + 90 * outputs:] == 7).all()
+
+
 @pytest.mark.parametrize("rows,count", [(8, 5), (8, 0), (50, 33), (50, 0), (300, 200), (300, 0), (300, -3), (20000, 19001), (20000, 40000)])
 def test_linear_counts(d3d, rows, count):
     inputs = 64 if rows > 300 else 512  # few rows: a sum shared by a cluster
