@@ -46,6 +46,8 @@ constexpr int kNumSMs = 148;  // B200: 2 dies x 74 SMs; grids of streaming kerne
 
 static inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 static inline size_t align_up(size_t x, size_t a) { return (x + a - 1) / a * a; }
+// Whether all of these addresses (null ones too) are multiples of `bytes`.
+template <class... P> bool on_multiples(size_t bytes, const P*... p) { return ((reinterpret_cast<uintptr_t>(p) % bytes == 0) && ...); }
 static inline size_t next_pow2(size_t x) {
   size_t y = 1;
   while (y < x) y <<= 1;

@@ -715,9 +715,8 @@ int check_scan(int dtype, const ScanArgs& a) {
   D3D_REQUIRE(a.rows >= 0 && a.channels >= 1 && a.seqs >= 0 && a.x_ld >= a.channels && a.gates_ld >= a.channels && a.offsets,
               D3D_ERR_INVALID_ARGUMENT);
   D3D_REQUIRE(a.rows < (1ll << 31) && a.channels <= (1 << 16), D3D_ERR_TOO_LARGE);
-  const int esize = (int)dtype_size(dtype);
-  D3D_REQUIRE(reinterpret_cast<uintptr_t>(a.x) % esize == 0 && reinterpret_cast<uintptr_t>(a.gates) % esize == 0 &&
-                  reinterpret_cast<uintptr_t>(a.grad) % esize == 0,
+  D3D_REQUIRE(on_multiples(dtype_size(dtype), a.x, a.gates, a.out, a.grad, a.grad_x, a.grad_gates) &&
+                  on_multiples(4, a.offsets, a.initial, a.final_state, a.states, a.grad_final, a.grad_initial),
               D3D_ERR_INVALID_ARGUMENT);
   return D3D_OK;
 }
@@ -838,8 +837,7 @@ extern "C" int d3d_gated_recurrence_step(int dtype, const void* x, int64_t x_ld,
   D3D_REQUIRE(rows >= 0 && channels >= 1 && x_ld >= channels && gates_ld >= channels, D3D_ERR_INVALID_ARGUMENT);
   if (rows == 0) return D3D_OK;
   const int esize = (int)dtype_size(dtype);
-  D3D_REQUIRE(x && gates && state && state_out && out && reinterpret_cast<uintptr_t>(x) % esize == 0 &&
-                  reinterpret_cast<uintptr_t>(gates) % esize == 0 && reinterpret_cast<uintptr_t>(out) % esize == 0,
+  D3D_REQUIRE(x && gates && state && state_out && out && on_multiples(esize, x, gates, out) && on_multiples(4, state, state_out),
               D3D_ERR_INVALID_ARGUMENT);
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   auto wide_rows = [esize](const void* p, int64_t ld) { return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld * esize % 16 == 0; };

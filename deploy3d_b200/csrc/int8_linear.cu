@@ -786,7 +786,8 @@ extern "C" int d3d_int8_linear(int dtype, const int8_t* x, int64_t x_ld, const f
                   ceil_div(rows, kTileRows) * ceil_div(outputs, 16) < (1ll << 30),
               D3D_ERR_TOO_LARGE);
   if (rows == 0) return D3D_OK;
-  D3D_REQUIRE(x && x_scales && weight && weight_scales && out && reinterpret_cast<uintptr_t>(out) % esize == 0,
+  D3D_REQUIRE(x && x_scales && weight && weight_scales && out && on_multiples(esize, out) &&
+                  on_multiples(4, x_scales, num_rows, weight_scales, bias),
               D3D_ERR_INVALID_ARGUMENT);
   const size_t need = d3d_int8_linear_workspace(x, x_ld, rows, weight, weight_ld, inputs, outputs);
   D3D_REQUIRE(need == 0 || (workspace && reinterpret_cast<uintptr_t>(workspace) % 256 == 0), D3D_ERR_INVALID_ARGUMENT);

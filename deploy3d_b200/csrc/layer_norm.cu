@@ -483,7 +483,6 @@ template <class F> int by_type(int dtype, F f) {
 bool rows_wide(const void* p, int64_t ld, int esize) {
   return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld * esize % 16 == 0;
 }
-bool rows_aligned(const void* p, int esize) { return reinterpret_cast<uintptr_t>(p) % esize == 0; }
 
 // CTAs of `kernel` that fill the GPU once.
 template <class K> int resident(K kernel, int threads, size_t smem) {
@@ -529,8 +528,7 @@ extern "C" int d3d_layer_norm(int dtype, const void* x, int64_t x_ld, const void
               D3D_ERR_INVALID_ARGUMENT);
   D3D_REQUIRE(channels <= kMaxChannels, D3D_ERR_TOO_LARGE);
   if (rows == 0) return D3D_OK;
-  D3D_REQUIRE(x && out && rows_aligned(x, esize) && rows_aligned(residual, esize) && rows_aligned(out, esize) &&
-                  rows_aligned(total, esize),
+  D3D_REQUIRE(x && out && on_multiples(esize, x, residual, out, total) && on_multiples(4, weight, bias, num_rows, mean, rstd),
               D3D_ERR_INVALID_ARGUMENT);
   NormArgs a = {};
   a.x = x, a.x_ld = x_ld, a.residual = residual, a.residual_ld = residual_ld, a.weight = weight, a.bias = bias, a.eps = eps;
@@ -552,7 +550,7 @@ extern "C" int d3d_layer_norm_int8(int dtype, const void* x, int64_t x_ld, const
               D3D_ERR_INVALID_ARGUMENT);
   D3D_REQUIRE(channels <= kMaxChannels, D3D_ERR_TOO_LARGE);
   if (rows == 0) return D3D_OK;
-  D3D_REQUIRE(x && q && scales && rows_aligned(x, esize) && rows_aligned(residual, esize) && rows_aligned(total, esize),
+  D3D_REQUIRE(x && q && scales && on_multiples(esize, x, residual, total) && on_multiples(4, weight, bias, num_rows, scales),
               D3D_ERR_INVALID_ARGUMENT);
   NormArgs a = {};
   a.x = x, a.x_ld = x_ld, a.residual = residual, a.residual_ld = residual_ld, a.weight = weight, a.bias = bias, a.eps = eps;
@@ -570,7 +568,7 @@ extern "C" int d3d_quantize_rows(int dtype, const void* x, int64_t x_ld, int64_t
   D3D_REQUIRE(rows >= 0 && channels >= 1 && x_ld >= channels && q_ld >= channels, D3D_ERR_INVALID_ARGUMENT);
   D3D_REQUIRE(channels <= kMaxChannels, D3D_ERR_TOO_LARGE);
   if (rows == 0) return D3D_OK;
-  D3D_REQUIRE(x && q && scales && rows_aligned(x, esize), D3D_ERR_INVALID_ARGUMENT);
+  D3D_REQUIRE(x && q && scales && on_multiples(esize, x) && on_multiples(4, num_rows, scales), D3D_ERR_INVALID_ARGUMENT);
   NormArgs a = {};
   a.x = x, a.x_ld = x_ld, a.rows = rows, a.channels = channels, a.num_rows = num_rows, a.q = q, a.q_ld = q_ld, a.scales = scales;
   const bool wide = channels * esize % 16 == 0 && rows_wide(x, x_ld, esize) && reinterpret_cast<uintptr_t>(q) % 8 == 0 && q_ld % 8 == 0;
@@ -594,9 +592,9 @@ extern "C" int d3d_layer_norm_backward(int dtype, const void* grad, int64_t grad
               D3D_ERR_INVALID_ARGUMENT);
   D3D_REQUIRE(channels <= kMaxChannels, D3D_ERR_TOO_LARGE);
   D3D_REQUIRE(rows == 0 || (x && grad && mean && rstd && grad_x), D3D_ERR_INVALID_ARGUMENT);
-  D3D_REQUIRE(rows_aligned(x, esize) && rows_aligned(grad, esize) && rows_aligned(grad_total, esize) && rows_aligned(grad_x, esize),
+  D3D_REQUIRE(on_multiples(esize, x, grad, grad_total, grad_x) && on_multiples(4, weight, mean, rstd, num_rows, grad_weight, grad_bias),
               D3D_ERR_INVALID_ARGUMENT);
-  D3D_REQUIRE(workspace && reinterpret_cast<uintptr_t>(workspace) % 4 == 0, D3D_ERR_INVALID_ARGUMENT);
+  D3D_REQUIRE(workspace && on_multiples(4, workspace), D3D_ERR_INVALID_ARGUMENT);
   D3D_REQUIRE(workspace_bytes >= d3d_layer_norm_backward_workspace(rows, channels), D3D_ERR_WORKSPACE_TOO_SMALL);
   NormBackwardArgs a = {};
   a.grad = grad, a.grad_ld = grad_ld, a.x = x, a.x_ld = x_ld, a.grad_total = grad_total, a.grad_total_ld = grad_total_ld;

@@ -57,6 +57,43 @@ def test_entry_points_refuse_bad_arguments(d3d):
         assert step(**bad) == BAD, bad
 
 
+def test_entry_points_refuse_addresses_off_their_elements(d3d):
+    """Every pointer that a kernel would follow, one byte off: two-byte features, four-byte parameters, states, scales, counts."""
+    from deploy3d_b200 import _lib
+    lib, F = _lib.lib(), _lib.D3D_HALF
+    V = ctypes.c_void_p
+    odd, half = V(4097), V(4098)
+
+    def refuses(fn, good, pointers):
+        """`good` would be launched; with any of the pointers off its elements it is refused."""
+        for name, size in pointers.items():
+            for bad in (odd, half) if size == 4 else (odd,):
+                assert fn(*dict(good, **{name: bad}).values()) == BAD, (fn.__name__, name, bad.value)
+    norm = dict(dt=F, x=ONE, ld=16, res=ONE, rld=16, w=ONE, b=ONE, eps=1e-5, rows=4, ch=16, num=ONE, total=ONE, out=ONE, mean=ONE,
+                rstd=ONE, st=None)
+    refuses(lib.d3d_layer_norm, norm, dict(x=2, res=2, total=2, out=2, w=4, b=4, num=4, mean=4, rstd=4))
+    norm8 = dict(dt=F, x=ONE, ld=16, res=ONE, rld=16, w=ONE, b=ONE, eps=1e-5, rows=4, ch=16, num=ONE, total=ONE, q=ONE, qld=16,
+                 s=ONE, st=None)
+    refuses(lib.d3d_layer_norm_int8, norm8, dict(x=2, res=2, total=2, w=4, b=4, num=4, s=4))
+    quant = dict(dt=F, x=ONE, ld=16, rows=4, ch=16, num=ONE, q=ONE, qld=16, s=ONE, st=None)
+    refuses(lib.d3d_quantize_rows, quant, dict(x=2, num=4, s=4))
+    back = dict(dt=F, g=ONE, gld=16, x=ONE, ld=16, t=ONE, tld=16, w=ONE, m=ONE, r=ONE, rows=4, ch=16, num=ONE, gx=ONE, gw=ONE,
+                gb=ONE, ws=ONE, nb=1 << 20, st=None)
+    refuses(lib.d3d_layer_norm_backward, back, dict(g=2, x=2, t=2, gx=2, w=4, m=4, r=4, num=4, gw=4, gb=4, ws=4))
+    lin = dict(dt=F, x=ONE, ld=16, s=ONE, rows=100, num=ONE, w=ONE, wld=16, ws=ONE, b=ONE, k=16, n=16, out=ONE, work=ONE, nb=1 << 20,
+               st=None)
+    refuses(lib.d3d_int8_linear, lin, dict(out=2, s=4, num=4, ws=4, b=4))
+    for rows in (100, 200):  # one tile, several
+        scan = dict(dt=F, x=ONE, ld=16, g=ONE, gld=16, offs=ONE, seqs=2, rows=rows, ch=16, rev=0, init=ONE, out=ONE, fin=ONE, states=ONE,
+                    ws=ONE, nb=1 << 20, st=None)
+        refuses(lib.d3d_gated_recurrence, scan, dict(x=2, g=2, out=2, offs=4, init=4, fin=4, states=4))
+        back = dict(dt=F, d=ONE, dld=16, x=ONE, ld=16, g=ONE, gld=16, offs=ONE, seqs=2, rows=rows, ch=16, rev=0, states=ONE, init=ONE,
+                    gf=ONE, gx=ONE, gg=ONE, gi=ONE, ws=ONE, nb=1 << 20, st=None)
+        refuses(lib.d3d_gated_recurrence_backward, back, dict(d=2, x=2, g=2, gx=2, gg=2, offs=4, states=4, init=4, gf=4, gi=4))
+    step = dict(dt=F, x=ONE, ld=16, g=ONE, gld=16, s=ONE, so=ONE, out=ONE, rows=4, ch=16, st=None)
+    refuses(lib.d3d_gated_recurrence_step, step, dict(x=2, g=2, out=2, s=4, so=4))
+
+
 def test_operators_refuse_what_they_cannot_run(d3d):
     x = torch.zeros((4, 16))
     with pytest.raises(ValueError):
