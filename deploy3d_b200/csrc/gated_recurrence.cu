@@ -173,7 +173,7 @@ template <int V> __device__ __forceinline__ Vec<V> load_state(const float* p, in
   Vec<V> r = all<V>(0.f);
   if (p)
 #pragma unroll
-    for (int e = 0; e < V; ++e) r.v[e] = __ldg(p + s * channels + c + e);
+    for (int e = 0; e < V; ++e) r.v[e] = load_fresh(p + s * channels + c + e);
   return r;
 }
 template <int V> __device__ __forceinline__ void store_state(float* p, int64_t s, int channels, int c, const Vec<V>& h) {
@@ -187,7 +187,7 @@ __device__ __forceinline__ int sequence_of(const ScanArgs& a, int64_t t) {
   int lo = 0, n = a.seqs;
   while (n > 1) {
     const int step = (n + 31) / 32, at = lo + lane_id() * step;
-    const unsigned before = __ballot_sync(0xffffffffu, at < lo + n && __ldg(a.offsets + at) <= t);
+    const unsigned before = __ballot_sync(0xffffffffu, at < lo + n && load_fresh(a.offsets + at) <= t);
     const int k = before ? __popc(before) - 1 : 0, end = lo + n;
     lo += k * step;
     if (lo > end - 1) lo = end - 1;  // offsets out of order
@@ -200,8 +200,8 @@ __device__ __forceinline__ int sequence_of(const ScanArgs& a, int64_t t) {
 struct Finder {
   int s;
   __device__ __forceinline__ int of(const ScanArgs& a, int64_t t) {
-    while (s + 1 < a.seqs && __ldg(a.offsets + s + 1) <= t) ++s;
-    while (s > 0 && __ldg(a.offsets + s) > t) --s;
+    while (s + 1 < a.seqs && load_fresh(a.offsets + s + 1) <= t) ++s;
+    while (s > 0 && load_fresh(a.offsets + s) > t) --s;
     return s;
   }
 };
@@ -224,7 +224,7 @@ __device__ __forceinline__ Marks mark_ends(const ScanArgs& a, const Place<V, kLa
   for (int base = owner; base < a.seqs; base += 32) {
     const int s = base + lane_id();
     const bool in = s < a.seqs;
-    const int64_t b = in ? (int64_t)__ldg(a.offsets + s) - low : kSpan, e = in ? (int64_t)__ldg(a.offsets + s + 1) - 1 - low : kSpan;
+    const int64_t b = in ? (int64_t)load_fresh(a.offsets + s) - low : kSpan, e = in ? (int64_t)load_fresh(a.offsets + s + 1) - 1 - low : kSpan;
     if (b <= e) {
       if (b >= 0 && b < kSpan) first[kSpan > 32 ? (int)b >> 5 : 0] |= 1u << ((int)b & 31);
       if (e >= 0 && e < kSpan) last[kSpan > 32 ? (int)e >> 5 : 0] |= 1u << ((int)e & 31);
@@ -243,7 +243,7 @@ __device__ __forceinline__ Marks mark_ends(const ScanArgs& a, const Place<V, kLa
     f = __brevll(l) >> (64 - kSpan), l = __brevll(up) >> (64 - kSpan);
   }
   const int shift = lane_id() / kLanes * kRows;
-  const uint32_t live = at.there & at.span(at.low_row(), __ldg(a.offsets), __ldg(a.offsets + a.seqs));
+  const uint32_t live = at.there & at.span(at.low_row(), load_fresh(a.offsets), load_fresh(a.offsets + a.seqs));
   const uint32_t starts = (uint32_t)(f >> shift) & live, ends = (uint32_t)(l >> shift) & live;
   return {live, starts | ends << 16, owner};
 }
@@ -354,8 +354,8 @@ __device__ __forceinline__ void pass_empty(const ScanArgs& a, const Place<V, kLa
   const int tiles = a.tiles > 0 ? a.tiles : 1, low = at.slab * V * kLanes;
   const int high = low + V * kLanes < a.channels ? low + V * kLanes : a.channels;
   for (int64_t s = (int64_t)at.tile * kThreads + threadIdx.x; s < a.seqs; s += (int64_t)tiles * kThreads)
-    if (__ldg(a.offsets + s + 1) <= __ldg(a.offsets + s))
-      for (int c = low; c < high; ++c) to[s * a.channels + c] = from ? __ldg(from + s * a.channels + c) : 0.f;
+    if (load_fresh(a.offsets + s + 1) <= load_fresh(a.offsets + s))
+      for (int c = low; c < high; ++c) to[s * a.channels + c] = from ? load_fresh(from + s * a.channels + c) : 0.f;
 }
 
 // The map of a thread's rows, those from the last start of a sequence on: what was in front of it is gone.  Rows between two ends of
@@ -409,7 +409,7 @@ scan_maps_kernel(const ScanArgs a) {
 // CTA; 256 threads of each take kHeld tiles into registers, chain them, and are chained by shuffles and through shared memory.
 constexpr int kHeld = 16, kCarryThreads = 512, kCarryChannels = 2, kCarryWarps = kCarryThreads / 32;
 __global__ void __launch_bounds__(kCarryThreads)
-carry_kernel(const float2* __restrict__ maps, float* __restrict__ into, int tiles, int channels, int backward) {
+carry_kernel(const float2* maps, float* __restrict__ into, int tiles, int channels, int backward) {
   __shared__ float2 totals[kCarryWarps][kCarryChannels];
   __shared__ float starts[kCarryWarps][kCarryChannels];
   const int lane = lane_id(), warp = threadIdx.x >> 5, ch = threadIdx.x % kCarryChannels, c = blockIdx.x * kCarryChannels + ch;
@@ -653,8 +653,8 @@ scan_backward_rows_kernel(const ScanArgs a) {
 // One row a sequence: the state is read, moved on and written; state_out may be state.
 template <class T, int V>
 __global__ void __launch_bounds__(256)
-step_kernel(const T* __restrict__ x, int64_t x_ld, const T* __restrict__ gates, int64_t gates_ld, const float* state,
-            float* state_out, T* __restrict__ out, int64_t rows, int channels) {
+step_kernel(const T* x, int64_t x_ld, const T* gates, int64_t gates_ld, const float* state,
+            float* state_out, T* out, int64_t rows, int channels) {
   using P = Pack<T, V>;
   pdl_wait();
   pdl_release();

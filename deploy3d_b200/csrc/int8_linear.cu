@@ -32,12 +32,6 @@ struct LinearArgs {
   int inputs, outputs;
 };
 
-__device__ __forceinline__ int64_t live_rows(int64_t rows, const int32_t* num_rows) {
-  if (!num_rows) return rows;
-  const int64_t n = __ldg(num_rows);
-  return n < 0 ? 0 : n < rows ? n : rows;
-}
-
 // ---- little work ------------------------------------------------------------------------------------------------------
 // A warp per output channel: its weights stream by once, eight pieces of a lane on their way, and are multiplied with those of kM
 // rows.  kBytes: what one load takes (16 where rows start on 16 bytes, else one).
@@ -52,8 +46,8 @@ dot_kernel(const LinearArgs a) {
   const int n = blockIdx.x * 8 + (threadIdx.x >> 5), lane = lane_id();
   if (n >= a.outputs) return;
   const int8_t* w = a.w + (int64_t)n * a.w_ld;
-  const float ws = __ldg(a.w_scale + n), b = a.bias ? __ldg(a.bias + n) : 0.f;
-  const float xs = lane < kM && m0 + lane < rows ? __ldg(a.x_scale + m0 + lane) : 0.f;
+  const float ws = load_fresh(a.w_scale + n), b = a.bias ? load_fresh(a.bias + n) : 0.f;
+  const float xs = lane < kM && m0 + lane < rows ? load_fresh(a.x_scale + m0 + lane) : 0.f;
   const int8_t* x[kM];
   int acc[kM];
 #pragma unroll
@@ -354,11 +348,11 @@ linear_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__
       if (next_t != of_tile) {
         const int2 tile = tiles.at(next_t);
         m = (tile.x * kCta + (int)rank) * kTileRows + quarter * 32, n_tile = tile.y * p.cols, of_tile = next_t;
-        next_x = m + lane < rows ? __ldg(p.l.x_scale + m + lane) : 0.f;
+        next_x = m + lane < rows ? load_fresh(p.l.x_scale + m + lane) : 0.f;
       }
       const int n = n_tile + piece * kCols + lane;
       const bool in = lane < kCols && n < p.l.outputs;
-      next_w = in ? __ldg(p.l.w_scale + n) : 0.f, next_b = in && p.l.bias ? __ldg(p.l.bias + n) : 0.f;
+      next_w = in ? load_fresh(p.l.w_scale + n) : 0.f, next_b = in && p.l.bias ? load_fresh(p.l.bias + n) : 0.f;
     };
     ask();
     int buf = 0, acc_phase = 0;
@@ -530,8 +524,8 @@ few_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
       mbar_drain(&sh->drained, 0);
     }
   } else {
-    if (mine) ws = __ldg(p.l.w_scale + n), b = p.l.bias ? __ldg(p.l.bias + n) : 0.f;
-    if ((int)threadIdx.x < rows) sh->x_scale[threadIdx.x] = __ldg(p.l.x_scale + threadIdx.x);
+    if (mine) ws = load_fresh(p.l.w_scale + n), b = p.l.bias ? load_fresh(p.l.bias + n) : 0.f;
+    if ((int)threadIdx.x < rows) sh->x_scale[threadIdx.x] = load_fresh(p.l.x_scale + threadIdx.x);
     asm volatile("bar.sync 1, 128;" ::: "memory");
     if (k1 > k0) ok = __all_sync(0xffffffffu, mbar_wait(&sh->done, 0, abort_flag, 4, kWaitLimitCycles));
     tc_fence_after();
@@ -579,7 +573,7 @@ few_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
 
 // Rows of bytes that do not start on 16 bytes: copied so that they do.
 __global__ void __launch_bounds__(256)
-repitch_kernel(const int8_t* __restrict__ from, int64_t from_ld, int8_t* __restrict__ to, int64_t to_ld, int64_t rows, int channels,
+repitch_kernel(const int8_t* from, int64_t from_ld, int8_t* to, int64_t to_ld, int64_t rows, int channels,
                const int32_t* num_rows) {
   pdl_release();
   pdl_wait();

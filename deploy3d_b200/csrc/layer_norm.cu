@@ -31,12 +31,6 @@ struct NormArgs {
   float* scales;
 };
 
-__device__ __forceinline__ int64_t live_rows(int64_t rows, const int32_t* num_rows) {
-  if (!num_rows) return rows;
-  const int64_t n = __ldg(num_rows);
-  return n < 0 ? 0 : n < rows ? n : rows;
-}
-
 struct Add {
   __device__ __forceinline__ float operator()(float a, float b) const { return a + b; }
 };
@@ -167,14 +161,14 @@ template <int V, int kVecs, int kLanes> struct Columns {
   // The caller's barrier before the first use.
   __device__ __forceinline__ Columns(Store& shared, const float* p, float without, int lane, int channels) : store(shared) {
     if constexpr (kShared) {
-      for (int c = threadIdx.x; c < kWidth; c += threads_for<kLanes>()) shared[c] = c >= channels ? 0.f : p ? __ldg(p + c) : without;
+      for (int c = threadIdx.x; c < kWidth; c += threads_for<kLanes>()) shared[c] = c >= channels ? 0.f : p ? load_fresh(p + c) : without;
     } else {
 #pragma unroll
       for (int k = 0; k < kVecs; ++k)
 #pragma unroll
         for (int e = 0; e < V; ++e) {
           const int c = (k * kLanes + lane) * V + e;
-          held[k].v[e] = c >= channels ? 0.f : p ? __ldg(p + c) : without;
+          held[k].v[e] = c >= channels ? 0.f : p ? load_fresh(p + c) : without;
         }
     }
   }
@@ -322,7 +316,7 @@ norm_backward_kernel(const NormBackwardArgs a) {
     const bool has = at < rows;
     in[I].load(has, lane, channels);
     grad[I].load(has, lane, channels);
-    next_mean[I] = has ? __ldg(a.mean + at) : 0.f, next_rstd[I] = has ? __ldg(a.rstd + at) : 0.f;
+    next_mean[I] = has ? load_fresh(a.mean + at) : 0.f, next_rstd[I] = has ? load_fresh(a.rstd + at) : 0.f;
   };
   load(std::integral_constant<int, 0>(), row);
   load(std::integral_constant<int, 1>(), row + stride);
@@ -416,7 +410,7 @@ norm_backward_kernel(const NormBackwardArgs a) {
 
 // Sums the CTAs' partial gradients in a fixed order: eight columns to a CTA, 64 threads of each take the partials in turn.
 __global__ void __launch_bounds__(512)
-norm_columns_kernel(const float* __restrict__ partial, int parts, int channels, float* __restrict__ grad_weight,
+norm_columns_kernel(const float* partial, int parts, int channels, float* __restrict__ grad_weight,
                     float* __restrict__ grad_bias) {
   __shared__ float s[16][8];
   pdl_release();

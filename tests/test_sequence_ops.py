@@ -1,5 +1,7 @@
 """What the voxel-sequence operators refuse, and their formulas' gradients against differences (CPU)."""
 import ctypes
+import os
+import re
 
 import numpy as np
 import pytest
@@ -92,6 +94,16 @@ def test_entry_points_refuse_addresses_off_their_elements(d3d):
         refuses(lib.d3d_gated_recurrence_backward, back, dict(d=2, x=2, g=2, gx=2, gg=2, offs=4, states=4, init=4, gf=4, gi=4))
     step = dict(dt=F, x=ONE, ld=16, g=ONE, gld=16, s=ONE, so=ONE, out=ONE, rows=4, ch=16, st=None)
     refuses(lib.d3d_gated_recurrence_step, step, dict(x=2, g=2, out=2, s=4, so=4))
+
+
+def test_kernels_read_what_may_still_be_written_by_plain_loads():
+    """The kernels live while the one in front of them still writes, so none of their loads may be of the kind that takes memory
+    for constant as long as the kernel lives: __ldg, or what a const __restrict__ argument allows a plain load to become."""
+    root = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "deploy3d_b200", "csrc")
+    for name in ("layer_norm.cu", "int8_linear.cu", "gated_recurrence.cu", "packed.cuh"):
+        text = re.sub(r"//[^\n]*", "", open(os.path.join(root, name)).read())
+        assert "__ldg(" not in text and ".nc." not in text, name
+        assert not re.search(r"const \w+\s*\*\s*__restrict__", text), name
 
 
 def test_operators_refuse_what_they_cannot_run(d3d):
