@@ -115,6 +115,7 @@ struct TcArgs {
   int stages, k_blocks, accs;
   uint32_t stage_bytes;
   uint32_t idesc;
+  uint32_t wait_limit;  // cycles after which a wait gives up
   int out_piece;   // bytes, 16 at most, that the output's rows start on; with 16 it has a map
 };
 
@@ -123,7 +124,7 @@ struct Shared {
   uint64_t empty[kMaxStages];  // MMA -> TMA
   uint64_t acc_full[kMaxAcc];   // MMA -> epilogue
   uint64_t acc_empty[kMaxAcc];  // epilogue -> MMA
-  uint64_t drained;            // MMA, where a wait has given up: the products on their way
+  uint64_t drained;            // MMA: all products
   uint32_t tmem;
   int abort;
   alignas(16) float scale[kEpilogueWarps][2][32];  // of a warp's piece: weight scales, bias
@@ -174,6 +175,13 @@ template <int kCta> __device__ __forceinline__ void commit(uint64_t* bar) {
   else
     asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
                  ::"r"(smem_u32(bar)), "h"((uint16_t)3) : "memory");
+}
+// The same for this CTA's barrier alone.
+template <int kCta> __device__ __forceinline__ void commit_here(uint64_t* bar) {
+  if (kCta == 1)
+    umma_commit(bar);
+  else
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
 template <int kCta> __device__ __forceinline__ void alloc_tmem(uint32_t* dst) {
   if (kCta == 1) {
@@ -271,7 +279,7 @@ linear_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__
         const int2 tile = tiles.at(t);
         const int m0 = (tile.x * kCta + (int)rank) * kTileRows, n0 = tile.y * p.cols + (int)rank * (p.cols / kCta);
         for (int k = 0; k < p.k_blocks; ++k) {
-          ok = mbar_wait(&sh->empty[stage], phase ^ 1, abort_flag, 1, kWaitLimitCycles);
+          ok = mbar_wait(&sh->empty[stage], phase ^ 1, abort_flag, 1, p.wait_limit);
           if (!ok) break;
           unsigned char* a = ring + stage * p.stage_bytes;
           if (rank == 0) mbar_arrive_expect_tx(&sh->full[stage], kCta * p.stage_bytes);
@@ -280,9 +288,10 @@ linear_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__
           if (++stage == p.stages) stage = 0, phase ^= 1;
         }
       }
-      // The CTAs do not end with copies on their way, whoever has given up (those of both count here).
-      if (rank == 0)
-        for (int s = 0; s < p.stages; ++s) mbar_drain(&sh->full[s], s < stage ? phase : phase ^ 1);
+      // The CTAs do not end with copies on their way, whoever has given up.  Those of both count on the leader's barriers; but where
+      // that has given up first the other one's last ones do not, so the other one waits for the products of what it has
+      // brought, or as long as no copy takes.
+      mbar_drain_ring(rank == 0 ? sh->full : sh->empty, p.stages, stage, phase);
     }
   } else if (warp == kEpilogueWarps + 1) {
     // The whole warp walks by counters and one lane of it waits and issues: what feeds an MMA has to be the same for all lanes in a
@@ -295,7 +304,7 @@ linear_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__
       int stage = 0, phase = 0, buf = 0, acc_phase = 0;
       bool bad = false;
       for (int t = tiles.first; t < tiles.count; t += tiles.step) {
-        if (!bad) bad = !mbar_wait(&sh->acc_empty[buf], acc_phase ^ 1, abort_flag, 2, kWaitLimitCycles);
+        if (!bad) bad = !mbar_wait(&sh->acc_empty[buf], acc_phase ^ 1, abort_flag, 2, p.wait_limit);
         bad = __any_sync(0xffffffffu, bad);
         if (bad) break;
         tc_fence_after();
@@ -305,7 +314,7 @@ linear_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__
           const uint64_t da = (uint64_t)kHigh << 32 | low, db = (uint64_t)kHigh << 32 | (low + (kABytes >> 4));
           const int n = k == p.k_blocks - 1 ? last : 4;
           if (elect_one()) {
-            if (!bad) bad = !mbar_wait(&sh->full[stage], phase, abort_flag, 3, kWaitLimitCycles);
+            if (!bad) bad = !mbar_wait(&sh->full[stage], phase, abort_flag, 3, p.wait_limit);
             if (!bad) {
               tc_fence_after();
               // 32 channels further is 32 bytes further
@@ -322,8 +331,9 @@ linear_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__
         }
         if (++buf == p.accs) buf = 0, acc_phase ^= 1;
       }
-      if (__any_sync(0xffffffffu, bad) && elect_one()) {
-        commit<kCta>(&sh->drained);
+      // Nor with products on their way: the epilogue may have given up on what has been issued here.
+      if (elect_one()) {
+        commit_here<kCta>(&sh->drained);
         mbar_drain(&sh->drained, 0);
       }
     }
@@ -357,7 +367,7 @@ linear_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__
     ask();
     int buf = 0, acc_phase = 0;
     for (int t = tiles.first; t < tiles.count; t += tiles.step) {
-      const bool ok = mbar_wait(&sh->acc_full[buf], acc_phase, abort_flag, 4, kWaitLimitCycles);
+      const bool ok = mbar_wait(&sh->acc_full[buf], acc_phase, abort_flag, 4, p.wait_limit);
       if (!__all_sync(0xffffffffu, ok)) break;
       tc_fence_after();
       // What the MMA warp waits for is that all have loaded, not that they are done.
@@ -438,7 +448,7 @@ struct FewArgs {
   int cols;        // rows of the input, rounded up to 16
   int k_blocks, splits, stages;
   int share;       // rows whose sums a CTA of a cluster adds up: every splits-th
-  uint32_t stage_bytes, tmem_cols, idesc;
+  uint32_t stage_bytes, tmem_cols, idesc, wait_limit;
 };
 struct FewShared {
   uint64_t full[kMaxStages], empty[kMaxStages], done, drained;
@@ -485,14 +495,14 @@ few_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
     if (lane == 0) {
       int stage = 0, phase = 0;
       for (int k = k0; k < k1; ++k) {
-        if (!mbar_wait(&sh->empty[stage], phase ^ 1, abort_flag, 1, kWaitLimitCycles)) break;
+        if (!mbar_wait(&sh->empty[stage], phase ^ 1, abort_flag, 1, p.wait_limit)) break;
         unsigned char* a = ring + stage * p.stage_bytes;
         mbar_arrive_expect_tx(&sh->full[stage], p.stage_bytes);
         tma_load_2d(&map_w, &sh->full[stage], a, k * kBlockK, n0);
         tma_load_2d(&map_x, &sh->full[stage], a + kABytes, k * kBlockK, 0);
         if (++stage == p.stages) stage = 0, phase ^= 1;
       }
-      for (int s = 0; s < p.stages; ++s) mbar_drain(&sh->full[s], s < stage ? phase : phase ^ 1);
+      mbar_drain_ring(sh->full, p.stages, stage, phase);
     }
   } else if (warp == 5) {
     constexpr uint32_t kHigh = 64u | (1u << 14) | (2u << 29);
@@ -505,7 +515,7 @@ few_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
       const uint64_t da = (uint64_t)kHigh << 32 | low, db = (uint64_t)kHigh << 32 | (low + (kABytes >> 4));
       const int steps = k == p.k_blocks - 1 ? last : 4;
       if (elect_one()) {
-        if (!bad) bad = !mbar_wait(&sh->full[stage], phase, abort_flag, 3, kWaitLimitCycles);
+        if (!bad) bad = !mbar_wait(&sh->full[stage], phase, abort_flag, 3, p.wait_limit);
         if (!bad) {
           tc_fence_after();
           mma_i8<1>(tmem, da, db, p.idesc, k > k0);
@@ -519,7 +529,8 @@ few_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
       __syncwarp();
       if (++stage == p.stages) stage = 0, phase ^= 1;
     }
-    if (__any_sync(0xffffffffu, bad) && elect_one()) {
+    // products are seen out as above, also where it is the epilogue that has given up on them
+    if (elect_one()) {
       umma_commit(&sh->drained);
       mbar_drain(&sh->drained, 0);
     }
@@ -527,7 +538,7 @@ few_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
     if (mine) ws = load_fresh(p.l.w_scale + n), b = p.l.bias ? load_fresh(p.l.bias + n) : 0.f;
     if ((int)threadIdx.x < rows) sh->x_scale[threadIdx.x] = load_fresh(p.l.x_scale + threadIdx.x);
     asm volatile("bar.sync 1, 128;" ::: "memory");
-    if (k1 > k0) ok = __all_sync(0xffffffffu, mbar_wait(&sh->done, 0, abort_flag, 4, kWaitLimitCycles));
+    if (k1 > k0) ok = __all_sync(0xffffffffu, mbar_wait(&sh->done, 0, abort_flag, 4, p.wait_limit));
     tc_fence_after();
     __syncwarp();
     if (p.splits > 1) asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
@@ -664,6 +675,7 @@ template <class T> int launch_few(const LinearArgs& a, cudaStream_t st) {
   p.stages = (int)((227 * 1024 - fixed) / p.stage_bytes);
   if (p.stages > kMaxStages) p.stages = kMaxStages;
   p.tmem_cols = 32;
+  p.wait_limit = wait_limit();
   p.idesc = (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(p.cols >> 3) << 17) | ((uint32_t)(kTileRows >> 4) << 24);
   CUtensorMap map_w, map_x;
   if (!make_map(&map_w, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, a.w, a.inputs, a.outputs, a.w_ld, kBlockK, kTileRows) ||
@@ -690,6 +702,7 @@ template <int kCta, class T> int launch_tiles(const LinearArgs& a, int cols, cud
   if (p.stages > kMaxStages) p.stages = kMaxStages;
   // D 32-bit integers, A and B signed
   p.idesc = (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(cols >> 3) << 17) | ((uint32_t)(kCta * kTileRows >> 4) << 24);
+  p.wait_limit = wait_limit();
   p.out_piece = 16;
   while ((reinterpret_cast<uintptr_t>(a.out) | (uintptr_t)a.outputs * sizeof(T)) % p.out_piece) p.out_piece /= 2;
   CUtensorMap map_x, map_w, map_out = {};

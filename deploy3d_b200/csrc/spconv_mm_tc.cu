@@ -1179,6 +1179,7 @@ extern "C" int d3d_debug_take_kernel_error(int* code) {
 
 // Debug aid without a reference counterpart: after how many cycles a bounded wait of the tensor-core kernel gives up, for every
 // later launch of this process (0 = the usual second).  Not thread-safe.
+uint32_t d3d::wait_limit() { return g_wait_limit; }
 extern "C" int d3d_debug_set_wait_limit(int cycles) {
   D3D_REQUIRE(cycles >= 0, D3D_ERR_INVALID_ARGUMENT);
   d3d::g_wait_limit = cycles ? (uint32_t)cycles : d3d::kWaitLimitCycles;

@@ -65,6 +65,14 @@ __device__ __forceinline__ void mbar_drain(uint64_t* bar, uint32_t parity) {
   while (!mbar_try_wait(bar, parity) && (uint32_t)clock() - t0 <= kWaitLimitCycles) {
   }
 }
+// The same for the stages of a ring, all within one limit: those below `stage` in the phase that was under way, the others in
+// the one before.
+__device__ __forceinline__ void mbar_drain_ring(uint64_t* bars, int stages, int stage, uint32_t phase) {
+  const uint32_t t0 = (uint32_t)clock();
+  for (int s = 0; s < stages; ++s)
+    while (!mbar_try_wait(&bars[s], s < stage ? phase : phase ^ 1) && (uint32_t)clock() - t0 <= kWaitLimitCycles) {
+    }
+}
 __device__ __forceinline__ void tma_load_2d(const CUtensorMap* map, uint64_t* bar, void* dst, int x, int y) {
   asm volatile(
       "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"

@@ -69,9 +69,10 @@ const char* d3d_status_string(int status);
 /* Debug aid (no reference counterpart; the reference only prints CUDA errors, trt/include/common/macros.h:14-34):
  * synchronises the device, returns in *code the error word a kernel of this library raised when one of its bounded
  * waits expired (0 = none) and clears it.  The word is one per process: a wait of a tensor-core kernel (SPConvMM; the products
- * of 8-bit rows, whose codes are above 100) gives up after about one second of wall clock (far beyond any hand-over of a running kernel; a context that is
- * time-sliced away for longer would trip it too), the CTA then drains, part of the output stays unwritten, and the
- * asynchronous enqueue that launched it has long returned D3D_OK.  Not thread-safe. */
+ * of 8-bit rows, whose codes are above 100) gives up after about one second of wall clock (far beyond any hand-over of a
+ * running kernel; a context that is time-sliced away for longer would trip it too), the CTA then sees its copies and
+ * products out, the launch's output is not to be used, and the asynchronous enqueue that launched it has long returned
+ * D3D_OK.  Not thread-safe. */
 int d3d_debug_take_kernel_error(int* code);
 /* Debug aid (no reference counterpart): after how many cycles such a wait gives up, for every later launch of the process;
  * 0 = the usual second.  Tests shorten it.  Not thread-safe. */

@@ -559,6 +559,48 @@ def test_linear_counts(d3d, rows, count):
         check_linear(x[:n], s[:n], w, ws, None, out[:n])
 
 
+@pytest.fixture
+def wait_limit():
+    """Sets the cycles after which a bounded wait gives up; the usual second again afterwards."""
+    from deploy3d_b200 import _lib
+    set_to = lambda cycles: _lib.check("d3d_debug_set_wait_limit", _lib.lib().d3d_debug_set_wait_limit(cycles))
+    yield set_to
+    set_to(0)
+
+
+def kernel_error():
+    import ctypes
+    from deploy3d_b200 import _lib
+    code = ctypes.c_int(-1)
+    _lib.check("d3d_debug_take_kernel_error", _lib.lib().d3d_debug_take_kernel_error(ctypes.byref(code)))
+    return code.value
+
+
+@pytest.mark.parametrize("rows,inputs,outputs,base", [
+    (20000, 512, 512, 100), (128, 8192, 256, 100),      # a CTA to a tile: several tiles each, long sums
+    (9600, 2048, 1024, 100), (9600, 8192, 512, 100),    # two CTAs to a tile
+    (20, 200, 20000, 200), (20, 8192, 512, 200)])       # few rows: a CTA to a sum, a cluster to a sum
+def test_linear_whose_wait_gives_up(d3d, wait_limit, rows, inputs, outputs, base):
+    """A wait that gives up ends the launch with an error word, wherever in the kernel it happens; a launch without one is right, and
+    so are those after the limit is the usual one again."""
+    x, w = int8(1, rows, inputs), int8(2, outputs, inputs)
+    s, ws = 0.01 * normal(3, rows).abs(), 0.01 * normal(4, outputs)
+    want = d3d.int8_linear(x, s, w, ws)
+    assert kernel_error() == 0
+    codes = set()
+    for cycles in (1, 200, 700, 2000, 6000):
+        wait_limit(cycles)
+        got = d3d.int8_linear(x, s, w, ws)
+        code = kernel_error()
+        codes.add(code)
+        assert code == 0 or base < code <= base + 4
+        assert code or torch.equal(got, want)
+    wait_limit(0)
+    assert codes - {0}, "no wait gave up"
+    for _ in range(3):
+        assert torch.equal(d3d.int8_linear(x, s, w, ws), want) and kernel_error() == 0
+
+
 def test_linear_of_rows_that_are_not_finite(d3d):
     """A row with a NaN in it is NaN behind the product, and no other is."""
     for rows in (4, 200):
