@@ -55,11 +55,21 @@ struct ScanArgs {
 
 __device__ __forceinline__ bool is_reset(float a) { return __float_as_int(a) < 0; }
 __device__ __forceinline__ float reset_mark() { return __int_as_float((int)0x80000000u); }
+// a h + b for the factor of several rows.  As a product of many gates it may have become zero although none of them is; walked row by
+// row an infinite state stays one, so it does here: zero is taken as 2^-149 times 2^-149, which no number is left of.
+__device__ __forceinline__ float carry_on(float a, float b, float h) {
+  const float least = __int_as_float(1);
+  return fmaf(a == 0.f ? least : a, h * (a == 0.f ? least : 1.f), b);
+}
 // The map (a, b) at h.
-__device__ __forceinline__ float apply(float a, float b, float h) { return is_reset(a) ? b : fmaf(a, h, b); }
+__device__ __forceinline__ float apply(float a, float b, float h) {
+  const float r = carry_on(a, b, h);
+  return is_reset(a) ? b : r;
+}
 // (a, b) after (pa, pb).
 __device__ __forceinline__ void after(float& a, float& b, float pa, float pb) {
-  if (!is_reset(a)) b = fmaf(a, pb, b), a *= pa;
+  b = apply(a, b, pb);
+  a = is_reset(a) ? a : a * pa;
 }
 
 // f = sigmoid(gate) and 1 - f.  With t = exp(-|gate|) the smaller one is t / (1 + t), the other one a difference that loses

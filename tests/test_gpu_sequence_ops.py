@@ -286,6 +286,39 @@ def test_sequences_do_not_touch_each_other(d3d, dtype, channels):
             assert torch.equal(a[rows_ok], b[rows_ok]) if len(a) == rows else torch.equal(a[seqs_ok], b[seqs_ok])
 
 
+def check_not_finite(got, want, limit, dtype, what):
+    """Infinities and NaN where the definition, walked row by row, has them; the others within their bound."""
+    got, fine = ref.as64(got), np.isfinite(want)
+    assert np.array_equal(got[~fine], want[~fine], equal_nan=True), what
+    ref.assert_within(got[fine], want[fine], (limit + ref.half_step(dtype) * (np.abs(want) + limit) + ref.smallest(dtype))[fine], what)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("reverse", [False, True])
+@pytest.mark.parametrize("rows,channels", [(90, 8), (700, 5), (1500, 24), (1500, 72)])
+def test_states_that_are_not_finite(d3d, dtype, reverse, rows, channels):
+    """An infinite state stays one whatever tiles lie behind it, although the product of their gates, 0.27 and less each, is no number
+    any more; opposite ones make NaN.  The same for gradients, walked the other way."""
+    x, g = features(1, rows, channels, dtype), (-1 - normal(2, rows, channels).abs()).to(dtype)
+    grad, offs = normal(3, rows, channels).to(dtype), [0, rows // 9, rows - rows // 9, rows]
+    initial, gf = normal(4, 3, channels), normal(5, 3, channels)
+    inf, a, b = float("inf"), rows // 4, rows - rows // 5
+    x[a, 0], x[a, 1], x[b, 1], initial[1, 2], x[a, 3] = inf, inf, -inf, -inf, float("nan")
+    grad[a, 0], grad[b, 1], grad[a, 2], gf[1, 4] = inf, -inf, inf, inf
+    offsets = torch.tensor(offs, dtype=torch.int32, device=DEV)
+    h, final, states = d3d.gated_recurrence(x, g, offsets, initial, reverse=reverse, with_states=True)
+    got = d3d.gated_recurrence_backward(grad, x, g, offsets, states, initial, gf, reverse=reverse)
+    x64, g64, i64 = ref.as64(x), ref.as64(g), ref.as64(initial)
+    with np.errstate(invalid="ignore"):
+        want, off, wfinal, foff, _, _ = ref.recurrence(x64, g64, offs, i64, reverse, dtype)
+        back = ref.recurrence_backward(ref.as64(grad), x64, g64, offs, i64, ref.as64(gf), reverse, dtype)
+        assert np.isinf(want).sum() > rows / 2 and np.isnan(want).any() and np.isinf(back[0][0]).any()
+        check_not_finite(h, want, off, dtype, "h")
+        check_not_finite(final, wfinal, foff, torch.float32, "final")
+        for t, (w, o), what in zip(got, back, ("dx", "dgates", "dinitial")):
+            check_not_finite(t, w, o, torch.float32 if what == "dinitial" else dtype, what)
+
+
 def test_recurrence_gates_at_their_ends(d3d):
     """Gates so large that nothing is added or kept, also in 32 bits: the state passes unchanged or is the row."""
     x = features(1, 300, 16, torch.float32)
