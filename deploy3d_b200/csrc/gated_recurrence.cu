@@ -73,7 +73,8 @@ __device__ __forceinline__ void after(float& a, float& b, float pa, float pb) {
 }
 
 // f = sigmoid(gate) and 1 - f.  With t = exp(-|gate|) the smaller one is t / (1 + t), the other one a difference that loses
-// nothing; with t = exp(-gate) the same from f = 1 / (1 + t) and 1 - f = t f, where f is taken as the difference while t < 1.
+// nothing; with t = exp(-gate) the smaller one is t / (1 + t) while t < 1, then 1 / (1 + t), zero where t is infinite (463 k x 64 bf16
+// 70.2 us; by exp(-|gate|) 76.8).
 // Neither has a sign, NaN included: the sign of a map means a reset.
 // Features of 32 bits: exponential and quotient to two units of the last place.  Of 16 bits: the hardware's base-two exponential,
 // whose argument is rounded to |gate| 2^-24 (so that 1 - f is off by that much, relatively; the gate itself came rounded to 2^-9
@@ -86,17 +87,16 @@ template <class T, int V> __device__ __forceinline__ void gate_of(const Vec<V>& 
       f.v[e] = g.v[e] >= 0.f ? large : small, rest.v[e] = g.v[e] >= 0.f ? small : large;
     }
   } else {
-    Vec<V> y = mul(g, all<V>(-1.44269504f)), t, r;
+    const Vec<V> y = mul(g, all<V>(-1.44269504f));
+    Vec<V> t, r;
 #pragma unroll
-    for (int e = 0; e < V; ++e) {
-      // 2^100 is as good as infinity: of any 16-bit state nothing is left, and 1 - f is one
-      asm("min.NaN.f32 %0, %0, 0f42C80000;" : "+f"(y.v[e]));
-      asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(t.v[e]) : "f"(y.v[e]));
-    }
+    for (int e = 0; e < V; ++e) asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(t.v[e]) : "f"(y.v[e]));
     const Vec<V> d = add(t, all<V>(1.f));
 #pragma unroll
     for (int e = 0; e < V; ++e) asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r.v[e]) : "f"(d.v[e]));
-    rest = mul(t, r);
+    const Vec<V> large = fma(r, all<V>(-1.f), all<V>(1.f));
+#pragma unroll
+    for (int e = 0; e < V; ++e) rest.v[e] = t.v[e] < 1.f ? t.v[e] * r.v[e] : large.v[e];
     f = fma(rest, all<V>(-1.f), all<V>(1.f));
 #pragma unroll
     for (int e = 0; e < V; ++e) f.v[e] = t.v[e] < 1.f ? f.v[e] : r.v[e];

@@ -334,6 +334,33 @@ def test_recurrence_gates_at_their_ends(d3d):
     assert torch.equal(d3d.gated_recurrence(x, inf, offsets, initial)[0], initial.expand(300, 16))
 
 
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_recurrence_gates_at_their_ends_in_16_bits(d3d, dtype):
+    """The same, for states as large as 32 bits hold; gates between have their part of such a state."""
+    lowest = torch.finfo(dtype).min
+    x = features(1, 300, 16, dtype)
+    offsets = torch.tensor([0, 300], dtype=torch.int32, device=DEV)
+    for size in (1.0, 3e38):
+        initial = size * normal(2, 1, 16).sign()
+        for gate in (-200.0, lowest, float("-inf")):
+            g = torch.full_like(x, gate)
+            out, final = d3d.gated_recurrence(x, g, offsets, initial)
+            assert torch.equal(out, x) and torch.equal(final, x[-1:].float())
+            one = d3d.gated_recurrence_step(x[:1], g[:1], initial)
+            assert torch.equal(one[0], x[:1]) and torch.equal(one[1], x[:1].float())
+            assert torch.equal(d3d.gated_recurrence(x, -g, offsets, initial)[1], initial)
+            _, _, states = d3d.gated_recurrence(x, g, offsets, initial, with_states=True)
+            dx, dg, di = d3d.gated_recurrence_backward(x, x, g, offsets, states, initial)
+            assert torch.equal(dx, x) and not dg.any() and not di.any()
+    g = (-60 - 26 * torch.rand((300, 16), generator=torch.Generator(device=DEV).manual_seed(3), device=DEV)).to(dtype)
+    state, zero = 1e38 * normal(4, 300, 16), torch.zeros_like(x)
+    singles = list(range(301))
+    want, off, wfinal, foff, _, _ = ref.recurrence(ref.as64(zero), ref.as64(g), singles, ref.as64(state), False, dtype)
+    for got in (d3d.gated_recurrence(zero, g, torch.tensor(singles, dtype=torch.int32, device=DEV), state),
+                d3d.gated_recurrence_step(zero, g, state)):
+        ref.assert_within(got[1], wfinal, foff + ref.U32 * np.abs(wfinal), "state")
+
+
 @pytest.mark.parametrize("offs", [[5, 3], [-4, 50], [0, 500], [20, 10, 60, 0, 99], [-9, -3], [400, 600]])
 def test_offsets_out_of_order_stay_inside_the_tensors(d3d, offs):
     """Nothing is said about the results; rows behind the tensors' own are not touched."""
