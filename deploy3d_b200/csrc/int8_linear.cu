@@ -752,11 +752,15 @@ template <class T> int launch_linear(const LinearArgs& a, cudaStream_t st) {
 // Whether the integer units' dot products are taken: where there is so little to multiply that setting up the tensor cores takes
 // longer (us, dot products / tensor cores, launched on their own: one row 256 -> 512 4.1 / 6.3, 1024 -> 1024 4.2 / 6.3; behind
 // other kernels, where the setting up is hidden, they are equal up to 2048 -> 2048, 5.4 / 4.7, and at 4096 -> 4096 8.2 / 5.6),
-// and for few rows that do not start on 16 bytes, where a copy of all weights to better places takes longer (dot products / copy and
-// tensor cores, 1001 -> 5000, one row, four, six: 6.5 / 12.5, 10.6 / 16.5, 14.7 / 16.6; 3802 -> 3731: 12.6 / 18.9, 21.5 / 22.8,
-// 33.1 / 22.9).
-bool little(int64_t rows, int64_t inputs, int64_t outputs, bool aligned) {
-  return (rows <= 64 && rows * inputs * outputs <= (1 << 22)) || (!aligned && rows <= 4);
+// and for few rows by weights that do not start on 16 bytes, where a copy of all weights to better places takes longer (dot products
+// / copy and tensor cores, 1001 -> 5000, one row, four, six: 6.5 / 12.5, 10.6 / 16.5, 14.7 / 16.6; 3802 -> 3731: 12.6 / 18.9,
+// 21.5 / 22.8, 33.1 / 22.9).  Where only the rows do not, the dot products read the weights by bytes too, and it is the rows that the
+// others copy: twice as much work and short sums are still little (one row 512 -> 16000 4.9 / 7.2, 1008 -> 8000 6.8 / 7.2,
+// 1024 -> 16384 8.2 / 7.4, 2048 -> 3584 8.8 / 7.2, 4096 -> 4096 13.2 / 7.5, four rows 33 / 7.5).
+bool little(int64_t rows, int64_t inputs, int64_t outputs, bool aligned_rows, bool aligned_weights) {
+  const int64_t work = rows * inputs * outputs;
+  if (rows <= 64 && work <= (1 << 22)) return true;
+  return aligned_weights ? !aligned_rows && rows * inputs <= 1024 && work <= (1 << 23) : rows <= 4;
 }
 
 size_t repitched(const void* p, int64_t ld, int64_t rows, int channels) {
@@ -778,7 +782,7 @@ using namespace d3d;
 
 extern "C" size_t d3d_int8_linear_workspace(const int8_t* x, int64_t x_ld, int64_t rows, const int8_t* weight, int64_t weight_ld,
                                             int inputs, int outputs) {
-  if (inputs < 1 || outputs < 1 || little(rows, inputs, outputs, aligned_rows(x, x_ld) && aligned_rows(weight, weight_ld))) return 0;
+  if (inputs < 1 || outputs < 1 || little(rows, inputs, outputs, aligned_rows(x, x_ld), aligned_rows(weight, weight_ld))) return 0;
   return repitched(x, x_ld, rows, inputs) + repitched(weight, weight_ld, outputs, inputs);
 }
 
@@ -801,9 +805,8 @@ extern "C" int d3d_int8_linear(int dtype, const int8_t* x, int64_t x_ld, const f
   D3D_REQUIRE(workspace_bytes >= need, D3D_ERR_WORKSPACE_TOO_SMALL);
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   LinearArgs a = {x, weight, x_ld, weight_ld, x_scales, weight_scales, bias, out, rows, num_rows, inputs, outputs};
-  const bool aligned = aligned_rows(x, x_ld) && aligned_rows(weight, weight_ld);
-  const bool dot = little(rows, inputs, outputs, aligned);
-  if (!aligned && !dot) {
+  const bool dot = little(rows, inputs, outputs, aligned_rows(x, x_ld), aligned_rows(weight, weight_ld));
+  if (!dot) {
     uint8_t* ws = reinterpret_cast<uint8_t*>(workspace);
     const int64_t pitch = (int64_t)align_up(inputs, 16);
     if (!aligned_rows(x, x_ld)) {

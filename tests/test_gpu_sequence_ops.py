@@ -587,6 +587,21 @@ def test_linear_by_tiles_of_every_width(d3d, rows, inputs, outputs):
         check_linear(x, s, w, ws, b, d3d.int8_linear(x, s, w, ws, b, dtype=dtype))
 
 
+@pytest.mark.parametrize("rows", [1, 2, 3, 4, 5, 20, 100])
+@pytest.mark.parametrize("layouts", [("odd", "dense"), ("columns", "odd"), ("odd", "columns")])
+@pytest.mark.parametrize("inputs,outputs", [(1024, 5000), (2080, 2500), (48, 40)])
+def test_linear_of_one_side_off_its_places(d3d, rows, layouts, inputs, outputs):
+    dtype = TYPES[(rows + outputs) % 3]
+    x, w = int8(1, rows, inputs, layouts[0]), int8(2, outputs, inputs, layouts[1])
+    s, ws, b = 0.01 * normal(3, rows).abs(), 0.01 * normal(4, outputs), normal(5, outputs)
+    check_linear(x, s, w, ws, b, d3d.int8_linear(x, s, w, ws, b, dtype=dtype))
+    out = torch.full((rows, outputs), 7.0, device=DEV, dtype=dtype)
+    d3d.int8_linear(x, s, w, ws, b, dtype=dtype, num_rows=live(rows - 1), out=out)
+    assert (out[rows - 1:] == 7).all()
+    if rows > 1:
+        check_linear(x[:-1], s[:-1], w, ws, b, out[:-1])
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("outputs", [24, 20, 18, 17, 264, 260, 258, 257])
 @pytest.mark.parametrize("start", [0, 1, 2, 4, 8])

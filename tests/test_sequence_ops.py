@@ -96,6 +96,16 @@ def test_entry_points_refuse_addresses_off_their_elements(d3d):
     refuses(lib.d3d_gated_recurrence_step, step, dict(x=2, g=2, out=2, s=4, so=4))
 
 
+def test_few_rows_off_their_places_are_copied_and_not_all_weights_read_by_bytes(d3d):
+    from deploy3d_b200 import _lib
+    need = lambda x, rows, w: _lib.lib().d3d_int8_linear_workspace(ctypes.c_void_p(x), 4096, rows, ctypes.c_void_p(w), 4096, 4096, 4096)
+    for rows in (1, 4):
+        assert need(4097, rows, 4096) == 4096 * rows      # the rows go to the workspace
+        assert need(4097, rows, 4097) == need(4096, rows, 4097) == 0  # the weights are read where they are
+        assert need(4096, rows, 4096) == 0
+    assert need(4097, 5, 4097) == 4096 * (5 + 4096) and need(4096, 5, 4097) == 4096 * 4096
+
+
 def test_kernels_read_what_may_still_be_written_by_plain_loads():
     """The kernels live while the one in front of them still writes, so none of their loads may be of the kind that takes memory
     for constant as long as the kernel lives: __ldg, or what a const __restrict__ argument allows a plain load to become."""
