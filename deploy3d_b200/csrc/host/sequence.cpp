@@ -104,6 +104,10 @@ at::Tensor output(PyObject* o, std::initializer_list<int64_t> shape, at::ScalarT
   dense_tensor(o, "out", shape, type, device);
   return THPVariable_Unpack(o);
 }
+// `out`, where it was given, has other contents now: autograd refuses to go back through what it has kept of the old ones.
+void wrote(PyObject* o, const at::Tensor& out) {
+  if (o != Py_None && !out.is_inference()) out.unsafeGetTensorImpl()->bump_version();
+}
 void* at_of(const at::Tensor& t) { return t.defined() && t.numel() ? t.data_ptr() : nullptr; }
 float* floats_of(const at::Tensor& t) { return static_cast<float*>(at_of(t)); }
 
@@ -167,6 +171,7 @@ PyObject* layer_norm(Args a, Py_ssize_t n) {
     return f_layer_norm(dtype_of(x.t), x.p(), x.ld, r.p(), r.ld, weight, bias, eps, x.rows, (int)x.channels, count, at_of(total),
                         at_of(out), floats_of(mean), floats_of(rstd), stream);
   });
+  wrote(a[7], out);
   if (!total.defined() && !mean.defined()) return THPVariable_Wrap(out);
   return tuple_of({out, total, mean, rstd});
 }
@@ -259,6 +264,7 @@ PyObject* int8_linear(Args a, Py_ssize_t n) {
     return f_int8_linear(dtype_of(out), px, x.ld, scales, x.rows, count, pw, w.ld, w_scales, bias, (int)x.channels, (int)w.rows,
                          at_of(out), at_of(ws), bytes, stream);
   });
+  wrote(a[7], out);
   return THPVariable_Wrap(out);
 }
 
@@ -294,6 +300,7 @@ PyObject* gated_recurrence(Args a, Py_ssize_t n) {
                               (int)x.channels, reverse, initial, at_of(out), floats_of(final_state), floats_of(states), at_of(ws),
                               bytes, stream);
   });
+  wrote(a[6], out);
   return tuple_of({out, final_state, states});
 }
 
@@ -333,6 +340,7 @@ PyObject* gated_recurrence_step(Args a, Py_ssize_t n) {
     return f_gated_recurrence_step(dtype_of(x.t), x.p(), x.ld, g.p(), g.ld, state, floats_of(next), at_of(out), x.rows,
                                    (int)x.channels, stream);
   });
+  wrote(a[3], next);
   return tuple_of({out, next});
 }
 

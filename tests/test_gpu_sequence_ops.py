@@ -810,6 +810,28 @@ def test_results_in_place_of_the_features(d3d):
                 assert torch.equal(again, want)
 
 
+def test_autograd_notices_what_was_written_over(d3d):
+    """A tensor that autograd has kept and that an operator is then given as `out`: going back raises, as behind torch's own
+    operators in place, and does not use the new contents.  Tensors of inference mode have no such count."""
+    x, offsets = features(1, 40, 16, torch.float32), torch.tensor([0, 40], dtype=torch.int32, device=DEV)
+    q, s = d3d.quantize_rows(x)
+    calls = [lambda out: d3d.layer_norm(x, None, out=out), lambda out: d3d.gated_recurrence(x, x, offsets, out=out),
+             lambda out: d3d.gated_recurrence_step(x, x, x, state_out=out),
+             lambda out: d3d.int8_linear(q, s, q[:16], s[:16], dtype=torch.float32, out=out)]
+    for call in calls:
+        a, kept = normal(2, 40, 16).requires_grad_(), normal(3, 40, 16)
+        y = (a * kept).sum()
+        before = kept._version
+        call(kept)
+        assert kept._version == before + 1
+        with pytest.raises(RuntimeError):
+            y.backward()
+        with torch.inference_mode():
+            buf = torch.empty((40, 16), device=DEV)
+        call(buf)
+        assert torch.equal(buf, kept) and x._version == 0
+
+
 def test_refusals_on_the_gpu(d3d):
     """Shapes, types and devices that do not fit raise before anything is launched."""
     x, g = features(1, 8, 16, torch.float16), features(2, 8, 16, torch.float16)
