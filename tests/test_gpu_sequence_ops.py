@@ -123,6 +123,21 @@ def test_norm_rows_keep_to_themselves(d3d):
             assert got[5].isnan().all() and got[40].isnan().all() and (got[66] == 0).all()
 
 
+@pytest.mark.parametrize("dtype,mean,rows,channels", [
+    (torch.float32, 1e4, 300, 64), (torch.float32, -3e4, 65, 1001), (torch.float32, 1e4, 9, 4096), (torch.float16, 200.0, 300, 64),
+    (torch.float16, -200.0, 77, 131), (torch.bfloat16, 30.0, 513, 256), (torch.bfloat16, -30.0, 5, 8191)])
+def test_norm_of_rows_far_from_zero(d3d, dtype, mean, rows, channels):
+    """A mean far above the spread, of either sign: what a difference of two large sums, or of squares, would lose."""
+    x, grad = (mean + normal(1, rows, channels)).to(dtype), normal(3, rows, channels).to(dtype)
+    weight, bias = 1 + 0.2 * normal(4, channels), 0.1 * normal(5, channels)
+    y, m, r = d3d.layer_norm(x, weight, bias, EPS, with_stats=True)
+    check_norm(x, weight, bias, y, m, r)
+    got = d3d.layer_norm_backward(grad, x, weight, m, r)
+    want = ref.norm_backward(ref.as64(grad), ref.as64(x), ref.as64(weight), ref.as64(m), ref.as64(r))
+    for g, (w, limit), what in zip(got, want, ("dx", "dweight", "dbias")):
+        ref.assert_within(g, w, limit + ref.half_step(g.dtype) * (np.abs(w) + limit) + ref.smallest(g.dtype), what)
+
+
 def test_norm_backward_is_the_same_every_time(d3d):
     x, g = features(1, 20011, 64, torch.bfloat16), features(2, 20011, 64, torch.bfloat16)
     w = normal(4, 64)
@@ -458,6 +473,62 @@ def test_offsets_out_of_order_over_several_tiles(d3d):
             d3d.gated_recurrence_backward(x, x, x, offsets, states, reverse=reverse)
             torch.cuda.synchronize()
             assert (buf[:32] == 5).all() and (buf[32 + rows:] == 5).all()
+
+
+def walk64(a, b):
+    """h[t] = a[t] h[t-1] + b[t] from h = 0, along the rows, in 64 bits on the GPU: blocks of rows side by side, then their ends one
+    after the other, then what comes into each block."""
+    rows, channels = a.shape
+    block = int(rows ** 0.5)
+    many = -(-rows // block)
+    a, b = (torch.nn.functional.pad(t, (0, 0, 0, many * block - rows)).view(many, block, channels).clone() for t in (a, b))
+    for t in range(1, block):
+        b[:, t] += a[:, t] * b[:, t - 1]
+        a[:, t] *= a[:, t - 1]
+    into = torch.zeros((many, channels), dtype=a.dtype, device=a.device)
+    for t in range(1, many):
+        into[t] = a[t - 1, -1] * into[t - 1] + b[t - 1, -1]
+    return (b + a * into[:, None]).view(-1, channels)[:rows]
+
+
+@pytest.mark.parametrize("reverse", [False, True])
+@pytest.mark.parametrize("rows", [600001, 4300007])
+def test_recurrence_of_one_sequence_over_many_tiles(d3d, reverse, rows):
+    """17 channels in 16 bits go by tiles of 128 rows.  4096 tiles are what the chain over them takes at a time, 32768 what a
+    dimension of the grid does.  With gates around 8 a state lasts for thousands of rows, and with means of 1 it is of the size
+    of the rows, so that what comes into a tile counts.  Definition and bounds are those of tests/_sequence.py, for all rows at once."""
+    channels, dtype = 17, torch.float16
+    x, g, grad = ((mean + normal(seed, rows, channels)).to(dtype) for seed, mean in ((1, 1.0), (3, 8.0), (4, 1.0)))
+    offsets = torch.tensor([0, rows], dtype=torch.int32, device=DEV)
+    initial, gf = 100 * normal(5, 1, channels), 100 * normal(6, 1, channels)
+    h, final, states = d3d.gated_recurrence(x, g, offsets, initial, reverse=reverse, with_states=True)
+    dx, dg, di = d3d.gated_recurrence_backward(grad, x, g, offsets, states, initial, gf, reverse=reverse)
+    turn = (lambda t: t.flip(0)) if reverse else (lambda t: t)
+    x, gate, grad = (turn(t).double() for t in (x, g, grad))
+    f, add, k = torch.sigmoid(gate), torch.sigmoid(-gate), ref.K + ref.PER_GATE * gate.abs()
+    first, last = torch.zeros_like(f), torch.zeros_like(f)
+    first[0], last[-1] = f[0], f[-1]
+    del gate
+
+    def check(got, want, off, what, rnd=dtype):
+        off = off + ref.half_step(rnd) * (want.abs() + off) + ref.smallest(rnd)
+        assert ((got.double() - want).abs() <= off).all(), what
+    want = walk64(f, add * x + first * initial)
+    size = walk64(f, add * x.abs() + first * initial.abs())
+    off = walk64(f, ref.U32 * k * size)
+    check(turn(h), want, off, "h")
+    check(final, want[-1:], off[-1:], "final", torch.float32)
+    before, before_off = torch.cat([initial.double(), want[:-1]]), torch.cat([0 * off[:1], off[:-1]])
+    del want, size, off
+    back = lambda a, b: walk64(a.flip(0), b.flip(0)).flip(0)
+    into = lambda t, end: torch.cat([t[1:], end])  # of what leaves a row: what comes into the one in front of it
+    q, size = back(f, f * grad + last * gf), back(f, f * grad.abs() + last * gf.abs())
+    check(di, q[:1], (e := back(f, ref.U32 * (1 + k) * size))[:1], "dinitial", torch.float32)
+    delta, dsize = grad + into(q, gf.double()), grad.abs() + into(size, gf.abs().double())
+    doff = into(e, 0 * e[:1]) + ref.U32 * dsize
+    check(turn(dx), delta * add, add * (doff + ref.U32 * k * dsize), "dx")
+    check(turn(dg), delta * (before - x) * f * add, f * add * (doff * (before - x).abs() + dsize * before_off +
+                                                               ref.U32 * k * dsize * (before.abs() + x.abs())), "dgates")
 
 
 # ---- streams, graphs ------------------------------------------------------------------------------------------------
