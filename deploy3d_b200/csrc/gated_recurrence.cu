@@ -8,11 +8,12 @@
 // waits for another CTA, and every sum is made in one order.  A row that starts a sequence is the map c -> b whatever c is, also
 // where c is not finite: its a is -0, and the sign says that what came before is not looked at (products keep it, f is never
 // negative).
-// The rows are read twice, the second time in part from L2.  One kernel that hands the state from tile to tile would read them
-// once, but 3618 tiles would wait for each other through memory (not built).  Measured: 463 k x 64 bf16 73 us, maps 30, chain 8,
-// rows 31 to 41 by what L2 still holds (178 MB of features in and out, floor 27 us); 120 k x 128 fp16 with gradients 107 us, maps 21
-// and 19, chains 5 and 5, rows 21 and 45.  Maps are bound by instructions (23 an element, 2.9 a cycle issued of 4), the rows by
-// their bytes, backward by the 16 warps an SM that 128 registers leave.
+// The rows are read twice, the second time in part from L2, and the gate is evaluated both times.  One kernel that hands the state
+// from tile to tile would do either once; it has not been built, so what its waits would cost is not known.  Measured: 463 k x 64 bf16
+// 73 us, maps 30, chain 8, rows 31 to 40 by what L2 still holds (178 MB of features in and out, floor 27 us); 120 k x 128 fp16 with
+// gradients 109 us, maps 21 and 20, chains 5 and 5, rows 21 and 47.  Maps are bound by instructions (23 an element, 2.9 a cycle
+// issued of 4), the rows by their bytes, backward by the 16 warps an SM that 128 registers leave.  Forward the last kernel
+// spills 32 bytes a thread of paired 16-bit rows (64 registers, for four CTAs an SM).
 #include <cstring>
 #include <type_traits>
 

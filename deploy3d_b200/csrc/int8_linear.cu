@@ -6,7 +6,7 @@
 // channels: operands by TMA in 128-byte rows (128 channels of the sum a stage), several accumulators in tensor memory so that
 // the epilogue of one tile runs beside the products of the next.  Up to kFewRows rows: the other way round, tiles of 128 output
 // channels by all rows.  Little work is left to the integer units.
-// Measured: 8192 x 4096 -> 8192 bf16 167 us, 3.29 Pop/s, the tensor cores 88 % busy (in a row of calls the power cap makes it 176 to
+// Measured: 8192 x 4096 -> 8192 bf16 170 us, 3.2 Pop/s, the tensor cores 87 % busy (in a row of calls the power cap makes it 175 to
 // 205); short sums are bound by what happens to an output piece, accumulator to registers to shared memory to memory, one after
 // the other: 238 k x 64 -> 192 fp16 33 us, 3.2 TB/s, tensor cores 4 %; one row 4096 -> 4096 5.5 us, 3 TB/s of weights.
 #include <mutex>

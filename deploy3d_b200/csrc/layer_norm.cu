@@ -3,11 +3,14 @@
 //   dx = rstd (g - <g> - xhat <g xhat>),  g = dy w,  xhat = (t - mean) rstd,  dw = sum dy xhat,  db = sum dy
 //   s = max |y| / 127,  q = rint(y / s)
 // All of them move bytes: every tensor is read and written once, in 16-byte pieces, a row stays in the registers of
-// the threads that share it, and mean, variance and the two means of the backward pass are exact sums over those
+// the threads that share it, and mean, variance and the two means of the backward pass are sums in 32 bits over those
 // registers (the variance of differences to the mean, not a difference of two large sums).
 // Measured, of the 6.55 TB/s that a copy gets: a norm with a residual of 120 k x 128 bf16 20.9 us, 5.9 TB/s; norm and backward pass
 // of 238 k x 64 bf16 13.4 + 27.5 + 5.5 us (five passes over the rows, some of them from L2), of 4099 x 4096 in 32 bits 22 + 36 +
-// 7 us; a norm of 66 k x 256 bf16 in 8 bits 25.5 us, 2.0 TB/s, bound by the instructions of norm and rounding.
+// 7 us; a norm of 66 k x 256 bf16 with a residual in 8 bits 28 us, 4.2 TB/s of 118 MB: neither the bytes nor the instructions (2.0 a
+// cycle of 4) are all there can be; a row is a chain of three sums and the rounding, with 24 warps an SM to hide it.
+// Not all fits the registers: spilled are 96 to 136 bytes a thread backward for 16-bit rows of 8 to 1024 channels (80 registers, for
+// three CTAs an SM), 200 to 570 for the longest rows, 50 to 70 forward for up to 512 channels in 32 bits, 16 in 8 bits.
 #include <type_traits>
 
 #include "common.cuh"

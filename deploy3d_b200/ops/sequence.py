@@ -4,9 +4,10 @@ norm, its rows in 8-bit integers, and a gated linear recurrence.  The reference 
 Features are CUDA tensors ``[rows, channels]`` in float32, float16 or bfloat16 and may be columns of a wider tensor (their
 channels side by side); parameters, scales and states are float32.  Everything runs on the current stream of the features'
 device.  ``num_rows``, an int32 tensor of one element on the device, says how many rows are live, as the counts of the voxel
-operators do: rows behind are neither read nor written (in a tensor the call has made itself they hold nothing).  ``out``
-takes the result where given: dense, of the right shape and type; it may be the (dense) features themselves.  Backward passes are functions of their own; nothing here
-records autograd history.
+operators do: rows behind are not written, and what they hold does not matter (in a tensor the call has made itself they hold
+nothing).  ``out`` takes the result where given: dense, of the right shape and type; it may be the (dense) features themselves.
+Backward passes are functions of their own: nothing here records autograd history, also where features or parameters require
+gradients.
 """
 import torch
 
@@ -43,7 +44,7 @@ def layer_norm_int8(feats, weight, bias=None, eps=1e-5, residual=None, num_rows=
 
 def quantize_rows(feats, num_rows=None):
     """(int8 [rows, channels], float32 [rows]): scale = max |row| / 127, row / scale to the nearest integer, ties to even.  Rows
-    of zeros have scale 0, rows that are not finite zeros and scale NaN.  At most 8192 channels.  The rows lie a multiple of
+    of zeros, or of less than 127 times the smallest normal float, have scale 0, rows that are not finite zeros and scale NaN.  At most 8192 channels.  The rows lie a multiple of
     16 bytes apart."""
     return (_NATIVE or _native()).quantize_rows(feats, num_rows)
 
@@ -63,8 +64,10 @@ def gated_recurrence(feats, gates, seq_offsets, initial=None, reverse=False, wit
 
     seq_offsets int32 [sequences + 1] on the device, ascending: sequence s are the rows seq_offsets[s] .. seq_offsets[s+1]-1, walked
     downwards with `reverse`; equal ones are a sequence without rows.  initial float32 [sequences, channels]: h in front of the
-    first row walked (None: zeros).  Rows outside all sequences are not written, and what they hold does not matter.  Returns (h in the type of
-    feats, h of the last row walked of every sequence in float32); with `with_states` also what the backward pass needs."""
+    first row walked (None: zeros).  Rows outside all sequences are not written, and what they hold does not matter.  An
+    infinite h stays infinite to the end of its sequence (NaN where f is zero in float or an infinite row is against it).
+    Returns (h in the type of feats, h of the last row walked of every sequence in float32); with `with_states` also what the
+    backward pass needs."""
     return (_NATIVE or _native()).gated_recurrence(feats, gates, seq_offsets, initial, reverse, with_states, out)
 
 

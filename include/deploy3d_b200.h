@@ -489,7 +489,8 @@ int d3d_yolox3d_decode_enqueue(const d3d_yolox3d_decode_params* p, const d3d_ten
  * (at least the row's own), so that inputs may be columns of a wider tensor; outputs without one are dense.  Rows that start
  * on 16 bytes and are multiples of 16 bytes apart are read in wider pieces than others.  The kernels are launched as programmatic
  * dependents: they may start before the kernel in front of them has ended, and wait for it before they touch memory.
- * `num_rows`: the live rows, int32 [1] on the device, or NULL for all of them; rows behind are neither read nor written.
+ * `num_rows`: the live rows, int32 [1] on the device, or NULL for all of them; rows behind are not written, and what they
+ * hold does not matter.
  * An address that is not a multiple of its elements' size is refused (D3D_ERR_INVALID_ARGUMENT).
  * ------------------------------------------------------------------------------------------- */
 /* out = (t - mean) * rstd * weight + bias over the channels, t = x, or the sum x + residual rounded to the type, which is then
