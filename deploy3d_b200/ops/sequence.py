@@ -65,8 +65,8 @@ def gated_recurrence(feats, gates, seq_offsets, initial=None, reverse=False, wit
     seq_offsets int32 [sequences + 1] on the device, ascending: sequence s are the rows seq_offsets[s] .. seq_offsets[s+1]-1, walked
     downwards with `reverse`; equal ones are a sequence without rows.  initial float32 [sequences, channels]: h in front of the
     first row walked (None: zeros).  Rows outside all sequences are not written, and what they hold does not matter.  An
-    infinite h stays infinite to the end of its sequence (NaN where f is zero in float or an infinite row is against it).
-    Returns (h in the type of feats, h of the last row walked of every sequence in float32); with `with_states` also what the
+    infinite h stays infinite to the end of its sequence; behind a gate whose f is zero in float32 or an infinite row against it,
+    it may be NaN instead.  Returns (h in the type of feats, h of the last row walked of every sequence in float32); with `with_states` also what the
     backward pass needs."""
     return (_NATIVE or _native()).gated_recurrence(feats, gates, seq_offsets, initial, reverse, with_states, out)
 
