@@ -530,8 +530,9 @@ int d3d_int8_linear(int dtype, const int8_t* x, int64_t x_ld, const float* x_sca
  * (NULL: zeros); final_state [seqs][channels] (or NULL): h of the last one, initial where there is none.  Rows outside all
  * sequences are not written, and what they hold does not matter.  h is held in float; sequences do not touch each other,
  * whatever their values.  An infinite h stays infinite to the sequence's end; behind a gate whose f is zero in float (below
- * -87 for 16-bit gates, -103 for float ones) or an infinite x against it, it may be NaN instead.  out may be x where that is dense.  states: NULL, or [d3d_gated_recurrence_state_rows(rows)][channels],
- * what the backward pass needs.  rows < 2^31, channels <= 65536.  The workspace (of both directions) is 256-byte aligned; it may
+ * -87 for 16-bit gates, -103 for float ones) or an infinite x against it, it may be NaN instead.  out may be x where that is
+ * dense.  states: NULL, or [d3d_gated_recurrence_state_rows(rows)][channels], what the backward pass needs.  rows < 2^31,
+ * channels <= 65536.  The workspace (of both directions) is 256-byte aligned; it may
  * be NULL where its size is 0, up to 128 rows. */
 int64_t d3d_gated_recurrence_state_rows(int64_t rows);
 size_t d3d_gated_recurrence_workspace(int64_t rows, int channels);
